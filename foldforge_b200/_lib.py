@@ -118,6 +118,16 @@ SIGNATURES: dict[str, list] = {
     "ffb_transition_gemm_prepare": [c_void_p] * 5 + [c_int, c_int, c_void_p, c_void_p],
     "ffb_transition_gemm_fwd": [c_void_p, c_void_p, c_void_p, c_void_p, ctypes.c_size_t, c_i64, c_int, c_int,
                                 c_void_p],
+    # training operators
+    "ffb_layernorm_train_fwd": [c_void_p] * 8 + [c_i64, c_int, c_float, c_int, c_void_p],
+    "ffb_layernorm_bwd_workspace_bytes": [c_i64, c_int, c_int],
+    "ffb_layernorm_bwd": [c_void_p] * 12 + [ctypes.c_size_t, c_i64, c_int, c_int, c_void_p],
+    "ffb_checkpoint_pack": [c_void_p] * 3 + [c_i64, c_int, c_int, c_void_p],
+    "ffb_checkpoint_unpack": [c_void_p] * 3 + [c_i64, c_int, c_int, c_void_p],
+    "ffb_weight_grad_workspace_bytes": [c_i64, c_int, c_int],
+    "ffb_weight_grad": [c_void_p] * 6 + [ctypes.c_size_t, c_i64, c_int, c_int, c_void_p],
+    "ffb_swiglu_train_fwd": [c_void_p] * 4 + [c_i64, c_int, c_int, c_void_p],
+    "ffb_swiglu_bwd": [c_void_p] * 6 + [c_i64, c_int, c_int, c_void_p],
 }
 
 #: entry points that return a size_t instead of a status
@@ -128,7 +138,8 @@ SIZE_RESULT = {"ffb_apb_packed_bytes", "ffb_apb_workspace_bytes", "ffb_single_tr
                "ffb_apb_single_workspace_bytes", "ffb_trimul_f32_workspace_bytes", "ffb_triattn_f32_workspace_bytes",
                "ffb_transition_f32_workspace_bytes", "ffb_apb_f32_workspace_bytes", "ffb_opm_packed_bytes",
                "ffb_opm_workspace_bytes", "ffb_pwa_packed_bytes", "ffb_pwa_workspace_bytes",
-               "ffb_transition_gemm_packed_bytes", "ffb_transition_gemm_workspace_bytes"}
+               "ffb_transition_gemm_packed_bytes", "ffb_transition_gemm_workspace_bytes",
+               "ffb_layernorm_bwd_workspace_bytes", "ffb_weight_grad_workspace_bytes"}
 
 STATUS = {0: "FFB_OK", 1: "FFB_ERR_ARG", 2: "FFB_ERR_UNSUPPORTED", 3: "FFB_ERR_CUDA", 4: "FFB_ERR_DEVICE"}
 

@@ -159,5 +159,43 @@ int generic_apb(const float* s, const float* z, const uint8_t* mask, const Gener
                 float* out, void* workspace, int B, int N, int cs, int cz, int H, float gate_bias, int masked_zero,
                 cudaStream_t stream);
 
+// ---- training operators (train.cu, wgrad.cu); codes / scales: an 8-bit checkpoint (mx8.cuh)
+constexpr int kMaxNormChannels = 8192;  // a row is held in one block's registers
+struct LayerNormTrain {
+  const void* x;
+  void* y;
+  const float *gamma, *beta;
+  float *mean, *rstd;
+  uint8_t *codes, *scales;  // null: no checkpoint is written
+  int64_t rows;
+  int c;
+  float eps;
+};
+struct LayerNormBwd {
+  const void *dy, *x;              // x null: the input comes from codes / scales
+  const uint8_t *codes, *scales;
+  const float *mean, *rstd, *gamma;
+  const void* residual;            // added to dx where not null
+  void* dx;
+  float *dgamma, *dbeta;           // null: not wanted
+  void* workspace;
+  int64_t rows;
+  int c;
+};
+size_t ln_bwd_workspace_bytes(int64_t rows, int c, int is_f32);
+int launch_ln_train(const LayerNormTrain& p, int is_f32, cudaStream_t stream);
+int launch_ln_bwd(const LayerNormBwd& p, int is_f32, cudaStream_t stream);
+int launch_checkpoint_pack(const void* x, uint8_t* codes, uint8_t* scales, int64_t rows, int c, int is_f32,
+                           cudaStream_t stream);
+int launch_checkpoint_unpack(const uint8_t* codes, const uint8_t* scales, void* x, int64_t rows, int c, int is_f32,
+                             cudaStream_t stream);
+int launch_swiglu_train(const void* ab, void* out, uint8_t* codes, uint8_t* scales, int64_t rows, int h, int is_f32,
+                        cudaStream_t stream);
+int launch_swiglu_bwd(const void* dh, const void* ab, const uint8_t* codes, const uint8_t* scales, void* dab, void* out,
+                      int64_t rows, int h, int is_f32, cudaStream_t stream);
+size_t weight_grad_workspace_bytes(int64_t rows, int n, int k);
+int weight_grad_forward(const void* dy, const void* x, const uint8_t* codes, const uint8_t* scales, float* dw,
+                        void* workspace, int64_t rows, int n, int k, const DeviceInfo& info, cudaStream_t stream);
+
 }  // namespace ffb
 

@@ -348,6 +348,45 @@ size_t ffb_dit_workspace_bytes(int S, int L);
 int ffb_dit_fwd(const void* x, const uint8_t* mask, const void* packed, const void* tables, void* out, void* workspace,
                 size_t workspace_bytes, int S, int L, void* stream);
 
+/* ---- Training operators. `rows` is the product of a tensor's leading axes, its last axis dense.
+ * A checkpoint is a row's channels in 8 bits: codes [rows, c] (e4m3) and scales [rows, ceil(c / 32)]
+ * (one byte a block of 32 channels; code value * 2^(byte - 127)), the scale being the smallest power
+ * of two that brings the block's largest finite magnitude to at most 448. Values that are not finite
+ * come back as NaN. `dtype` (ffb_dtype) is the activations'; statistics and the gradients of weights
+ * are fp32. rows may be 0 (weight gradients are then 0). Results do not depend on timing: every sum
+ * has a fixed order.
+ *
+ * ffb_layernorm_train_fwd: y = (x - mean) rstd gamma + beta with mean, rstd [rows] kept for the
+ *   backward pass; codes / scales (both or neither) receive x's checkpoint. gamma, beta may be NULL.
+ * ffb_layernorm_bwd: x (codes, scales NULL) or its checkpoint (x NULL): xh = (x - mean) rstd,
+ *   w = gamma dy, dx = rstd (w - mean_c(w) - xh mean_c(w xh)) (+ residual where not NULL),
+ *   dgamma = sum_rows dy xh, dbeta = sum_rows dy (each NULL where not wanted). c <= 8192.
+ * ffb_checkpoint_pack / _unpack: a checkpoint written from x, and read back.
+ * ffb_weight_grad: dw [n, k] fp32 = dy^T x over the rows: dy [rows, n] bf16, x [rows, k] bf16 or its
+ *   checkpoint.
+ * ffb_swiglu_train_fwd: out [rows, h] = silu(a) b of ab [rows, 2 h] = [a | b]; codes / scales (both or
+ *   neither) receive ab's checkpoint.
+ * ffb_swiglu_bwd: dab [rows, 2 h] from dh [rows, h] and ab or its checkpoint: da = dh b s (1 + a (1 - s)),
+ *   db = dh a s, s = sigmoid(a); out (or NULL) receives silu(a) b again.
+ * No output may alias an input. */
+int ffb_layernorm_train_fwd(const void* x, void* y, const float* gamma, const float* beta, float* mean, float* rstd,
+                            uint8_t* codes, uint8_t* scales, int64_t rows, int c, float eps, int dtype, void* stream);
+size_t ffb_layernorm_bwd_workspace_bytes(int64_t rows, int c, int dtype);
+int ffb_layernorm_bwd(const void* dy, const void* x, const uint8_t* codes, const uint8_t* scales, const float* mean,
+                      const float* rstd, const float* gamma, const void* residual, void* dx, float* dgamma,
+                      float* dbeta, void* workspace, size_t workspace_bytes, int64_t rows, int c, int dtype,
+                      void* stream);
+int ffb_checkpoint_pack(const void* x, uint8_t* codes, uint8_t* scales, int64_t rows, int c, int dtype, void* stream);
+int ffb_checkpoint_unpack(const uint8_t* codes, const uint8_t* scales, void* x, int64_t rows, int c, int dtype,
+                          void* stream);
+size_t ffb_weight_grad_workspace_bytes(int64_t rows, int n, int k);
+int ffb_weight_grad(const void* dy, const void* x, const uint8_t* codes, const uint8_t* scales, float* dw,
+                    void* workspace, size_t workspace_bytes, int64_t rows, int n, int k, void* stream);
+int ffb_swiglu_train_fwd(const void* ab, void* out, uint8_t* codes, uint8_t* scales, int64_t rows, int h, int dtype,
+                         void* stream);
+int ffb_swiglu_bwd(const void* dh, const void* ab, const uint8_t* codes, const uint8_t* scales, void* dab, void* out,
+                   int64_t rows, int h, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
