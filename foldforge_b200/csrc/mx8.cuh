@@ -17,16 +17,10 @@ namespace ffb {
 
 constexpr int kMxBlock = 32;
 
-// |x| where x is finite, else 0 (a NaN compares false)
-__device__ __forceinline__ float mx_magnitude(float x) {
-  const float a = fabsf(x);
-  return a <= 3.402823466e38f ? a : 0.f;
-}
-
-// The scale byte of a block from its largest finite magnitude: the biased exponent less 8, one more
-// where the mantissa is above 1.75 (adding 0x1FFFFF carries into the exponent exactly then).
-__device__ __forceinline__ uint32_t mx_scale_byte(float largest) {
-  const int e = static_cast<int>((__float_as_uint(largest) + 0x1FFFFFu) >> 23) - 8;
+// The scale byte of a block from the bits of its largest finite magnitude: the biased exponent less 8, one
+// more where the mantissa is above 1.75 (adding 0x1FFFFF carries into the exponent exactly then).
+__device__ __forceinline__ uint32_t mx_scale_byte(uint32_t largest) {
+  const int e = static_cast<int>((largest + 0x1FFFFFu) >> 23) - 8;
   return static_cast<uint32_t>(e > 0 ? e : 0);
 }
 
@@ -42,24 +36,11 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// x * inv, or NaN where x is not finite (the conversion above would make 448 of an infinity)
-__device__ __forceinline__ float mx_scaled(float x, float inv) {
-  return fabsf(x) <= 3.402823466e38f ? x * inv : __uint_as_float(0x7FFFFFFFu);
-}
-
 // two codes to fp32 (exact)
 __device__ __forceinline__ float2 e4m3x2_value(uint32_t pair) {
   uint32_t h;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(pair)));
   return __half22float2(*reinterpret_cast<__half2*>(&h));
-}
-
-// the largest magnitude over the `LANES` consecutive lanes that share a block
-template <int LANES>
-__device__ __forceinline__ float mx_block_max(float a) {
-#pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xFFFFFFFFu, a, o));
-  return a;
 }
 
 // ------------------------------------------------------------------ vectors of VEC elements
@@ -73,16 +54,14 @@ template <>
 struct MxCodes<1> { using type = uint8_t; };
 
 template <int VEC>
-__device__ __forceinline__ typename MxCodes<VEC>::type mx_encode(const float (&f)[VEC], float inv) {
+__device__ __forceinline__ typename MxCodes<VEC>::type mx_encode(const float (&f)[VEC]) {
   if constexpr (VEC == 1) {
-    const float v = mx_scaled(f[0], inv);
-    return static_cast<uint8_t>(e4m3x2(v, 0.f));
+    return static_cast<uint8_t>(e4m3x2(f[0], 0.f));
   } else {
     uint32_t w[VEC / 4];
 #pragma unroll
     for (int i = 0; i < VEC / 4; ++i)
-      w[i] = e4m3x2(mx_scaled(f[4 * i], inv), mx_scaled(f[4 * i + 1], inv)) |
-             (e4m3x2(mx_scaled(f[4 * i + 2], inv), mx_scaled(f[4 * i + 3], inv)) << 16);
+      w[i] = e4m3x2(f[4 * i], f[4 * i + 1]) | (e4m3x2(f[4 * i + 2], f[4 * i + 3]) << 16);
     if constexpr (VEC == 8)
       return make_uint2(w[0], w[1]);
     else
@@ -113,26 +92,99 @@ __device__ __forceinline__ void mx_decode(typename MxCodes<VEC>::type codes, flo
   }
 }
 
-// VEC elements of type T to and from fp32: VEC is a 16-byte load's worth (8 bf16, 4 fp32), or 1
+// VEC elements of type T as they lie in memory: VEC is a 16-byte load's worth (8 bf16, 4 fp32), or 1.
+// Kernels hold rows in this form (bf16 in half the registers of fp32) and widen on use.
 template <typename T, int VEC>
-__device__ __forceinline__ void load_vec(const T* p, float (&f)[VEC]) {
+struct Raw {
+  using type = uint4;
+};
+template <typename T>
+struct Raw<T, 1> {
+  using type = T;
+};
+
+// a load of data that is read once (kept out of the way of what is read again)
+template <typename T, int VEC>
+__device__ __forceinline__ typename Raw<T, VEC>::type load_raw(const T* p) {
+  if constexpr (VEC == 1)
+    return *p;
+  else
+    return __ldcs(reinterpret_cast<const uint4*>(p));
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ typename Raw<T, VEC>::type zero_raw() {
+  if constexpr (VEC == 1)
+    return static_cast<T>(0.f);
+  else
+    return make_uint4(0, 0, 0, 0);
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void widen(const typename Raw<T, VEC>::type& v, float (&f)[VEC]) {
   if constexpr (VEC == 1) {
-    f[0] = static_cast<float>(*p);
-  } else if constexpr (sizeof(T) == 4) {
-    const float4 v = *reinterpret_cast<const float4*>(p);
-    f[0] = v.x;
-    f[1] = v.y;
-    f[2] = v.z;
-    f[3] = v.w;
+    f[0] = static_cast<float>(v);
   } else {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      f[2 * i] = __uint_as_float(w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      if constexpr (sizeof(T) == 4) {
+        f[i] = __uint_as_float(w[i]);
+      } else {
+        f[2 * i] = __uint_as_float(w[i] << 16);
+        f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      }
     }
   }
+}
+
+// The bits (fp32) of the largest magnitude among VEC elements: magnitudes order as their bits do, an
+// infinity or a NaN above every finite one. bf16 pairs are compared two at a time.
+template <typename T, int VEC>
+__device__ __forceinline__ uint32_t max_magnitude(const typename Raw<T, VEC>::type& v) {
+  if constexpr (VEC == 1) {
+    return __float_as_uint(static_cast<float>(v)) & 0x7FFFFFFFu;
+  } else if constexpr (sizeof(T) == 4) {
+    return max(max(v.x & 0x7FFFFFFFu, v.y & 0x7FFFFFFFu), max(v.z & 0x7FFFFFFFu, v.w & 0x7FFFFFFFu));
+  } else {
+    const uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
+    return max(m << 16, m & 0xFFFF0000u);
+  }
+}
+
+// The codes of a thread's VEC elements and the scale byte of their block, whose 32 channels lie in
+// 32 / VEC consecutive lanes. All of a warp's threads call this together. `f` holds the widened elements.
+template <typename T, int VEC>
+__device__ __forceinline__ typename MxCodes<VEC>::type mx_quantise(const typename Raw<T, VEC>::type& v,
+                                                                   const float (&f)[VEC], uint32_t& byte) {
+  constexpr uint32_t kInfinity = 0x7F800000u;
+  uint32_t m = max_magnitude<T, VEC>(v);
+#pragma unroll
+  for (int o = kMxBlock / VEC / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  float q[VEC];
+  if (__any_sync(0xFFFFFFFFu, m >= kInfinity)) {
+    // rare: somewhere in the warp's blocks a value is not finite. It becomes NaN (the conversion to e4m3
+    // would make 448 of an infinity) and the scale is that of the others.
+    m = 0;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const uint32_t a = __float_as_uint(f[j]) & 0x7FFFFFFFu;
+      m = max(m, a < kInfinity ? a : 0u);
+    }
+#pragma unroll
+    for (int o = kMxBlock / VEC / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    byte = mx_scale_byte(m);
+    const float inv = mx_inverse_scale(byte);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+      q[j] = (__float_as_uint(f[j]) & 0x7FFFFFFFu) < kInfinity ? f[j] * inv : __uint_as_float(0x7FFFFFFFu);
+  } else {
+    byte = mx_scale_byte(m);
+    const float inv = mx_inverse_scale(byte);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) q[j] = f[j] * inv;
+  }
+  return mx_encode<VEC>(q);
 }
 
 template <typename T, int VEC>
@@ -140,7 +192,7 @@ __device__ __forceinline__ void store_vec(T* p, const float (&f)[VEC]) {
   if constexpr (VEC == 1) {
     *p = static_cast<T>(f[0]);  // round to nearest even
   } else if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+    __stcs(reinterpret_cast<float4*>(p), make_float4(f[0], f[1], f[2], f[3]));
   } else {
     uint32_t w[4];
 #pragma unroll
@@ -148,7 +200,7 @@ __device__ __forceinline__ void store_vec(T* p, const float (&f)[VEC]) {
       const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
       w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
   }
 }
 

@@ -88,7 +88,7 @@ int ffb_layernorm_bwd(const void* dy, const void* x, const uint8_t* codes, const
     return fail(FFB_ERR_ARG, "layernorm_bwd: misaligned pointer");
   if (dgamma || dbeta) {
     const size_t need = ln_bwd_workspace_bytes(rows, c, dtype == FFB_F32);
-    if (!workspace || workspace_bytes < need)
+    if (need > 0 && (!workspace || workspace_bytes < need))
       return fail(FFB_ERR_ARG, "layernorm_bwd: workspace %zu < %zu bytes", workspace ? workspace_bytes : 0, need);
     if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return fail(FFB_ERR_ARG, "layernorm_bwd: misaligned workspace");
   }

@@ -521,72 +521,78 @@ class Checkpoint8(NamedTuple):
 
 
 class LayerNormSaved(NamedTuple):
-    """What a LayerNorm's backward pass reads: the input or its checkpoint, and each row's statistics."""
+    """What a LayerNorm's backward pass reads: the input or its checkpoint, and each row's mean and
+    1 / sqrt(var + eps) (``stats [2, ...]``, fp32)."""
 
     x: Tensor | Checkpoint8
-    mean: Tensor
-    rstd: Tensor
+    stats: Tensor
 
 
 def _on_device(t: Tensor, name: str, *args) -> None:
-    """Call an entry point on ``t``'s device, on that device's current stream."""
-    if t.device.index == torch.cuda.current_device():
-        _lib.call(name, *args, _stream())
+    """Call an entry point on ``t``'s device, on that device's current stream. Pointers are passed as
+    they come from ``data_ptr()`` (``None`` for an absent tensor): ``ctypes`` converts them itself."""
+    index = t.device.index
+    if index == torch.cuda.current_device():
+        _lib.call(name, *args, torch.cuda.current_stream(index).cuda_stream)
     else:
-        with torch.cuda.device(t.device):
-            _lib.call(name, *args, _stream())
+        with torch.cuda.device(index):
+            _lib.call(name, *args, torch.cuda.current_stream(index).cuda_stream)
 
 
-def _train_input(name: str, x: Tensor, *others: Tensor | None, dtypes=(torch.bfloat16, torch.float32)) -> Tensor:
-    _need_cuda(x, *others)
+def _dense(t: Tensor) -> Tensor:
+    """``t`` outside autograd, dense."""
+    if t.requires_grad:
+        t = t.detach()
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _train_input(name: str, x: Tensor, dtypes=_DTYPES) -> Tensor:
+    _need_cuda(x)
     if x.dtype not in dtypes:
         raise _lib.UnsupportedCall(name, 2, f"dtype {x.dtype} (takes {', '.join(str(d) for d in dtypes)})")
     if x.dim() == 0 or x.shape[-1] == 0:
         raise _lib.UnsupportedCall(name, 2, f"shape {tuple(x.shape)} has no channels")
-    for t in others:
-        if t is not None and t.device != x.device:
-            raise _lib.UnsupportedCall(name, 2, f"tensors on {x.device} and {t.device}")
-    return x.detach().contiguous()
+    return _dense(x)
 
 
-def _like(name: str, what: str, t: Tensor, shape, dtype: torch.dtype) -> Tensor:
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
-        raise _lib.UnsupportedCall(name, 2, f"{what} is {t.dtype} {tuple(t.shape)}, not {dtype} {tuple(shape)}")
-    return t.detach().contiguous()
+def _beside(name: str, what: str, x: Tensor, t: Tensor, shape, dtype: torch.dtype) -> Tensor:
+    """``t``, which has to lie on ``x``'s device with this shape and dtype, dense."""
+    if t.shape != shape or t.dtype != dtype or t.device != x.device:
+        raise _lib.UnsupportedCall(name, 2, f"{what} is {t.dtype} {tuple(t.shape)} on {t.device}, not {dtype} "
+                                            f"{tuple(shape)} on {x.device}")
+    return _dense(t)
 
 
-def _vector(name: str, what: str, t: Tensor | None, c: int) -> Tensor | None:
+def _vector(name: str, what: str, x: Tensor, t: Tensor | None) -> Tensor | None:
+    """A norm's weight or bias beside ``x [..., c]``, in fp32."""
     if t is None:
         return None
-    if tuple(t.shape) != (c,):
-        raise _lib.UnsupportedCall(name, 2, f"{what} {tuple(t.shape)} is not [{c}]")
-    return _f32(t)
+    if t.shape != x.shape[-1:] or t.device != x.device or not t.is_floating_point():
+        raise _lib.UnsupportedCall(name, 2, f"{what} is {t.dtype} {tuple(t.shape)} on {t.device}, beside "
+                                            f"{tuple(x.shape)} on {x.device}")
+    return t if t.dtype == torch.float32 and t.is_contiguous() else _f32(t)
+
+
+def _at(t: Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
 
 
 def _new_checkpoint(x: Tensor) -> Checkpoint8:
-    c = x.shape[-1]
-    codes = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    scales = torch.empty((*x.shape[:-1], -(-c // MX_BLOCK)), dtype=torch.uint8, device=x.device)
+    codes = torch.empty_like(x, dtype=torch.float8_e4m3fn)
+    scales = torch.empty((*x.shape[:-1], -(-x.shape[-1] // MX_BLOCK)), dtype=torch.uint8, device=x.device)
     return Checkpoint8(codes, scales, x.dtype)
 
 
-def _kept(name: str, kept: Tensor | Checkpoint8, shape, dtype: torch.dtype):
-    """``(x, codes, scales)`` of a kept activation, the absent ones ``None``, checked against the shape
-    and dtype it has to have."""
+def _kept(name: str, x: Tensor, kept: Tensor | Checkpoint8, shape, dtype: torch.dtype):
+    """``(tensor, codes, scales)`` of a kept activation, the absent ones ``None``: checked against the
+    shape and dtype it has to have beside ``x``."""
     if not isinstance(kept, Checkpoint8):
-        return _like(name, "the kept activation", kept, shape, dtype), None, None
+        return _beside(name, "the kept activation", x, kept, shape, dtype), None, None
     if kept.dtype != dtype:
         raise _lib.UnsupportedCall(name, 2, f"the checkpoint is of a {kept.dtype} activation, not {dtype}")
-    codes = _like(name, "codes", kept.codes, shape, torch.float8_e4m3fn)
-    scales = _like(name, "scales", kept.scales, (*shape[:-1], -(-shape[-1] // MX_BLOCK)), torch.uint8)
-    return None, codes, scales
-
-
-def _devices(name: str, x: Tensor, kept: Tensor | Checkpoint8) -> None:
-    tensors = (kept.codes, kept.scales) if isinstance(kept, Checkpoint8) else (kept,)
-    for t in tensors:
-        if t.device != x.device:
-            raise _lib.UnsupportedCall(name, 2, f"tensors on {x.device} and {t.device}")
+    codes = _beside(name, "codes", x, kept.codes, shape, torch.float8_e4m3fn)
+    blocks = (*shape[:-1], -(-shape[-1] // MX_BLOCK))
+    return None, codes, _beside(name, "scales", x, kept.scales, blocks, torch.uint8)
 
 
 def checkpoint_pack(x: Tensor) -> Checkpoint8:
@@ -594,21 +600,21 @@ def checkpoint_pack(x: Tensor) -> Checkpoint8:
     x = _train_input("checkpoint_pack", x)
     kept = _new_checkpoint(x)
     c = x.shape[-1]
-    _on_device(x, "ffb_checkpoint_pack", _ptr(x), _ptr(kept.codes), _ptr(kept.scales), x.numel() // c, c,
+    _on_device(x, "ffb_checkpoint_pack", x.data_ptr(), kept.codes.data_ptr(), kept.scales.data_ptr(), x.numel() // c, c,
                _DTYPES[x.dtype])
     return kept
 
 
 def checkpoint_unpack(kept: Checkpoint8) -> Tensor:
     """The activation a checkpoint stands for, in the dtype it had."""
-    codes = kept.codes
-    _train_input("checkpoint_unpack", codes, kept.scales, dtypes=(torch.float8_e4m3fn,))
+    name = "checkpoint_unpack"
+    codes = _train_input(name, kept.codes, dtypes=(torch.float8_e4m3fn,))
     if kept.dtype not in _DTYPES:
-        raise _lib.UnsupportedCall("checkpoint_unpack", 2, f"dtype {kept.dtype}")
-    _, codes, scales = _kept("checkpoint_unpack", kept, codes.shape, kept.dtype)
-    x = torch.empty(codes.shape, dtype=kept.dtype, device=codes.device)
+        raise _lib.UnsupportedCall(name, 2, f"dtype {kept.dtype}")
+    _, codes, scales = _kept(name, codes, kept, codes.shape, kept.dtype)
+    x = torch.empty_like(codes, dtype=kept.dtype)
     c = codes.shape[-1]
-    _on_device(codes, "ffb_checkpoint_unpack", _ptr(codes), _ptr(scales), _ptr(x), codes.numel() // c, c,
+    _on_device(codes, "ffb_checkpoint_unpack", codes.data_ptr(), scales.data_ptr(), x.data_ptr(), codes.numel() // c, c,
                _DTYPES[kept.dtype])
     return x
 
@@ -616,18 +622,20 @@ def checkpoint_unpack(kept: Checkpoint8) -> Tensor:
 def layer_norm_train(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float = 1e-5, *,
                      checkpoint: bool = False) -> tuple[Tensor, LayerNormSaved]:
     """LayerNorm over the last axis (at most 8192 channels) and what its backward pass reads: the input
-    itself, or with ``checkpoint`` its 8-bit checkpoint (the input need not be kept then)."""
-    x = _train_input("layer_norm_train", x, weight, bias)
+    itself (which may not change until then), or with ``checkpoint`` its 8-bit checkpoint."""
+    name = "layer_norm_train"
+    x = _train_input(name, x)
+    w, b = _vector(name, "weight", x, weight), _vector(name, "bias", x, bias)
     c = x.shape[-1]
-    w, b = _vector("layer_norm_train", "weight", weight, c), _vector("layer_norm_train", "bias", bias, c)
+    rows = x.numel() // c
     y = torch.empty_like(x)
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    rstd = torch.empty_like(mean)
+    stats = torch.empty((2, *x.shape[:-1]), dtype=torch.float32, device=x.device)
+    mean = stats.data_ptr()
     kept = _new_checkpoint(x) if checkpoint else None
-    codes, scales = (kept.codes, kept.scales) if checkpoint else (None, None)
-    _on_device(x, "ffb_layernorm_train_fwd", _ptr(x), _ptr(y), _ptr(w), _ptr(b), _ptr(mean), _ptr(rstd), _ptr(codes),
-               _ptr(scales), x.numel() // c, c, ctypes.c_float(eps), _DTYPES[x.dtype])
-    return y, LayerNormSaved(kept if checkpoint else x, mean, rstd)
+    codes, scales = (kept.codes.data_ptr(), kept.scales.data_ptr()) if checkpoint else (None, None)
+    _on_device(x, "ffb_layernorm_train_fwd", x.data_ptr(), y.data_ptr(), _at(w), _at(b), mean, mean + 4 * rows, codes,
+               scales, rows, c, eps, _DTYPES[x.dtype])
+    return y, LayerNormSaved(kept if checkpoint else x, stats)
 
 
 def layer_norm_backward(dy: Tensor, saved: LayerNormSaved, weight: Tensor | None, *, bias: bool = True,
@@ -636,23 +644,23 @@ def layer_norm_backward(dy: Tensor, saved: LayerNormSaved, weight: Tensor | None
     reaches x around the norm) in ``dy``'s dtype, the others fp32, reduced over the rows in a fixed order
     (``None`` without ``weight`` / ``bias``)."""
     name = "layer_norm_backward"
-    dy = _train_input(name, dy, weight, residual, saved.mean, saved.rstd)
-    _devices(name, dy, saved.x)
+    dy = _train_input(name, dy)
     c = dy.shape[-1]
     rows = dy.numel() // c
-    x, codes, scales = _kept(name, saved.x, dy.shape, dy.dtype)
-    mean = _like(name, "mean", saved.mean, dy.shape[:-1], torch.float32)
-    rstd = _like(name, "rstd", saved.rstd, dy.shape[:-1], torch.float32)
-    w = _vector(name, "weight", weight, c)
+    x, codes, scales = _kept(name, dy, saved.x, dy.shape, dy.dtype)
+    stats = _beside(name, "stats", dy, saved.stats, (2, *dy.shape[:-1]), torch.float32)
+    w = _vector(name, "weight", dy, weight)
     if residual is not None:
-        residual = _like(name, "residual", residual, dy.shape, dy.dtype)
+        residual = _beside(name, "residual", dy, residual, dy.shape, dy.dtype)
     dx = torch.empty_like(dy)
-    dweight = None if w is None else torch.empty(c, dtype=torch.float32, device=dy.device)
+    dweight = None if w is None else torch.empty_like(w)
     dbias = torch.empty(c, dtype=torch.float32, device=dy.device) if bias else None
-    ws = _workspace(_lib.load().ffb_layernorm_bwd_workspace_bytes(rows, c, _DTYPES[dy.dtype]), dy.device)
-    _on_device(dy, "ffb_layernorm_bwd", _ptr(dy), _ptr(x), _ptr(codes), _ptr(scales), _ptr(mean), _ptr(rstd), _ptr(w),
-               _ptr(residual), _ptr(dx), _ptr(dweight), _ptr(dbias), _ptr(ws), ctypes.c_size_t(ws.numel()), rows, c,
-               _DTYPES[dy.dtype])
+    dtype = _DTYPES[dy.dtype]
+    size = _lib.load().ffb_layernorm_bwd_workspace_bytes(rows, c, dtype)
+    ws = torch.empty(size, dtype=torch.uint8, device=dy.device) if size else None
+    mean = stats.data_ptr()
+    _on_device(dy, "ffb_layernorm_bwd", dy.data_ptr(), _at(x), _at(codes), _at(scales), mean, mean + 4 * rows, _at(w),
+               _at(residual), dx.data_ptr(), _at(dweight), _at(dbias), _at(ws), size, rows, c, dtype)
     return dx, dweight, dbias
 
 
@@ -661,23 +669,23 @@ def weight_grad(dy: Tensor, x: Tensor | Checkpoint8) -> Tensor:
     bf16, ``x [..., k]`` bf16 or its checkpoint."""
     name = "weight_grad"
     dy = _train_input(name, dy, dtypes=(torch.bfloat16,))
-    _devices(name, dy, x)
     shape = x.codes.shape if isinstance(x, Checkpoint8) else x.shape
-    if tuple(shape[:-1]) != tuple(dy.shape[:-1]) or len(shape) == 0 or shape[-1] == 0:
+    if len(shape) == 0 or shape[-1] == 0 or shape[:-1] != dy.shape[:-1]:
         raise _lib.UnsupportedCall(name, 2, f"rows of dy {tuple(dy.shape)} and x {tuple(shape)}")
     n, k = dy.shape[-1], shape[-1]
     rows = dy.numel() // n
-    x, codes, scales = _kept(name, x, shape, torch.bfloat16)
+    x, codes, scales = _kept(name, dy, x, shape, torch.bfloat16)
     dw = torch.empty((n, k), dtype=torch.float32, device=dy.device)
-    ws = _workspace(_lib.load().ffb_weight_grad_workspace_bytes(rows, n, k), dy.device)
-    _on_device(dy, "ffb_weight_grad", _ptr(dy), _ptr(x), _ptr(codes), _ptr(scales), _ptr(dw), _ptr(ws),
-               ctypes.c_size_t(ws.numel()), rows, n, k)
+    size = _lib.load().ffb_weight_grad_workspace_bytes(rows, n, k)
+    ws = torch.empty(size, dtype=torch.uint8, device=dy.device) if size else None
+    _on_device(dy, "ffb_weight_grad", dy.data_ptr(), _at(x), _at(codes), _at(scales), dw.data_ptr(), _at(ws), size, rows,
+               n, k)
     return dw
 
 
 def swiglu_train(ab: Tensor, *, checkpoint: bool = False) -> tuple[Tensor, Tensor | Checkpoint8]:
     """``silu(a) b [..., h]`` of ``ab [..., 2 h] = [a | b]`` (bf16 or fp32) and what its backward pass
-    reads: ``ab`` itself, or with ``checkpoint`` its 8-bit checkpoint."""
+    reads: ``ab`` itself (which may not change until then), or with ``checkpoint`` its 8-bit checkpoint."""
     name = "swiglu_train"
     ab = _train_input(name, ab)
     if ab.shape[-1] % 2:
@@ -685,8 +693,8 @@ def swiglu_train(ab: Tensor, *, checkpoint: bool = False) -> tuple[Tensor, Tenso
     h = ab.shape[-1] // 2
     out = torch.empty((*ab.shape[:-1], h), dtype=ab.dtype, device=ab.device)
     kept = _new_checkpoint(ab) if checkpoint else None
-    codes, scales = (kept.codes, kept.scales) if checkpoint else (None, None)
-    _on_device(ab, "ffb_swiglu_train_fwd", _ptr(ab), _ptr(out), _ptr(codes), _ptr(scales), out.numel() // h, h,
+    codes, scales = (kept.codes.data_ptr(), kept.scales.data_ptr()) if checkpoint else (None, None)
+    _on_device(ab, "ffb_swiglu_train_fwd", ab.data_ptr(), out.data_ptr(), codes, scales, out.numel() // h, h,
                _DTYPES[ab.dtype])
     return out, kept if checkpoint else ab
 
@@ -696,11 +704,10 @@ def swiglu_backward(dh: Tensor, saved: Tensor | Checkpoint8, *, output: bool = F
     again, as the squeeze's weight gradient needs it: ``(dab, h)``."""
     name = "swiglu_backward"
     dh = _train_input(name, dh)
-    _devices(name, dh, saved)
     h = dh.shape[-1]
-    ab, codes, scales = _kept(name, saved, (*dh.shape[:-1], 2 * h), dh.dtype)
+    ab, codes, scales = _kept(name, dh, saved, (*dh.shape[:-1], 2 * h), dh.dtype)
     dab = torch.empty((*dh.shape[:-1], 2 * h), dtype=dh.dtype, device=dh.device)
     out = torch.empty_like(dh) if output else None
-    _on_device(dh, "ffb_swiglu_bwd", _ptr(dh), _ptr(ab), _ptr(codes), _ptr(scales), _ptr(dab), _ptr(out),
+    _on_device(dh, "ffb_swiglu_bwd", dh.data_ptr(), _at(ab), _at(codes), _at(scales), dab.data_ptr(), _at(out),
                dh.numel() // h, h, _DTYPES[dh.dtype])
     return (dab, out) if output else dab

@@ -16,7 +16,7 @@ F32, BF16 = 1, 0
 def test_cpu_tensors_are_refused():
     x = torch.randn(4, 64)
     w = torch.ones(64)
-    saved = kernels.LayerNormSaved(x, torch.zeros(4), torch.ones(4))
+    saved = kernels.LayerNormSaved(x, torch.ones(2, 4))
     for call in (lambda: kernels.layer_norm_train(x, w, w), lambda: kernels.layer_norm_backward(x, saved, w),
                  lambda: kernels.checkpoint_pack(x), lambda: kernels.weight_grad(x.bfloat16(), x.bfloat16()),
                  lambda: kernels.swiglu_train(x), lambda: kernels.swiglu_backward(x, torch.randn(4, 128)),
@@ -35,7 +35,7 @@ def on_gpu(monkeypatch):
 
 def test_dtypes_and_shapes_are_refused(on_gpu):
     x, w = torch.randn(4, 64), torch.ones(64)
-    saved = kernels.LayerNormSaved(x, torch.zeros(4), torch.ones(4))
+    saved = kernels.LayerNormSaved(x, torch.ones(2, 4))
     kept = kernels.Checkpoint8(x.to(torch.float8_e4m3fn), torch.zeros(4, 2, dtype=torch.uint8), torch.float32)
     bad = [
         lambda: kernels.layer_norm_train(x.half(), w, w),
@@ -45,8 +45,8 @@ def test_dtypes_and_shapes_are_refused(on_gpu):
         lambda: kernels.layer_norm_train(torch.empty(4, 0), None, None),
         lambda: kernels.layer_norm_backward(x[:3], saved, w),
         lambda: kernels.layer_norm_backward(x.bfloat16(), saved, w),
-        lambda: kernels.layer_norm_backward(x, saved._replace(mean=torch.zeros(4, 1)), w),
-        lambda: kernels.layer_norm_backward(x, saved._replace(rstd=torch.ones(4).double()), w),
+        lambda: kernels.layer_norm_backward(x, saved._replace(stats=torch.zeros(2, 4, 1)), w),
+        lambda: kernels.layer_norm_backward(x, saved._replace(stats=torch.ones(2, 4).double()), w),
         lambda: kernels.layer_norm_backward(x, saved, w, residual=x[:, :32]),
         lambda: kernels.layer_norm_backward(x, saved._replace(x=kept._replace(scales=kept.scales[:, :1])), w),
         lambda: kernels.layer_norm_backward(x, saved._replace(x=kept._replace(dtype=torch.bfloat16)), w),
