@@ -124,7 +124,7 @@ SIGNATURES: dict[str, list] = {
     "ffb_layernorm_bwd": [c_void_p] * 12 + [ctypes.c_size_t, c_i64, c_int, c_int, c_void_p],
     "ffb_checkpoint_pack": [c_void_p] * 3 + [c_i64, c_int, c_int, c_void_p],
     "ffb_checkpoint_unpack": [c_void_p] * 3 + [c_i64, c_int, c_int, c_void_p],
-    "ffb_weight_grad_workspace_bytes": [c_i64, c_int, c_int],
+    "ffb_weight_grad_workspace_bytes": [c_i64, c_int, c_int, c_int],
     "ffb_weight_grad": [c_void_p] * 6 + [ctypes.c_size_t, c_i64, c_int, c_int, c_void_p],
     "ffb_swiglu_train_fwd": [c_void_p] * 4 + [c_i64, c_int, c_int, c_void_p],
     "ffb_swiglu_bwd": [c_void_p] * 6 + [c_i64, c_int, c_int, c_void_p],

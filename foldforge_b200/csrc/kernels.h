@@ -193,7 +193,7 @@ int launch_swiglu_train(const void* ab, void* out, uint8_t* codes, uint8_t* scal
                         cudaStream_t stream);
 int launch_swiglu_bwd(const void* dh, const void* ab, const uint8_t* codes, const uint8_t* scales, void* dab, void* out,
                       int64_t rows, int h, int is_f32, cudaStream_t stream);
-size_t weight_grad_workspace_bytes(int64_t rows, int n, int k);
+size_t weight_grad_workspace_bytes(int64_t rows, int n, int k, bool codes);
 int weight_grad_forward(const void* dy, const void* x, const uint8_t* codes, const uint8_t* scales, float* dw,
                         void* workspace, int64_t rows, int n, int k, const DeviceInfo& info, cudaStream_t stream);
 

@@ -22,6 +22,7 @@ int element_size(int dtype) { return dtype == FFB_F32 ? 4 : 2; }
 bool off_element(const void* p, int dtype) {
   return (reinterpret_cast<uintptr_t>(p) & static_cast<uintptr_t>(element_size(dtype) - 1)) != 0;
 }
+bool off_vector(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
 bool off_word(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) != 0; }
 
 // a bf16 / fp32 tensor or its checkpoint: exactly one of the two
@@ -125,8 +126,8 @@ int ffb_checkpoint_unpack(const uint8_t* codes, const uint8_t* scales, void* x, 
                      "checkpoint_unpack launch");
 }
 
-size_t ffb_weight_grad_workspace_bytes(int64_t rows, int n, int k) {
-  return (rows <= 0 || n <= 0 || k <= 0) ? 0 : weight_grad_workspace_bytes(rows, n, k);
+size_t ffb_weight_grad_workspace_bytes(int64_t rows, int n, int k, int checkpoint) {
+  return (rows <= 0 || n <= 0 || k <= 0) ? 0 : weight_grad_workspace_bytes(rows, n, k, checkpoint != 0);
 }
 
 int ffb_weight_grad(const void* dy, const void* x, const uint8_t* codes, const uint8_t* scales, float* dw,
@@ -148,11 +149,11 @@ int ffb_weight_grad(const void* dy, const void* x, const uint8_t* codes, const u
   st = check_kept("weight_grad", x, codes, scales);
   if (st != FFB_OK) return st;
   if (!dy) return fail(FFB_ERR_ARG, "weight_grad: null pointer");
-  if (off_element(dy, FFB_BF16) || off_element(x, FFB_BF16)) return fail(FFB_ERR_ARG, "weight_grad: misaligned pointer");
-  const size_t need = weight_grad_workspace_bytes(rows, n, k);
+  if (off_vector(dy) || off_vector(x) || off_vector(codes)) return fail(FFB_ERR_ARG, "weight_grad: misaligned pointer");
+  const size_t need = weight_grad_workspace_bytes(rows, n, k, codes != nullptr);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(FFB_ERR_ARG, "weight_grad: workspace %zu < %zu bytes", workspace ? workspace_bytes : 0, need);
-  if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return fail(FFB_ERR_ARG, "weight_grad: misaligned workspace");
+  if (off_vector(workspace)) return fail(FFB_ERR_ARG, "weight_grad: misaligned workspace");
   st = device_info(&info);
   if (st != FFB_OK) return st;
   return weight_grad_forward(dy, x, codes, scales, dw, workspace, rows, n, k, info, as_stream(stream));

@@ -573,6 +573,11 @@ def _vector(name: str, what: str, x: Tensor, t: Tensor | None) -> Tensor | None:
     return t if t.dtype == torch.float32 and t.is_contiguous() else _f32(t)
 
 
+def _aligned(t: Tensor | None) -> Tensor | None:
+    """``t`` from a 16-byte boundary on (a copy of a view that is not)."""
+    return t if t is None or t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _at(t: Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
@@ -675,8 +680,9 @@ def weight_grad(dy: Tensor, x: Tensor | Checkpoint8) -> Tensor:
     n, k = dy.shape[-1], shape[-1]
     rows = dy.numel() // n
     x, codes, scales = _kept(name, dy, x, shape, torch.bfloat16)
+    dy, x, codes = _aligned(dy), _aligned(x), _aligned(codes)
     dw = torch.empty((n, k), dtype=torch.float32, device=dy.device)
-    size = _lib.load().ffb_weight_grad_workspace_bytes(rows, n, k)
+    size = _lib.load().ffb_weight_grad_workspace_bytes(rows, n, k, codes is not None)
     ws = torch.empty(size, dtype=torch.uint8, device=dy.device) if size else None
     _on_device(dy, "ffb_weight_grad", dy.data_ptr(), _at(x), _at(codes), _at(scales), dw.data_ptr(), _at(ws), size, rows,
                n, k)

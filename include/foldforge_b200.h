@@ -363,7 +363,7 @@ int ffb_dit_fwd(const void* x, const uint8_t* mask, const void* packed, const vo
  *   dgamma = sum_rows dy xh, dbeta = sum_rows dy (each NULL where not wanted). c <= 8192.
  * ffb_checkpoint_pack / _unpack: a checkpoint written from x, and read back.
  * ffb_weight_grad: dw [n, k] fp32 = dy^T x over the rows: dy [rows, n] bf16, x [rows, k] bf16 or its
- *   checkpoint.
+ *   checkpoint (`checkpoint` of the workspace's size); dy, x and codes 16-byte aligned.
  * ffb_swiglu_train_fwd: out [rows, h] = silu(a) b of ab [rows, 2 h] = [a | b]; codes / scales (both or
  *   neither) receive ab's checkpoint.
  * ffb_swiglu_bwd: dab [rows, 2 h] from dh [rows, h] and ab or its checkpoint: da = dh b s (1 + a (1 - s)),
@@ -379,7 +379,7 @@ int ffb_layernorm_bwd(const void* dy, const void* x, const uint8_t* codes, const
 int ffb_checkpoint_pack(const void* x, uint8_t* codes, uint8_t* scales, int64_t rows, int c, int dtype, void* stream);
 int ffb_checkpoint_unpack(const uint8_t* codes, const uint8_t* scales, void* x, int64_t rows, int c, int dtype,
                           void* stream);
-size_t ffb_weight_grad_workspace_bytes(int64_t rows, int n, int k);
+size_t ffb_weight_grad_workspace_bytes(int64_t rows, int n, int k, int checkpoint);
 int ffb_weight_grad(const void* dy, const void* x, const uint8_t* codes, const uint8_t* scales, float* dw,
                     void* workspace, size_t workspace_bytes, int64_t rows, int n, int k, void* stream);
 int ffb_swiglu_train_fwd(const void* ab, void* out, uint8_t* codes, uint8_t* scales, int64_t rows, int h, int dtype,

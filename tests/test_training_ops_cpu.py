@@ -106,7 +106,7 @@ def test_entry_points_check_their_arguments():
     assert lib.ffb_checkpoint_unpack(z, q, p, 4, 8, BF16, z) == 1
     assert lib.ffb_checkpoint_unpack(p, q, odd, 4, 8, F32, z) == 1
     wg = lib.ffb_weight_grad
-    need = lib.ffb_weight_grad_workspace_bytes(100000, 64, 64)
+    need = lib.ffb_weight_grad_workspace_bytes(100000, 64, 64, 0)
     assert need > 0
     assert wg(p, q, z, z, r, z, size(0), 100000, 64, 64, z) == 1
     assert wg(p, q, z, z, r, p, size(need - 1), 100000, 64, 64, z) == 1
@@ -114,6 +114,11 @@ def test_entry_points_check_their_arguments():
     assert wg(p, q, z, z, r, p, size(need), 1 << 31, 64, 64, z) == 2
     assert wg(p, q, r, z, r, p, size(need), 100000, 64, 64, z) == 1
     assert wg(p, q, z, z, z, p, size(need), 100000, 64, 64, z) == 1
+    assert wg(ctypes.c_void_p(0x10002), q, z, z, r, p, size(need), 100000, 64, 64, z) == 1
+    # rows that are padded into the workspace
+    padded = lib.ffb_weight_grad_workspace_bytes(100000, 65, 64, 0)
+    assert padded > 100000 * 72 * 2 and lib.ffb_weight_grad_workspace_bytes(100000, 64, 72, 1) > 100000 * 72 * 2
+    assert wg(p, q, z, z, r, p, size(padded - 1), 100000, 65, 64, z) == 1
     assert lib.ffb_swiglu_train_fwd(p, p, z, z, 4, 8, BF16, z) == 1
     assert lib.ffb_swiglu_train_fwd(p, q, z, r, 4, 8, BF16, z) == 1
     assert lib.ffb_swiglu_bwd(p, q, z, z, q, z, 4, 8, BF16, z) == 1
