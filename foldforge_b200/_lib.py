@@ -210,7 +210,7 @@ def _stage_launches(name: str, args) -> int:
 def call(name: str, *args) -> None:
     """Call an entry point; raise on a non-OK status."""
     global launch_count
-    lib = load()
+    lib = load() if _lib is None else _lib
     status = getattr(lib, name)(*args)
     if status == 0:
         if name in ("ffb_trimul_fwd_stages", "ffb_triattn_fwd_stages"):

@@ -13,6 +13,19 @@ from foldforge_b200 import _lib, kernels
 F32, BF16 = 1, 0
 
 
+def checkpoint(rows: int, c: int, dtype: torch.dtype) -> kernels.Checkpoint8:
+    size = -(-rows * c // 16) * 16 + rows * -(-c // 32)
+    return kernels.Checkpoint8(torch.zeros(size, dtype=torch.uint8), torch.Size((rows, c)), dtype)
+
+
+def test_checkpoint_parts():
+    kept = checkpoint(3, 65, torch.bfloat16)
+    assert kept.codes.shape == (3, 65) and kept.codes.dtype == torch.float8_e4m3fn
+    assert kept.scales.shape == (3, 3) and kept.scales.dtype == torch.uint8
+    assert (kept.scales.data_ptr() - kept.codes.data_ptr()) == 208  # 195 codes, to the next 16 bytes
+    assert kept.data.numel() == 208 + 9
+
+
 def test_cpu_tensors_are_refused():
     x = torch.randn(4, 64)
     w = torch.ones(64)
@@ -20,9 +33,7 @@ def test_cpu_tensors_are_refused():
     for call in (lambda: kernels.layer_norm_train(x, w, w), lambda: kernels.layer_norm_backward(x, saved, w),
                  lambda: kernels.checkpoint_pack(x), lambda: kernels.weight_grad(x.bfloat16(), x.bfloat16()),
                  lambda: kernels.swiglu_train(x), lambda: kernels.swiglu_backward(x, torch.randn(4, 128)),
-                 lambda: kernels.checkpoint_unpack(kernels.Checkpoint8(x.to(torch.float8_e4m3fn),
-                                                                       torch.zeros(4, 2, dtype=torch.uint8),
-                                                                       torch.float32))):
+                 lambda: kernels.checkpoint_unpack(checkpoint(4, 64, torch.float32))):
         with pytest.raises(_lib.UnsupportedCall, match="CUDA device"):
             call()
 
@@ -36,7 +47,7 @@ def on_gpu(monkeypatch):
 def test_dtypes_and_shapes_are_refused(on_gpu):
     x, w = torch.randn(4, 64), torch.ones(64)
     saved = kernels.LayerNormSaved(x, torch.ones(2, 4))
-    kept = kernels.Checkpoint8(x.to(torch.float8_e4m3fn), torch.zeros(4, 2, dtype=torch.uint8), torch.float32)
+    kept = checkpoint(4, 64, torch.float32)
     bad = [
         lambda: kernels.layer_norm_train(x.half(), w, w),
         lambda: kernels.layer_norm_train(x, w[:63], w),
@@ -45,15 +56,18 @@ def test_dtypes_and_shapes_are_refused(on_gpu):
         lambda: kernels.layer_norm_train(torch.empty(4, 0), None, None),
         lambda: kernels.layer_norm_backward(x[:3], saved, w),
         lambda: kernels.layer_norm_backward(x.bfloat16(), saved, w),
-        lambda: kernels.layer_norm_backward(x, saved._replace(stats=torch.zeros(2, 4, 1)), w),
+        lambda: kernels.layer_norm_backward(x, saved._replace(stats=torch.zeros(2, 5)), w),
         lambda: kernels.layer_norm_backward(x, saved._replace(stats=torch.ones(2, 4).double()), w),
         lambda: kernels.layer_norm_backward(x, saved, w, residual=x[:, :32]),
-        lambda: kernels.layer_norm_backward(x, saved._replace(x=kept._replace(scales=kept.scales[:, :1])), w),
+        lambda: kernels.layer_norm_backward(x, saved._replace(x=kept._replace(data=kept.data[:-1])), w),
         lambda: kernels.layer_norm_backward(x, saved._replace(x=kept._replace(dtype=torch.bfloat16)), w),
         lambda: kernels.checkpoint_pack(x.to(torch.int32)),
-        lambda: kernels.checkpoint_unpack(kept._replace(scales=kept.scales[:2])),
+        lambda: kernels.checkpoint_unpack(kept._replace(data=kept.data[:200])),
         lambda: kernels.checkpoint_unpack(kept._replace(dtype=torch.float16)),
-        lambda: kernels.checkpoint_unpack(kept._replace(codes=x)),
+        lambda: kernels.checkpoint_unpack(kept._replace(data=kept.data.view(torch.int8))),
+        lambda: kernels.checkpoint_unpack(kept._replace(shape=torch.Size((4, 32)))),
+        lambda: kernels.checkpoint_unpack(kept._replace(shape=torch.Size(()))),
+        lambda: kernels.weight_grad(x.bfloat16(), checkpoint(5, 64, torch.bfloat16)),
         lambda: kernels.weight_grad(x, x),
         lambda: kernels.weight_grad(x.bfloat16(), x),
         lambda: kernels.weight_grad(x.bfloat16(), x[:3].bfloat16()),
