@@ -183,8 +183,8 @@ struct LayerNormBwd {
   int c;
 };
 size_t ln_bwd_workspace_bytes(int64_t rows, int c, int is_f32);
-int launch_ln_train(const LayerNormTrain& p, int is_f32, cudaStream_t stream);
-int launch_ln_bwd(const LayerNormBwd& p, int is_f32, cudaStream_t stream);
+int launch_ln_train(const LayerNormTrain& p, int is_f32, int* err, cudaStream_t stream);
+int launch_ln_bwd(const LayerNormBwd& p, int is_f32, int* err, cudaStream_t stream);
 int launch_checkpoint_pack(const void* x, uint8_t* codes, uint8_t* scales, int64_t rows, int c, int is_f32,
                            cudaStream_t stream);
 int launch_checkpoint_unpack(const uint8_t* codes, const uint8_t* scales, void* x, int64_t rows, int c, int is_f32,

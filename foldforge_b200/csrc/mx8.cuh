@@ -12,6 +12,9 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
+#include <string.h>
+
+#include "common.cuh"
 
 namespace ffb {
 
@@ -44,6 +47,123 @@ __device__ __forceinline__ float2 e4m3x2_value(uint32_t pair) {
 }
 
 // ------------------------------------------------------------------ vectors of VEC elements
+// VEC fp32 values of a thread, in pairs on the paired fp32 pipe (or a single one)
+template <int VEC>
+struct Lanes {
+  uint64_t p[VEC / 2];
+  __device__ __forceinline__ Lanes() {}
+  __device__ __forceinline__ explicit Lanes(float x) {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) p[i] = f32x2(x, x);
+  }
+  template <typename F>
+  __device__ __forceinline__ Lanes each(F&& f) const {
+    Lanes r;
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) {
+      float a, b;
+      f32x2_split(p[i], a, b);
+      a = f(a);
+      b = f(b);
+      r.p[i] = f32x2(a, b);
+    }
+    return r;
+  }
+  // f(this value, the other's)
+  template <typename F>
+  __device__ __forceinline__ Lanes apply(const Lanes& o, F&& f) const {
+    Lanes r;
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) {
+      float a, b, c, d;
+      f32x2_split(p[i], a, b);
+      f32x2_split(o.p[i], c, d);
+      c = f(a, c);
+      d = f(b, d);
+      r.p[i] = f32x2(c, d);
+    }
+    return r;
+  }
+  __device__ __forceinline__ float sum() const {
+    uint64_t t = p[0];
+#pragma unroll
+    for (int i = 1; i < VEC / 2; ++i) t = add_f32x2(t, p[i]);
+    float a, b;
+    f32x2_split(t, a, b);
+    return a + b;
+  }
+  __device__ __forceinline__ float get(int j) const {
+    float a, b;
+    f32x2_split(p[j / 2], a, b);
+    return j & 1 ? b : a;
+  }
+};
+template <>
+struct Lanes<1> {
+  float f;
+  __device__ __forceinline__ Lanes() {}
+  __device__ __forceinline__ explicit Lanes(float x) : f(x) {}
+  template <typename F>
+  __device__ __forceinline__ Lanes each(F&& g) const {
+    return Lanes(g(f));
+  }
+  template <typename F>
+  __device__ __forceinline__ Lanes apply(const Lanes& o, F&& g) const {
+    return Lanes(g(f, o.f));
+  }
+  __device__ __forceinline__ float sum() const { return f; }
+  __device__ __forceinline__ float get(int) const { return f; }
+};
+template <int VEC>
+__device__ __forceinline__ Lanes<VEC> operator+(const Lanes<VEC>& a, const Lanes<VEC>& b) {
+  Lanes<VEC> r;
+  if constexpr (VEC == 1) {
+    r.f = a.f + b.f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) r.p[i] = add_f32x2(a.p[i], b.p[i]);
+  }
+  return r;
+}
+template <int VEC>
+__device__ __forceinline__ Lanes<VEC> operator*(const Lanes<VEC>& a, const Lanes<VEC>& b) {
+  Lanes<VEC> r;
+  if constexpr (VEC == 1) {
+    r.f = a.f * b.f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) r.p[i] = mul_f32x2(a.p[i], b.p[i]);
+  }
+  return r;
+}
+template <int VEC>
+__device__ __forceinline__ Lanes<VEC> fma(const Lanes<VEC>& a, const Lanes<VEC>& b, const Lanes<VEC>& c) {
+  Lanes<VEC> r;
+  if constexpr (VEC == 1) {
+    r.f = fmaf(a.f, b.f, c.f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) r.p[i] = fma_f32x2(a.p[i], b.p[i], c.p[i]);
+  }
+  return r;
+}
+// VEC values of a weight vector (16-byte aligned where VEC > 1)
+template <int VEC>
+__device__ __forceinline__ Lanes<VEC> load_weight(const float* p) {
+  Lanes<VEC> r;
+  if constexpr (VEC == 1) {
+    r.f = __ldg(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i) {
+      const float4 v = __ldg(reinterpret_cast<const float4*>(p) + i);
+      r.p[2 * i] = f32x2(v.x, v.y);
+      r.p[2 * i + 1] = f32x2(v.z, v.w);
+    }
+  }
+  return r;
+}
+
 template <int VEC>
 struct MxCodes;  // VEC code bytes as one machine word
 template <>
@@ -54,42 +174,41 @@ template <>
 struct MxCodes<1> { using type = uint8_t; };
 
 template <int VEC>
-__device__ __forceinline__ typename MxCodes<VEC>::type mx_encode(const float (&f)[VEC]) {
+__device__ __forceinline__ typename MxCodes<VEC>::type mx_encode(const Lanes<VEC>& v) {
+  typename MxCodes<VEC>::type out;
   if constexpr (VEC == 1) {
-    return static_cast<uint8_t>(e4m3x2(f[0], 0.f));
+    out = static_cast<uint8_t>(e4m3x2(v.f, 0.f));
   } else {
     uint32_t w[VEC / 4];
 #pragma unroll
-    for (int i = 0; i < VEC / 4; ++i)
-      w[i] = e4m3x2(f[4 * i], f[4 * i + 1]) | (e4m3x2(f[4 * i + 2], f[4 * i + 3]) << 16);
-    if constexpr (VEC == 8)
-      return make_uint2(w[0], w[1]);
-    else
-      return w[0];
+    for (int i = 0; i < VEC / 4; ++i) {
+      float a, b, c, d;
+      f32x2_split(v.p[2 * i], a, b);
+      f32x2_split(v.p[2 * i + 1], c, d);
+      w[i] = e4m3x2(a, b) | (e4m3x2(c, d) << 16);
+    }
+    memcpy(&out, w, sizeof(out));
   }
+  return out;
 }
 
+// VEC codes as fp32, without their scale (exact)
 template <int VEC>
-__device__ __forceinline__ void mx_decode(typename MxCodes<VEC>::type codes, float scale, float (&f)[VEC]) {
+__device__ __forceinline__ Lanes<VEC> mx_codes_value(const typename MxCodes<VEC>::type& codes) {
+  Lanes<VEC> v;
   if constexpr (VEC == 1) {
-    f[0] = e4m3x2_value(codes).x * scale;
+    v.f = e4m3x2_value(codes).x;
   } else {
     uint32_t w[VEC / 4];
-    if constexpr (VEC == 8) {
-      w[0] = codes.x;
-      w[1] = codes.y;
-    } else {
-      w[0] = codes;
-    }
+    memcpy(w, &codes, sizeof(codes));
 #pragma unroll
     for (int i = 0; i < VEC / 4; ++i) {
       const float2 lo = e4m3x2_value(w[i] & 0xFFFFu), hi = e4m3x2_value(w[i] >> 16);
-      f[4 * i] = lo.x * scale;
-      f[4 * i + 1] = lo.y * scale;
-      f[4 * i + 2] = hi.x * scale;
-      f[4 * i + 3] = hi.y * scale;
+      v.p[2 * i] = f32x2(lo.x, lo.y);
+      v.p[2 * i + 1] = f32x2(hi.x, hi.y);
     }
   }
+  return v;
 }
 
 // Eight codes times their scale as bf16, exactly (e4m3's 4 significant bits fit bf16's 8; only below 2^-126
@@ -123,11 +242,15 @@ __device__ __forceinline__ uint4 mx_decode_bf16(uint2 codes, uint32_t byte) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// VEC elements of type T as they lie in memory: VEC is a 16-byte load's worth (8 bf16, 4 fp32), or 1.
-// Kernels hold rows in this form (bf16 in half the registers of fp32) and widen on use.
+// VEC elements of type T as they lie in memory: whole 16-byte words, or one element. Kernels hold rows in
+// this form (bf16 in half the registers of fp32) and widen on use.
+template <int WORDS>
+struct Words {
+  uint4 w[WORDS];
+};
 template <typename T, int VEC>
 struct Raw {
-  using type = uint4;
+  using type = Words<VEC * sizeof(T) / 16>;
 };
 template <typename T>
 struct Raw<T, 1> {
@@ -137,34 +260,74 @@ struct Raw<T, 1> {
 // a load of data that is read once (kept out of the way of what is read again)
 template <typename T, int VEC>
 __device__ __forceinline__ typename Raw<T, VEC>::type load_raw(const T* p) {
-  if constexpr (VEC == 1)
+  if constexpr (VEC == 1) {
     return *p;
-  else
-    return __ldcs(reinterpret_cast<const uint4*>(p));
+  } else {
+    typename Raw<T, VEC>::type v;
+#pragma unroll
+    for (int i = 0; i < VEC * static_cast<int>(sizeof(T)) / 16; ++i) v.w[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+    return v;
+  }
+}
+
+// the same from shared memory
+template <typename T, int VEC>
+__device__ __forceinline__ typename Raw<T, VEC>::type shared_raw(const T* p) {
+  return *reinterpret_cast<const typename Raw<T, VEC>::type*>(p);
 }
 
 template <typename T, int VEC>
 __device__ __forceinline__ typename Raw<T, VEC>::type zero_raw() {
-  if constexpr (VEC == 1)
+  if constexpr (VEC == 1) {
     return static_cast<T>(0.f);
-  else
-    return make_uint4(0, 0, 0, 0);
+  } else {
+    typename Raw<T, VEC>::type v;
+#pragma unroll
+    for (int i = 0; i < VEC * static_cast<int>(sizeof(T)) / 16; ++i) v.w[i] = make_uint4(0, 0, 0, 0);
+    return v;
+  }
 }
 
 template <typename T, int VEC>
-__device__ __forceinline__ void widen(const typename Raw<T, VEC>::type& v, float (&f)[VEC]) {
+__device__ __forceinline__ Lanes<VEC> widen(const typename Raw<T, VEC>::type& v) {
+  Lanes<VEC> f;
   if constexpr (VEC == 1) {
-    f[0] = static_cast<float>(v);
+    f.f = static_cast<float>(v);
   } else {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < VEC * static_cast<int>(sizeof(T)) / 16; ++i) {
+      const uint32_t w[4] = {v.w[i].x, v.w[i].y, v.w[i].z, v.w[i].w};
       if constexpr (sizeof(T) == 4) {
-        f[i] = __uint_as_float(w[i]);
+        f.p[2 * i] = f32x2(__uint_as_float(w[0]), __uint_as_float(w[1]));
+        f.p[2 * i + 1] = f32x2(__uint_as_float(w[2]), __uint_as_float(w[3]));
       } else {
-        f[2 * i] = __uint_as_float(w[i] << 16);
-        f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f.p[4 * i + k] = f32x2(bf16_lo(w[k]), bf16_hi(w[k]));
       }
+    }
+  }
+  return f;
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void store_lanes(T* p, const Lanes<VEC>& f) {
+  if constexpr (VEC == 1) {
+    *p = static_cast<T>(f.f);  // round to nearest even
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC * static_cast<int>(sizeof(T)) / 16; ++i) {
+      uint32_t w[4];
+      if constexpr (sizeof(T) == 4) {
+        memcpy(w, &f.p[2 * i], 16);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float lo, hi;
+          f32x2_split(f.p[4 * i + k], lo, hi);
+          w[k] = pack_bf16(lo, hi);
+        }
+      }
+      __stcs(reinterpret_cast<uint4*>(p) + i, make_uint4(w[0], w[1], w[2], w[3]));
     }
   }
 }
@@ -175,64 +338,49 @@ template <typename T, int VEC>
 __device__ __forceinline__ uint32_t max_magnitude(const typename Raw<T, VEC>::type& v) {
   if constexpr (VEC == 1) {
     return __float_as_uint(static_cast<float>(v)) & 0x7FFFFFFFu;
-  } else if constexpr (sizeof(T) == 4) {
-    return max(max(v.x & 0x7FFFFFFFu, v.y & 0x7FFFFFFFu), max(v.z & 0x7FFFFFFFu, v.w & 0x7FFFFFFFu));
   } else {
-    const uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
-    return max(m << 16, m & 0xFFFF0000u);
+    constexpr uint32_t mask = sizeof(T) == 4 ? 0x7FFFFFFFu : 0x7FFF7FFFu;
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < VEC * static_cast<int>(sizeof(T)) / 16; ++i) {
+      const uint32_t a = v.w[i].x & mask, b = v.w[i].y & mask, c = v.w[i].z & mask, d = v.w[i].w & mask;
+      if constexpr (sizeof(T) == 4)
+        m = max(m, max(max(a, b), max(c, d)));
+      else
+        m = __vmaxu2(m, __vmaxu2(__vmaxu2(a, b), __vmaxu2(c, d)));
+    }
+    return sizeof(T) == 4 ? m : max(m << 16, m & 0xFFFF0000u);
   }
 }
 
 // The codes of a thread's VEC elements and the scale byte of their block, whose 32 channels lie in
 // 32 / VEC consecutive lanes. All of a warp's threads call this together. `f` holds the widened elements.
 template <typename T, int VEC>
-__device__ __forceinline__ typename MxCodes<VEC>::type mx_quantise(const typename Raw<T, VEC>::type& v,
-                                                                   const float (&f)[VEC], uint32_t& byte) {
+__device__ __forceinline__ typename MxCodes<VEC>::type mx_quantise(const typename Raw<T, VEC>::type& v, const Lanes<VEC>& f,
+                                                                   uint32_t& byte) {
   constexpr uint32_t kInfinity = 0x7F800000u;
   uint32_t m = max_magnitude<T, VEC>(v);
 #pragma unroll
   for (int o = kMxBlock / VEC / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-  float q[VEC];
   if (__any_sync(0xFFFFFFFFu, m >= kInfinity)) {
     // rare: somewhere in the warp's blocks a value is not finite. It becomes NaN (the conversion to e4m3
     // would make 448 of an infinity) and the scale is that of the others.
     m = 0;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const uint32_t a = __float_as_uint(f[j]) & 0x7FFFFFFFu;
+    f.each([&](float x) {
+      const uint32_t a = __float_as_uint(x) & 0x7FFFFFFFu;
       m = max(m, a < kInfinity ? a : 0u);
-    }
+      return x;
+    });
 #pragma unroll
     for (int o = kMxBlock / VEC / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
     byte = mx_scale_byte(m);
     const float inv = mx_inverse_scale(byte);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j)
-      q[j] = (__float_as_uint(f[j]) & 0x7FFFFFFFu) < kInfinity ? f[j] * inv : __uint_as_float(0x7FFFFFFFu);
-  } else {
-    byte = mx_scale_byte(m);
-    const float inv = mx_inverse_scale(byte);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) q[j] = f[j] * inv;
+    return mx_encode<VEC>(f.each([&](float x) {
+      return (__float_as_uint(x) & 0x7FFFFFFFu) < kInfinity ? x * inv : __uint_as_float(0x7FFFFFFFu);
+    }));
   }
-  return mx_encode<VEC>(q);
-}
-
-template <typename T, int VEC>
-__device__ __forceinline__ void store_vec(T* p, const float (&f)[VEC]) {
-  if constexpr (VEC == 1) {
-    *p = static_cast<T>(f[0]);  // round to nearest even
-  } else if constexpr (sizeof(T) == 4) {
-    __stcs(reinterpret_cast<float4*>(p), make_float4(f[0], f[1], f[2], f[3]));
-  } else {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
-  }
+  byte = mx_scale_byte(m);
+  return mx_encode<VEC>(f * Lanes<VEC>(mx_inverse_scale(byte)));
 }
 
 }  // namespace ffb

@@ -40,23 +40,6 @@ __device__ __forceinline__ void group_sum(float (&v)[NSUM], float* scratch, int&
   }
 }
 
-// VEC values of a weight vector (fp32; 16-byte aligned where VEC > 1)
-template <int VEC>
-__device__ __forceinline__ void load_weight(const float* p, float (&f)[VEC]) {
-  if constexpr (VEC == 1) {
-    f[0] = __ldg(p);
-  } else {
-#pragma unroll
-    for (int j = 0; j < VEC; j += 4) {
-      const float4 v = __ldg(reinterpret_cast<const float4*>(p + j));
-      f[j] = v.x;
-      f[j + 1] = v.y;
-      f[j + 2] = v.z;
-      f[j + 3] = v.w;
-    }
-  }
-}
-
 // ------------------------------------------------------------------ LayerNorm forward
 // GROUP threads hold U rows in registers (NV vectors of VEC channels a thread and row), so that U rows'
 // loads are in flight at once; mean and variance in two passes over the registers, one read and one
@@ -91,12 +74,7 @@ __global__ void __launch_bounds__(kThreads)
   for (int u = 0; u < U; ++u) {
     mean[u] = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      float f[VEC];
-      widen<T, VEC>(v[u][i], f);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) mean[u] += f[j];
-    }
+    for (int i = 0; i < NV; ++i) mean[u] += widen<T, VEC>(v[u][i]).sum();
   }
   group_sum<GROUP>(mean, scratch, turn);
 #pragma unroll
@@ -105,14 +83,8 @@ __global__ void __launch_bounds__(kThreads)
     rstd[u] = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int col = (i * GROUP + t) * VEC;
-      float f[VEC];
-      widen<T, VEC>(v[u][i], f);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float d = f[j] - mean[u];
-        rstd[u] += col < c ? d * d : 0.f;
-      }
+      const Lanes<VEC> d = widen<T, VEC>(v[u][i]) + Lanes<VEC>(-mean[u]);
+      rstd[u] += (i * GROUP + t) * VEC < c ? (d * d).sum() : 0.f;
     }
   }
   group_sum<GROUP>(rstd, scratch, turn);
@@ -128,20 +100,13 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int col = (i * GROUP + t) * VEC;
-    float w[VEC], b[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      w[j] = 1.f;
-      b[j] = 0.f;
-    }
-    if (col < c && gamma != nullptr) load_weight<VEC>(gamma + col, w);
-    if (col < c && beta != nullptr) load_weight<VEC>(beta + col, b);
+    const Lanes<VEC> w = col < c && gamma != nullptr ? load_weight<VEC>(gamma + col) : Lanes<VEC>(1.f);
+    const Lanes<VEC> b = col < c && beta != nullptr ? load_weight<VEC>(beta + col) : Lanes<VEC>(0.f);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t row = row0 + u * kGroups;
       const bool in = row < rows && col < c;
-      float f[VEC];
-      widen<T, VEC>(v[u][i], f);
+      const Lanes<VEC> f = widen<T, VEC>(v[u][i]);
       if (codes != nullptr) {
         uint32_t byte;
         const auto q = mx_quantise<T, VEC>(v[u][i], f, byte);
@@ -150,11 +115,59 @@ __global__ void __launch_bounds__(kThreads)
           if (t % kLanes == 0) scales[row * blocks + col / kMxBlock] = static_cast<uint8_t>(byte);
         }
       }
-      if (in) {
+      if (in)
+        store_lanes<T, VEC>(y + row * c + col, fma((f + Lanes<VEC>(-mean[u])) * Lanes<VEC>(rstd[u]), w, b));
+    }
+  }
+}
+
+// The block's sums of each channel over its rows (dg, db: a thread's, over the rows it took) to row
+// blockIdx.x of the partial sums.
+template <int VEC, int NV, int GROUP>
+__device__ __forceinline__ void write_column_sums(Lanes<VEC> (&dg)[NV], Lanes<VEC> (&db)[NV], float* dgamma, float* dbeta,
+                                                  int64_t partial_stride, int c) {
+  const int t = threadIdx.x % GROUP;
+  if (dgamma == nullptr && dbeta == nullptr) return;
+  float* pg = dgamma == nullptr ? nullptr : dgamma + blockIdx.x * partial_stride;
+  float* pb = dbeta == nullptr ? nullptr : dbeta + blockIdx.x * partial_stride;
+  if constexpr (GROUP == kThreads) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) f[j] = fmaf((f[j] - mean[u]) * rstd[u], w[j], b[j]);
-        store_vec<T, VEC>(y + row * c + col, f);
+    for (int i = 0; i < NV; ++i) {
+      const int col = (i * GROUP + t) * VEC;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        if (col < c && pg != nullptr) pg[col + j] = dg[i].get(j);
+        if (col < c && pb != nullptr) pb[col + j] = db[i].get(j);
       }
+    }
+  } else {
+    // the block's groups, added warp by warp into shared memory (a warp's groups by shuffles first)
+    __shared__ float sum[2][NV * 32 * VEC];
+#pragma unroll
+    for (int o = 16; o >= GROUP; o >>= 1) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        dg[i] = dg[i].each([&](float v) { return v + __shfl_xor_sync(0xFFFFFFFFu, v, o); });
+        db[i] = db[i].each([&](float v) { return v + __shfl_xor_sync(0xFFFFFFFFu, v, o); });
+      }
+    }
+    for (int w = 0; w < kWarps; ++w) {
+      if (threadIdx.x / 32 == w && (threadIdx.x & 31) < GROUP) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            const int at = (i * GROUP + t) * VEC + j;
+            sum[0][at] = w == 0 ? dg[i].get(j) : sum[0][at] + dg[i].get(j);
+            sum[1][at] = w == 0 ? db[i].get(j) : sum[1][at] + db[i].get(j);
+          }
+        }
+      }
+      __syncthreads();
+    }
+    for (int at = threadIdx.x; at < c; at += kThreads) {
+      if (pg != nullptr) pg[at] = sum[0][at];
+      if (pb != nullptr) pb[at] = sum[1][at];
     }
   }
 }
@@ -179,11 +192,9 @@ __global__ void __launch_bounds__(kThreads)
   const int t = threadIdx.x % GROUP;
   const int blocks = (c + kMxBlock - 1) / kMxBlock;
   const float inv_c = 1.0f / static_cast<float>(c);
-  float dg[NV][VEC], db[NV][VEC];
+  Lanes<VEC> dg[NV], db[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) dg[i][j] = db[i][j] = 0.f;
+  for (int i = 0; i < NV; ++i) dg[i] = db[i] = Lanes<VEC>(0.f);
 
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * (kGroups * U); base < rows;
        base += static_cast<int64_t>(gridDim.x) * (kGroups * U)) {
@@ -212,14 +223,14 @@ __global__ void __launch_bounds__(kThreads)
         }
       }
     }
-    // the normalised input of row u, vector i (channels past the row's end: 0 for dy, so no sum sees it)
-    auto normalised = [&](int u, int i, float(&xh)[VEC]) {
+    // The normalised input of row u, vector i. The mean is taken off first: x rstd - mean rstd would leave
+    // rounding errors of mean rstd where a row hardly varies.
+    auto normalised = [&](int u, int i) {
+      const Lanes<VEC> centre(-mean[u]), r(rstd[u]);
       if constexpr (MX)
-        mx_decode<VEC>(vc[u][i], mx_scale(vs[u][i]), xh);
+        return fma(mx_codes_value<VEC>(vc[u][i]), Lanes<VEC>(mx_scale(vs[u][i])), centre) * r;
       else
-        widen<T, VEC>(vx[u][i], xh);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) xh[j] = (xh[j] - mean[u]) * rstd[u];
+        return (widen<T, VEC>(vx[u][i]) + centre) * r;
     };
     float s[2 * U];
 #pragma unroll
@@ -227,24 +238,15 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int col = (i * GROUP + t) * VEC;
-      float g[VEC];
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) g[j] = 1.f;
-      if (col < c && gamma != nullptr) load_weight<VEC>(gamma + col, g);
+      const Lanes<VEC> g = col < c && gamma != nullptr ? load_weight<VEC>(gamma + col) : Lanes<VEC>(1.f);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (row0 + u * kGroups < rows && col < c) {
-          float xh[VEC], d[VEC];
-          normalised(u, i, xh);
-          widen<T, VEC>(vd[u][i], d);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            dg[i][j] = fmaf(d[j], xh[j], dg[i][j]);
-            db[i][j] += d[j];
-            const float w = d[j] * g[j];
-            s[2 * u] += w;
-            s[2 * u + 1] = fmaf(w, xh[j], s[2 * u + 1]);
-          }
+          const Lanes<VEC> xh = normalised(u, i), d = widen<T, VEC>(vd[u][i]), w = d * g;
+          dg[i] = fma(d, xh, dg[i]);
+          db[i] = db[i] + d;
+          s[2 * u] += w.sum();
+          s[2 * u + 1] += (w * xh).sum();
         }
       }
     }
@@ -252,77 +254,318 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int col = (i * GROUP + t) * VEC;
-      float g[VEC];
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) g[j] = 1.f;
-      if (col < c && gamma != nullptr) load_weight<VEC>(gamma + col, g);
+      const Lanes<VEC> g = col < c && gamma != nullptr ? load_weight<VEC>(gamma + col) : Lanes<VEC>(1.f);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int64_t row = row0 + u * kGroups;
         if (row < rows && col < c) {
           const float c1 = s[2 * u] * inv_c, c2 = s[2 * u + 1] * inv_c;
           const int64_t at = row * c + col;
-          float xh[VEC], d[VEC];
-          normalised(u, i, xh);
-          widen<T, VEC>(vd[u][i], d);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) d[j] = rstd[u] * (d[j] * g[j] - c1 - xh[j] * c2);
-          if (residual != nullptr) {
-            float r[VEC];
-            widen<T, VEC>(load_raw<T, VEC>(residual + at), r);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) d[j] += r[j];
-          }
-          store_vec<T, VEC>(dx + at, d);
+          const Lanes<VEC> w = widen<T, VEC>(vd[u][i]) * g;
+          Lanes<VEC> o = fma(normalised(u, i), Lanes<VEC>(-c2), w + Lanes<VEC>(-c1)) * Lanes<VEC>(rstd[u]);
+          if (residual != nullptr) o = o + widen<T, VEC>(load_raw<T, VEC>(residual + at));
+          store_lanes<T, VEC>(dx + at, o);
         }
       }
     }
   }
-  if (dgamma == nullptr && dbeta == nullptr) return;
-  float* pg = dgamma == nullptr ? nullptr : dgamma + blockIdx.x * partial_stride;
-  float* pb = dbeta == nullptr ? nullptr : dbeta + blockIdx.x * partial_stride;
-  if constexpr (GROUP == kThreads) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int col = (i * GROUP + t) * VEC;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        if (col < c && pg != nullptr) pg[col + j] = dg[i][j];
-        if (col < c && pb != nullptr) pb[col + j] = db[i][j];
-      }
+  write_column_sums<VEC, NV, GROUP>(dg, db, dgamma, dbeta, partial_stride, c);
+}
+
+// ------------------------------------------------------------------ LayerNorm, rows streamed
+// The same sums where rows are whole 16-byte words (c a multiple of 16): a team (a warp, or the block for
+// rows that a warp's registers cannot hold) takes RS = rows at a time, which lie next to one another in
+// memory, and has them copied to its own ring of kRing slots in shared memory by bulk copies. The loads in
+// flight then do not depend on registers or occupancy, and cost one thread a few instructions.
+constexpr int kRing = 3;
+
+template <int TEAM>
+__device__ __forceinline__ void team_sync() {
+  if constexpr (TEAM == 32)
+    __syncwarp();
+  else
+    __syncthreads();
+}
+
+// whether all of a team's threads say so, as all of them learn
+template <int TEAM>
+__device__ __forceinline__ bool team_all(bool yes) {
+  if constexpr (TEAM == 32)
+    return __all_sync(0xFFFFFFFFu, yes);
+  else
+    return __syncthreads_and(yes);
+}
+
+// A team's ring: `streams` tensors with rows of row_bytes[k] bytes; a slot holds RS rows of each, one
+// tensor after the other.
+template <int TEAM, int RS>
+struct Ring {
+  uint8_t* slots;
+  uint64_t* full;
+  int streams, slot_bytes;
+  const uint8_t* base[3];
+  int row_bytes[3];
+  int64_t rows, teams, first;  // this team's chunks of RS rows: first, first + teams, ..
+
+  __device__ __forceinline__ Ring(uint8_t* smem, uint64_t* bars, int64_t all_rows) : streams(0), slot_bytes(0), rows(all_rows) {
+    constexpr int kTeams = kThreads / TEAM;
+    const int team = threadIdx.x / TEAM;
+    slots = smem;
+    full = bars + team * kRing;
+    teams = static_cast<int64_t>(gridDim.x) * kTeams;
+    first = static_cast<int64_t>(blockIdx.x) * kTeams + team;
+    if (threadIdx.x % TEAM == 0) {
+      for (int i = 0; i < kRing; ++i) mbar_init(&full[i], 1);
+      fence_mbar_init();
     }
-  } else {
-    // the block's groups, added warp by warp into shared memory (the two rows of a warp's halves first)
-    __shared__ float sum[2][NV * 32 * VEC];
-    if constexpr (GROUP == 16) {
+  }
+  __device__ __forceinline__ void add(const void* p, int bytes) {
+    base[streams] = static_cast<const uint8_t*>(p);
+    row_bytes[streams] = bytes;
+    slot_bytes += RS * bytes;
+    ++streams;
+  }
+  // after the last add: the team's part of shared memory
+  __device__ __forceinline__ void place() { slots += static_cast<int64_t>(threadIdx.x / TEAM) * kRing * slot_bytes; }
+  __device__ __forceinline__ int64_t row(int turn) const { return (first + turn * teams) * RS; }
+  // one thread: the copies of the team's chunk number `turn`
+  __device__ __forceinline__ void fetch(int turn) {
+    const int64_t at = row(turn);
+    if (at >= rows) return;
+    const int n = rows - at < RS ? static_cast<int>(rows - at) : RS;
+    uint64_t* bar = &full[turn % kRing];
+    uint8_t* dst = slots + turn % kRing * slot_bytes;
+    int bytes = 0;
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      if (k < streams) bytes += n * row_bytes[k];
+    mbar_arrive_expect_tx(bar, bytes);
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      if (k < streams) {
+        bulk_load(dst, base[k] + at * row_bytes[k], n * row_bytes[k], bar);
+        dst += RS * row_bytes[k];
+      }
+  }
+  // False (for the whole team) where the copies never came: the error word says so, and the other slots'
+  // copies have had the same time to land.
+  __device__ __forceinline__ bool wait(int turn, int* err) {
+    return team_all<TEAM>(mbar_wait(&full[turn % kRing], (turn / kRing) & 1, err, kErrTimeoutLoad));
+  }
+  // row r of a slot's tensor k (whose rows follow those of the tensors before it)
+  template <typename P>
+  __device__ __forceinline__ const P* at(int turn, int offset) const {
+    return reinterpret_cast<const P*>(slots + turn % kRing * slot_bytes + offset);
+  }
+};
+
+template <typename T, int VEC, int NV, int GROUP, int U>
+__global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
+    ln_train_stream_kernel(const T* __restrict__ x, T* __restrict__ y, const float* __restrict__ gamma,
+                           const float* __restrict__ beta, float* __restrict__ mean_out, float* __restrict__ rstd_out,
+                           uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t rows, int c, float eps,
+                           int* err) {
+  constexpr int kTeam = GROUP <= 32 ? 32 : kThreads;
+  constexpr int kGroups = kTeam / GROUP;  // rows of a team side by side
+  constexpr int RS = kGroups * U;
+  constexpr int kLanes = kMxBlock / VEC;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t bars[kThreads / kTeam * kRing];
+  __shared__ float scratch[2 * U * kWarps];
+  int turn_of = 0;
+  const int t = threadIdx.x % GROUP, g = threadIdx.x % kTeam / GROUP;
+  const bool leader = threadIdx.x % kTeam == 0;
+  const int blocks = (c + kMxBlock - 1) / kMxBlock;
+  const float inv_c = 1.0f / static_cast<float>(c);
+  Ring<kTeam, RS> ring(smem, bars, rows);
+  ring.add(x, c * static_cast<int>(sizeof(T)));
+  ring.place();
+  __syncthreads();
+  if (leader)
+    for (int i = 0; i < kRing; ++i) ring.fetch(i);
+  Lanes<VEC> w[NV], b[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int col = (i * GROUP + t) * VEC;
+    w[i] = col < c && gamma != nullptr ? load_weight<VEC>(gamma + col) : Lanes<VEC>(1.f);
+    b[i] = col < c && beta != nullptr ? load_weight<VEC>(beta + col) : Lanes<VEC>(0.f);
+  }
+  for (int turn = 0; ring.row(turn) < rows; ++turn) {
+    if (!ring.wait(turn, err)) break;
+    const int64_t row0 = ring.row(turn) + g;
+    const T* have = ring.template at<T>(turn, 0) + g * c;
+    typename Raw<T, VEC>::type v[U][NV];
+    float mean[U], rstd[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      mean[u] = 0.f;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          dg[i][j] += __shfl_xor_sync(0xFFFFFFFFu, dg[i][j], 16);
-          db[i][j] += __shfl_xor_sync(0xFFFFFFFFu, db[i][j], 16);
-        }
+        const int col = (i * GROUP + t) * VEC;
+        v[u][i] = row0 + u * kGroups < rows && col < c ? shared_raw<T, VEC>(have + u * kGroups * c + col) : zero_raw<T, VEC>();
+        mean[u] += widen<T, VEC>(v[u][i]).sum();
       }
     }
-    for (int w = 0; w < kWarps; ++w) {
-      if (threadIdx.x / 32 == w && (threadIdx.x & 31) < GROUP) {
+    // the slot is in registers: the next rows may come
+    team_sync<kTeam>();
+    if (leader) ring.fetch(turn + kRing);
+    group_sum<GROUP>(mean, scratch, turn_of);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
+    for (int u = 0; u < U; ++u) {
+      mean[u] *= inv_c;
+      rstd[u] = 0.f;
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const int at = (i * GROUP + t) * VEC + j;
-            sum[0][at] = w == 0 ? dg[i][j] : sum[0][at] + dg[i][j];
-            sum[1][at] = w == 0 ? db[i][j] : sum[1][at] + db[i][j];
+      for (int i = 0; i < NV; ++i) {
+        const Lanes<VEC> d = widen<T, VEC>(v[u][i]) + Lanes<VEC>(-mean[u]);
+        rstd[u] += (i * GROUP + t) * VEC < c ? (d * d).sum() : 0.f;
+      }
+    }
+    group_sum<GROUP>(rstd, scratch, turn_of);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      rstd[u] = rsqrtf(rstd[u] * inv_c + eps);
+      const int64_t row = row0 + u * kGroups;
+      if (t == 0 && row < rows) {
+        mean_out[row] = mean[u];
+        rstd_out[row] = rstd[u];
+      }
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int col = (i * GROUP + t) * VEC;
+        const bool in = row < rows && col < c;
+        const Lanes<VEC> f = widen<T, VEC>(v[u][i]);
+        if (codes != nullptr) {
+          uint32_t byte;
+          const auto q = mx_quantise<T, VEC>(v[u][i], f, byte);
+          if (in) {
+            *reinterpret_cast<typename MxCodes<VEC>::type*>(codes + row * c + col) = q;
+            if (t % kLanes == 0) scales[row * blocks + col / kMxBlock] = static_cast<uint8_t>(byte);
           }
         }
+        if (in) store_lanes<T, VEC>(y + row * c + col, fma((f + Lanes<VEC>(-mean[u])) * Lanes<VEC>(rstd[u]), w[i], b[i]));
       }
-      __syncthreads();
-    }
-    for (int at = threadIdx.x; at < c; at += kThreads) {
-      if (pg != nullptr) pg[at] = sum[0][at];
-      if (pb != nullptr) pb[at] = sum[1][at];
     }
   }
+}
+
+template <typename T, int VEC, int NV, int GROUP, int U, bool MX>
+__global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
+    ln_bwd_stream_kernel(const T* __restrict__ dy, const T* __restrict__ x, const uint8_t* __restrict__ codes,
+                         const uint8_t* __restrict__ scales, const float* __restrict__ mean_in,
+                         const float* __restrict__ rstd_in, const float* __restrict__ gamma,
+                         const T* __restrict__ residual, T* __restrict__ dx, float* __restrict__ dgamma,
+                         float* __restrict__ dbeta, int64_t partial_stride, int64_t rows, int c, int* err) {
+  constexpr int kTeam = GROUP <= 32 ? 32 : kThreads;
+  constexpr int kGroups = kTeam / GROUP;
+  constexpr int RS = kGroups * U;
+  using Codes = typename MxCodes<VEC>::type;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t bars[kThreads / kTeam * kRing];
+  __shared__ float scratch[4 * kWarps];
+  int turn_of = 0;
+  const int t = threadIdx.x % GROUP, g = threadIdx.x % kTeam / GROUP;
+  const bool leader = threadIdx.x % kTeam == 0;
+  const int blocks = (c + kMxBlock - 1) / kMxBlock;
+  const float inv_c = 1.0f / static_cast<float>(c);
+  Ring<kTeam, RS> ring(smem, bars, rows);
+  ring.add(dy, c * static_cast<int>(sizeof(T)));
+  if constexpr (MX)
+    ring.add(codes, c);
+  else
+    ring.add(x, c * static_cast<int>(sizeof(T)));
+  if (residual != nullptr) ring.add(residual, c * static_cast<int>(sizeof(T)));
+  ring.place();
+  __syncthreads();
+  if (leader)
+    for (int i = 0; i < kRing; ++i) ring.fetch(i);
+  Lanes<VEC> dg[NV], db[NV], w[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int col = (i * GROUP + t) * VEC;
+    dg[i] = db[i] = Lanes<VEC>(0.f);
+    w[i] = col < c && gamma != nullptr ? load_weight<VEC>(gamma + col) : Lanes<VEC>(1.f);
+  }
+  // a chunk's statistics (and scales) are loaded while the one before it is worked on
+  float mean[U], rstd[U];
+  uint8_t scale[MX ? U : 1][NV];
+  auto load_statistics = [&](int64_t row0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = row0 + g + u * kGroups;
+      const bool in = row < rows;
+      mean[u] = in ? __ldg(mean_in + row) : 0.f;
+      rstd[u] = in ? __ldg(rstd_in + row) : 0.f;
+      if constexpr (MX) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int col = (i * GROUP + t) * VEC;
+          scale[u][i] = in && col < c ? __ldg(scales + row * blocks + col / kMxBlock) : 0;
+        }
+      }
+    }
+  };
+  load_statistics(ring.row(0));
+  for (int turn = 0; ring.row(turn) < rows; ++turn) {
+    float m[U], r[U], scaled[MX ? U : 1][NV];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      m[u] = -mean[u];
+      r[u] = rstd[u];
+      if constexpr (MX)
+#pragma unroll
+        for (int i = 0; i < NV; ++i) scaled[u][i] = mx_scale(scale[u][i]);
+    }
+    load_statistics(ring.row(turn + 1));
+    if (!ring.wait(turn, err)) break;
+    const int64_t row0 = ring.row(turn) + g;
+    const T* have_dy = ring.template at<T>(turn, 0) + g * c;
+    const uint8_t* have_x = ring.template at<uint8_t>(turn, RS * c * static_cast<int>(sizeof(T)));
+    const T* have_res = ring.template at<T>(turn, RS * c * static_cast<int>(sizeof(T) + (MX ? 1 : sizeof(T)))) + g * c;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = row0 + u * kGroups;
+      const bool live = row < rows;
+      Lanes<VEC> xh[NV], d[NV];
+      float s[2] = {0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int col = (i * GROUP + t) * VEC;
+        const bool in = live && col < c;
+        const int at = u * kGroups * c + col;
+        d[i] = widen<T, VEC>(in ? shared_raw<T, VEC>(have_dy + at) : zero_raw<T, VEC>());
+        // the mean is taken off first: x rstd - mean rstd would leave rounding errors of mean rstd where a
+        // row hardly varies. Where dy is 0 (past a row's end) no sum sees xh.
+        if constexpr (MX) {
+          const Codes q = in ? *reinterpret_cast<const Codes*>(have_x + g * c + at) : Codes{};
+          xh[i] = fma(mx_codes_value<VEC>(q), Lanes<VEC>(scaled[u][i]), Lanes<VEC>(m[u])) * Lanes<VEC>(r[u]);
+        } else {
+          const typename Raw<T, VEC>::type q = in ? shared_raw<T, VEC>(reinterpret_cast<const T*>(have_x) + g * c + at) : zero_raw<T, VEC>();
+          xh[i] = (widen<T, VEC>(q) + Lanes<VEC>(m[u])) * Lanes<VEC>(r[u]);
+        }
+        if (live) {
+          dg[i] = fma(d[i], xh[i], dg[i]);
+          db[i] = db[i] + d[i];
+          d[i] = d[i] * w[i];
+          s[0] += d[i].sum();
+          s[1] += (d[i] * xh[i]).sum();
+        }
+      }
+      group_sum<GROUP>(s, scratch, turn_of);
+      const Lanes<VEC> c1(-s[0] * inv_c), c2(-s[1] * inv_c), scale_out(r[u]);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int col = (i * GROUP + t) * VEC;
+        if (live && col < c) {
+          Lanes<VEC> o = fma(xh[i], c2, d[i] + c1) * scale_out;
+          if (residual != nullptr) o = o + widen<T, VEC>(shared_raw<T, VEC>(have_res + u * kGroups * c + col));
+          store_lanes<T, VEC>(dx + row * c + col, o);
+        }
+      }
+    }
+    team_sync<kTeam>();
+    if (leader) ring.fetch(turn + kRing);
+  }
+  write_column_sums<VEC, NV, GROUP>(dg, db, dgamma, dbeta, partial_stride, c);
 }
 
 // out[col] = sum over `parts` rows of partial sums, in a fixed order: 32 columns a block, 32 rows at
@@ -398,10 +641,8 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const T* __restrict__ x,
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const P p(first + u * kThreads, total, c, per_row);
-    float f[VEC];
-    widen<T, VEC>(v[u], f);
     uint32_t byte;
-    const auto q = mx_quantise<T, VEC>(v[u], f, byte);
+    const auto q = mx_quantise<T, VEC>(v[u], widen<T, VEC>(v[u]), byte);
     if (p.in) {
       *reinterpret_cast<typename MxCodes<VEC>::type*>(codes + p.at) = q;
       if (threadIdx.x % P::kLanes == 0) scales[p.block] = static_cast<uint8_t>(byte);
@@ -427,9 +668,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const P p(first + u * kThreads, total, c, per_row);
-    float f[VEC];
-    mx_decode<VEC>(v[u], mx_scale(s[u]), f);
-    if (p.in) store_vec<T, VEC>(x + p.at, f);
+    if (p.in) store_lanes<T, VEC>(x + p.at, mx_codes_value<VEC>(v[u]) * Lanes<VEC>(mx_scale(s[u])));
   }
 }
 
@@ -472,9 +711,7 @@ __global__ void __launch_bounds__(kThreads)
   for (int u = 0; u < U; ++u) {
     const uint32_t id = first + u * kThreads;
     const bool in = id < total;
-    float a[VEC], b[VEC];
-    widen<T, VEC>(va[u], a);
-    widen<T, VEC>(vb[u], b);
+    const Lanes<VEC> a = widen<T, VEC>(va[u]), b = widen<T, VEC>(vb[u]);
     if (codes != nullptr) {
       uint32_t ea, eb;
       const auto qa = mx_quantise<T, VEC>(va[u], a, ea);
@@ -489,14 +726,11 @@ __global__ void __launch_bounds__(kThreads)
         }
       }
     }
-    if (in) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const Gate g(a[j]);
-        a[j] = a[j] * g.f * g.u * b[j];
-      }
-      store_vec<T, VEC>(out + static_cast<int64_t>(id) * VEC, a);
-    }
+    if (in)
+      store_lanes<T, VEC>(out + static_cast<int64_t>(id) * VEC, a.each([](float v) {
+                            const Gate g(v);
+                            return v * g.f * g.u;
+                          }) * b);
   }
 }
 
@@ -536,53 +770,72 @@ __global__ void __launch_bounds__(kThreads)
   for (int u = 0; u < U; ++u) {
     const uint32_t id = first + u * kThreads;
     if (id >= total) continue;
-    float a[VEC], b[VEC], d[VEC];
-    widen<T, VEC>(vd[u], d);
+    const Lanes<VEC> d = widen<T, VEC>(vd[u]);
+    Lanes<VEC> a, b;
     if constexpr (MX) {
-      mx_decode<VEC>(ca[u], mx_scale(sa[u]), a);
-      mx_decode<VEC>(cb[u], mx_scale(sb[u]), b);
+      a = mx_codes_value<VEC>(ca[u]) * Lanes<VEC>(mx_scale(sa[u]));
+      b = mx_codes_value<VEC>(cb[u]) * Lanes<VEC>(mx_scale(sb[u]));
     } else {
-      widen<T, VEC>(va[u], a);
-      widen<T, VEC>(vb[u], b);
+      a = widen<T, VEC>(va[u]);
+      b = widen<T, VEC>(vb[u]);
     }
-    float o[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const Gate g(a[j]);
-      const float unit = a[j] * g.f * g.u;
-      o[j] = unit * b[j];
-      const float da = d[j] * b[j] * g.f * (1.0f + a[j] * g.c) * g.u;
-      b[j] = d[j] * unit;
-      a[j] = da;
-    }
-    store_vec<T, VEC>(dab + at[u], a);
-    store_vec<T, VEC>(dab + at[u] + h, b);
-    if (out != nullptr) store_vec<T, VEC>(out + static_cast<int64_t>(id) * VEC, o);
+    const Lanes<VEC> unit = a.each([](float v) {
+      const Gate g(v);
+      return v * g.f * g.u;
+    });
+    // the gate's factors one at a time: d b f first, so that a large 1 + a (1 - s) meets it when it is small
+    Lanes<VEC> da = d * b;
+    da = a.apply(da, [](float v, float w) {
+      const Gate g(v);
+      return w * g.f * (1.0f + v * g.c) * g.u;
+    });
+    store_lanes<T, VEC>(dab + at[u], da);
+    store_lanes<T, VEC>(dab + at[u] + h, d * unit);
+    if (out != nullptr) store_lanes<T, VEC>(out + static_cast<int64_t>(id) * VEC, unit * b);
   }
 }
 
 // ------------------------------------------------------------------ launches
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// How a row of c channels is held: 16-byte vectors where the rows allow them (every pointer 16-byte
-// aligned, c a whole number of vectors), the fewest threads that hold it with at most 32 channels a
-// thread, and U rows at a time where a row leaves few registers in use. Calls
-// f(VEC, NV, GROUP, U as integral constants).
-template <typename T, typename F>
-int dispatch_row(int c, bool vector, F&& f) {
-  constexpr int kVec = 16 / sizeof(T);
 #define FFB_ROW(V, N, G, U)                                                                                   \
   if (c <= (V) * (N) * (G))                                                                                   \
   return f(std::integral_constant<int, V>{}, std::integral_constant<int, N>{}, std::integral_constant<int, G>{}, \
            std::integral_constant<int, U>{})
+
+// How a row of c channels is held, for rows that are streamed: vectors of 16 bytes, two a thread where the
+// row allows it (fewer threads, fewer shuffles to add them up; more would leave few registers), and U rows
+// of a group at a time so that a chunk is a few KB. Calls f(VEC, NV, GROUP, U as integral constants).
+template <typename T, typename F>
+int dispatch_stream(int c, F&& f) {
+  constexpr int kVec = 16 / sizeof(T);
+  if constexpr (kVec == 8) {
+    FFB_ROW(8, 2, 4, 2);
+    FFB_ROW(8, 2, 8, 2);
+    FFB_ROW(8, 2, 16, 2);
+    FFB_ROW(8, 2, 32, 2);
+    FFB_ROW(8, 4, 32, 1);
+    FFB_ROW(8, 2, kThreads, 1);
+    FFB_ROW(8, 4, kThreads, 1);
+  } else {
+    FFB_ROW(4, 2, 8, 2);
+    FFB_ROW(4, 2, 16, 2);
+    FFB_ROW(4, 2, 32, 2);
+    FFB_ROW(4, 4, 32, 1);
+    FFB_ROW(4, 2, kThreads, 1);
+    FFB_ROW(4, 8, kThreads, 1);
+  }
+  return static_cast<int>(cudaErrorInvalidValue);
+}
+
+// The same for rows that are not: vectors where every pointer is 16-byte aligned and c a whole number of
+// them, else single elements; the fewest threads that hold a row with at most 32 channels a thread.
+template <typename T, typename F>
+int dispatch_row(int c, bool vector, F&& f) {
+  constexpr int kVec = 16 / sizeof(T);
   if (vector) {
-    FFB_ROW(kVec, 1, 16, 4);
-    FFB_ROW(kVec, 1, 32, 4);
-    FFB_ROW(kVec, 2, 32, 2);
-    FFB_ROW(kVec, 3, 32, 2);
-    FFB_ROW(kVec, 4, 32, 1);
-    FFB_ROW(kVec, 1, kThreads, 4);
-    FFB_ROW(kVec, 2, kThreads, 2);
+    FFB_ROW(kVec, 1, 32, 2);
+    FFB_ROW(kVec, 32 / kVec, 32, 1);
     FFB_ROW(kVec, 32 / kVec, kThreads, 1);
   } else {
     FFB_ROW(1, 2, 32, 4);
@@ -590,29 +843,61 @@ int dispatch_row(int c, bool vector, F&& f) {
     FFB_ROW(1, 8, kThreads, 2);
     FFB_ROW(1, 32, kThreads, 1);
   }
-#undef FFB_ROW
   return static_cast<int>(cudaErrorInvalidValue);
 }
+#undef FFB_ROW
 
 constexpr int kLnBlocks = 148 * 2;  // blocks (rows of partial sums) of the backward pass at most
 
+// Whether rows of c channels are streamed: 16-byte words (every pointer is aligned) of 16 channels, and a
+// block's rings, whose rows take `row_bytes` over all tensors, fit shared memory (fp32 rows of above 6000
+// channels with a residual do not).
 template <typename T>
-int ln_bwd_blocks(int64_t rows, int c, bool vector) {
-  int blocks = 0;
-  dispatch_row<T>(c, vector, [&](auto, auto, auto g, auto u) {
-    constexpr int per = kThreads / decltype(g)::value * decltype(u)::value;  // rows a block takes at a time
-    const int64_t want = (rows + per - 1) / per;
-    blocks = static_cast<int>(want < kLnBlocks ? want : kLnBlocks);
+bool ln_streams(bool whole, int c, int row_bytes) {
+  int per = 0;
+  dispatch_stream<T>(c, [&](auto, auto, auto g, auto u) {
+    per = kThreads / decltype(g)::value * decltype(u)::value;
     return 0;
   });
+  return whole && c % 16 == 0 && static_cast<int64_t>(kRing) * per * row_bytes <= 200 * 1024;
+}
+
+// blocks of a backward pass whose blocks take `per` rows at a time
+int ln_blocks(int64_t rows, int64_t per) {
+  const int64_t want = (rows + per - 1) / per;
+  return static_cast<int>(want < kLnBlocks ? want : kLnBlocks);
+}
+template <typename T>
+int ln_bwd_blocks(int64_t rows, int c, bool stream, bool vector) {
+  int blocks = 0;
+  auto count = [&](auto, auto, auto g, auto u) {
+    blocks = ln_blocks(rows, kThreads / decltype(g)::value * decltype(u)::value);
+    return 0;
+  };
+  if (stream)
+    dispatch_stream<T>(c, count);
+  else
+    dispatch_row<T>(c, vector, count);
   return blocks;
 }
 
 template <typename T>
-int ln_train(const LayerNormTrain& p, cudaStream_t stream) {
-  const bool vector = aligned(p.x) && aligned(p.y) && aligned(p.codes) && aligned(p.gamma) && aligned(p.beta) &&
-                      p.c % (16 / sizeof(T)) == 0;
-  return dispatch_row<T>(p.c, vector, [&](auto v, auto n, auto g, auto u) {
+int ln_train(const LayerNormTrain& p, int* err, cudaStream_t stream) {
+  const bool whole = aligned(p.x) && aligned(p.y) && aligned(p.codes) && aligned(p.gamma) && aligned(p.beta);
+  if (ln_streams<T>(whole, p.c, p.c * sizeof(T)))
+    return dispatch_stream<T>(p.c, [&](auto v, auto n, auto g, auto u) {
+      constexpr int V = decltype(v)::value, N = decltype(n)::value, G = decltype(g)::value, U = decltype(u)::value;
+      constexpr int per = kThreads / G * U;  // rows of a block at a time
+      auto kernel = ln_train_stream_kernel<T, V, N, G, U>;
+      const int smem = kRing * per * p.c * static_cast<int>(sizeof(T));
+      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      if (e != cudaSuccess) return static_cast<int>(e);
+      kernel<<<ln_blocks(p.rows, per), kThreads, smem, stream>>>(static_cast<const T*>(p.x), static_cast<T*>(p.y), p.gamma,
+                                                                p.beta, p.mean, p.rstd, p.codes, p.scales, p.rows, p.c,
+                                                                p.eps, err);
+      return static_cast<int>(cudaGetLastError());
+    });
+  return dispatch_row<T>(p.c, whole && p.c % (16 / sizeof(T)) == 0, [&](auto v, auto n, auto g, auto u) {
     constexpr int V = decltype(v)::value, N = decltype(n)::value, G = decltype(g)::value, U = decltype(u)::value;
     constexpr int per = kThreads / G * U;
     // a launch's grid is 31 bits wide
@@ -628,31 +913,49 @@ int ln_train(const LayerNormTrain& p, cudaStream_t stream) {
 }
 
 template <typename T>
-int ln_bwd(const LayerNormBwd& p, cudaStream_t stream) {
+int ln_bwd(const LayerNormBwd& p, int* err, cudaStream_t stream) {
   const bool mx = p.codes != nullptr;
-  const bool vector = aligned(p.dy) && aligned(p.dx) && aligned(p.residual) && aligned(p.gamma) &&
-                      aligned(mx ? static_cast<const void*>(p.codes) : p.x) && p.c % (16 / sizeof(T)) == 0;
-  const int grid = ln_bwd_blocks<T>(p.rows, p.c, vector);
-  return dispatch_row<T>(p.c, vector, [&](auto v, auto n, auto g, auto u) {
-    constexpr int V = decltype(v)::value, N = decltype(n)::value, G = decltype(g)::value, U = decltype(u)::value;
-    const bool sums = p.dgamma != nullptr || p.dbeta != nullptr;
-    // one block writes the gradients itself; several leave rows [dgamma | dbeta] of partial sums
-    float* part = static_cast<float*>(p.workspace);
-    float* dg = !sums ? nullptr : grid == 1 ? p.dgamma : part;
-    float* db = !sums ? nullptr : grid == 1 ? p.dbeta : part + p.c;
-    auto launch = [&](auto m) {
-      ln_bwd_kernel<T, V, N, G, U, decltype(m)::value><<<grid, kThreads, 0, stream>>>(
-          static_cast<const T*>(p.dy), static_cast<const T*>(p.x), p.codes, p.scales, p.mean, p.rstd, p.gamma,
-          static_cast<const T*>(p.residual), static_cast<T*>(p.dx), dg, db, 2 * static_cast<int64_t>(p.c), p.rows, p.c);
-    };
-    if (mx)
-      launch(std::true_type{});
-    else
-      launch(std::false_type{});
-    if (sums && grid > 1)
-      ln_grad_reduce_kernel<<<(2 * p.c + 31) / 32, 1024, 0, stream>>>(part, p.dgamma, p.dbeta, grid, p.c);
-    return static_cast<int>(cudaGetLastError());
-  });
+  const bool whole = aligned(p.dy) && aligned(p.dx) && aligned(p.residual) && aligned(p.gamma) &&
+                     aligned(mx ? static_cast<const void*>(p.codes) : p.x);
+  const int row_bytes = p.c * static_cast<int>(sizeof(T)), all_bytes = row_bytes + (mx ? p.c : row_bytes) + (p.residual != nullptr ? row_bytes : 0);
+  const bool streamed = ln_streams<T>(whole, p.c, all_bytes), vector = whole && p.c % (16 / sizeof(T)) == 0;
+  const int grid = ln_bwd_blocks<T>(p.rows, p.c, streamed, vector);
+  const bool sums = p.dgamma != nullptr || p.dbeta != nullptr;
+  // one block writes the gradients itself; several leave rows [dgamma | dbeta] of partial sums
+  float* part = static_cast<float*>(p.workspace);
+  float* dg = !sums ? nullptr : grid == 1 ? p.dgamma : part;
+  float* db = !sums ? nullptr : grid == 1 ? p.dbeta : part + p.c;
+  const int64_t stride = 2 * static_cast<int64_t>(p.c);
+  const T* dy = static_cast<const T*>(p.dy);
+  const T* x = static_cast<const T*>(p.x);
+  const T* residual = static_cast<const T*>(p.residual);
+  T* dx = static_cast<T*>(p.dx);
+  int rc;
+  if (streamed)
+    rc = dispatch_stream<T>(p.c, [&](auto v, auto n, auto g, auto u) {
+      constexpr int V = decltype(v)::value, N = decltype(n)::value, G = decltype(g)::value, U = decltype(u)::value;
+      constexpr int per = kThreads / G * U;
+      const int smem = kRing * per * all_bytes;
+      auto kernel = mx ? ln_bwd_stream_kernel<T, V, N, G, U, true> : ln_bwd_stream_kernel<T, V, N, G, U, false>;
+      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      if (e != cudaSuccess) return static_cast<int>(e);
+      kernel<<<grid, kThreads, smem, stream>>>(dy, x, p.codes, p.scales, p.mean, p.rstd, p.gamma, residual, dx, dg, db,
+                                               stride, p.rows, p.c, err);
+      return static_cast<int>(cudaGetLastError());
+    });
+  else
+    rc = dispatch_row<T>(p.c, vector, [&](auto v, auto n, auto g, auto u) {
+      constexpr int V = decltype(v)::value, N = decltype(n)::value, G = decltype(g)::value, U = decltype(u)::value;
+      auto kernel = mx ? ln_bwd_kernel<T, V, N, G, U, true> : ln_bwd_kernel<T, V, N, G, U, false>;
+      kernel<<<grid, kThreads, 0, stream>>>(dy, x, p.codes, p.scales, p.mean, p.rstd, p.gamma, residual, dx, dg, db, stride,
+                                            p.rows, p.c);
+      return static_cast<int>(cudaGetLastError());
+    });
+  if (rc == 0 && sums && grid > 1) {
+    ln_grad_reduce_kernel<<<(2 * p.c + 31) / 32, 1024, 0, stream>>>(part, p.dgamma, p.dbeta, grid, p.c);
+    rc = static_cast<int>(cudaGetLastError());
+  }
+  return rc;
 }
 
 // Elementwise work on `rows` rows of `per_row` units (vectors, or blocks of 32 channels times their
@@ -762,18 +1065,21 @@ int swiglu_bwd(const void* dh, const void* ab, const uint8_t* codes, const uint8
 }  // namespace
 
 size_t ln_bwd_workspace_bytes(int64_t rows, int c, int is_f32) {
-  // the tensors' alignment is not known here: room for the form with more blocks
-  const int a = is_f32 ? ln_bwd_blocks<float>(rows, c, true) : ln_bwd_blocks<__nv_bfloat16>(rows, c, true);
-  const int b = is_f32 ? ln_bwd_blocks<float>(rows, c, false) : ln_bwd_blocks<__nv_bfloat16>(rows, c, false);
-  const int blocks = a > b ? a : b;
-  return blocks > 1 ? static_cast<size_t>(blocks) * 2 * c * sizeof(float) : 0;
+  // the tensors' alignment is not known here: room for the form with the most blocks
+  int most = 0;
+  for (int form = 0; form < 3; ++form) {
+    const bool stream = form == 0, vector = form == 1;
+    const int blocks = is_f32 ? ln_bwd_blocks<float>(rows, c, stream, vector) : ln_bwd_blocks<__nv_bfloat16>(rows, c, stream, vector);
+    if (blocks > most) most = blocks;
+  }
+  return most > 1 ? static_cast<size_t>(most) * 2 * c * sizeof(float) : 0;
 }
 
-int launch_ln_train(const LayerNormTrain& p, int is_f32, cudaStream_t stream) {
-  return is_f32 ? ln_train<float>(p, stream) : ln_train<__nv_bfloat16>(p, stream);
+int launch_ln_train(const LayerNormTrain& p, int is_f32, int* err, cudaStream_t stream) {
+  return is_f32 ? ln_train<float>(p, err, stream) : ln_train<__nv_bfloat16>(p, err, stream);
 }
-int launch_ln_bwd(const LayerNormBwd& p, int is_f32, cudaStream_t stream) {
-  return is_f32 ? ln_bwd<float>(p, stream) : ln_bwd<__nv_bfloat16>(p, stream);
+int launch_ln_bwd(const LayerNormBwd& p, int is_f32, int* err, cudaStream_t stream) {
+  return is_f32 ? ln_bwd<float>(p, err, stream) : ln_bwd<__nv_bfloat16>(p, err, stream);
 }
 int launch_checkpoint_pack(const void* x, uint8_t* codes, uint8_t* scales, int64_t rows, int c, int is_f32,
                            cudaStream_t stream) {

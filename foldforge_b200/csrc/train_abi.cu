@@ -55,7 +55,7 @@ int ffb_layernorm_train_fwd(const void* x, void* y, const float* gamma, const fl
   st = device_info(&info);
   if (st != FFB_OK) return st;
   const LayerNormTrain p{x, y, gamma, beta, mean, rstd, codes, scales, rows, c, eps};
-  return cuda_status(launch_ln_train(p, dtype == FFB_F32, as_stream(stream)), "layernorm_train_fwd launch");
+  return cuda_status(launch_ln_train(p, dtype == FFB_F32, info.err, as_stream(stream)), "layernorm_train_fwd launch");
 }
 
 size_t ffb_layernorm_bwd_workspace_bytes(int64_t rows, int c, int dtype) {
@@ -96,7 +96,7 @@ int ffb_layernorm_bwd(const void* dy, const void* x, const uint8_t* codes, const
   st = device_info(&info);
   if (st != FFB_OK) return st;
   const LayerNormBwd p{dy, x, codes, scales, mean, rstd, gamma, residual, dx, dgamma, dbeta, workspace, rows, c};
-  return cuda_status(launch_ln_bwd(p, dtype == FFB_F32, as_stream(stream)), "layernorm_bwd launch");
+  return cuda_status(launch_ln_bwd(p, dtype == FFB_F32, info.err, as_stream(stream)), "layernorm_bwd launch");
 }
 
 int ffb_checkpoint_pack(const void* x, uint8_t* codes, uint8_t* scales, int64_t rows, int c, int dtype, void* stream) {
