@@ -92,6 +92,15 @@ struct Lanes {
     f32x2_split(t, a, b);
     return a + b;
   }
+  // the sum of products with `o`
+  __device__ __forceinline__ float dot(const Lanes& o) const {
+    uint64_t t = mul_f32x2(p[0], o.p[0]);
+#pragma unroll
+    for (int i = 1; i < VEC / 2; ++i) t = fma_f32x2(p[i], o.p[i], t);
+    float a, b;
+    f32x2_split(t, a, b);
+    return a + b;
+  }
   __device__ __forceinline__ float get(int j) const {
     float a, b;
     f32x2_split(p[j / 2], a, b);
@@ -112,6 +121,7 @@ struct Lanes<1> {
     return Lanes(g(f, o.f));
   }
   __device__ __forceinline__ float sum() const { return f; }
+  __device__ __forceinline__ float dot(const Lanes& o) const { return f * o.f; }
   __device__ __forceinline__ float get(int) const { return f; }
 };
 template <int VEC>
@@ -332,6 +342,12 @@ __device__ __forceinline__ void store_lanes(T* p, const Lanes<VEC>& f) {
   }
 }
 
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
 // The bits (fp32) of the largest magnitude among VEC elements: magnitudes order as their bits do, an
 // infinity or a NaN above every finite one. bf16 pairs are compared two at a time.
 template <typename T, int VEC>
@@ -347,7 +363,7 @@ __device__ __forceinline__ uint32_t max_magnitude(const typename Raw<T, VEC>::ty
       if constexpr (sizeof(T) == 4)
         m = max(m, max(max(a, b), max(c, d)));
       else
-        m = __vmaxu2(m, __vmaxu2(__vmaxu2(a, b), __vmaxu2(c, d)));
+        m = max_u16x2(m, max_u16x2(max_u16x2(a, b), max_u16x2(c, d)));
     }
     return sizeof(T) == 4 ? m : max(m << 16, m & 0xFFFF0000u);
   }

@@ -359,7 +359,8 @@ struct Ring {
   }
 };
 
-template <typename T, int VEC, int NV, int GROUP, int U>
+// FULL: c fills the group's vectors, so that no lane has to look whether its channels are there.
+template <typename T, int VEC, int NV, int GROUP, int U, bool FULL>
 __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
     ln_train_stream_kernel(const T* __restrict__ x, T* __restrict__ y, const float* __restrict__ gamma,
                            const float* __restrict__ beta, float* __restrict__ mean_out, float* __restrict__ rstd_out,
@@ -371,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
   constexpr int kLanes = kMxBlock / VEC;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t bars[kThreads / kTeam * kRing];
-  __shared__ float scratch[2 * U * kWarps];
+  __shared__ float scratch[2 * kWarps];
   int turn_of = 0;
   const int t = threadIdx.x % GROUP, g = threadIdx.x % kTeam / GROUP;
   const bool leader = threadIdx.x % kTeam == 0;
@@ -387,68 +388,62 @@ __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int col = (i * GROUP + t) * VEC;
-    w[i] = col < c && gamma != nullptr ? load_weight<VEC>(gamma + col) : Lanes<VEC>(1.f);
-    b[i] = col < c && beta != nullptr ? load_weight<VEC>(beta + col) : Lanes<VEC>(0.f);
+    w[i] = (FULL || col < c) && gamma != nullptr ? load_weight<VEC>(gamma + col) : Lanes<VEC>(1.f);
+    b[i] = (FULL || col < c) && beta != nullptr ? load_weight<VEC>(beta + col) : Lanes<VEC>(0.f);
   }
   for (int turn = 0; ring.row(turn) < rows; ++turn) {
     if (!ring.wait(turn, err)) break;
     const int64_t row0 = ring.row(turn) + g;
     const T* have = ring.template at<T>(turn, 0) + g * c;
-    typename Raw<T, VEC>::type v[U][NV];
-    float mean[U], rstd[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      mean[u] = 0.f;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int col = (i * GROUP + t) * VEC;
-        v[u][i] = row0 + u * kGroups < rows && col < c ? shared_raw<T, VEC>(have + u * kGroups * c + col) : zero_raw<T, VEC>();
-        mean[u] += widen<T, VEC>(v[u][i]).sum();
-      }
-    }
-    // the slot is in registers: the next rows may come
-    team_sync<kTeam>();
-    if (leader) ring.fetch(turn + kRing);
-    group_sum<GROUP>(mean, scratch, turn_of);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      mean[u] *= inv_c;
-      rstd[u] = 0.f;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const Lanes<VEC> d = widen<T, VEC>(v[u][i]) + Lanes<VEC>(-mean[u]);
-        rstd[u] += (i * GROUP + t) * VEC < c ? (d * d).sum() : 0.f;
-      }
-    }
-    group_sum<GROUP>(rstd, scratch, turn_of);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      rstd[u] = rsqrtf(rstd[u] * inv_c + eps);
       const int64_t row = row0 + u * kGroups;
+      typename Raw<T, VEC>::type v[NV];
+      Lanes<VEC> f[NV];
+      float mean[1] = {0.f}, rstd[1] = {0.f};
+      // a row past the last one reads what the slot held before, and nothing of it is kept
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int col = (i * GROUP + t) * VEC;
+        v[i] = FULL || col < c ? shared_raw<T, VEC>(have + u * kGroups * c + col) : zero_raw<T, VEC>();
+        f[i] = widen<T, VEC>(v[i]);
+        mean[0] += f[i].sum();
+      }
+      group_sum<GROUP>(mean, scratch, turn_of);
+      const float m = mean[0] * inv_c;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const Lanes<VEC> d = f[i] + Lanes<VEC>(-m);
+        const float q = d.dot(d);
+        rstd[0] += FULL || (i * GROUP + t) * VEC < c ? q : 0.f;
+      }
+      group_sum<GROUP>(rstd, scratch, turn_of);
+      const float r = rsqrtf(rstd[0] * inv_c + eps);
       if (t == 0 && row < rows) {
-        mean_out[row] = mean[u];
-        rstd_out[row] = rstd[u];
+        mean_out[row] = m;
+        rstd_out[row] = r;
       }
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int col = (i * GROUP + t) * VEC;
-        const bool in = row < rows && col < c;
-        const Lanes<VEC> f = widen<T, VEC>(v[u][i]);
+        const bool in = row < rows && (FULL || col < c);
         if (codes != nullptr) {
           uint32_t byte;
-          const auto q = mx_quantise<T, VEC>(v[u][i], f, byte);
+          const auto q = mx_quantise<T, VEC>(v[i], f[i], byte);
           if (in) {
             *reinterpret_cast<typename MxCodes<VEC>::type*>(codes + row * c + col) = q;
             if (t % kLanes == 0) scales[row * blocks + col / kMxBlock] = static_cast<uint8_t>(byte);
           }
         }
-        if (in) store_lanes<T, VEC>(y + row * c + col, fma((f + Lanes<VEC>(-mean[u])) * Lanes<VEC>(rstd[u]), w[i], b[i]));
+        if (in) store_lanes<T, VEC>(y + row * c + col, fma((f[i] + Lanes<VEC>(-m)) * Lanes<VEC>(r), w[i], b[i]));
       }
     }
+    team_sync<kTeam>();
+    if (leader) ring.fetch(turn + kRing);
   }
 }
 
-template <typename T, int VEC, int NV, int GROUP, int U, bool MX>
+template <typename T, int VEC, int NV, int GROUP, int U, bool MX, bool FULL>
 __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
     ln_bwd_stream_kernel(const T* __restrict__ dy, const T* __restrict__ x, const uint8_t* __restrict__ codes,
                          const uint8_t* __restrict__ scales, const float* __restrict__ mean_in,
@@ -483,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
   for (int i = 0; i < NV; ++i) {
     const int col = (i * GROUP + t) * VEC;
     dg[i] = db[i] = Lanes<VEC>(0.f);
-    w[i] = col < c && gamma != nullptr ? load_weight<VEC>(gamma + col) : Lanes<VEC>(1.f);
+    w[i] = (FULL || col < c) && gamma != nullptr ? load_weight<VEC>(gamma + col) : Lanes<VEC>(1.f);
   }
   // a chunk's statistics (and scales) are loaded while the one before it is worked on
   float mean[U], rstd[U];
@@ -499,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           const int col = (i * GROUP + t) * VEC;
-          scale[u][i] = in && col < c ? __ldg(scales + row * blocks + col / kMxBlock) : 0;
+          scale[u][i] = in && (FULL || col < c) ? __ldg(scales + row * blocks + col / kMxBlock) : 0;
         }
       }
     }
@@ -521,6 +516,7 @@ __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
     const T* have_dy = ring.template at<T>(turn, 0) + g * c;
     const uint8_t* have_x = ring.template at<uint8_t>(turn, RS * c * static_cast<int>(sizeof(T)));
     const T* have_res = ring.template at<T>(turn, RS * c * static_cast<int>(sizeof(T) + (MX ? 1 : sizeof(T)))) + g * c;
+    const bool whole = ring.row(turn) + RS <= rows;  // the same for the team
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t row = row0 + u * kGroups;
@@ -530,33 +526,40 @@ __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int col = (i * GROUP + t) * VEC;
-        const bool in = live && col < c;
         const int at = u * kGroups * c + col;
-        d[i] = widen<T, VEC>(in ? shared_raw<T, VEC>(have_dy + at) : zero_raw<T, VEC>());
+        d[i] = widen<T, VEC>(FULL || col < c ? shared_raw<T, VEC>(have_dy + at) : zero_raw<T, VEC>());
         // the mean is taken off first: x rstd - mean rstd would leave rounding errors of mean rstd where a
         // row hardly varies. Where dy is 0 (past a row's end) no sum sees xh.
         if constexpr (MX) {
-          const Codes q = in ? *reinterpret_cast<const Codes*>(have_x + g * c + at) : Codes{};
+          const Codes q = FULL || col < c ? *reinterpret_cast<const Codes*>(have_x + g * c + at) : Codes{};
           xh[i] = fma(mx_codes_value<VEC>(q), Lanes<VEC>(scaled[u][i]), Lanes<VEC>(m[u])) * Lanes<VEC>(r[u]);
         } else {
-          const typename Raw<T, VEC>::type q = in ? shared_raw<T, VEC>(reinterpret_cast<const T*>(have_x) + g * c + at) : zero_raw<T, VEC>();
-          xh[i] = (widen<T, VEC>(q) + Lanes<VEC>(m[u])) * Lanes<VEC>(r[u]);
-        }
-        if (live) {
-          dg[i] = fma(d[i], xh[i], dg[i]);
-          db[i] = db[i] + d[i];
-          d[i] = d[i] * w[i];
-          s[0] += d[i].sum();
-          s[1] += (d[i] * xh[i]).sum();
+          xh[i] = (widen<T, VEC>(FULL || col < c ? shared_raw<T, VEC>(reinterpret_cast<const T*>(have_x) + g * c + at)
+                                                 : zero_raw<T, VEC>()) +
+                   Lanes<VEC>(m[u])) *
+                  Lanes<VEC>(r[u]);
         }
       }
+      if (!whole && !live) {  // the slot holds what was there before
+#pragma unroll
+        for (int i = 0; i < NV; ++i) d[i] = xh[i] = Lanes<VEC>(0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        dg[i] = fma(d[i], xh[i], dg[i]);
+        db[i] = db[i] + d[i];
+        d[i] = d[i] * w[i];
+        s[0] += d[i].sum();
+        s[1] += d[i].dot(xh[i]);
+      }
       group_sum<GROUP>(s, scratch, turn_of);
-      const Lanes<VEC> c1(-s[0] * inv_c), c2(-s[1] * inv_c), scale_out(r[u]);
+      // dx = rstd w - (rstd mean(w)) - xh (rstd mean(w xh))
+      const Lanes<VEC> c1(-s[0] * inv_c * r[u]), c2(-s[1] * inv_c * r[u]), c0(r[u]);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int col = (i * GROUP + t) * VEC;
-        if (live && col < c) {
-          Lanes<VEC> o = fma(xh[i], c2, d[i] + c1) * scale_out;
+        if (live && (FULL || col < c)) {
+          Lanes<VEC> o = fma(xh[i], c2, fma(d[i], c0, c1));
           if (residual != nullptr) o = o + widen<T, VEC>(shared_raw<T, VEC>(have_res + u * kGroups * c + col));
           store_lanes<T, VEC>(dx + row * c + col, o);
         }
@@ -888,7 +891,7 @@ int ln_train(const LayerNormTrain& p, int* err, cudaStream_t stream) {
     return dispatch_stream<T>(p.c, [&](auto v, auto n, auto g, auto u) {
       constexpr int V = decltype(v)::value, N = decltype(n)::value, G = decltype(g)::value, U = decltype(u)::value;
       constexpr int per = kThreads / G * U;  // rows of a block at a time
-      auto kernel = ln_train_stream_kernel<T, V, N, G, U>;
+      auto kernel = p.c == V * N * G ? ln_train_stream_kernel<T, V, N, G, U, true> : ln_train_stream_kernel<T, V, N, G, U, false>;
       const int smem = kRing * per * p.c * static_cast<int>(sizeof(T));
       const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
       if (e != cudaSuccess) return static_cast<int>(e);
@@ -936,7 +939,9 @@ int ln_bwd(const LayerNormBwd& p, int* err, cudaStream_t stream) {
       constexpr int V = decltype(v)::value, N = decltype(n)::value, G = decltype(g)::value, U = decltype(u)::value;
       constexpr int per = kThreads / G * U;
       const int smem = kRing * per * all_bytes;
-      auto kernel = mx ? ln_bwd_stream_kernel<T, V, N, G, U, true> : ln_bwd_stream_kernel<T, V, N, G, U, false>;
+      const bool full = p.c == V * N * G;
+      auto kernel = mx ? full ? ln_bwd_stream_kernel<T, V, N, G, U, true, true> : ln_bwd_stream_kernel<T, V, N, G, U, true, false>
+                       : full ? ln_bwd_stream_kernel<T, V, N, G, U, false, true> : ln_bwd_stream_kernel<T, V, N, G, U, false, false>;
       const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
       if (e != cudaSuccess) return static_cast<int>(e);
       kernel<<<grid, kThreads, smem, stream>>>(dy, x, p.codes, p.scales, p.mean, p.rstd, p.gamma, residual, dx, dg, db,
