@@ -369,15 +369,22 @@ __device__ __forceinline__ uint32_t max_magnitude(const typename Raw<T, VEC>::ty
   }
 }
 
+// the largest of the lanes that share a block (a whole warp for single elements)
+template <int VEC>
+__device__ __forceinline__ uint32_t mx_lanes_max(uint32_t m) {
+  if constexpr (VEC == 1) return __reduce_max_sync(0xFFFFFFFFu, m);
+#pragma unroll
+  for (int o = kMxBlock / VEC / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  return m;
+}
+
 // The codes of a thread's VEC elements and the scale byte of their block, whose 32 channels lie in
 // 32 / VEC consecutive lanes. All of a warp's threads call this together. `f` holds the widened elements.
 template <typename T, int VEC>
 __device__ __forceinline__ typename MxCodes<VEC>::type mx_quantise(const typename Raw<T, VEC>::type& v, const Lanes<VEC>& f,
                                                                    uint32_t& byte) {
   constexpr uint32_t kInfinity = 0x7F800000u;
-  uint32_t m = max_magnitude<T, VEC>(v);
-#pragma unroll
-  for (int o = kMxBlock / VEC / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  uint32_t m = mx_lanes_max<VEC>(max_magnitude<T, VEC>(v));
   if (__any_sync(0xFFFFFFFFu, m >= kInfinity)) {
     // rare: somewhere in the warp's blocks a value is not finite. It becomes NaN (the conversion to e4m3
     // would make 448 of an infinity) and the scale is that of the others.
@@ -387,8 +394,7 @@ __device__ __forceinline__ typename MxCodes<VEC>::type mx_quantise(const typenam
       m = max(m, a < kInfinity ? a : 0u);
       return x;
     });
-#pragma unroll
-    for (int o = kMxBlock / VEC / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    m = mx_lanes_max<VEC>(m);
     byte = mx_scale_byte(m);
     const float inv = mx_inverse_scale(byte);
     return mx_encode<VEC>(f.each([&](float x) {

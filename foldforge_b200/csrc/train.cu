@@ -122,12 +122,13 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // The block's sums of each channel over its rows (dg, db: a thread's, over the rows it took) to row
-// blockIdx.x of the partial sums.
+// blockIdx.x of the partial sums. `space` holds kWarps NV GROUP VEC floats unless the whole block shares
+// each row, and nobody uses it any more once the block has come here.
 template <int VEC, int NV, int GROUP>
 __device__ __forceinline__ void write_column_sums(Lanes<VEC> (&dg)[NV], Lanes<VEC> (&db)[NV], float* dgamma, float* dbeta,
-                                                  int64_t partial_stride, int c) {
-  const int t = threadIdx.x % GROUP;
+                                                  int64_t partial_stride, int c, float* space) {
   if (dgamma == nullptr && dbeta == nullptr) return;
+  const int t = threadIdx.x % GROUP;
   float* pg = dgamma == nullptr ? nullptr : dgamma + blockIdx.x * partial_stride;
   float* pb = dbeta == nullptr ? nullptr : dbeta + blockIdx.x * partial_stride;
   if constexpr (GROUP == kThreads) {
@@ -141,8 +142,9 @@ __device__ __forceinline__ void write_column_sums(Lanes<VEC> (&dg)[NV], Lanes<VE
       }
     }
   } else {
-    // the block's groups, added warp by warp into shared memory (a warp's groups by shuffles first)
-    __shared__ float sum[2][NV * 32 * VEC];
+    // a warp's groups by shuffles, then the warps through shared memory, each sum in a fixed order
+    constexpr int kColumns = NV * GROUP * VEC;
+    const int warp = threadIdx.x / 32;
 #pragma unroll
     for (int o = 16; o >= GROUP; o >>= 1) {
 #pragma unroll
@@ -151,23 +153,24 @@ __device__ __forceinline__ void write_column_sums(Lanes<VEC> (&dg)[NV], Lanes<VE
         db[i] = db[i].each([&](float v) { return v + __shfl_xor_sync(0xFFFFFFFFu, v, o); });
       }
     }
-    for (int w = 0; w < kWarps; ++w) {
-      if (threadIdx.x / 32 == w && (threadIdx.x & 31) < GROUP) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
+    for (int which = 0; which < 2; ++which) {
+      __syncthreads();
+      if ((threadIdx.x & 31) < GROUP) {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const int at = (i * GROUP + t) * VEC + j;
-            sum[0][at] = w == 0 ? dg[i].get(j) : sum[0][at] + dg[i].get(j);
-            sum[1][at] = w == 0 ? db[i].get(j) : sum[1][at] + db[i].get(j);
-          }
-        }
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            space[warp * kColumns + (i * GROUP + t) * VEC + j] = which == 0 ? dg[i].get(j) : db[i].get(j);
       }
       __syncthreads();
-    }
-    for (int at = threadIdx.x; at < c; at += kThreads) {
-      if (pg != nullptr) pg[at] = sum[0][at];
-      if (pb != nullptr) pb[at] = sum[1][at];
+      float* out = which == 0 ? pg : pb;
+      for (int at = threadIdx.x; at < c && out != nullptr; at += kThreads) {
+        float a = 0.f;
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) a += space[k * kColumns + at];
+        out[at] = a;
+      }
     }
   }
 }
@@ -269,7 +272,8 @@ __global__ void __launch_bounds__(kThreads)
       }
     }
   }
-  write_column_sums<VEC, NV, GROUP>(dg, db, dgamma, dbeta, partial_stride, c);
+  __shared__ float space[GROUP == kThreads ? 1 : kWarps * NV * GROUP * VEC];
+  write_column_sums<VEC, NV, GROUP>(dg, db, dgamma, dbeta, partial_stride, c, space);
 }
 
 // ------------------------------------------------------------------ LayerNorm, rows streamed
@@ -372,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
   constexpr int kLanes = kMxBlock / VEC;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t bars[kThreads / kTeam * kRing];
-  __shared__ float scratch[2 * kWarps];
+  __shared__ float scratch[2 * U * kWarps];
   int turn_of = 0;
   const int t = threadIdx.x % GROUP, g = threadIdx.x % kTeam / GROUP;
   const bool leader = threadIdx.x % kTeam == 0;
@@ -395,47 +399,85 @@ __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
     if (!ring.wait(turn, err)) break;
     const int64_t row0 = ring.row(turn) + g;
     const T* have = ring.template at<T>(turn, 0) + g * c;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t row = row0 + u * kGroups;
-      typename Raw<T, VEC>::type v[NV];
-      Lanes<VEC> f[NV];
-      float mean[1] = {0.f}, rstd[1] = {0.f};
-      // a row past the last one reads what the slot held before, and nothing of it is kept
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int col = (i * GROUP + t) * VEC;
-        v[i] = FULL || col < c ? shared_raw<T, VEC>(have + u * kGroups * c + col) : zero_raw<T, VEC>();
-        f[i] = widen<T, VEC>(v[i]);
-        mean[0] += f[i].sum();
+    // a row past the last one reads what the slot held before, and nothing of it is kept
+    auto read = [&](int u, int i) {
+      const int col = (i * GROUP + t) * VEC;
+      return FULL || col < c ? shared_raw<T, VEC>(have + u * kGroups * c + col) : zero_raw<T, VEC>();
+    };
+    auto squares = [&](const Lanes<VEC>& f, float m, int i) {
+      const Lanes<VEC> d = f + Lanes<VEC>(-m);
+      const float q = d.dot(d);
+      return FULL || (i * GROUP + t) * VEC < c ? q : 0.f;
+    };
+    auto finish = [&](const typename Raw<T, VEC>::type& v, const Lanes<VEC>& f, float m, float r, int64_t row, int i) {
+      const int col = (i * GROUP + t) * VEC;
+      const bool in = row < rows && (FULL || col < c);
+      if (codes != nullptr) {
+        uint32_t byte;
+        const auto q = mx_quantise<T, VEC>(v, f, byte);
+        if (in) {
+          *reinterpret_cast<typename MxCodes<VEC>::type*>(codes + row * c + col) = q;
+          if (t % kLanes == 0) scales[row * blocks + col / kMxBlock] = static_cast<uint8_t>(byte);
+        }
       }
-      group_sum<GROUP>(mean, scratch, turn_of);
-      const float m = mean[0] * inv_c;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const Lanes<VEC> d = f[i] + Lanes<VEC>(-m);
-        const float q = d.dot(d);
-        rstd[0] += FULL || (i * GROUP + t) * VEC < c ? q : 0.f;
-      }
-      group_sum<GROUP>(rstd, scratch, turn_of);
-      const float r = rsqrtf(rstd[0] * inv_c + eps);
+      if (in) store_lanes<T, VEC>(y + row * c + col, fma((f + Lanes<VEC>(-m)) * Lanes<VEC>(r), w[i], b[i]));
+    };
+    auto keep = [&](float m, float r, int64_t row) {
       if (t == 0 && row < rows) {
         mean_out[row] = m;
         rstd_out[row] = r;
       }
+    };
+    if constexpr (GROUP > 32) {
+      // the block's barriers cost more than reading the slot again: all rows of the chunk at a time
+      float m[U], r[U];
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int col = (i * GROUP + t) * VEC;
-        const bool in = row < rows && (FULL || col < c);
-        if (codes != nullptr) {
-          uint32_t byte;
-          const auto q = mx_quantise<T, VEC>(v[i], f[i], byte);
-          if (in) {
-            *reinterpret_cast<typename MxCodes<VEC>::type*>(codes + row * c + col) = q;
-            if (t % kLanes == 0) scales[row * blocks + col / kMxBlock] = static_cast<uint8_t>(byte);
-          }
+      for (int u = 0; u < U; ++u) {
+        m[u] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) m[u] += widen<T, VEC>(read(u, i)).sum();
+      }
+      group_sum<GROUP>(m, scratch, turn_of);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        m[u] *= inv_c;
+        r[u] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) r[u] += squares(widen<T, VEC>(read(u, i)), m[u], i);
+      }
+      group_sum<GROUP>(r, scratch, turn_of);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        r[u] = rsqrtf(r[u] * inv_c + eps);
+        keep(m[u], r[u], row0 + u);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const auto v = read(u, i);
+          finish(v, widen<T, VEC>(v), m[u], r[u], row0 + u, i);
         }
-        if (in) store_lanes<T, VEC>(y + row * c + col, fma((f[i] + Lanes<VEC>(-m)) * Lanes<VEC>(r), w[i], b[i]));
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t row = row0 + u * kGroups;
+        typename Raw<T, VEC>::type v[NV];
+        Lanes<VEC> f[NV];
+        float m[1] = {0.f}, r[1] = {0.f};
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          v[i] = read(u, i);
+          f[i] = widen<T, VEC>(v[i]);
+          m[0] += f[i].sum();
+        }
+        group_sum<GROUP>(m, scratch, turn_of);
+        m[0] *= inv_c;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) r[0] += squares(f[i], m[0], i);
+        group_sum<GROUP>(r, scratch, turn_of);
+        r[0] = rsqrtf(r[0] * inv_c + eps);
+        keep(m[0], r[0], row);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) finish(v[i], f[i], m[0], r[0], row, i);
       }
     }
     team_sync<kTeam>();
@@ -456,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
   using Codes = typename MxCodes<VEC>::type;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t bars[kThreads / kTeam * kRing];
-  __shared__ float scratch[4 * kWarps];
+  __shared__ float scratch[4 * U * kWarps];
   int turn_of = 0;
   const int t = threadIdx.x % GROUP, g = threadIdx.x % kTeam / GROUP;
   const bool leader = threadIdx.x % kTeam == 0;
@@ -517,58 +559,85 @@ __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
     const uint8_t* have_x = ring.template at<uint8_t>(turn, RS * c * static_cast<int>(sizeof(T)));
     const T* have_res = ring.template at<T>(turn, RS * c * static_cast<int>(sizeof(T) + (MX ? 1 : sizeof(T)))) + g * c;
     const bool whole = ring.row(turn) + RS <= rows;  // the same for the team
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
+    // dy and the normalised input of row u, vector i; 0 for a row past the last one (the slot holds what was
+    // there before). The mean is taken off first: x rstd - mean rstd would leave rounding errors of mean
+    // rstd where a row hardly varies. Where dy is 0 (past a row's end) no sum sees xh.
+    auto read = [&](int u, int i, Lanes<VEC>& d, Lanes<VEC>& xh) {
+      const int col = (i * GROUP + t) * VEC;
+      const int at = u * kGroups * c + col;
+      d = widen<T, VEC>(FULL || col < c ? shared_raw<T, VEC>(have_dy + at) : zero_raw<T, VEC>());
+      if constexpr (MX) {
+        const Codes q = FULL || col < c ? *reinterpret_cast<const Codes*>(have_x + g * c + at) : Codes{};
+        xh = fma(mx_codes_value<VEC>(q), Lanes<VEC>(scaled[u][i]), Lanes<VEC>(m[u])) * Lanes<VEC>(r[u]);
+      } else {
+        xh = (widen<T, VEC>(FULL || col < c ? shared_raw<T, VEC>(reinterpret_cast<const T*>(have_x) + g * c + at)
+                                            : zero_raw<T, VEC>()) +
+              Lanes<VEC>(m[u])) *
+             Lanes<VEC>(r[u]);
+      }
+      if (!whole && row0 + u * kGroups >= rows) d = xh = Lanes<VEC>(0.f);
+    };
+    // dgamma, dbeta and the row's sums; d becomes gamma dy
+    auto add = [&](int i, Lanes<VEC>& d, const Lanes<VEC>& xh, float& s0, float& s1) {
+      dg[i] = fma(d, xh, dg[i]);
+      db[i] = db[i] + d;
+      d = d * w[i];
+      s0 += d.sum();
+      s1 += d.dot(xh);
+    };
+    // dx = rstd w - rstd mean(w) - xh rstd mean(w xh)
+    auto finish = [&](int u, int i, const Lanes<VEC>& d, const Lanes<VEC>& xh, float s0, float s1) {
       const int64_t row = row0 + u * kGroups;
-      const bool live = row < rows;
-      Lanes<VEC> xh[NV], d[NV];
-      float s[2] = {0.f, 0.f};
+      const int col = (i * GROUP + t) * VEC;
+      if (row < rows && (FULL || col < c)) {
+        Lanes<VEC> o = fma(xh, Lanes<VEC>(-s1 * inv_c * r[u]), fma(d, Lanes<VEC>(r[u]), Lanes<VEC>(-s0 * inv_c * r[u])));
+        if (residual != nullptr) o = o + widen<T, VEC>(shared_raw<T, VEC>(have_res + u * kGroups * c + col));
+        store_lanes<T, VEC>(dx + row * c + col, o);
+      }
+    };
+    if constexpr (GROUP > 32) {
+      // the block's barriers cost more than reading the slot again: all rows of the chunk at a time
+      float s[2 * U];
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int col = (i * GROUP + t) * VEC;
-        const int at = u * kGroups * c + col;
-        d[i] = widen<T, VEC>(FULL || col < c ? shared_raw<T, VEC>(have_dy + at) : zero_raw<T, VEC>());
-        // the mean is taken off first: x rstd - mean rstd would leave rounding errors of mean rstd where a
-        // row hardly varies. Where dy is 0 (past a row's end) no sum sees xh.
-        if constexpr (MX) {
-          const Codes q = FULL || col < c ? *reinterpret_cast<const Codes*>(have_x + g * c + at) : Codes{};
-          xh[i] = fma(mx_codes_value<VEC>(q), Lanes<VEC>(scaled[u][i]), Lanes<VEC>(m[u])) * Lanes<VEC>(r[u]);
-        } else {
-          xh[i] = (widen<T, VEC>(FULL || col < c ? shared_raw<T, VEC>(reinterpret_cast<const T*>(have_x) + g * c + at)
-                                                 : zero_raw<T, VEC>()) +
-                   Lanes<VEC>(m[u])) *
-                  Lanes<VEC>(r[u]);
+      for (int u = 0; u < U; ++u) {
+        s[2 * u] = s[2 * u + 1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          Lanes<VEC> d, xh;
+          read(u, i, d, xh);
+          add(i, d, xh, s[2 * u], s[2 * u + 1]);
         }
-      }
-      if (!whole && !live) {  // the slot holds what was there before
-#pragma unroll
-        for (int i = 0; i < NV; ++i) d[i] = xh[i] = Lanes<VEC>(0.f);
-      }
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        dg[i] = fma(d[i], xh[i], dg[i]);
-        db[i] = db[i] + d[i];
-        d[i] = d[i] * w[i];
-        s[0] += d[i].sum();
-        s[1] += d[i].dot(xh[i]);
       }
       group_sum<GROUP>(s, scratch, turn_of);
-      // dx = rstd w - (rstd mean(w)) - xh (rstd mean(w xh))
-      const Lanes<VEC> c1(-s[0] * inv_c * r[u]), c2(-s[1] * inv_c * r[u]), c0(r[u]);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int col = (i * GROUP + t) * VEC;
-        if (live && (FULL || col < c)) {
-          Lanes<VEC> o = fma(xh[i], c2, fma(d[i], c0, c1));
-          if (residual != nullptr) o = o + widen<T, VEC>(shared_raw<T, VEC>(have_res + u * kGroups * c + col));
-          store_lanes<T, VEC>(dx + row * c + col, o);
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          Lanes<VEC> d, xh;
+          read(u, i, d, xh);
+          finish(u, i, d * w[i], xh, s[2 * u], s[2 * u + 1]);
         }
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        Lanes<VEC> xh[NV], d[NV];
+        float s[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NV; ++i) read(u, i, d[i], xh[i]);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) add(i, d[i], xh[i], s[0], s[1]);
+        group_sum<GROUP>(s, scratch, turn_of);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) finish(u, i, d[i], xh[i], s[0], s[1]);
       }
     }
     team_sync<kTeam>();
     if (leader) ring.fetch(turn + kRing);
   }
-  write_column_sums<VEC, NV, GROUP>(dg, db, dgamma, dbeta, partial_stride, c);
+  // the rings hold 24 rows or more, at least 72 bytes a channel: room for 32 bytes a lane's channel, of which at
+  // most half lie past the row
+  write_column_sums<VEC, NV, GROUP>(dg, db, dgamma, dbeta, partial_stride, c, reinterpret_cast<float*>(smem));
 }
 
 // out[col] = sum over `parts` rows of partial sums, in a fixed order: 32 columns a block, 32 rows at
@@ -818,14 +887,15 @@ int dispatch_stream(int c, F&& f) {
     FFB_ROW(8, 2, 16, 2);
     FFB_ROW(8, 2, 32, 2);
     FFB_ROW(8, 4, 32, 1);
-    FFB_ROW(8, 2, kThreads, 1);
+    FFB_ROW(8, 2, kThreads, 2);
     FFB_ROW(8, 4, kThreads, 1);
   } else {
     FFB_ROW(4, 2, 8, 2);
     FFB_ROW(4, 2, 16, 2);
     FFB_ROW(4, 2, 32, 2);
     FFB_ROW(4, 4, 32, 1);
-    FFB_ROW(4, 2, kThreads, 1);
+    FFB_ROW(4, 2, kThreads, 2);
+    FFB_ROW(4, 4, kThreads, 1);
     FFB_ROW(4, 8, kThreads, 1);
   }
   return static_cast<int>(cudaErrorInvalidValue);
