@@ -26,7 +26,11 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from foldforge_b200.engine import training
+
 Tensor = torch.Tensor
+#: channels of a LayerNorm whose gradient the b200 kernels take (a row is held in one block's registers)
+MAX_TRAINED_CHANNELS = 8192
 MASKED_UPDATES = ("zero", "compute")
 
 
@@ -61,6 +65,9 @@ class LayerNorm(nn.LayerNorm):
     backends = ("pytorch", "b200")
     dispatches_policy = True
 
+    #: what the b200 backend keeps for a backward pass (``foldforge_b200.engine.training``)
+    checkpoint: str | None = None
+
     def __init__(self, d, eps: float = 1e-5, bias: bool = True, elementwise_affine: bool = True) -> None:
         super().__init__(d, eps=eps, elementwise_affine=elementwise_affine, bias=bias)
         self.backend = "pytorch"
@@ -76,17 +83,26 @@ class LayerNorm(nn.LayerNorm):
         _check_backend(self, name)
         self.backend = name
 
+    def set_checkpoint(self, name: str | None) -> None:
+        self.checkpoint = training.check_name(name)
+
+    def _trains(self, x: Tensor) -> bool:
+        return self.checkpoint is not None and training.needs_gradient(self, x)
+
     def unsupported(self, x: Tensor) -> str | None:
         if self.backend == "pytorch":
             return None
-        reason = _cuda_reason(x)
+        trains = self._trains(x)
+        reason = _device_reason(x) if trains else _cuda_reason(x)
         if reason:
             return reason
         if x.dtype not in (torch.bfloat16, torch.float32):
             return f"dtype {x.dtype} (bf16 or fp32 only)"
         if len(self.normalized_shape) != 1:
             return "normalisation over more than one axis"
-        return None
+        if trains and self.normalized_shape[0] > MAX_TRAINED_CHANNELS:
+            return f"{self.normalized_shape[0]} channels (the b200 gradient takes at most {MAX_TRAINED_CHANNELS})"
+        return training.capture_reason() if trains else None
 
     def forward(self, x: Tensor) -> Tensor:
         return _dispatch(self, x)
@@ -99,6 +115,8 @@ class LayerNorm(nn.LayerNorm):
     def _forward_b200(self, x: Tensor) -> Tensor:
         from foldforge_b200 import kernels
 
+        if self._trains(x):
+            return training.layer_norm(x, self.weight, self.bias, self.eps, self.checkpoint)
         return kernels.layer_norm(x, self.weight, self.bias, self.eps)
 
 
@@ -109,7 +127,7 @@ def _check_backend(module: nn.Module, name: str) -> None:
         raise BackendUnsupported(message)
 
 
-def _cuda_reason(*ts: Tensor | None) -> str | None:
+def _device_reason(*ts: Tensor | None) -> str | None:
     for t in ts:
         if t is None:
             continue
@@ -117,7 +135,15 @@ def _cuda_reason(*ts: Tensor | None) -> str | None:
             return "tensor is not on a CUDA device"
         if torch.cuda.get_device_capability(t.device) != (10, 0):
             return "the b200 kernels need an sm_100 device"
-        if t.requires_grad and torch.is_grad_enabled():
+    return None
+
+
+def _cuda_reason(*ts: Tensor | None) -> str | None:
+    for t in ts:
+        reason = _device_reason(t)
+        if reason:
+            return reason
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
             return "autograd is not supported by the b200 kernels (inference only)"
     return None
 
@@ -404,7 +430,12 @@ class TriangleAttentionAF3(TriangleAttention):
 class Transition(_PairOp):
     """``x + W_sq(silu(W_a LN(x)) * W_b LN(x))`` (``legacy/primitives.py:20-37``,
     ``legacy/reference/transition.py:28-59``). On b200: the pair (128, 4) and single (384, 4)
-    widths in bf16 run the tcgen05 kernels, every other width and fp32 the SIMT path."""
+    widths in bf16 run the tcgen05 kernels, every other width and fp32 the SIMT path. With
+    ``checkpoint`` set it has a gradient there too (``foldforge_b200.engine.training``), for bf16
+    activations of widths that are a multiple of 8."""
+
+    #: what the b200 backend keeps for a backward pass
+    checkpoint: str | None = None
 
     def __init__(self, d_hidden: int, n: int = 4) -> None:
         super().__init__()
@@ -414,14 +445,31 @@ class Transition(_PairOp):
         self.expand_b = nn.Linear(d_hidden, n * d_hidden, bias=False)
         self.squeeze = nn.Linear(n * d_hidden, d_hidden, bias=False)
 
+    def set_checkpoint(self, name: str | None) -> None:
+        self.checkpoint = training.check_name(name)
+
+    def _trains(self, x: Tensor) -> bool:
+        return self.checkpoint is not None and training.needs_gradient(self, x)
+
+    def _training_reason(self, x: Tensor) -> str | None:
+        if x.dtype != torch.bfloat16:
+            return f"activations are {x.dtype}; the b200 gradient takes bf16 (master precision)"
+        if self.d % 8 or self.n * self.d % 16 or self.d > MAX_TRAINED_CHANNELS:
+            return f"widths ({self.d}, {self.n} x {self.d}) (the b200 gradient takes a multiple of 8)"
+        return training.capture_reason()
+
     def unsupported(self, x: Tensor, key_mask: Tensor | None = None) -> str | None:
         if self.backend == "pytorch":
             return None
-        reason = _cuda_reason(x, key_mask) or _library_reason()
+        trains = self._trains(x)
+        reason = (_device_reason(x, key_mask) if trains else _cuda_reason(x, key_mask)) or _library_reason()
         if reason:
             return reason
         if x.dtype not in (torch.bfloat16, torch.float32):
             return f"activations are {x.dtype}; the b200 kernels take bf16 (master) or fp32"
+        reason = self._training_reason(x) if trains else None
+        if reason:
+            return reason
         if key_mask is None:
             return None if x.dim() >= 2 else f"transition input {tuple(x.shape)} has no rows"
         if x.dim() == 4 and x.shape[1] != x.shape[2] or x.dim() not in (3, 4):
@@ -454,6 +502,17 @@ class Transition(_PairOp):
 
     @honours_dead
     def _forward_b200(self, x: Tensor, key_mask: Tensor | None = None) -> Tensor:
+        if not self._trains(x):
+            return self._run_b200(x, key_mask)
+        mask = None
+        if self._masked_zero() and key_mask is not None:
+            mask = key_mask.bool()
+            if x.dim() == 4:
+                mask = mask[:, :, None] & mask[:, None, :]
+        weights = (self.ln_in.weight, self.ln_in.bias, self.expand_a.weight, self.expand_b.weight, self.squeeze.weight)
+        return training.transition(x, mask, lambda t: self._run_b200(t, key_mask), self.checkpoint, self.ln_in.eps, *weights)
+
+    def _run_b200(self, x: Tensor, key_mask: Tensor | None) -> Tensor:
         from foldforge_b200 import kernels
 
         if not self._tensor_cores(x):
