@@ -7,6 +7,8 @@ missing or unloadable library raises :class:`LibraryMissing` at the first call.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 from pathlib import Path
 
@@ -185,6 +187,29 @@ def load() -> ctypes.CDLL:
             fn.restype = c_int
     _lib = lib
     return lib
+
+
+_binding = None
+
+
+def binding():
+    """The compiled torch-facing calls (``_binding.so``), bound to the loaded library's entry points."""
+    global _binding
+    if _binding is not None:
+        return _binding
+    path = _HERE / "_binding.so"
+    if not path.exists():
+        raise LibraryMissing(f"{path} is not built; run `python -m foldforge_b200.csrc.build`")
+    lib = load()
+    loader = importlib.machinery.ExtensionFileLoader("foldforge_b200._binding", str(path))
+    try:
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("foldforge_b200._binding", loader))
+        loader.exec_module(module)
+    except ImportError as exc:  # pragma: no cover - depends on the machine
+        raise LibraryMissing(f"cannot load {path}: {exc}") from exc
+    module.bind({name: ctypes.cast(getattr(lib, name), c_void_p).value for name in SIGNATURES})
+    _binding = module
+    return module
 
 
 #: kernels each forward entry point launches (the bench's count of this library's launches)

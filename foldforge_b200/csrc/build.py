@@ -16,6 +16,7 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 PKG = HERE.parent
 OUT = PKG / "_ffb.so"
+BINDING = PKG / "_binding.so"
 BUILD = PKG.parent / "_build"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr", "-Xptxas", "-v"]
@@ -55,7 +56,32 @@ def build(verbose: bool = False) -> Path:
         if res.returncode != 0:
             sys.stderr.write(res.stdout + res.stderr)
             raise RuntimeError("nvcc link failed")
+    build_binding()
     return OUT
+
+
+def build_binding() -> Path:
+    """``foldforge_b200/_binding.so``: the torch-facing calls of ``binding.cpp``, against the installed torch."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    src, header = HERE / "binding.cpp", PKG.parent / "include" / "foldforge_b200.h"
+    newest = max(src.stat().st_mtime, header.stat().st_mtime, Path(torch.__file__).stat().st_mtime)
+    if BINDING.exists() and BINDING.stat().st_mtime >= newest:
+        return BINDING
+    includes = [*cpp_extension.include_paths(), "/usr/local/cuda/include", sysconfig.get_paths()["include"]]
+    libs = Path(torch.__file__).parent / "lib"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_API_INCLUDE_EXTENSION_H",
+           *[f"-I{p}" for p in includes], str(src), "-o", str(BINDING), f"-L{libs}", f"-Wl,-rpath,{libs}", "-lc10", "-lc10_cuda",
+           "-ltorch_cpu", "-ltorch_python", "-ltorch"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError("the compiler failed on binding.cpp")
+    return BINDING
 
 
 if __name__ == "__main__":

@@ -504,13 +504,10 @@ def dit_forward(x: Tensor, mask: Tensor, packed: Tensor, tables: Tensor, *, work
 
 
 # --------------------------------------------------------------------------- training operators
-# csrc/train.cu, csrc/wgrad.cu. These return plain tensors outside autograd; the engine modules put
-# them behind autograd (``checkpoint`` of LayerNorm and Transition). The smallest calls take as long as
-# the host needs to issue them, so these wrappers pass ``data_ptr()`` as it is (``None``: absent;
-# ``ctypes`` converts both), take the stream's handle without a Stream object, and allocate little.
+# csrc/train.cu, csrc/wgrad.cu behind csrc/binding.cpp, which checks the tensors, makes the outputs and
+# calls the C ABI on the tensors' device and its current stream. These return plain tensors outside
+# autograd; the engine modules put them behind autograd (``checkpoint`` of LayerNorm and Transition).
 MX_BLOCK = 32  # channels that share a scale
-MAX_NORM_CHANNELS = 8192
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # absent from a build without CUDA
 
 
 class Checkpoint8(NamedTuple):
@@ -530,7 +527,7 @@ class Checkpoint8(NamedTuple):
     @property
     def scales(self) -> Tensor:
         """``[..., ceil(c / 32)]`` uint8"""
-        first, blocks = _scales_at(self.shape.numel()), -(-self.shape[-1] // MX_BLOCK)
+        first, blocks = -(-self.shape.numel() // 16) * 16, -(-self.shape[-1] // MX_BLOCK)
         return self.data[first:].view(*self.shape[:-1], blocks)
 
 
@@ -542,124 +539,33 @@ class LayerNormSaved(NamedTuple):
     stats: Tensor
 
 
-def _refuse(name: str, message: str):
-    raise _lib.UnsupportedCall(name, 2, message)
-
-
-def _on_device(t: Tensor, name: str, *args) -> None:
-    """Call an entry point on ``t``'s device, on that device's current stream."""
-    index = t.device.index
-    if index == torch.cuda.current_device():
-        _lib.call(name, *args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            _lib.call(name, *args, _raw_stream(index))
-
-
-def _dense(t: Tensor) -> Tensor:
-    """``t`` outside autograd, dense."""
-    if t.requires_grad:
-        t = t.detach()
-    return t if t.is_contiguous() else t.contiguous()
-
-
-def _train_input(name: str, x: Tensor, dtypes=_DTYPES) -> Tensor:
-    _need_cuda(x)
-    if x.dtype not in dtypes:
-        _refuse(name, f"dtype {x.dtype} (takes {', '.join(str(d) for d in dtypes)})")
-    if x.dim() == 0 or x.shape[-1] == 0:
-        _refuse(name, f"shape {tuple(x.shape)} has no channels")
-    return _dense(x)
-
-
-def _beside(name: str, what: str, x: Tensor, t: Tensor, shape, dtype: torch.dtype) -> Tensor:
-    """``t``, which has to lie on ``x``'s device with this shape and dtype, dense."""
-    if t.shape != shape or t.dtype != dtype or t.device != x.device:
-        _refuse(name, f"{what} is {t.dtype} {tuple(t.shape)} on {t.device}, not {dtype} {tuple(shape)} on {x.device}")
-    return _dense(t)
-
-
-def _vector(name: str, what: str, x: Tensor, t: Tensor) -> Tensor:
-    """A norm's weight or bias beside ``x [..., c]``, in fp32."""
-    if t.shape != x.shape[-1:] or t.device != x.device or not t.is_floating_point():
-        _refuse(name, f"{what} is {t.dtype} {tuple(t.shape)} on {t.device}, beside {tuple(x.shape)} on {x.device}")
-    return t if t.dtype == torch.float32 and t.is_contiguous() else _f32(t)
-
-
-def _at(t: Tensor | None) -> int | None:
-    return None if t is None else t.data_ptr()
-
-
-def _scales_at(codes: int) -> int:
-    """Where a checkpoint's scales start, behind its codes."""
-    return -(-codes // 16) * 16
-
-
-def _checkpoint_bytes(codes: int, c: int) -> int:
-    return _scales_at(codes) + codes // c * -(-c // MX_BLOCK)
-
-
-def _new_checkpoint(x: Tensor) -> Checkpoint8:
-    return Checkpoint8(x.new_empty(_checkpoint_bytes(x.numel(), x.shape[-1]), dtype=torch.uint8), x.shape, x.dtype)
-
-
-def _kept(name: str, x: Tensor, kept: Tensor | Checkpoint8, shape: torch.Size, dtype: torch.dtype):
-    """``(tensor, its address, that of the codes, that of the scales)`` of a kept activation, absent ones
-    ``None``: checked against the shape and dtype it has to have beside ``x``."""
+def _unpacked(name: str, kept: Tensor | Checkpoint8, shape, dtype: torch.dtype) -> tuple[Tensor, bool]:
+    """A kept activation's tensor and whether it is a checkpoint, one of the shape and dtype it has to have
+    (a tensor's are checked with its device)."""
     if not isinstance(kept, Checkpoint8):
-        kept = _beside(name, "the kept activation", x, kept, shape, dtype)
-        return kept, kept.data_ptr(), None, None
+        return kept, False
     if kept.shape != shape or kept.dtype != dtype:
-        _refuse(name, f"the checkpoint is of a {kept.dtype} {tuple(kept.shape)} activation, not {dtype} {tuple(shape)}")
-    codes = kept.shape.numel()
-    data = _beside(name, "the checkpoint", x, kept.data, (_checkpoint_bytes(codes, shape[-1]),), torch.uint8)
-    at = data.data_ptr()
-    return data, None, at, at + _scales_at(codes)
+        raise _lib.UnsupportedCall(name, 2, f"the checkpoint is of a {kept.dtype} {tuple(kept.shape)} activation, not "
+                                            f"{dtype} {tuple(shape)}")
+    return kept.data, True
 
 
 def checkpoint_pack(x: Tensor) -> Checkpoint8:
     """``x [..., c]`` (bf16 or fp32) as it is kept in 8 bits: 33 bytes for 32 channels."""
-    x = _train_input("checkpoint_pack", x)
-    kept = _new_checkpoint(x)
-    codes, n, c = kept.data.data_ptr(), x.numel(), x.shape[-1]
-    _on_device(x, "ffb_checkpoint_pack", x.data_ptr(), codes, codes + _scales_at(n), n // c, c, _DTYPES[x.dtype])
-    return kept
+    return Checkpoint8(_lib.binding().checkpoint_pack(x), x.shape, x.dtype)
 
 
 def checkpoint_unpack(kept: Checkpoint8) -> Tensor:
     """The activation a checkpoint stands for, in the dtype it had."""
-    name = "checkpoint_unpack"
-    _need_cuda(kept.data)
-    if kept.dtype not in _DTYPES or len(kept.shape) == 0 or kept.shape[-1] == 0:
-        _refuse(name, f"of a {kept.dtype} {tuple(kept.shape)} activation")
-    data, _, codes, scales = _kept(name, kept.data, kept, kept.shape, kept.dtype)
-    x = data.new_empty(kept.shape, dtype=kept.dtype)
-    c = kept.shape[-1]
-    _on_device(data, "ffb_checkpoint_unpack", codes, scales, x.data_ptr(), x.numel() // c, c, _DTYPES[kept.dtype])
-    return x
+    return _lib.binding().checkpoint_unpack(*kept)
 
 
 def layer_norm_train(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float = 1e-5, *,
                      checkpoint: bool = False) -> tuple[Tensor, LayerNormSaved]:
     """LayerNorm over the last axis (at most 8192 channels) and what its backward pass reads: the input
     itself (which may not change until then), or with ``checkpoint`` its 8-bit checkpoint."""
-    name = "layer_norm_train"
-    x = _train_input(name, x)
-    w = None if weight is None else _vector(name, "weight", x, weight)
-    b = None if bias is None else _vector(name, "bias", x, bias)
-    n, c = x.numel(), x.shape[-1]
-    rows = n // c
-    y = torch.empty_like(x)
-    stats = x.new_empty((2, rows), dtype=torch.float32) if w is None else w.new_empty((2, rows))
-    mean = stats.data_ptr()
-    kept, codes, scales = x, None, None
-    if checkpoint:
-        kept = _new_checkpoint(x)
-        codes = kept.data.data_ptr()
-        scales = codes + _scales_at(n)
-    _on_device(x, "ffb_layernorm_train_fwd", x.data_ptr(), y.data_ptr(), _at(w), _at(b), mean, mean + 4 * rows, codes,
-               scales, rows, c, eps, _DTYPES[x.dtype])
-    return y, LayerNormSaved(kept, stats)
+    y, kept, stats = _lib.binding().layer_norm_train(x, weight, bias, eps, checkpoint)
+    return y, LayerNormSaved(Checkpoint8(kept, x.shape, x.dtype) if checkpoint else kept, stats)
 
 
 def layer_norm_backward(dy: Tensor, saved: LayerNormSaved, weight: Tensor | None, *, bias: bool = True,
@@ -667,84 +573,29 @@ def layer_norm_backward(dy: Tensor, saved: LayerNormSaved, weight: Tensor | None
     """``(dx, dweight, dbias)`` of :func:`layer_norm_train`: ``dx`` (plus ``residual``, the gradient that
     reaches x around the norm) in ``dy``'s dtype, the others fp32, reduced over the rows in a fixed order
     (``None`` without ``weight`` / ``bias``)."""
-    name = "layer_norm_backward"
-    dy = _train_input(name, dy)
-    c = dy.shape[-1]
-    rows = dy.numel() // c
-    kept, x, codes, scales = _kept(name, dy, saved.x, dy.shape, dy.dtype)
-    stats = _beside(name, "stats", dy, saved.stats, (2, rows), torch.float32)
-    w = None if weight is None else _vector(name, "weight", dy, weight)
-    if residual is not None:
-        residual = _beside(name, "residual", dy, residual, dy.shape, dy.dtype)
-    dx = torch.empty_like(dy)
-    dweight = None if w is None else stats.new_empty(c)
-    dbias = stats.new_empty(c) if bias else None
-    dtype = _DTYPES[dy.dtype]
-    size = _lib.load().ffb_layernorm_bwd_workspace_bytes(rows, c, dtype)
-    ws = stats.new_empty(size, dtype=torch.uint8) if size else None
-    mean = stats.data_ptr()
-    _on_device(dy, "ffb_layernorm_bwd", dy.data_ptr(), x, codes, scales, mean, mean + 4 * rows, _at(w), _at(residual),
-               dx.data_ptr(), _at(dweight), _at(dbias), _at(ws), size, rows, c, dtype)
-    return dx, dweight, dbias
-
-
-def _aligned(t: Tensor) -> Tensor:
-    """``t`` from a 16-byte boundary on (a copy of a view that is not)."""
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    kept, packed = _unpacked("layer_norm_backward", saved.x, dy.shape, dy.dtype)
+    return _lib.binding().layer_norm_backward(dy, kept, packed, saved.stats, weight, bias, residual)
 
 
 def weight_grad(dy: Tensor, x: Tensor | Checkpoint8) -> Tensor:
     """A linear layer's weight gradient ``dy^T x`` (fp32, ``[n, k]``) over every leading axis: ``dy [..., n]``
     bf16, ``x [..., k]`` bf16 or its checkpoint."""
-    name = "weight_grad"
-    dy = _train_input(name, dy, (torch.bfloat16,))
-    shape = x.shape
-    if len(shape) == 0 or shape[-1] == 0 or shape[:-1] != dy.shape[:-1]:
-        _refuse(name, f"rows of dy {tuple(dy.shape)} and x {tuple(shape)}")
-    n, k = dy.shape[-1], shape[-1]
-    rows = dy.numel() // n
-    if isinstance(x, Checkpoint8):
-        x = x._replace(data=_aligned(x.data))
-    kept, at, codes, scales = _kept(name, dy, x, shape, torch.bfloat16)
-    dy = _aligned(dy)
-    if at is not None:
-        kept = _aligned(kept)
-        at = kept.data_ptr()
-    dw = dy.new_empty((n, k), dtype=torch.float32)
-    size = _lib.load().ffb_weight_grad_workspace_bytes(rows, n, k, codes is not None)
-    ws = dy.new_empty(size, dtype=torch.uint8) if size else None
-    _on_device(dy, "ffb_weight_grad", dy.data_ptr(), at, codes, scales, dw.data_ptr(), _at(ws), size, rows, n, k)
-    return dw
+    packed = isinstance(x, Checkpoint8)
+    return _lib.binding().weight_grad(dy, x.data if packed else x, packed, x.shape, x.dtype)
 
 
 def swiglu_train(ab: Tensor, *, checkpoint: bool = False) -> tuple[Tensor, Tensor | Checkpoint8]:
     """``silu(a) b [..., h]`` of ``ab [..., 2 h] = [a | b]`` (bf16 or fp32) and what its backward pass
     reads: ``ab`` itself (which may not change until then), or with ``checkpoint`` its 8-bit checkpoint."""
-    name = "swiglu_train"
-    ab = _train_input(name, ab)
-    n, c = ab.numel(), ab.shape[-1]
-    if c % 2:
-        _refuse(name, f"{c} channels are not [a | b]")
-    out = ab.new_empty((*ab.shape[:-1], c // 2))
-    kept, codes, scales = ab, None, None
-    if checkpoint:
-        kept = _new_checkpoint(ab)
-        codes = kept.data.data_ptr()
-        scales = codes + _scales_at(n)
-    _on_device(ab, "ffb_swiglu_train_fwd", ab.data_ptr(), out.data_ptr(), codes, scales, n // c, c // 2, _DTYPES[ab.dtype])
-    return out, kept
+    out, kept = _lib.binding().swiglu_train(ab, checkpoint)
+    return out, Checkpoint8(kept, ab.shape, ab.dtype) if checkpoint else kept
 
 
 def swiglu_backward(dh: Tensor, saved: Tensor | Checkpoint8, *, output: bool = False):
     """``dab [..., 2 h]`` of :func:`swiglu_train` from ``dh [..., h]``; with ``output`` also ``silu(a) b``
     again, as the squeeze's weight gradient needs it: ``(dab, h)``."""
-    name = "swiglu_backward"
-    dh = _train_input(name, dh)
-    h = dh.shape[-1]
-    shape = torch.Size((*dh.shape[:-1], 2 * h))
-    kept, ab, codes, scales = _kept(name, dh, saved, shape, dh.dtype)
-    dab = dh.new_empty(shape)
-    out = torch.empty_like(dh) if output else None
-    _on_device(dh, "ffb_swiglu_bwd", dh.data_ptr(), ab, codes, scales, dab.data_ptr(), _at(out), dh.numel() // h, h,
-               _DTYPES[dh.dtype])
+    kept, packed = saved, False
+    if isinstance(saved, Checkpoint8):
+        kept, packed = _unpacked("swiglu_backward", saved, (*dh.shape[:-1], 2 * dh.shape[-1]) if dh.dim() else (), dh.dtype)
+    dab, out = _lib.binding().swiglu_backward(dh, kept, packed, output)
     return (dab, out) if output else dab
