@@ -223,31 +223,33 @@ __device__ __forceinline__ Lanes<VEC> mx_codes_value(const typename MxCodes<VEC>
 
 // Eight codes times their scale as bf16, exactly (e4m3's 4 significant bits fit bf16's 8; only below 2^-126
 // may the result round). A code's exponent and mantissa, moved to bf16's fields as they are, stand for the
-// value times 2^-120 (biases 7 and 127), subnormal codes included; two multiplications by powers of two,
-// 2^120 and the scale, restore it (their product alone may leave bf16's range). Integer and paired bf16
-// operations only: the conversion instruction runs at a fraction of their rate.
+// value times 2^-120 (biases 7 and 127), subnormal codes included; a multiplication by 2^(byte - 7) makes
+// the value of it. Integer and paired bf16 operations only: the conversion instruction runs at a fraction
+// of their rate.
 __device__ __forceinline__ uint4 mx_decode_bf16(uint2 codes, uint32_t byte) {
   const uint32_t c[2] = {codes.x, codes.y};
   uint32_t w[4];
-  const uint32_t s16 = byte != 0 ? byte << 7 : 0x0040u;  // 2^(byte - 127) in bf16
-  const uint32_t scale = s16 | (s16 << 16);
+  const uint32_t scale = (byte + 120u) * 0x00800080u;  // 2^(byte - 7) twice, for bytes up to 134
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t t = __byte_perm(c[i / 2], 0, i & 1 ? 0x3424 : 0x1404);  // each code in the high byte of its half
-    uint32_t v = (t & 0x80008000u) | ((t >> 4) & 0x07F007F0u);
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(v) : "r"(v), "r"(0x7B807B80u));  // 2^120
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(v) : "r"(v), "r"(scale));
-    w[i] = v;
+    w[i] = (t & 0x80008000u) | ((t >> 4) & 0x07F007F0u);
   }
-  // NaN codes (all seven bits set)
+  // NaN codes (all seven bits set), or a scale of more than 2^7, whose product with 2^120 is past bf16's range
   const uint32_t n0 = ((c[0] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u, n1 = ((c[1] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-  if (n0 | n1) {
+  if ((n0 | n1) != 0 || byte > 134u) {
+    const uint32_t s16 = byte != 0 ? byte << 7 : 0x0040u;  // 2^(byte - 127) in bf16
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(w[i]) : "r"(w[i]), "r"(0x7B807B80u));  // 2^120
+      asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(w[i]) : "r"(w[i]), "r"(s16 | (s16 << 16)));
       const uint32_t n = (i < 2 ? n0 : n1) >> (16 * (i & 1));
       if (n & 0x80u) w[i] |= 0x00007FFFu;
       if (n & 0x8000u) w[i] |= 0x7FFF0000u;
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(w[i]) : "r"(w[i]), "r"(scale));
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }

@@ -365,9 +365,14 @@ __global__ void __launch_bounds__(kWgradThreads, 1)
     const int nn = n0 + group * kMine % BN;
     if (kk < p.k) {
       float* o = p.out + (static_cast<int64_t>(blockIdx.y) * p.n + nn) * p.k + kk;  // one split: split 0
+      if (nn + kMine <= p.n) {
 #pragma unroll
-      for (int i = 0; i < kMine; ++i)
-        if (nn + i < p.n) o[static_cast<int64_t>(i) * p.k] = acc[i];
+        for (int i = 0; i < kMine; ++i, o += p.k) *o = acc[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < kMine; ++i, o += p.k)
+          if (nn + i < p.n) *o = acc[i];
+      }
     }
   }
   tc_fence_before();
