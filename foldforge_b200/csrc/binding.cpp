@@ -59,6 +59,9 @@ int dtype_of(at::ScalarType t) { return t == at::kFloat ? FFB_F32 : FFB_BF16; }
 // Outside autograd and dense. (Called under a guard that records nothing.)
 Tensor dense(const Tensor& t) { return t.is_contiguous() ? t : t.contiguous(); }
 
+// a copy of a view that does not start on a 16-byte boundary
+Tensor aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone(); }
+
 // The first tensor of a call: bf16 (or fp32) rows of at least one channel on a CUDA device.
 Tensor rows_of(const char* name, const Tensor& x, bool fp32 = true) {
   if (x.scalar_type() != at::kBFloat16 && !(fp32 && x.scalar_type() == at::kFloat))
@@ -82,7 +85,7 @@ Tensor beside(const char* name, const char* what, const Tensor& x, const Tensor&
 Tensor vector(const char* name, const char* what, const Tensor& x, const Tensor& t) {
   if (t.dim() != 1 || t.size(0) != x.size(-1) || t.device() != x.device() || !t.is_floating_point())
     refuse(name, std::string(what) + " is " + text(t) + ", beside " + text(x));
-  return t.scalar_type() == at::kFloat ? dense(t) : t.to(at::kFloat).contiguous();
+  return aligned(t.scalar_type() == at::kFloat ? dense(t) : t.to(at::kFloat).contiguous());
 }
 
 Tensor bytes(const Tensor& x, int64_t n) { return at::empty({n}, x.options().dtype(at::kByte).requires_grad(false)); }
@@ -154,7 +157,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_train(const Tensor& x_in, const Op
                                                     bool checkpoint) {
   at::NoGradGuard no_grad;
   const char* name = "layer_norm_train";
-  Tensor x = rows_of(name, x_in);
+  const Tensor x = aligned(rows_of(name, x_in));
   OptTensor w, b;
   if (weight) w = vector(name, "weight", x, *weight);
   if (bias) b = vector(name, "bias", x, *bias);
@@ -179,13 +182,14 @@ std::tuple<Tensor, OptTensor, OptTensor> layer_norm_backward(const Tensor& dy_in
                                                              const OptTensor& weight, bool bias, const OptTensor& residual_in) {
   at::NoGradGuard no_grad;
   const char* name = "layer_norm_backward";
-  const Tensor dy = rows_of(name, dy_in);
+  const Tensor dy = aligned(rows_of(name, dy_in));
   const int64_t c = dy.size(-1), rows = dy.numel() / c;
-  const Kept k = kept_of(name, dy, kept, checkpoint, dy.sizes(), dy.scalar_type());
+  kept_of(name, dy, kept, checkpoint, dy.sizes(), dy.scalar_type());
+  const Kept k = kept_of(name, dy, aligned(dense(kept)), checkpoint, dy.sizes(), dy.scalar_type());
   const Tensor stats = beside(name, "stats", dy, stats_in, {2, rows}, at::kFloat);
   OptTensor w, residual, dweight, dbias, ws;
   if (weight) w = vector(name, "weight", dy, *weight);
-  if (residual_in) residual = beside(name, "residual", dy, *residual_in, dy.sizes(), dy.scalar_type());
+  if (residual_in) residual = aligned(beside(name, "residual", dy, *residual_in, dy.sizes(), dy.scalar_type()));
   need_cuda(name, dy);
   Call call(dy);
   const Tensor dx = like(dy, dy.sizes());
@@ -200,9 +204,6 @@ std::tuple<Tensor, OptTensor, OptTensor> layer_norm_backward(const Tensor& dy_in
                                     ws ? ws->data_ptr() : nullptr, size, rows, static_cast<int>(c), dtype, call.stream));
   return {dx, dweight, dbias};
 }
-
-// a copy of a view that does not start on a 16-byte boundary
-Tensor aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone(); }
 
 Tensor weight_grad(const Tensor& dy_in, const Tensor& kept, bool checkpoint, const std::vector<int64_t>& shape, at::ScalarType dtype) {
   at::NoGradGuard no_grad;

@@ -1,10 +1,12 @@
 // Training operators bound by memory: LayerNorm forward and backward, the 8-bit checkpoint
 // (mx8.cuh) packed and read back, and the gated unit silu(a) b forward and backward.
+#include <initializer_list>
 #include <type_traits>
 
 #include "abi_util.h"
 #include "common.cuh"
 #include "kernels.h"
+#include "launch.cuh"
 #include "mx8.cuh"
 
 namespace ffb {
@@ -40,87 +42,7 @@ __device__ __forceinline__ void group_sum(float (&v)[NSUM], float* scratch, int&
   }
 }
 
-// ------------------------------------------------------------------ LayerNorm forward
-// GROUP threads hold U rows in registers (NV vectors of VEC channels a thread and row), so that U rows'
-// loads are in flight at once; mean and variance in two passes over the registers, one read and one
-// write an element. Writes each row's mean and 1 / sqrt(var + eps) in fp32 for the backward pass and,
-// with `codes`, the input's 8-bit checkpoint.
-template <typename T, int VEC, int NV, int GROUP, int U>
-__global__ void __launch_bounds__(kThreads)
-    ln_train_kernel(const T* __restrict__ x, T* __restrict__ y, const float* __restrict__ gamma,
-                    const float* __restrict__ beta, float* __restrict__ mean_out, float* __restrict__ rstd_out,
-                    uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t rows, int c, float eps) {
-  constexpr int kGroups = kThreads / GROUP;
-  constexpr int kLanes = kMxBlock / VEC;  // lanes that share a block of 32 channels
-  __shared__ float scratch[2 * U * kWarps];
-  int turn = 0;
-  const int t = threadIdx.x % GROUP;
-  const int blocks = (c + kMxBlock - 1) / kMxBlock;
-  const float inv_c = 1.0f / static_cast<float>(c);
-  // rows row0 + u * kGroups; every thread takes part in the shuffles and barriers, row or not
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kGroups * U) + threadIdx.x / GROUP;
-  typename Raw<T, VEC>::type v[U][NV];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int64_t row = row0 + u * kGroups;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int col = (i * GROUP + t) * VEC;
-      v[u][i] = row < rows && col < c ? load_raw<T, VEC>(x + row * c + col) : zero_raw<T, VEC>();
-    }
-  }
-  float mean[U], rstd[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    mean[u] = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) mean[u] += widen<T, VEC>(v[u][i]).sum();
-  }
-  group_sum<GROUP>(mean, scratch, turn);
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    mean[u] *= inv_c;
-    rstd[u] = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const Lanes<VEC> d = widen<T, VEC>(v[u][i]) + Lanes<VEC>(-mean[u]);
-      rstd[u] += (i * GROUP + t) * VEC < c ? (d * d).sum() : 0.f;
-    }
-  }
-  group_sum<GROUP>(rstd, scratch, turn);
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    rstd[u] = rsqrtf(rstd[u] * inv_c + eps);
-    const int64_t row = row0 + u * kGroups;
-    if (t == 0 && row < rows) {
-      mean_out[row] = mean[u];
-      rstd_out[row] = rstd[u];
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int col = (i * GROUP + t) * VEC;
-    const Lanes<VEC> w = col < c && gamma != nullptr ? load_weight<VEC>(gamma + col) : Lanes<VEC>(1.f);
-    const Lanes<VEC> b = col < c && beta != nullptr ? load_weight<VEC>(beta + col) : Lanes<VEC>(0.f);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t row = row0 + u * kGroups;
-      const bool in = row < rows && col < c;
-      const Lanes<VEC> f = widen<T, VEC>(v[u][i]);
-      if (codes != nullptr) {
-        uint32_t byte;
-        const auto q = mx_quantise<T, VEC>(v[u][i], f, byte);
-        if (in) {
-          *reinterpret_cast<typename MxCodes<VEC>::type*>(codes + row * c + col) = q;
-          if (t % kLanes == 0) scales[row * blocks + col / kMxBlock] = static_cast<uint8_t>(byte);
-        }
-      }
-      if (in)
-        store_lanes<T, VEC>(y + row * c + col, fma((f + Lanes<VEC>(-mean[u])) * Lanes<VEC>(rstd[u]), w, b));
-    }
-  }
-}
-
+// ------------------------------------------------------------------ LayerNorm
 // The block's sums of each channel over its rows (dg, db: a thread's, over the rows it took) to row
 // blockIdx.x of the partial sums. `space` holds kWarps NV GROUP VEC floats unless the whole block shares
 // each row, and nobody uses it any more once the block has come here.
@@ -128,6 +50,7 @@ template <int VEC, int NV, int GROUP>
 __device__ __forceinline__ void write_column_sums(Lanes<VEC> (&dg)[NV], Lanes<VEC> (&db)[NV], float* dgamma, float* dbeta,
                                                   int64_t partial_stride, int c, float* space) {
   if (dgamma == nullptr && dbeta == nullptr) return;
+  let_next_kernel_start();
   const int t = threadIdx.x % GROUP;
   float* pg = dgamma == nullptr ? nullptr : dgamma + blockIdx.x * partial_stride;
   float* pb = dbeta == nullptr ? nullptr : dbeta + blockIdx.x * partial_stride;
@@ -175,113 +98,11 @@ __device__ __forceinline__ void write_column_sums(Lanes<VEC> (&dg)[NV], Lanes<VE
   }
 }
 
-// ------------------------------------------------------------------ LayerNorm backward
-// xh = (x - mean) rstd, w = gamma dy: dx = rstd (w - mean(w) - xh mean(w xh)) (+ residual). As above U
-// rows of a group are in flight at once. A thread keeps the same channels for every row it takes, so
-// the sums dgamma = sum dy xh and dbeta = sum dy stay in its registers until the end; the block's row
-// groups are then added in a fixed order and each block writes one row of partial sums, which
-// ln_grad_reduce_kernel adds in a fixed order: the result does not depend on timing.
-template <typename T, int VEC, int NV, int GROUP, int U, bool MX>
-__global__ void __launch_bounds__(kThreads)
-    ln_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const uint8_t* __restrict__ codes,
-                  const uint8_t* __restrict__ scales, const float* __restrict__ mean_in,
-                  const float* __restrict__ rstd_in, const float* __restrict__ gamma, const T* __restrict__ residual,
-                  T* __restrict__ dx, float* __restrict__ dgamma, float* __restrict__ dbeta, int64_t partial_stride,
-                  int64_t rows, int c) {
-  constexpr int kGroups = kThreads / GROUP;
-  using Codes = typename MxCodes<VEC>::type;
-  __shared__ float scratch[4 * U * kWarps];
-  int turn = 0;
-  const int t = threadIdx.x % GROUP;
-  const int blocks = (c + kMxBlock - 1) / kMxBlock;
-  const float inv_c = 1.0f / static_cast<float>(c);
-  Lanes<VEC> dg[NV], db[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) dg[i] = db[i] = Lanes<VEC>(0.f);
-
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * (kGroups * U); base < rows;
-       base += static_cast<int64_t>(gridDim.x) * (kGroups * U)) {
-    const int64_t row0 = base + threadIdx.x / GROUP;
-    typename Raw<T, VEC>::type vd[U][NV], vx[MX ? 1 : U][NV];
-    Codes vc[MX ? U : 1][NV];
-    uint8_t vs[MX ? U : 1][NV];
-    float mean[U], rstd[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t row = row0 + u * kGroups;
-      const bool live = row < rows;
-      mean[u] = live ? mean_in[row] : 0.f;
-      rstd[u] = live ? rstd_in[row] : 0.f;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int col = (i * GROUP + t) * VEC;
-        const bool in = live && col < c;
-        const int64_t at = row * c + col;
-        vd[u][i] = in ? load_raw<T, VEC>(dy + at) : zero_raw<T, VEC>();
-        if constexpr (MX) {
-          vc[u][i] = in ? __ldcs(reinterpret_cast<const Codes*>(codes + at)) : Codes{};
-          vs[u][i] = in ? scales[row * blocks + col / kMxBlock] : 0;
-        } else {
-          vx[u][i] = in ? load_raw<T, VEC>(x + at) : zero_raw<T, VEC>();
-        }
-      }
-    }
-    // The normalised input of row u, vector i. The mean is taken off first: x rstd - mean rstd would leave
-    // rounding errors of mean rstd where a row hardly varies.
-    auto normalised = [&](int u, int i) {
-      const Lanes<VEC> centre(-mean[u]), r(rstd[u]);
-      if constexpr (MX)
-        return fma(mx_codes_value<VEC>(vc[u][i]), Lanes<VEC>(mx_scale(vs[u][i])), centre) * r;
-      else
-        return (widen<T, VEC>(vx[u][i]) + centre) * r;
-    };
-    float s[2 * U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) s[2 * u] = s[2 * u + 1] = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int col = (i * GROUP + t) * VEC;
-      const Lanes<VEC> g = col < c && gamma != nullptr ? load_weight<VEC>(gamma + col) : Lanes<VEC>(1.f);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (row0 + u * kGroups < rows && col < c) {
-          const Lanes<VEC> xh = normalised(u, i), d = widen<T, VEC>(vd[u][i]), w = d * g;
-          dg[i] = fma(d, xh, dg[i]);
-          db[i] = db[i] + d;
-          s[2 * u] += w.sum();
-          s[2 * u + 1] += (w * xh).sum();
-        }
-      }
-    }
-    group_sum<GROUP>(s, scratch, turn);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int col = (i * GROUP + t) * VEC;
-      const Lanes<VEC> g = col < c && gamma != nullptr ? load_weight<VEC>(gamma + col) : Lanes<VEC>(1.f);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int64_t row = row0 + u * kGroups;
-        if (row < rows && col < c) {
-          const float c1 = s[2 * u] * inv_c, c2 = s[2 * u + 1] * inv_c;
-          const int64_t at = row * c + col;
-          const Lanes<VEC> w = widen<T, VEC>(vd[u][i]) * g;
-          Lanes<VEC> o = fma(normalised(u, i), Lanes<VEC>(-c2), w + Lanes<VEC>(-c1)) * Lanes<VEC>(rstd[u]);
-          if (residual != nullptr) o = o + widen<T, VEC>(load_raw<T, VEC>(residual + at));
-          store_lanes<T, VEC>(dx + at, o);
-        }
-      }
-    }
-  }
-  __shared__ float space[GROUP == kThreads ? 1 : kWarps * NV * GROUP * VEC];
-  write_column_sums<VEC, NV, GROUP>(dg, db, dgamma, dbeta, partial_stride, c, space);
-}
-
-// ------------------------------------------------------------------ LayerNorm, rows streamed
-// The same sums where rows are whole 16-byte words (c a multiple of 16): a team (a warp, or the block for
-// rows that a warp's registers cannot hold) takes RS = rows at a time, which lie next to one another in
-// memory, and has them copied to its own ring of kRing slots in shared memory by bulk copies. The loads in
-// flight then do not depend on registers or occupancy, and cost one thread a few instructions.
-constexpr int kRing = 3;
+// Rows are streamed: a team (a warp, or the block for rows that a warp's registers cannot hold) takes RS
+// rows at a time, which lie next to one another in memory, and has them copied to its own ring of slots in
+// shared memory by bulk copies. The loads in flight then do not depend on registers or occupancy, and cost
+// one thread a few instructions.
+constexpr int kRing = 3;  // slots at most
 
 template <int TEAM>
 __device__ __forceinline__ void team_sync() {
@@ -300,18 +121,25 @@ __device__ __forceinline__ bool team_all(bool yes) {
     return __syncthreads_and(yes);
 }
 
-// A team's ring: `streams` tensors with rows of row_bytes[k] bytes; a slot holds RS rows of each, one
-// tensor after the other.
-template <int TEAM, int RS>
+// bytes of a slot for `rows` rows of a tensor: they start at any of 16 bytes, and whole granules are copied
+__host__ __device__ constexpr int slot_part(int rows, int row_bytes) { return (rows * row_bytes + 30) / 16 * 16; }
+
+// A team's ring over `streams` tensors (16-byte aligned, rows of row_bytes[k] bytes); a slot holds RS rows of
+// each, one tensor after the other. WHOLE: rows are whole 16-byte granules in every tensor. Otherwise the
+// copies take the aligned granules around the rows, and the tensor's last bytes, where they do not fill one,
+// are written by the copying thread itself.
+template <int TEAM, int RS, bool WHOLE>
 struct Ring {
   uint8_t* slots;
   uint64_t* full;
+  int depth, slot, phase;  // slots, the one in use and the parity its next copies complete
   int streams, slot_bytes;
   const uint8_t* base[3];
   int row_bytes[3];
   int64_t rows, teams, first;  // this team's chunks of RS rows: first, first + teams, ..
 
-  __device__ __forceinline__ Ring(uint8_t* smem, uint64_t* bars, int64_t all_rows) : streams(0), slot_bytes(0), rows(all_rows) {
+  __device__ __forceinline__ Ring(uint8_t* smem, uint64_t* bars, int slots_of, int64_t all_rows)
+      : depth(slots_of), slot(0), phase(0), streams(0), slot_bytes(0), rows(all_rows) {
     constexpr int kTeams = kThreads / TEAM;
     const int team = threadIdx.x / TEAM;
     slots = smem;
@@ -326,50 +154,96 @@ struct Ring {
   __device__ __forceinline__ void add(const void* p, int bytes) {
     base[streams] = static_cast<const uint8_t*>(p);
     row_bytes[streams] = bytes;
-    slot_bytes += RS * bytes;
+    slot_bytes += part(bytes);
     ++streams;
   }
+  __device__ __forceinline__ static int part(int bytes) { return WHOLE ? RS * bytes : slot_part(RS, bytes); }
   // after the last add: the team's part of shared memory
-  __device__ __forceinline__ void place() { slots += static_cast<int64_t>(threadIdx.x / TEAM) * kRing * slot_bytes; }
+  __device__ __forceinline__ void place() { slots += static_cast<int64_t>(threadIdx.x / TEAM) * depth * slot_bytes; }
   __device__ __forceinline__ int64_t row(int turn) const { return (first + turn * teams) * RS; }
-  // one thread: the copies of the team's chunk number `turn`
-  __device__ __forceinline__ void fetch(int turn) {
+  // one thread: the copies of the team's chunk number `turn` into slot `to`
+  __device__ __forceinline__ void fetch(int turn, int to) {
     const int64_t at = row(turn);
     if (at >= rows) return;
     const int n = rows - at < RS ? static_cast<int>(rows - at) : RS;
-    uint64_t* bar = &full[turn % kRing];
-    uint8_t* dst = slots + turn % kRing * slot_bytes;
-    int bytes = 0;
+    uint64_t* bar = &full[to];
+    uint8_t* dst = slots + to * slot_bytes;
+    if constexpr (WHOLE) {
+      int all = 0;
 #pragma unroll
-    for (int k = 0; k < 3; ++k)
-      if (k < streams) bytes += n * row_bytes[k];
-    mbar_arrive_expect_tx(bar, bytes);
+      for (int k = 0; k < 3; ++k)
+        if (k < streams) all += n * row_bytes[k];
+      mbar_arrive_expect_tx(bar, all);
+#pragma unroll
+      for (int k = 0; k < 3; ++k)
+        if (k < streams) {
+          bulk_load(dst, base[k] + at * row_bytes[k], n * row_bytes[k], bar);
+          dst += RS * row_bytes[k];
+        }
+      return;
+    }
+    uint32_t bytes[3] = {0, 0, 0}, all = 0;
 #pragma unroll
     for (int k = 0; k < 3; ++k)
       if (k < streams) {
-        bulk_load(dst, base[k] + at * row_bytes[k], n * row_bytes[k], bar);
-        dst += RS * row_bytes[k];
+        const uint8_t* a = base[k] + at * row_bytes[k];
+        const uint8_t* stop = a + n * row_bytes[k];
+        const uint8_t* from = a - (reinterpret_cast<uintptr_t>(a) & 15u);
+        const uint8_t* end = base[k] + rows * row_bytes[k];
+        const uint8_t* whole = end - (reinterpret_cast<uintptr_t>(end) & 15u);  // granules past here are not the tensor's alone
+        const uint8_t* to_here = stop + ((16u - (reinterpret_cast<uintptr_t>(stop) & 15u)) & 15u);
+        if (to_here > whole) to_here = whole;
+        for (const uint8_t* q = to_here > from ? to_here : from; q < stop; ++q) dst[q - from] = __ldg(q);
+        bytes[k] = to_here > from ? static_cast<uint32_t>(to_here - from) : 0u;
+        all += bytes[k];
+        dst += slot_part(RS, row_bytes[k]);
       }
+    mbar_arrive_expect_tx(bar, all);
+    dst = slots + to * slot_bytes;
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      if (k < streams) {
+        const uint8_t* a = base[k] + at * row_bytes[k];
+        if (bytes[k] != 0) bulk_load(dst, a - (reinterpret_cast<uintptr_t>(a) & 15u), bytes[k], bar);
+        dst += slot_part(RS, row_bytes[k]);
+      }
+  }
+  __device__ __forceinline__ void start() {
+    for (int i = 0; i < depth; ++i) fetch(i, i);
   }
   // False (for the whole team) where the copies never came: the error word says so, and the other slots'
   // copies have had the same time to land.
-  __device__ __forceinline__ bool wait(int turn, int* err) {
-    return team_all<TEAM>(mbar_wait(&full[turn % kRing], (turn / kRing) & 1, err, kErrTimeoutLoad));
+  __device__ __forceinline__ bool wait(int* err) {
+    return team_all<TEAM>(mbar_wait(&full[slot], phase, err, kErrTimeoutLoad));
   }
-  // row r of a slot's tensor k (whose rows follow those of the tensors before it)
+  // the team has read chunk `turn`: its slot takes a later one
+  __device__ __forceinline__ void next(int turn) {
+    team_sync<TEAM>();
+    if (threadIdx.x % TEAM == 0) fetch(turn + depth, slot);
+    if (++slot == depth) {
+      slot = 0;
+      phase ^= 1;
+    }
+  }
+  // the first row of chunk `turn` in tensor k, whose part of a slot starts at `offset`
   template <typename P>
-  __device__ __forceinline__ const P* at(int turn, int offset) const {
-    return reinterpret_cast<const P*>(slots + turn % kRing * slot_bytes + offset);
+  __device__ __forceinline__ const P* at(int turn, int k, int offset) const {
+    const uint32_t shift = WHOLE ? 0 : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(base[k] + row(turn) * row_bytes[k])) & 15u;
+    return reinterpret_cast<const P*>(slots + slot * slot_bytes + offset + shift);
   }
 };
 
-// FULL: c fills the group's vectors, so that no lane has to look whether its channels are there.
-template <typename T, int VEC, int NV, int GROUP, int U, bool FULL>
+// ROWS says what is known of a row. kFullRows: c fills the group's vectors, so that no lane has to look
+// whether its channels are there; kWholeRows: c is a multiple of 16; kAnyRows: nothing.
+enum Rows : int { kAnyRows, kWholeRows, kFullRows };
+
+template <typename T, int VEC, int NV, int GROUP, int U, Rows ROWS>
 __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
-    ln_train_stream_kernel(const T* __restrict__ x, T* __restrict__ y, const float* __restrict__ gamma,
+    ln_train_kernel(const T* __restrict__ x, T* __restrict__ y, const float* __restrict__ gamma,
                            const float* __restrict__ beta, float* __restrict__ mean_out, float* __restrict__ rstd_out,
                            uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t rows, int c, float eps,
-                           int* err) {
+                           int slots, int* err) {
+  constexpr bool FULL = ROWS == kFullRows;
   constexpr int kTeam = GROUP <= 32 ? 32 : kThreads;
   constexpr int kGroups = kTeam / GROUP;  // rows of a team side by side
   constexpr int RS = kGroups * U;
@@ -379,15 +253,13 @@ __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
   __shared__ float scratch[2 * U * kWarps];
   int turn_of = 0;
   const int t = threadIdx.x % GROUP, g = threadIdx.x % kTeam / GROUP;
-  const bool leader = threadIdx.x % kTeam == 0;
   const int blocks = (c + kMxBlock - 1) / kMxBlock;
   const float inv_c = 1.0f / static_cast<float>(c);
-  Ring<kTeam, RS> ring(smem, bars, rows);
+  Ring<kTeam, RS, (ROWS > 0)> ring(smem, bars, slots, rows);
   ring.add(x, c * static_cast<int>(sizeof(T)));
   ring.place();
   __syncthreads();
-  if (leader)
-    for (int i = 0; i < kRing; ++i) ring.fetch(i);
+  if (threadIdx.x % kTeam == 0) ring.start();
   Lanes<VEC> w[NV], b[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -396,9 +268,9 @@ __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
     b[i] = (FULL || col < c) && beta != nullptr ? load_weight<VEC>(beta + col) : Lanes<VEC>(0.f);
   }
   for (int turn = 0; ring.row(turn) < rows; ++turn) {
-    if (!ring.wait(turn, err)) break;
+    if (!ring.wait(err)) break;
     const int64_t row0 = ring.row(turn) + g;
-    const T* have = ring.template at<T>(turn, 0) + g * c;
+    const T* have = ring.template at<T>(turn, 0, 0) + g * c;
     // a row past the last one reads what the slot held before, and nothing of it is kept
     auto read = [&](int u, int i) {
       const int col = (i * GROUP + t) * VEC;
@@ -480,18 +352,18 @@ __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
         for (int i = 0; i < NV; ++i) finish(v[i], f[i], m[0], r[0], row, i);
       }
     }
-    team_sync<kTeam>();
-    if (leader) ring.fetch(turn + kRing);
+    ring.next(turn);
   }
 }
 
-template <typename T, int VEC, int NV, int GROUP, int U, bool MX, bool FULL>
+template <typename T, int VEC, int NV, int GROUP, int U, bool MX, Rows ROWS>
 __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
-    ln_bwd_stream_kernel(const T* __restrict__ dy, const T* __restrict__ x, const uint8_t* __restrict__ codes,
+    ln_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const uint8_t* __restrict__ codes,
                          const uint8_t* __restrict__ scales, const float* __restrict__ mean_in,
                          const float* __restrict__ rstd_in, const float* __restrict__ gamma,
                          const T* __restrict__ residual, T* __restrict__ dx, float* __restrict__ dgamma,
-                         float* __restrict__ dbeta, int64_t partial_stride, int64_t rows, int c, int* err) {
+                         float* __restrict__ dbeta, int64_t partial_stride, int64_t rows, int c, int slots, int* err) {
+  constexpr bool FULL = ROWS == kFullRows;
   constexpr int kTeam = GROUP <= 32 ? 32 : kThreads;
   constexpr int kGroups = kTeam / GROUP;
   constexpr int RS = kGroups * U;
@@ -501,10 +373,9 @@ __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
   __shared__ float scratch[4 * U * kWarps];
   int turn_of = 0;
   const int t = threadIdx.x % GROUP, g = threadIdx.x % kTeam / GROUP;
-  const bool leader = threadIdx.x % kTeam == 0;
   const int blocks = (c + kMxBlock - 1) / kMxBlock;
   const float inv_c = 1.0f / static_cast<float>(c);
-  Ring<kTeam, RS> ring(smem, bars, rows);
+  Ring<kTeam, RS, (ROWS > 0)> ring(smem, bars, slots, rows);
   ring.add(dy, c * static_cast<int>(sizeof(T)));
   if constexpr (MX)
     ring.add(codes, c);
@@ -513,8 +384,7 @@ __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
   if (residual != nullptr) ring.add(residual, c * static_cast<int>(sizeof(T)));
   ring.place();
   __syncthreads();
-  if (leader)
-    for (int i = 0; i < kRing; ++i) ring.fetch(i);
+  if (threadIdx.x % kTeam == 0) ring.start();
   Lanes<VEC> dg[NV], db[NV], w[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -553,11 +423,12 @@ __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
         for (int i = 0; i < NV; ++i) scaled[u][i] = mx_scale(scale[u][i]);
     }
     load_statistics(ring.row(turn + 1));
-    if (!ring.wait(turn, err)) break;
+    if (!ring.wait(err)) break;
     const int64_t row0 = ring.row(turn) + g;
-    const T* have_dy = ring.template at<T>(turn, 0) + g * c;
-    const uint8_t* have_x = ring.template at<uint8_t>(turn, RS * c * static_cast<int>(sizeof(T)));
-    const T* have_res = ring.template at<T>(turn, RS * c * static_cast<int>(sizeof(T) + (MX ? 1 : sizeof(T)))) + g * c;
+    const int row_bytes = c * static_cast<int>(sizeof(T)), part = ring.part(row_bytes);
+    const T* have_dy = ring.template at<T>(turn, 0, 0) + g * c;
+    const uint8_t* have_x = ring.template at<uint8_t>(turn, 1, part);
+    const T* have_res = residual == nullptr ? nullptr : ring.template at<T>(turn, 2, part + ring.part(MX ? c : row_bytes)) + g * c;
     const bool whole = ring.row(turn) + RS <= rows;  // the same for the team
     // dy and the normalised input of row u, vector i; 0 for a row past the last one (the slot holds what was
     // there before). The mean is taken off first: x rstd - mean rstd would leave rounding errors of mean
@@ -632,11 +503,8 @@ __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
         for (int i = 0; i < NV; ++i) finish(u, i, d[i], xh[i], s[0], s[1]);
       }
     }
-    team_sync<kTeam>();
-    if (leader) ring.fetch(turn + kRing);
+    ring.next(turn);
   }
-  // the rings hold 24 rows or more, at least 72 bytes a channel: room for 32 bytes a lane's channel, of which at
-  // most half lie past the row
   write_column_sums<VEC, NV, GROUP>(dg, db, dgamma, dbeta, partial_stride, c, reinterpret_cast<float*>(smem));
 }
 
@@ -649,6 +517,7 @@ __global__ void __launch_bounds__(1024)
   const int lane = threadIdx.x & 31, r = threadIdx.x / 32;
   const int col = blockIdx.x * 32 + lane;
   float v = 0.f;
+  wait_for_kernel_before();
   if (col < 2 * c)
     for (int p = r; p < parts; p += 32) v += part[static_cast<int64_t>(p) * (2 * c) + col];
   s[r][lane] = v;
@@ -661,17 +530,6 @@ __global__ void __launch_bounds__(1024)
     if (out != nullptr) out[col < c ? col : col - c] = a;
   }
 }
-
-// Division of 32-bit numbers below 2^31 by a fixed one: a multiplication and a shift (Granlund and
-// Montgomery, "Division by invariant integers using multiplication", 1994).
-struct Divisor {
-  uint32_t d, m, shift;
-  __host__ explicit Divisor(uint32_t n) : d(n), shift(0) {
-    while ((uint64_t(1) << shift) < n) ++shift;
-    m = static_cast<uint32_t>(((uint64_t(1) << 32) * ((uint64_t(1) << shift) - n)) / n + 1);
-  }
-  __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return (__umulhi(m, n) + n) >> shift; }
-};
 
 // ------------------------------------------------------------------ 8-bit checkpoints
 // A thread takes VEC channels of U places, a block's width apart, all loaded before the first is used;
@@ -875,13 +733,20 @@ bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0
   return f(std::integral_constant<int, V>{}, std::integral_constant<int, N>{}, std::integral_constant<int, G>{}, \
            std::integral_constant<int, U>{})
 
-// How a row of c channels is held, for rows that are streamed: vectors of 16 bytes, two a thread where the
-// row allows it (fewer threads, fewer shuffles to add them up; more would leave few registers), and U rows
-// of a group at a time so that a chunk is a few KB. Calls f(VEC, NV, GROUP, U as integral constants).
+// How a row of c channels is held: vectors of 16 bytes where it is a whole number of them, two a thread
+// where the row allows it (fewer threads, fewer shuffles to add them up; more would leave few registers),
+// else single elements, 32 lanes side by side; and U rows of a group at a time so that a chunk is a few KB.
+// Calls f(VEC, NV, GROUP, U as integral constants).
 template <typename T, typename F>
-int dispatch_stream(int c, F&& f) {
+int dispatch_row(int c, F&& f) {
   constexpr int kVec = 16 / sizeof(T);
-  if constexpr (kVec == 8) {
+  if (c % kVec != 0) {
+    FFB_ROW(1, 2, 32, 4);
+    FFB_ROW(1, 8, 32, 2);
+    FFB_ROW(1, 32, 32, 1);
+    FFB_ROW(1, 8, kThreads, 2);
+    FFB_ROW(1, 32, kThreads, 1);
+  } else if constexpr (kVec == 8) {
     FFB_ROW(8, 2, 4, 2);
     FFB_ROW(8, 2, 8, 2);
     FFB_ROW(8, 2, 16, 2);
@@ -894,27 +759,9 @@ int dispatch_stream(int c, F&& f) {
     FFB_ROW(4, 2, 16, 2);
     FFB_ROW(4, 2, 32, 2);
     FFB_ROW(4, 4, 32, 1);
-    FFB_ROW(4, 2, kThreads, 2);
+    FFB_ROW(4, 8, 32, 1);
     FFB_ROW(4, 4, kThreads, 1);
     FFB_ROW(4, 8, kThreads, 1);
-  }
-  return static_cast<int>(cudaErrorInvalidValue);
-}
-
-// The same for rows that are not: vectors where every pointer is 16-byte aligned and c a whole number of
-// them, else single elements; the fewest threads that hold a row with at most 32 channels a thread.
-template <typename T, typename F>
-int dispatch_row(int c, bool vector, F&& f) {
-  constexpr int kVec = 16 / sizeof(T);
-  if (vector) {
-    FFB_ROW(kVec, 1, 32, 2);
-    FFB_ROW(kVec, 32 / kVec, 32, 1);
-    FFB_ROW(kVec, 32 / kVec, kThreads, 1);
-  } else {
-    FFB_ROW(1, 2, 32, 4);
-    FFB_ROW(1, 8, 32, 2);
-    FFB_ROW(1, 8, kThreads, 2);
-    FFB_ROW(1, 32, kThreads, 1);
   }
   return static_cast<int>(cudaErrorInvalidValue);
 }
@@ -922,65 +769,55 @@ int dispatch_row(int c, bool vector, F&& f) {
 
 constexpr int kLnBlocks = 148 * 2;  // blocks (rows of partial sums) of the backward pass at most
 
-// Whether rows of c channels are streamed: 16-byte words (every pointer is aligned) of 16 channels, and a
-// block's rings, whose rows take `row_bytes` over all tensors, fit shared memory (fp32 rows of above 6000
-// channels with a residual do not).
-template <typename T>
-bool ln_streams(bool whole, int c, int row_bytes) {
-  int per = 0;
-  dispatch_stream<T>(c, [&](auto, auto, auto g, auto u) {
-    per = kThreads / decltype(g)::value * decltype(u)::value;
-    return 0;
-  });
-  return whole && c % 16 == 0 && static_cast<int64_t>(kRing) * per * row_bytes <= 200 * 1024;
-}
-
-// blocks of a backward pass whose blocks take `per` rows at a time
+// blocks of a launch whose blocks take `per` rows at a time
 int ln_blocks(int64_t rows, int64_t per) {
   const int64_t want = (rows + per - 1) / per;
   return static_cast<int>(want < kLnBlocks ? want : kLnBlocks);
 }
 template <typename T>
-int ln_bwd_blocks(int64_t rows, int c, bool stream, bool vector) {
+int ln_bwd_blocks(int64_t rows, int c) {
   int blocks = 0;
-  auto count = [&](auto, auto, auto g, auto u) {
+  dispatch_row<T>(c, [&](auto, auto, auto g, auto u) {
     blocks = ln_blocks(rows, kThreads / decltype(g)::value * decltype(u)::value);
     return 0;
-  };
-  if (stream)
-    dispatch_stream<T>(c, count);
-  else
-    dispatch_row<T>(c, vector, count);
+  });
   return blocks;
+}
+
+// A launch's shared memory: the teams' rings, three slots deep where they fit (two for fp32 rows of above
+// 6000 channels with a residual), and room for the column sums behind them in time.
+struct LnShared {
+  int slots, bytes;
+};
+template <int V, int N, int G, int U>
+LnShared ln_shared(std::initializer_list<int> row_bytes) {
+  constexpr int team = G <= 32 ? 32 : kThreads, rows = team / G * U;
+  int slot = 0;
+  for (int b : row_bytes)
+    if (b > 0) slot += slot_part(rows, b);
+  slot *= kThreads / team;
+  const int slots = kRing * slot <= 216 * 1024 ? kRing : 2;
+  const int sums = G <= 32 ? kWarps * N * G * V * static_cast<int>(sizeof(float)) : 0;
+  return {slots, slots * slot > sums ? slots * slot : sums};
 }
 
 template <typename T>
 int ln_train(const LayerNormTrain& p, int* err, cudaStream_t stream) {
-  const bool whole = aligned(p.x) && aligned(p.y) && aligned(p.codes) && aligned(p.gamma) && aligned(p.beta);
-  if (ln_streams<T>(whole, p.c, p.c * sizeof(T)))
-    return dispatch_stream<T>(p.c, [&](auto v, auto n, auto g, auto u) {
-      constexpr int V = decltype(v)::value, N = decltype(n)::value, G = decltype(g)::value, U = decltype(u)::value;
-      constexpr int per = kThreads / G * U;  // rows of a block at a time
-      auto kernel = p.c == V * N * G ? ln_train_stream_kernel<T, V, N, G, U, true> : ln_train_stream_kernel<T, V, N, G, U, false>;
-      const int smem = kRing * per * p.c * static_cast<int>(sizeof(T));
-      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-      if (e != cudaSuccess) return static_cast<int>(e);
-      kernel<<<ln_blocks(p.rows, per), kThreads, smem, stream>>>(static_cast<const T*>(p.x), static_cast<T*>(p.y), p.gamma,
-                                                                p.beta, p.mean, p.rstd, p.codes, p.scales, p.rows, p.c,
-                                                                p.eps, err);
-      return static_cast<int>(cudaGetLastError());
-    });
-  return dispatch_row<T>(p.c, whole && p.c % (16 / sizeof(T)) == 0, [&](auto v, auto n, auto g, auto u) {
+  return dispatch_row<T>(p.c, [&](auto v, auto n, auto g, auto u) {
     constexpr int V = decltype(v)::value, N = decltype(n)::value, G = decltype(g)::value, U = decltype(u)::value;
-    constexpr int per = kThreads / G * U;
-    // a launch's grid is 31 bits wide
-    for (int64_t first = 0; first < p.rows; first += int64_t(1) << 30) {
-      const int64_t rows = p.rows - first < (int64_t(1) << 30) ? p.rows - first : int64_t(1) << 30;
-      ln_train_kernel<T, V, N, G, U><<<static_cast<int>((rows + per - 1) / per), kThreads, 0, stream>>>(
-          static_cast<const T*>(p.x) + first * p.c, static_cast<T*>(p.y) + first * p.c, p.gamma, p.beta, p.mean + first,
-          p.rstd + first, p.codes == nullptr ? nullptr : p.codes + first * p.c,
-          p.codes == nullptr ? nullptr : p.scales + first * ((p.c + kMxBlock - 1) / kMxBlock), rows, p.c, p.eps);
+    const LnShared smem = ln_shared<V, N, G, U>({p.c * static_cast<int>(sizeof(T))});
+    auto kernel = ln_train_kernel<T, V, N, G, U, kAnyRows>;
+    if constexpr (V > 1) {
+      if (p.c == V * N * G)
+        kernel = ln_train_kernel<T, V, N, G, U, kFullRows>;
+      else if (p.c % 16 == 0)
+        kernel = ln_train_kernel<T, V, N, G, U, kWholeRows>;
     }
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem.bytes);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    kernel<<<ln_blocks(p.rows, kThreads / G * U), kThreads, smem.bytes, stream>>>(
+        static_cast<const T*>(p.x), static_cast<T*>(p.y), p.gamma, p.beta, p.mean, p.rstd, p.codes, p.scales, p.rows, p.c,
+        p.eps, smem.slots, err);
     return static_cast<int>(cudaGetLastError());
   });
 }
@@ -988,47 +825,33 @@ int ln_train(const LayerNormTrain& p, int* err, cudaStream_t stream) {
 template <typename T>
 int ln_bwd(const LayerNormBwd& p, int* err, cudaStream_t stream) {
   const bool mx = p.codes != nullptr;
-  const bool whole = aligned(p.dy) && aligned(p.dx) && aligned(p.residual) && aligned(p.gamma) &&
-                     aligned(mx ? static_cast<const void*>(p.codes) : p.x);
-  const int row_bytes = p.c * static_cast<int>(sizeof(T)), all_bytes = row_bytes + (mx ? p.c : row_bytes) + (p.residual != nullptr ? row_bytes : 0);
-  const bool streamed = ln_streams<T>(whole, p.c, all_bytes), vector = whole && p.c % (16 / sizeof(T)) == 0;
-  const int grid = ln_bwd_blocks<T>(p.rows, p.c, streamed, vector);
+  const int grid = ln_bwd_blocks<T>(p.rows, p.c);
   const bool sums = p.dgamma != nullptr || p.dbeta != nullptr;
   // one block writes the gradients itself; several leave rows [dgamma | dbeta] of partial sums
   float* part = static_cast<float*>(p.workspace);
   float* dg = !sums ? nullptr : grid == 1 ? p.dgamma : part;
   float* db = !sums ? nullptr : grid == 1 ? p.dbeta : part + p.c;
-  const int64_t stride = 2 * static_cast<int64_t>(p.c);
-  const T* dy = static_cast<const T*>(p.dy);
-  const T* x = static_cast<const T*>(p.x);
-  const T* residual = static_cast<const T*>(p.residual);
-  T* dx = static_cast<T*>(p.dx);
-  int rc;
-  if (streamed)
-    rc = dispatch_stream<T>(p.c, [&](auto v, auto n, auto g, auto u) {
-      constexpr int V = decltype(v)::value, N = decltype(n)::value, G = decltype(g)::value, U = decltype(u)::value;
-      constexpr int per = kThreads / G * U;
-      const int smem = kRing * per * all_bytes;
-      const bool full = p.c == V * N * G;
-      auto kernel = mx ? full ? ln_bwd_stream_kernel<T, V, N, G, U, true, true> : ln_bwd_stream_kernel<T, V, N, G, U, true, false>
-                       : full ? ln_bwd_stream_kernel<T, V, N, G, U, false, true> : ln_bwd_stream_kernel<T, V, N, G, U, false, false>;
-      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-      if (e != cudaSuccess) return static_cast<int>(e);
-      kernel<<<grid, kThreads, smem, stream>>>(dy, x, p.codes, p.scales, p.mean, p.rstd, p.gamma, residual, dx, dg, db,
-                                               stride, p.rows, p.c, err);
-      return static_cast<int>(cudaGetLastError());
-    });
-  else
-    rc = dispatch_row<T>(p.c, vector, [&](auto v, auto n, auto g, auto u) {
-      constexpr int V = decltype(v)::value, N = decltype(n)::value, G = decltype(g)::value, U = decltype(u)::value;
-      auto kernel = mx ? ln_bwd_kernel<T, V, N, G, U, true> : ln_bwd_kernel<T, V, N, G, U, false>;
-      kernel<<<grid, kThreads, 0, stream>>>(dy, x, p.codes, p.scales, p.mean, p.rstd, p.gamma, residual, dx, dg, db, stride,
-                                            p.rows, p.c);
-      return static_cast<int>(cudaGetLastError());
-    });
+  const int row = p.c * static_cast<int>(sizeof(T));
+  int rc = dispatch_row<T>(p.c, [&](auto v, auto n, auto g, auto u) {
+    constexpr int V = decltype(v)::value, N = decltype(n)::value, G = decltype(g)::value, U = decltype(u)::value;
+    const LnShared smem = ln_shared<V, N, G, U>({row, mx ? p.c : row, p.residual != nullptr ? row : 0});
+    auto kernel = mx ? ln_bwd_kernel<T, V, N, G, U, true, kAnyRows> : ln_bwd_kernel<T, V, N, G, U, false, kAnyRows>;
+    if constexpr (V > 1) {
+      if (p.c == V * N * G)
+        kernel = mx ? ln_bwd_kernel<T, V, N, G, U, true, kFullRows> : ln_bwd_kernel<T, V, N, G, U, false, kFullRows>;
+      else if (p.c % 16 == 0)
+        kernel = mx ? ln_bwd_kernel<T, V, N, G, U, true, kWholeRows> : ln_bwd_kernel<T, V, N, G, U, false, kWholeRows>;
+    }
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem.bytes);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    kernel<<<grid, kThreads, smem.bytes, stream>>>(
+        static_cast<const T*>(p.dy), static_cast<const T*>(p.x), p.codes, p.scales, p.mean, p.rstd, p.gamma,
+        static_cast<const T*>(p.residual), static_cast<T*>(p.dx), dg, db, 2 * static_cast<int64_t>(p.c), p.rows, p.c, smem.slots, err);
+    return static_cast<int>(cudaGetLastError());
+  });
   if (rc == 0 && sums && grid > 1) {
-    ln_grad_reduce_kernel<<<(2 * p.c + 31) / 32, 1024, 0, stream>>>(part, p.dgamma, p.dbeta, grid, p.c);
-    rc = static_cast<int>(cudaGetLastError());
+    rc = launch_after(ln_grad_reduce_kernel, (2 * p.c + 31) / 32, 1024, 0, stream, static_cast<const float*>(part), p.dgamma,
+                      p.dbeta, grid, p.c);
   }
   return rc;
 }
@@ -1140,14 +963,8 @@ int swiglu_bwd(const void* dh, const void* ab, const uint8_t* codes, const uint8
 }  // namespace
 
 size_t ln_bwd_workspace_bytes(int64_t rows, int c, int is_f32) {
-  // the tensors' alignment is not known here: room for the form with the most blocks
-  int most = 0;
-  for (int form = 0; form < 3; ++form) {
-    const bool stream = form == 0, vector = form == 1;
-    const int blocks = is_f32 ? ln_bwd_blocks<float>(rows, c, stream, vector) : ln_bwd_blocks<__nv_bfloat16>(rows, c, stream, vector);
-    if (blocks > most) most = blocks;
-  }
-  return most > 1 ? static_cast<size_t>(most) * 2 * c * sizeof(float) : 0;
+  const int blocks = is_f32 ? ln_bwd_blocks<float>(rows, c) : ln_bwd_blocks<__nv_bfloat16>(rows, c);
+  return blocks > 1 ? static_cast<size_t>(blocks) * 2 * c * sizeof(float) : 0;
 }
 
 int launch_ln_train(const LayerNormTrain& p, int is_f32, int* err, cudaStream_t stream) {

@@ -49,7 +49,7 @@ int ffb_layernorm_train_fwd(const void* x, void* y, const float* gamma, const fl
   if ((codes == nullptr) != (scales == nullptr))
     return fail(FFB_ERR_ARG, "layernorm_train_fwd: codes and scales go together");
   if (x == y) return fail(FFB_ERR_ARG, "layernorm_train_fwd: y must not alias x");
-  if (off_element(x, dtype) || off_element(y, dtype) || off_word(gamma) || off_word(beta) || off_word(mean) || off_word(rstd))
+  if (off_vector(x) || off_vector(y) || off_vector(codes) || off_vector(gamma) || off_vector(beta) || off_word(mean) || off_word(rstd))
     return fail(FFB_ERR_ARG, "layernorm_train_fwd: misaligned pointer");
   DeviceInfo info;
   st = device_info(&info);
@@ -84,8 +84,8 @@ int ffb_layernorm_bwd(const void* dy, const void* x, const uint8_t* codes, const
   if (st != FFB_OK) return st;
   if (!dy || !mean || !rstd || !dx) return fail(FFB_ERR_ARG, "layernorm_bwd: null pointer");
   if (dx == dy || dx == x || dx == residual) return fail(FFB_ERR_ARG, "layernorm_bwd: dx must not alias an input");
-  if (off_element(dy, dtype) || off_element(x, dtype) || off_element(residual, dtype) || off_element(dx, dtype) ||
-      off_word(mean) || off_word(rstd) || off_word(gamma))
+  if (off_vector(dy) || off_vector(x) || off_vector(codes) || off_vector(residual) || off_vector(dx) || off_vector(gamma) ||
+      off_word(mean) || off_word(rstd))
     return fail(FFB_ERR_ARG, "layernorm_bwd: misaligned pointer");
   if (dgamma || dbeta) {
     const size_t need = ln_bwd_workspace_bytes(rows, c, dtype == FFB_F32);

@@ -25,6 +25,7 @@
 #include "abi_util.h"
 #include "common.cuh"
 #include "kernels.h"
+#include "launch.cuh"
 #include "mx8.cuh"
 
 namespace ffb {
@@ -235,6 +236,7 @@ __global__ void __launch_bounds__(kWgradThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s.tmem_base;
+  wait_for_kernel_before();  // the padded copies of the operands, where there are some
 
   const int quarter = warp & 3, group = warp / 4;  // TMEM lanes 32 quarter.., columns kMine group..
   const uint32_t mine = (static_cast<uint32_t>(quarter * 32) << 16) + group * kMine;
@@ -359,6 +361,7 @@ __global__ void __launch_bounds__(kWgradThreads, 1)
     copy_async_wait<0>();
   }
   while (ok && drained < chunks) drain();
+  let_next_kernel_start();
   if (ok) {
     // a lane is a channel of X, a column one of dY: each store of a warp writes 32 neighbours of a row of dW
     const int kk = k0 + (group * kMine / BN) * 128 + quarter * 32 + lane;
@@ -384,43 +387,70 @@ __global__ void __launch_bounds__(kWgradThreads, 1)
 }
 
 // ---- operands that neither TMA nor the fill warps take: bf16 rows of a multiple of 8 channels, the last
-// ones 0, from bf16 rows of any width or from a checkpoint's. A thread writes 8 channels; its
-// reads are single elements, which neighbours take from the same cache lines.
+// ones 0, from bf16 rows of any width or from a checkpoint's (16-byte aligned tensors). A thread writes 8
+// channels: it takes the two aligned words (16 bytes, or 8 of codes) that hold them and shifts.
 struct PadJob {
-  const __nv_bfloat16* x;  // null: from codes / scales
-  const uint8_t* codes;
-  const uint8_t* scales;
+  const uint8_t* from;    // bf16 rows, or codes
+  const uint8_t* scales;  // null: from bf16
   uint4* out;
-  int width, pieces;       // channels of a row, and pieces of 8 of a row of `out`
-  int64_t total;           // pieces of all rows (0: nothing to do)
+  int64_t bytes;          // of `from`
+  int width;
+  uint32_t total;         // pieces of 8 channels of all rows (0: nothing to do)
+  Divisor pieces;         // of a row of `out`
 };
+
+// the aligned word at `at`, put together from its elements where the tensor ends inside it
+template <typename Word, int SIZE>
+__device__ __forceinline__ Word pad_word(const PadJob& j, int64_t at) {
+  if (at + static_cast<int64_t>(sizeof(Word)) <= j.bytes) return __ldg(reinterpret_cast<const Word*>(j.from + at));
+  uint32_t w[sizeof(Word) / 4] = {};
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(Word)); i += SIZE)
+    if (at + i < j.bytes) {
+      const uint32_t e = SIZE == 1 ? static_cast<uint32_t>(__ldg(j.from + at + i))
+                                   : static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(j.from + at + i)));
+      w[i / 4] |= e << (8 * (i & 3));
+    }
+  Word out;
+  memcpy(&out, w, sizeof(out));
+  return out;
+}
 
 __global__ void __launch_bounds__(256) wgrad_pad_kernel(PadJob first, PadJob second) {
   for (int which = 0; which < 2; ++which) {
     const PadJob& j = which == 0 ? first : second;
     const int blocks = (j.width + kMxBlock - 1) / kMxBlock;
-    for (int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; id < j.total; id += static_cast<int64_t>(gridDim.x) * 256) {
-      const int64_t row = id / j.pieces;
-      const int col = static_cast<int>(id - row * j.pieces) * 8;
-      const int64_t at = row * j.width + col;
-      const int left = j.width - col;
-      uint32_t w[4] = {0, 0, 0, 0};
-      if (j.x != nullptr) {
+    for (uint32_t id = blockIdx.x * 256 + threadIdx.x; id < j.total; id += gridDim.x * 256) {
+      const uint32_t row = j.pieces.quotient(id);
+      const int col = static_cast<int>(id - row * j.pieces.d) * 8;
+      const int left = j.width - col;  // channels there are: the others become 0
+      const int64_t at = static_cast<int64_t>(row) * j.width + col;
+      uint4 v;
+      if (j.scales == nullptr) {
+        const uint32_t shift = static_cast<uint32_t>(2 * at) & 15u;
+        const uint4 lo = pad_word<uint4, 2>(j, 2 * at - shift), hi = pad_word<uint4, 2>(j, 2 * at - shift + 16);
+        uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < left) w[i / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(j.x) + at + i)) << (16 * (i & 1));
+        for (int i = 0; i < 6; ++i) w[i] = shift & 8u ? w[i + 2] : w[i];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = shift & 4u ? w[i + 1] : w[i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (shift & 2u) * 8);
+        v = make_uint4(w[0], w[1], w[2], w[3]);
       } else {
-        uint32_t c[2] = {0, 0};
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < left) c[i / 4] |= static_cast<uint32_t>(__ldg(j.codes + at + i)) << (8 * (i & 3));
-        const uint4 v = mx_decode_bf16(make_uint2(c[0], c[1]), __ldg(j.scales + row * blocks + col / kMxBlock));
-        w[0] = v.x;
-        w[1] = v.y;
-        w[2] = v.z;
-        w[3] = v.w;
+        const uint32_t shift = static_cast<uint32_t>(at) & 7u;
+        const uint2 lo = pad_word<uint2, 1>(j, at - shift), hi = pad_word<uint2, 1>(j, at - shift + 8);
+        const uint32_t w0 = shift & 4u ? lo.y : lo.x, w1 = shift & 4u ? hi.x : lo.y, w2 = shift & 4u ? hi.y : hi.x;
+        const uint2 c = make_uint2(__funnelshift_r(w0, w1, (shift & 3u) * 8), __funnelshift_r(w1, w2, (shift & 3u) * 8));
+        v = mx_decode_bf16(c, __ldg(j.scales + static_cast<int64_t>(row) * blocks + col / kMxBlock));
       }
-      j.out[id] = make_uint4(w[0], w[1], w[2], w[3]);
+      if (left < 8) {
+        uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = left >= 2 * i + 2 ? w[i] : left == 2 * i + 1 ? w[i] & 0xFFFFu : 0u;
+        v = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      j.out[id] = v;
     }
   }
 }
@@ -437,6 +467,7 @@ __global__ void __launch_bounds__(256)
   float a[VEC];
 #pragma unroll
   for (int i = 0; i < VEC; ++i) a[i] = 0.f;
+  wait_for_kernel_before();
   if (at < count) {
     const float* p = part + at;
 #pragma unroll 4
@@ -470,15 +501,19 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// Many splits are shared out over the block's warps (a place's sum would wait for one load after another),
-// few are added by one thread.
+// Many splits are shared out over the block's groups of threads (a place's sum would wait for one load after
+// another), few are added by one thread.
+template <int VEC, int GROUPS>
+int launch_reduce(const float* part, float* out, int splits, int64_t count, cudaStream_t stream) {
+  constexpr int places = 256 / GROUPS * VEC;
+  return launch_after(wgrad_reduce_kernel<VEC, GROUPS>, static_cast<unsigned>((count + places - 1) / places), 256, 0, stream, part,
+                      out, splits, count);
+}
 template <int VEC>
-void launch_reduce(const float* part, float* out, int splits, int64_t count, cudaStream_t stream) {
-  const int64_t places = count / VEC;
-  if (splits > 8)
-    wgrad_reduce_kernel<VEC, 8><<<static_cast<int>((places + 31) / 32), 256, 0, stream>>>(part, out, splits, count);
-  else
-    wgrad_reduce_kernel<VEC, 1><<<static_cast<int>((places + 255) / 256), 256, 0, stream>>>(part, out, splits, count);
+int launch_reduce(const float* part, float* out, int splits, int64_t count, cudaStream_t stream) {
+  return splits > 32  ? launch_reduce<VEC, 32>(part, out, splits, count, stream)
+         : splits > 8 ? launch_reduce<VEC, 8>(part, out, splits, count, stream)
+                      : launch_reduce<VEC, 1>(part, out, splits, count, stream);
 }
 
 struct WgradPlan {
@@ -514,21 +549,24 @@ WgradPlan plan(int64_t rows, int n, int k) {
 }
 
 template <int MB, int BN, bool CODES>
-int launch(const CUtensorMap& x, const CUtensorMap& dy, const WgradParams& p, const WgradPlan& plan, cudaStream_t stream) {
+int launch(const CUtensorMap& x, const CUtensorMap& dy, const WgradParams& p, const WgradPlan& plan, bool after, cudaStream_t stream) {
   constexpr size_t smem = sizeof(WgradSmem<MB, BN, CODES>) + 1024;
   static_assert(smem <= 232448, "weight-gradient shared memory exceeds the per-CTA limit");
   auto kernel = wgrad_kernel<MB, BN, CODES>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return static_cast<int>(e);
-  kernel<<<dim3(plan.tiles, plan.splits), kWgradThreads, smem, stream>>>(x, dy, p);
+  const dim3 grid(plan.tiles, plan.splits);
+  if (after) return launch_after(kernel, grid, kWgradThreads, smem, stream, x, dy, p);
+  kernel<<<grid, kWgradThreads, smem, stream>>>(x, dy, p);
   return static_cast<int>(cudaGetLastError());
 }
 
 template <bool CODES>
-int launch_tile(const CUtensorMap& x, const CUtensorMap& dy, const WgradParams& p, const WgradPlan& plan, cudaStream_t s) {
-  if (plan.bn == 256) return launch<1, 256, CODES>(x, dy, p, plan, s);
-  if (plan.mb == 2) return plan.bn == 64 ? launch<2, 64, CODES>(x, dy, p, plan, s) : launch<2, 128, CODES>(x, dy, p, plan, s);
-  return plan.bn == 64 ? launch<1, 64, CODES>(x, dy, p, plan, s) : launch<1, 128, CODES>(x, dy, p, plan, s);
+int launch_tile(const CUtensorMap& x, const CUtensorMap& dy, const WgradParams& p, const WgradPlan& plan, bool after,
+                cudaStream_t s) {
+  if (plan.bn == 256) return launch<1, 256, CODES>(x, dy, p, plan, after, s);
+  if (plan.mb == 2) return plan.bn == 64 ? launch<2, 64, CODES>(x, dy, p, plan, after, s) : launch<2, 128, CODES>(x, dy, p, plan, after, s);
+  return plan.bn == 64 ? launch<1, 64, CODES>(x, dy, p, plan, after, s) : launch<1, 128, CODES>(x, dy, p, plan, after, s);
 }
 
 int panel_map(CUtensorMap* map, const void* base, int64_t rows, int width, int pitch) {
@@ -559,24 +597,41 @@ int weight_grad_forward(const void* dy, const void* x, const uint8_t* codes, con
   const WgradPlan pl = plan(rows, n, k);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   uint8_t* pad = ws + partial_bytes(pl, n, k);
-  PadJob jobs[2] = {};
   const bool pad_dy = n % 8 != 0, pad_x = k % (codes != nullptr ? 16 : 8) != 0;
+  const void* const from_dy = dy;
+  const void* const from_x = codes != nullptr ? static_cast<const void*>(codes) : x;
+  const uint8_t* const from_scales = codes != nullptr ? scales : nullptr;
+  uint8_t *pad_for_dy = nullptr, *pad_for_x = nullptr;
   if (pad_dy) {
-    jobs[0] = PadJob{static_cast<const __nv_bfloat16*>(dy), nullptr, nullptr, reinterpret_cast<uint4*>(pad), n, padded(n) / 8, rows * (padded(n) / 8)};
-    dy = pad;
+    dy = pad_for_dy = pad;
     pad += pad_bytes(rows, n);
   }
   if (pad_x) {
-    jobs[1] = PadJob{static_cast<const __nv_bfloat16*>(x), codes, scales, reinterpret_cast<uint4*>(pad), k, padded(k) / 8, rows * (padded(k) / 8)};
-    x = pad;
+    x = pad_for_x = pad;
     codes = nullptr;
   }
   int rc = 0;
   if (pad_dy || pad_x) {
-    const int64_t most = jobs[0].total > jobs[1].total ? jobs[0].total : jobs[1].total;
-    const int64_t blocks = (most + 255) / 256;
-    wgrad_pad_kernel<<<static_cast<int>(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, stream>>>(jobs[0], jobs[1]);
-    rc = static_cast<int>(cudaGetLastError());
+    // so many rows at a time that their pieces are counted in 31 bits; a multiple of 16, so that each piece
+    // of a tensor starts on a 16-byte boundary
+    const int64_t most = (int64_t(1) << 30) / (padded(n > k ? n : k) / 8) / 16 * 16;
+    for (int64_t first = 0; first < rows && rc == 0; first += most) {
+      const int64_t part = rows - first < most ? rows - first : most;
+      auto job = [&](const void* from, const uint8_t* s, uint8_t* out, int width) {
+        const int pieces = padded(width) / 8, size = s != nullptr ? 1 : 2;
+        return PadJob{static_cast<const uint8_t*>(from) + first * width * size,
+                      s != nullptr ? s + first * ((width + kMxBlock - 1) / kMxBlock) : nullptr,
+                      out != nullptr ? reinterpret_cast<uint4*>(out) + first * pieces : nullptr,
+                      part * width * size,
+                      width,
+                      out != nullptr ? static_cast<uint32_t>(part * pieces) : 0u,
+                      Divisor(static_cast<uint32_t>(pieces))};
+      };
+      const PadJob a = job(from_dy, nullptr, pad_for_dy, n), b = job(from_x, from_scales, pad_for_x, k);
+      const uint32_t blocks = ((a.total > b.total ? a.total : b.total) + 255) / 256;
+      wgrad_pad_kernel<<<blocks < 148 * 16 ? blocks : 148 * 16, 256, 0, stream>>>(a, b);
+      rc = static_cast<int>(cudaGetLastError());
+    }
     if (rc != 0) return cuda_status(rc, "weight_grad launch");
   }
   CUtensorMap mx, md;
@@ -593,15 +648,13 @@ int weight_grad_forward(const void* dy, const void* x, const uint8_t* codes, con
   p.k = k;
   p.out = pl.splits > 1 ? reinterpret_cast<float*>(ws) : dw;
   p.err = info.err;
-  rc = codes != nullptr ? launch_tile<true>(mx, md, p, pl, stream) : launch_tile<false>(mx, md, p, pl, stream);
+  const bool after = pad_dy || pad_x;
+  rc = codes != nullptr ? launch_tile<true>(mx, md, p, pl, after, stream) : launch_tile<false>(mx, md, p, pl, after, stream);
   if (rc == 0 && pl.splits > 1) {
     const int64_t count = static_cast<int64_t>(n) * k;
     const float* part = reinterpret_cast<const float*>(ws);
-    if (count % 4 == 0 && aligned16(dw))
-      launch_reduce<4>(part, dw, pl.splits, count, stream);
-    else
-      launch_reduce<1>(part, dw, pl.splits, count, stream);
-    rc = static_cast<int>(cudaGetLastError());
+    rc = count % 4 == 0 && aligned16(dw) ? launch_reduce<4>(part, dw, pl.splits, count, stream)
+                                         : launch_reduce<1>(part, dw, pl.splits, count, stream);
   }
   return cuda_status(rc, "weight_grad launch");
 }

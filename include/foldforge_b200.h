@@ -360,7 +360,8 @@ int ffb_dit_fwd(const void* x, const uint8_t* mask, const void* packed, const vo
  *   backward pass; codes / scales (both or neither) receive x's checkpoint. gamma, beta may be NULL.
  * ffb_layernorm_bwd: x (codes, scales NULL) or its checkpoint (x NULL): xh = (x - mean) rstd,
  *   w = gamma dy, dx = rstd (w - mean_c(w) - xh mean_c(w xh)) (+ residual where not NULL),
- *   dgamma = sum_rows dy xh, dbeta = sum_rows dy (each NULL where not wanted). c <= 8192.
+ *   dgamma = sum_rows dy xh, dbeta = sum_rows dy (each NULL where not wanted). Both: c <= 8192, and all
+ *   but mean, rstd and scales 16-byte aligned.
  * ffb_checkpoint_pack / _unpack: a checkpoint written from x, and read back.
  * ffb_weight_grad: dw [n, k] fp32 = dy^T x over the rows: dy [rows, n] bf16, x [rows, k] bf16 or its
  *   checkpoint (`checkpoint` of the workspace's size); dy, x and codes 16-byte aligned.
