@@ -128,6 +128,44 @@ def test_layer_norm_options(c, mx):
     run_layer_norm(70, c, BF16, mx, residual=True)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_layer_norm_widest_rows_with_residual(dtype):
+    run_layer_norm(5, 8192, dtype, False, residual=True)
+    run_layer_norm(300, 6160, dtype, True, residual=True)
+
+
+@pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("c", [64, 129])
+def test_layer_norm_takes_any_layout(c, mx):
+    """Rows in another order of memory, a start off 16 bytes, weights of another dtype, an expanded gradient."""
+    g = gen(12)
+    w, b = 1 + 0.3 * torch.randn(c, device="cuda", generator=g), torch.randn(c, device="cuda", generator=g)
+    x = activation(g, 30, c, BF16).view(5, 6, c).transpose(0, 1)
+    dy = gradient(g, 1, 30 * c + 1, BF16).view(-1)[1:].view(6, 5, c)
+    w16 = w.to(BF16)
+    y, saved = kernels.layer_norm_train(x, w16, torch.cat([b, b])[c:][:c], checkpoint=mx)
+    dx, dw, db = kernels.layer_norm_backward(dy, saved, w16)
+    (ry, rdx, rdw, rdb), (ey, edx, edw, edb) = ref.layer_norm(x.reshape(30, c), dy.reshape(30, c), w16, b, 1e-5, mx)
+    assert y.shape == x.shape and dx.shape == dy.shape
+    assert ref.worst(y.reshape(30, c), ry, ey, BF16) <= 1 and ref.worst(dx.reshape(30, c), rdx, edx, BF16) <= 1
+    assert ref.worst(dw, rdw, edw, F32) <= 1 and ref.worst(db, rdb, edb, F32) <= 1
+    one = dy[:1, :1].expand(6, 5, c)
+    dx, _, _ = kernels.layer_norm_backward(one, saved, w16)
+    (_, rdx, *_), (_, edx, *_) = ref.layer_norm(x.reshape(30, c), one.reshape(30, c), w16, b, 1e-5, mx)
+    assert ref.worst(dx.reshape(30, c), rdx, edx, BF16) <= 1
+
+
+def test_layer_norm_row_that_does_not_vary():
+    """The normalised row is 0 to the last bit, whatever its value: y is the bias, dx has no x in it."""
+    w, b = torch.full((96,), 3.0, device="cuda"), torch.randn(96, device="cuda", generator=gen(13))
+    x = torch.tensor([[5.0], [-1e30], [0.0], [1e-30]], device="cuda").expand(4, 96).contiguous()
+    y, saved = kernels.layer_norm_train(x, w, b)
+    assert torch.equal(y, b.expand(4, 96))
+    dy = gradient(gen(14), 4, 96, F32)
+    _, dw, _ = kernels.layer_norm_backward(dy, saved, w)
+    assert torch.equal(dw, torch.zeros_like(dw))
+
+
 def test_layer_norm_of_no_rows():
     w = torch.ones(16, device="cuda")
     x = torch.empty(0, 16, device="cuda")
@@ -246,6 +284,19 @@ def test_swiglu(rows, h, dtype, mx):
         assert torch.equal(kernels.checkpoint_unpack(saved).double(), ref.rounded_to_8_bits(ab).to(dtype).double())
 
 
+@pytest.mark.parametrize("h", [32, 40])
+@pytest.mark.parametrize("mx", [False, True])
+def test_swiglu_takes_any_layout(h, mx):
+    g = gen(15)
+    ab = activation(g, 1, 21 * 2 * h + 1, BF16).view(-1)[1:].view(7, 3, 2 * h)
+    dh = gradient(g, 21, h, BF16).view(3, 7, h).transpose(0, 1)
+    out, saved = kernels.swiglu_train(ab, checkpoint=mx)
+    dab = kernels.swiglu_backward(dh, saved)
+    (rh, rdab, _), (eh, edab, _) = ref.swiglu(ab.reshape(21, 2 * h), dh.reshape(21, h), mx)
+    assert ref.worst(out.reshape(21, h), rh, eh, BF16) <= 1
+    assert ref.worst(dab.reshape(21, 2 * h), rdab, edab, BF16) <= 1
+
+
 def test_swiglu_far_from_zero():
     """Gates whose exponential overflows: silu(a) is a or -0, its derivative 1 or 0."""
     a = torch.tensor([1e4, -1e4, 3e38, -3e38, 90.0, -90.0, 0.0, -0.0], device="cuda")
@@ -262,6 +313,42 @@ def test_swiglu_far_from_zero():
     assert torch.isfinite(dab).all()
     assert ref.worst(dab[:, :8], rdab[:, :8], edab[:, :8], F32) <= 1
     assert ref.worst(dab[:, 8:], rdab[:, 8:], edab[:, 8:], F32) <= 1
+
+
+# --------------------------------------------------------------------------- offsets past 32 bits
+def test_offsets_past_32_bits():
+    """More than 2^32 elements: the last rows come out as they do in a call of their own. (Each of these
+    tensors is about 9 GB; whole-tensor copies are let go before the next ones are made.)"""
+    c, tail = 264, 40
+    rows = (1 << 32) // c + 1000
+    x = torch.zeros(rows, c, dtype=BF16, device="cuda")
+    x[-tail:] = activation(gen(41), tail, c, BF16)
+    w, b = torch.rand(c, device="cuda", generator=gen(42)), torch.rand(c, device="cuda", generator=gen(43))
+    small_y, small = kernels.layer_norm_train(x[-tail:], w, b, checkpoint=True)
+    y, saved = kernels.layer_norm_train(x, w, b, checkpoint=True)
+    assert torch.equal(y[-tail:], small_y)
+    assert torch.equal(saved.x.codes[-tail:].view(torch.uint8), small.x.codes.view(torch.uint8))
+    assert torch.equal(saved.x.scales[-tail:], small.x.scales) and torch.equal(saved.stats[:, -tail:], small.stats)
+    small_dx, small_dw, small_db = kernels.layer_norm_backward(x[-tail:], small, w)
+    del y
+    dx, dw, db = kernels.layer_norm_backward(x, saved, w)  # the gradient is 0 but for the last rows
+    assert torch.equal(dx[-tail:], small_dx) and not dx[: rows - tail].any()
+    bound = 512 * ref.STEP * (x[-tail:].double().abs().sum(0) * 40)
+    assert ((dw - small_dw).abs() <= bound).all() and ((db - small_db).abs() <= bound).all()
+    del dx
+    whole = kernels.checkpoint_unpack(saved.x)
+    assert torch.equal(whole[-tail:], kernels.checkpoint_unpack(small.x))
+    del whole
+    for kept, few in ((saved.x, small.x), (x, x[-tail:])):
+        got = kernels.weight_grad(x, kept)
+        want, allowed = ref.weight_grad(x[-tail:], x[-tail:], few is small.x)
+        assert ref.worst(got, want, allowed, F32) <= 1
+    del saved
+    out, kept = kernels.swiglu_train(x, checkpoint=True)
+    few_out, few_kept = kernels.swiglu_train(x[-tail:], checkpoint=True)
+    assert torch.equal(out[-tail:], few_out)
+    dab = kernels.swiglu_backward(out, kept)
+    assert torch.equal(dab[-tail:], kernels.swiglu_backward(few_out, few_kept)) and not dab[: rows - tail].any()
 
 
 # --------------------------------------------------------------------------- use
