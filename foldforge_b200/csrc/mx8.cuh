@@ -380,31 +380,43 @@ __device__ __forceinline__ uint32_t mx_lanes_max(uint32_t m) {
   return m;
 }
 
-// The codes of a thread's VEC elements and the scale byte of their block, whose 32 channels lie in
-// 32 / VEC consecutive lanes. All of a warp's threads call this together. `f` holds the widened elements.
-template <typename T, int VEC>
-__device__ __forceinline__ typename MxCodes<VEC>::type mx_quantise(const typename Raw<T, VEC>::type& v, const Lanes<VEC>& f,
-                                                                   uint32_t& byte) {
+// The codes of N vectors of VEC elements of a thread, and the scale byte of each one's block, whose 32
+// channels lie in 32 / VEC consecutive lanes. All of a warp's threads call this together. `f` holds the
+// widened elements.
+template <typename T, int VEC, int N>
+__device__ __forceinline__ void mx_quantise(const typename Raw<T, VEC>::type (&v)[N], const Lanes<VEC> (&f)[N],
+                                            typename MxCodes<VEC>::type (&codes)[N], uint32_t (&byte)[N]) {
   constexpr uint32_t kInfinity = 0x7F800000u;
-  uint32_t m = mx_lanes_max<VEC>(max_magnitude<T, VEC>(v));
-  if (__any_sync(0xFFFFFFFFu, m >= kInfinity)) {
+  uint32_t m[N], top = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    m[i] = mx_lanes_max<VEC>(max_magnitude<T, VEC>(v[i]));
+    top = max(top, m[i]);
+  }
+  if (__any_sync(0xFFFFFFFFu, top >= kInfinity)) {
     // rare: somewhere in the warp's blocks a value is not finite. It becomes NaN (the conversion to e4m3
     // would make 448 of an infinity) and the scale is that of the others.
-    m = 0;
-    f.each([&](float x) {
-      const uint32_t a = __float_as_uint(x) & 0x7FFFFFFFu;
-      m = max(m, a < kInfinity ? a : 0u);
-      return x;
-    });
-    m = mx_lanes_max<VEC>(m);
-    byte = mx_scale_byte(m);
-    const float inv = mx_inverse_scale(byte);
-    return mx_encode<VEC>(f.each([&](float x) {
-      return (__float_as_uint(x) & 0x7FFFFFFFu) < kInfinity ? x * inv : __uint_as_float(0x7FFFFFFFu);
-    }));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      uint32_t largest = 0;
+      f[i].each([&](float x) {
+        const uint32_t a = __float_as_uint(x) & 0x7FFFFFFFu;
+        largest = max(largest, a < kInfinity ? a : 0u);
+        return x;
+      });
+      byte[i] = mx_scale_byte(mx_lanes_max<VEC>(largest));
+      const float inv = mx_inverse_scale(byte[i]);
+      codes[i] = mx_encode<VEC>(f[i].each([&](float x) {
+        return (__float_as_uint(x) & 0x7FFFFFFFu) < kInfinity ? x * inv : __uint_as_float(0x7FFFFFFFu);
+      }));
+    }
+    return;
   }
-  byte = mx_scale_byte(m);
-  return mx_encode<VEC>(f * Lanes<VEC>(mx_inverse_scale(byte)));
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    byte[i] = mx_scale_byte(m[i]);
+    codes[i] = mx_encode<VEC>(f[i] * Lanes<VEC>(mx_inverse_scale(byte[i])));
+  }
 }
 
 }  // namespace ffb

@@ -43,6 +43,18 @@ __device__ __forceinline__ void group_sum(float (&v)[NSUM], float* scratch, int&
 }
 
 // ------------------------------------------------------------------ LayerNorm
+template <int VEC>
+__device__ __forceinline__ void store_sums(float* p, const Lanes<VEC>& v) {
+  if (VEC > 1 && (reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
+#pragma unroll
+    for (int j = 0; j + 4 <= VEC; j += 4)
+      *reinterpret_cast<float4*>(p + j) = make_float4(v.get(j), v.get(j + 1), v.get(j + 2), v.get(j + 3));
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) p[j] = v.get(j);
+  }
+}
+
 // The block's sums of each channel over its rows (dg, db: a thread's, over the rows it took) to row
 // blockIdx.x of the partial sums. `space` holds kWarps NV GROUP VEC floats unless the whole block shares
 // each row, and nobody uses it any more once the block has come here.
@@ -58,11 +70,8 @@ __device__ __forceinline__ void write_column_sums(Lanes<VEC> (&dg)[NV], Lanes<VE
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int col = (i * GROUP + t) * VEC;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        if (col < c && pg != nullptr) pg[col + j] = dg[i].get(j);
-        if (col < c && pb != nullptr) pb[col + j] = db[i].get(j);
-      }
+      if (col < c && pg != nullptr) store_sums<VEC>(pg + col, dg[i]);
+      if (col < c && pb != nullptr) store_sums<VEC>(pb + col, db[i]);
     }
   } else {
     // a warp's groups by shuffles, then the warps through shared memory, each sum in a fixed order
@@ -281,18 +290,26 @@ __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
       const float q = d.dot(d);
       return FULL || (i * GROUP + t) * VEC < c ? q : 0.f;
     };
-    auto finish = [&](const typename Raw<T, VEC>::type& v, const Lanes<VEC>& f, float m, float r, int64_t row, int i) {
-      const int col = (i * GROUP + t) * VEC;
-      const bool in = row < rows && (FULL || col < c);
+    auto finish = [&](const typename Raw<T, VEC>::type (&v)[NV], const Lanes<VEC> (&f)[NV], float m, float r, int64_t row) {
       if (codes != nullptr) {
-        uint32_t byte;
-        const auto q = mx_quantise<T, VEC>(v, f, byte);
-        if (in) {
-          *reinterpret_cast<typename MxCodes<VEC>::type*>(codes + row * c + col) = q;
-          if (t % kLanes == 0) scales[row * blocks + col / kMxBlock] = static_cast<uint8_t>(byte);
+        typename MxCodes<VEC>::type q[NV];
+        uint32_t byte[NV];
+        mx_quantise<T, VEC, NV>(v, f, q, byte);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int col = (i * GROUP + t) * VEC;
+          if (row < rows && (FULL || col < c)) {
+            *reinterpret_cast<typename MxCodes<VEC>::type*>(codes + row * c + col) = q[i];
+            if (t % kLanes == 0) scales[row * blocks + col / kMxBlock] = static_cast<uint8_t>(byte[i]);
+          }
         }
       }
-      if (in) store_lanes<T, VEC>(y + row * c + col, fma((f + Lanes<VEC>(-m)) * Lanes<VEC>(r), w[i], b[i]));
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int col = (i * GROUP + t) * VEC;
+        if (row < rows && (FULL || col < c))
+          store_lanes<T, VEC>(y + row * c + col, fma((f[i] + Lanes<VEC>(-m)) * Lanes<VEC>(r), w[i], b[i]));
+      }
     };
     auto keep = [&](float m, float r, int64_t row) {
       if (t == 0 && row < rows) {
@@ -300,56 +317,38 @@ __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
         rstd_out[row] = r;
       }
     };
-    if constexpr (GROUP > 32) {
-      // the block's barriers cost more than reading the slot again: all rows of the chunk at a time
-      float m[U], r[U];
+    // rows of a block together: a barrier for all of them
+    constexpr int kTogether = GROUP > 32 ? U : 1;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
+    for (int u0 = 0; u0 < U; u0 += kTogether) {
+      typename Raw<T, VEC>::type v[kTogether][NV];
+      Lanes<VEC> f[kTogether][NV];
+      float m[kTogether], r[kTogether];
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) {
         m[u] = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) m[u] += widen<T, VEC>(read(u, i)).sum();
+        for (int i = 0; i < NV; ++i) {
+          v[u][i] = read(u0 + u, i);
+          f[u][i] = widen<T, VEC>(v[u][i]);
+          m[u] += f[u][i].sum();
+        }
       }
       group_sum<GROUP>(m, scratch, turn_of);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
+      for (int u = 0; u < kTogether; ++u) {
         m[u] *= inv_c;
         r[u] = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) r[u] += squares(widen<T, VEC>(read(u, i)), m[u], i);
+        for (int i = 0; i < NV; ++i) r[u] += squares(f[u][i], m[u], i);
       }
       group_sum<GROUP>(r, scratch, turn_of);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
+      for (int u = 0; u < kTogether; ++u) {
+        const int64_t row = row0 + (u0 + u) * kGroups;
         r[u] = rsqrtf(r[u] * inv_c + eps);
-        keep(m[u], r[u], row0 + u);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const auto v = read(u, i);
-          finish(v, widen<T, VEC>(v), m[u], r[u], row0 + u, i);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int64_t row = row0 + u * kGroups;
-        typename Raw<T, VEC>::type v[NV];
-        Lanes<VEC> f[NV];
-        float m[1] = {0.f}, r[1] = {0.f};
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          v[i] = read(u, i);
-          f[i] = widen<T, VEC>(v[i]);
-          m[0] += f[i].sum();
-        }
-        group_sum<GROUP>(m, scratch, turn_of);
-        m[0] *= inv_c;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) r[0] += squares(f[i], m[0], i);
-        group_sum<GROUP>(r, scratch, turn_of);
-        r[0] = rsqrtf(r[0] * inv_c + eps);
-        keep(m[0], r[0], row);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) finish(v[i], f[i], m[0], r[0], row, i);
+        keep(m[u], r[u], row);
+        finish(v[u], f[u], m[u], r[u], row);
       }
     }
     ring.next(turn);
@@ -568,14 +567,18 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const T* __restrict__ x,
     const P p(first + u * kThreads, total, c, per_row);
     v[u] = p.in ? load_raw<T, VEC>(x + p.at) : zero_raw<T, VEC>();
   }
+  Lanes<VEC> f[U];
+  typename MxCodes<VEC>::type q[U];
+  uint32_t byte[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) f[u] = widen<T, VEC>(v[u]);
+  mx_quantise<T, VEC, U>(v, f, q, byte);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const P p(first + u * kThreads, total, c, per_row);
-    uint32_t byte;
-    const auto q = mx_quantise<T, VEC>(v[u], widen<T, VEC>(v[u]), byte);
     if (p.in) {
-      *reinterpret_cast<typename MxCodes<VEC>::type*>(codes + p.at) = q;
-      if (threadIdx.x % P::kLanes == 0) scales[p.block] = static_cast<uint8_t>(byte);
+      *reinterpret_cast<typename MxCodes<VEC>::type*>(codes + p.at) = q[u];
+      if (threadIdx.x % P::kLanes == 0) scales[p.block] = static_cast<uint8_t>(byte[u]);
     }
   }
 }
@@ -641,18 +644,20 @@ __global__ void __launch_bounds__(kThreads)
   for (int u = 0; u < U; ++u) {
     const uint32_t id = first + u * kThreads;
     const bool in = id < total;
-    const Lanes<VEC> a = widen<T, VEC>(va[u]), b = widen<T, VEC>(vb[u]);
+    const typename Raw<T, VEC>::type v[2] = {va[u], vb[u]};
+    const Lanes<VEC> f[2] = {widen<T, VEC>(va[u]), widen<T, VEC>(vb[u])};
+    const Lanes<VEC>&a = f[0], &b = f[1];
     if (codes != nullptr) {
-      uint32_t ea, eb;
-      const auto qa = mx_quantise<T, VEC>(va[u], a, ea);
-      const auto qb = mx_quantise<T, VEC>(vb[u], b, eb);
+      typename MxCodes<VEC>::type q[2];
+      uint32_t byte[2];
+      mx_quantise<T, VEC, 2>(v, f, q, byte);
       if (in) {
-        *reinterpret_cast<typename MxCodes<VEC>::type*>(codes + at[u]) = qa;
-        *reinterpret_cast<typename MxCodes<VEC>::type*>(codes + at[u] + h) = qb;
+        *reinterpret_cast<typename MxCodes<VEC>::type*>(codes + at[u]) = q[0];
+        *reinterpret_cast<typename MxCodes<VEC>::type*>(codes + at[u] + h) = q[1];
         if (threadIdx.x % kLanes == 0) {  // whole blocks: the scales of a row are 2 h / 32
           uint8_t* s = scales + at[u] / kMxBlock;
-          s[0] = static_cast<uint8_t>(ea);
-          s[h / kMxBlock] = static_cast<uint8_t>(eb);
+          s[0] = static_cast<uint8_t>(byte[0]);
+          s[h / kMxBlock] = static_cast<uint8_t>(byte[1]);
         }
       }
     }
