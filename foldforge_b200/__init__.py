@@ -4,7 +4,9 @@
   (op classes with ``pytorch`` / ``b200`` backends, backend plan, guard, observations,
   ``run_block``).
 * :mod:`foldforge_b200.kernels` -- torch-facing wrappers of the C ABI
-  (``include/foldforge_b200.h``) implemented by ``_ffb.so``.
+  (``include/foldforge_b200.h``) implemented by ``_ffb.so``; among them the training operators
+  (LayerNorm and the gated unit with their backward passes, 8-bit checkpoints, weight gradients).
+* :mod:`foldforge_b200.engine.training` -- gradients of the engine ops on b200.
 * :func:`load` -- the path's share of ``foldforge.load(..., backend=...)``
   (``src/foldforge/models/__init__.py:134-148``): a Pairformer trunk from engine-key block
   state dicts, configured for a precision and given its backends by a plan.

@@ -1,5 +1,15 @@
 // Training operators bound by memory: LayerNorm forward and backward, the 8-bit checkpoint
 // (mx8.cuh) packed and read back, and the gated unit silu(a) b forward and backward.
+//
+// Measured on one B200 (device time, L2 holding other data; a plain copy moves 6.5 TB/s):
+//   LayerNorm, 262144 x 128 bf16 (a pair tensor of 512 tokens)   forward 21 us (6.4 TB/s), writing a
+//     checkpoint too 29 us (5.8); backward 36 us (5.6), from a checkpoint 37 us (4.6), and 3 us for the sums
+//     over the blocks. With rows loaded straight to registers instead of rings the four took 32 / 43 / 45 / 50 us:
+//     what was in flight was limited by the registers, at 16 warps an SM. With a checkpoint the conversions
+//     weigh as well (58 and 60% of issue slots in a profile of these two at 30 and 39 us).
+//   LayerNorm, 4099 x 4096 bf16 with a checkpoint   19 us + 25 us + 4 us
+//   checkpoint, 524288 x 64 bf16   packed in 15 us, read back in 12 us
+//   gated unit, 65536 x 2 x 512 bf16 with a checkpoint   49 us (5.5 TB/s), backward 50 us (4.1)
 #include <initializer_list>
 #include <type_traits>
 
@@ -15,7 +25,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 
-// Sums `v` over the GROUP threads that share a row (16, 32 or the whole block). The block form
+// Sums `v` over the GROUP threads that share a row (4 to 32, or the whole block). The block form
 // needs all threads; `scratch` holds one slot a warp and is used in turn (two buffers) so that one
 // barrier a sum is enough.
 template <int GROUP, int NSUM>
@@ -43,6 +53,7 @@ __device__ __forceinline__ void group_sum(float (&v)[NSUM], float* scratch, int&
 }
 
 // ------------------------------------------------------------------ LayerNorm
+// VEC sums to fp32 memory of any alignment
 template <int VEC>
 __device__ __forceinline__ void store_sums(float* p, const Lanes<VEC>& v) {
   if (VEC > 1 && (reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
@@ -246,12 +257,15 @@ struct Ring {
 // whether its channels are there; kWholeRows: c is a multiple of 16; kAnyRows: nothing.
 enum Rows : int { kAnyRows, kWholeRows, kFullRows };
 
+// ---- forward. GROUP threads hold a row in registers (NV vectors of VEC channels a thread): mean and variance
+// in two passes over the registers, one read and one write an element. Writes each row's mean and
+// 1 / sqrt(var + eps) in fp32 for the backward pass and, with `codes`, the input's 8-bit checkpoint.
 template <typename T, int VEC, int NV, int GROUP, int U, Rows ROWS>
 __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
     ln_train_kernel(const T* __restrict__ x, T* __restrict__ y, const float* __restrict__ gamma,
-                           const float* __restrict__ beta, float* __restrict__ mean_out, float* __restrict__ rstd_out,
-                           uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t rows, int c, float eps,
-                           int slots, int* err) {
+                    const float* __restrict__ beta, float* __restrict__ mean_out, float* __restrict__ rstd_out,
+                    uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t rows, int c, float eps, int slots,
+                    int* err) {
   constexpr bool FULL = ROWS == kFullRows;
   constexpr int kTeam = GROUP <= 32 ? 32 : kThreads;
   constexpr int kGroups = kTeam / GROUP;  // rows of a team side by side
@@ -355,13 +369,18 @@ __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
   }
 }
 
+// ---- backward. xh = (x - mean) rstd, w = gamma dy: dx = rstd (w - mean(w) - xh mean(w xh)) (+ residual). A
+// thread keeps the same channels for every row it takes, so the sums dgamma = sum dy xh and dbeta = sum dy
+// stay in its registers until the end; the block's row groups are then added in a fixed order and each
+// block writes one row of partial sums, which ln_grad_reduce_kernel adds in a fixed order: the result does
+// not depend on timing.
 template <typename T, int VEC, int NV, int GROUP, int U, bool MX, Rows ROWS>
 __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
     ln_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const uint8_t* __restrict__ codes,
-                         const uint8_t* __restrict__ scales, const float* __restrict__ mean_in,
-                         const float* __restrict__ rstd_in, const float* __restrict__ gamma,
-                         const T* __restrict__ residual, T* __restrict__ dx, float* __restrict__ dgamma,
-                         float* __restrict__ dbeta, int64_t partial_stride, int64_t rows, int c, int slots, int* err) {
+                  const uint8_t* __restrict__ scales, const float* __restrict__ mean_in,
+                  const float* __restrict__ rstd_in, const float* __restrict__ gamma, const T* __restrict__ residual,
+                  T* __restrict__ dx, float* __restrict__ dgamma, float* __restrict__ dbeta, int64_t partial_stride,
+                  int64_t rows, int c, int slots, int* err) {
   constexpr bool FULL = ROWS == kFullRows;
   constexpr int kTeam = GROUP <= 32 ? 32 : kThreads;
   constexpr int kGroups = kTeam / GROUP;

@@ -19,7 +19,18 @@
 // The tensor core truncates as it adds to a TMEM accumulator, and the bias grows with the number of
 // additions (1.5e-6 of |dW| after 220 of them). So the products of kChunk stages go to one of two
 // accumulators, and the warps add it to fp32 registers (round to nearest) while the other one
-// fills: chains of 4 kChunk additions, however many rows there are.
+// fills: chains of 4 kChunk additions, however many rows there are (2e-7 of |dW|).
+//
+// Measured on one B200: n 512, k 128, 262144 rows with an 8-bit X (303 MB, 34 GFLOP; 46 us of copying, 21 us
+// of tensor work) in 52 us + 4 us for the sum over the splits. It waits for memory:
+// with 128 KB of dY in flight an SM, 5.8 TB/s means a latency of about 3 us (by count, not measured). Steps on
+// the way, each timed with the L2 full of lines to write back: loads and conversions in turn 156 us, a stage
+// ahead in registers 90, codes by cp.async and the warps in groups 70, 256 channels of dY as the N side 65 to
+// 68; the same kernel that took 68 so took 52 over clean lines, the way all times here are taken. In a loop
+// over three inputs 64 us with the sum; 3 groups of fill warps 64, chunks of 16 stages 65.
+// Rows that have to be padded (n 129, k 68, 90000 rows): 14 us for that, 12 for the products, 4 for the sum.
+// Reading such rows through the codes' rings took 97 us for the products alone (lines to write back) where
+// padding and products took 18 + 14.
 #include <string.h>
 
 #include "abi_util.h"
