@@ -20,6 +20,9 @@ using at::Tensor;
 using OptTensor = std::optional<Tensor>;
 
 constexpr int64_t kBlock = 32;  // channels of a checkpoint that share a scale
+constexpr int64_t kMostChannels = int64_t(1) << 30;
+// of a weight gradient
+constexpr int64_t kMostGradRows = (int64_t(1) << 31) - 4096 - 1, kMostGradChannels = int64_t(1) << 20;
 
 struct Entries {
   decltype(&ffb_last_error) last_error;
@@ -62,11 +65,20 @@ Tensor dense(const Tensor& t) { return t.is_contiguous() ? t : t.contiguous(); }
 // a copy of a view that does not start on a 16-byte boundary
 Tensor aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone(); }
 
-// The first tensor of a call: bf16 (or fp32) rows of at least one channel on a CUDA device.
-Tensor rows_of(const char* name, const Tensor& x, bool fp32 = true) {
+// The entry points take channels as an int: wider rows are refused before they are narrowed.
+void check_channels(const char* name, c10::IntArrayRef shape) {
+  if (shape.back() < 0 || shape.back() > kMostChannels) refuse(name, std::to_string(shape.back()) + " channels");
+}
+
+// The first tensor of a call: bf16 (or fp32) rows of at least one channel.
+void check_rows(const char* name, const Tensor& x, bool fp32 = true) {
   if (x.scalar_type() != at::kBFloat16 && !(fp32 && x.scalar_type() == at::kFloat))
     refuse(name, std::string("dtype ") + c10::toString(x.scalar_type()) + (fp32 ? " (takes bf16 or fp32)" : " (takes bf16)"));
   if (x.dim() == 0 || x.size(-1) == 0) refuse(name, "shape " + text(x.sizes()) + " has no channels");
+  check_channels(name, x.sizes());
+}
+Tensor rows_of(const char* name, const Tensor& x) {
+  check_rows(name, x);
   return dense(x);
 }
 
@@ -144,6 +156,7 @@ Tensor checkpoint_unpack(const Tensor& data_in, const std::vector<int64_t>& shap
   const char* name = "checkpoint_unpack";
   if ((dtype != at::kBFloat16 && dtype != at::kFloat) || shape.empty() || shape.back() == 0)
     refuse(name, std::string("of a ") + c10::toString(dtype) + " " + text(shape) + " activation");
+  check_channels(name, shape);
   const Kept k = kept_of(name, data_in, data_in, true, shape, dtype);
   need_cuda(name, data_in);
   Call call(data_in);
@@ -208,11 +221,14 @@ std::tuple<Tensor, OptTensor, OptTensor> layer_norm_backward(const Tensor& dy_in
 Tensor weight_grad(const Tensor& dy_in, const Tensor& kept, bool checkpoint, const std::vector<int64_t>& shape, at::ScalarType dtype) {
   at::NoGradGuard no_grad;
   const char* name = "weight_grad";
-  Tensor dy = rows_of(name, dy_in, false);
-  if (shape.empty() || shape.back() == 0 || c10::IntArrayRef(shape).slice(0, shape.size() - 1) != dy.sizes().slice(0, dy.dim() - 1))
-    refuse(name, "rows of dy " + text(dy.sizes()) + " and x " + text(shape));
+  check_rows(name, dy_in, false);
+  if (shape.empty() || shape.back() <= 0 || c10::IntArrayRef(shape).slice(0, shape.size() - 1) != dy_in.sizes().slice(0, dy_in.dim() - 1))
+    refuse(name, "rows of dy " + text(dy_in.sizes()) + " and x " + text(shape));
   if (dtype != at::kBFloat16) refuse(name, std::string("x is ") + c10::toString(dtype) + " (takes bf16)");
-  const int64_t n = dy.size(-1), k = shape.back(), rows = dy.numel() / n;
+  const int64_t n = dy_in.size(-1), k = shape.back(), rows = dy_in.numel() / n;
+  if (rows > kMostGradRows || n > kMostGradChannels || k > kMostGradChannels)
+    refuse(name, std::to_string(rows) + " rows of " + std::to_string(n) + " and " + std::to_string(k) + " channels");
+  Tensor dy = dense(dy_in);
   kept_of(name, dy, kept, checkpoint, shape, dtype);
   need_cuda(name, dy);
   Call call(dy);

@@ -32,6 +32,9 @@ int check_kept(const char* what, const void* x, const uint8_t* codes, const uint
   return FFB_OK;
 }
 
+// a weight gradient past what the kernels count (rows as TMA coordinates, tiles in 32 bits)
+bool wide_grad(int64_t rows, int n, int k) { return rows >= (int64_t(1) << 31) - 4096 || n > (1 << 20) || k > (1 << 20); }
+
 cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
 
 }  // namespace
@@ -127,14 +130,15 @@ int ffb_checkpoint_unpack(const uint8_t* codes, const uint8_t* scales, void* x, 
 }
 
 size_t ffb_weight_grad_workspace_bytes(int64_t rows, int n, int k, int checkpoint) {
-  return (rows <= 0 || n <= 0 || k <= 0) ? 0 : weight_grad_workspace_bytes(rows, n, k, checkpoint != 0);
+  if (rows <= 0 || n <= 0 || k <= 0 || wide_grad(rows, n, k)) return 0;
+  return weight_grad_workspace_bytes(rows, n, k, checkpoint != 0);
 }
 
 int ffb_weight_grad(const void* dy, const void* x, const uint8_t* codes, const uint8_t* scales, float* dw,
                     void* workspace, size_t workspace_bytes, int64_t rows, int n, int k, void* stream) {
   if (rows < 0 || n <= 0 || k <= 0)
     return fail(FFB_ERR_ARG, "weight_grad: rows=%lld n=%d k=%d", (long long)rows, n, k);
-  if (rows >= (int64_t(1) << 31) - 4096 || n > (1 << 20) || k > (1 << 20))
+  if (wide_grad(rows, n, k))
     return fail(FFB_ERR_UNSUPPORTED, "weight_grad: rows=%lld n=%d k=%d", (long long)rows, n, k);
   if (!dw) return fail(FFB_ERR_ARG, "weight_grad: null pointer");
   if (off_word(dw)) return fail(FFB_ERR_ARG, "weight_grad: misaligned pointer");

@@ -85,6 +85,36 @@ def test_dtypes_and_shapes_are_refused():
 
 
 @needs_library
+def test_sizes_past_the_entry_points_are_refused():
+    """Rows wider than the entry points' 32-bit counts, from a single element (nothing is copied or made)."""
+    def of(*shape, dtype=torch.bfloat16):
+        return torch.zeros(1, dtype=dtype).expand(*shape)
+
+    wide, tall, norm = 2**32 + 128, 2**31, torch.ones(128)
+    byte = torch.zeros(1, dtype=torch.uint8)
+    refused = [
+        lambda: kernels.checkpoint_pack(of(1, wide)),
+        lambda: kernels.checkpoint_unpack(kernels.Checkpoint8(byte, torch.Size((1, wide)), torch.bfloat16)),
+        lambda: kernels.layer_norm_train(of(1, wide), None, None),
+        lambda: kernels.layer_norm_train(of(wide), None, None, checkpoint=True),
+        lambda: kernels.layer_norm_backward(of(1, wide), kernels.LayerNormSaved(of(1, wide), torch.zeros(2, 1)), norm),
+        lambda: kernels.swiglu_train(of(1, wide, dtype=torch.float32)),
+        lambda: kernels.swiglu_backward(of(1, wide), of(1, 2 * wide)),
+        lambda: kernels.weight_grad(of(4, wide), of(4, 8)),
+        lambda: kernels.weight_grad(of(4, 8), of(4, wide)),
+        lambda: kernels.weight_grad(of(4, 8), of(4, 2**20 + 1)),
+        lambda: kernels.weight_grad(of(4, 2**20 + 1), of(4, 8)),
+        lambda: kernels.weight_grad(of(tall, 8), of(tall, 8)),
+    ]
+    for i, call in enumerate(refused):
+        with pytest.raises(_lib.UnsupportedCall) as refusal:
+            call()
+        assert "channels" in str(refusal.value), i
+    size = _lib.load().ffb_weight_grad_workspace_bytes
+    assert size(100, 2**31 - 1, 64, 0) == size(100, 64, 2**31 - 1, 1) == size(2**62, 64, 64, 0) == 0
+
+
+@needs_library
 def test_entry_points_check_their_arguments():
     """Bad arguments come back as a status before anything is launched (no GPU is touched)."""
     lib = _lib.load()
