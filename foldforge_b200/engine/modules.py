@@ -504,6 +504,9 @@ class Transition(_PairOp):
     def _forward_b200(self, x: Tensor, key_mask: Tensor | None = None) -> Tensor:
         if not self._trains(x):
             return self._run_b200(x, key_mask)
+        # weights in training change from step to step, through .data too, which leaves their version as it
+        # was: they are packed again, so that both passes see the same ones
+        self._packed = None
         mask = None
         if self._masked_zero() and key_mask is not None:
             mask = key_mask.bool()

@@ -142,6 +142,31 @@ def test_a_block_trains_where_it_can():
     assert rel(gz, wz) < 2 * TOL and rel(gs, ws) < 2 * TOL
 
 
+@pytest.mark.parametrize("d,n,shape", [(128, 4, (1, 9, 9)), (384, 4, (1, 9)), (64, 4, (3, 5))])
+def test_a_training_step_sees_weights_changed_through_data(d, n, shape):
+    """``p.data`` leaves a parameter's address and version as they were; an optimiser's step changes the
+    version. Both reach the next forward pass, and the next one without gradients."""
+    def fresh(state):
+        m = Transition(d, n).cuda()
+        m.load_state_dict(state)
+        m.set_backend("b200")
+        m.set_checkpoint("exact")
+        return m
+
+    op = fresh(randomised(Transition(d, n), 3).state_dict())
+    x = torch.randn(*shape, d, generator=torch.Generator().manual_seed(4)).to(BF16).cuda()
+    first = op(x)
+    op.squeeze.weight.data.mul_(-2.0)
+    second = op(x)
+    assert not torch.equal(first, second)
+    assert torch.equal(second, fresh(op.state_dict())(x))
+    with torch.no_grad():
+        assert torch.equal(op(x), second)
+    second.float().sum().backward()
+    torch.optim.SGD(op.parameters(), lr=0.1).step()
+    assert torch.equal(op(x), fresh(op.state_dict())(x))
+
+
 def test_a_captured_training_step_calls_the_kernels():
     """Autograd under capture is refused; the same step from the kernels' functions is captured, replayed
     on new inputs, and agrees with autograd's."""
