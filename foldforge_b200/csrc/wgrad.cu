@@ -31,6 +31,8 @@
 // Rows that have to be padded (n 129, k 68, 90000 rows): 14 us for that, 12 for the products, 4 for the sum.
 // Reading such rows through the codes' rings took 97 us for the products alone (lines to write back) where
 // padding and products took 18 + 14.
+// A bf16 library product with a bf16 result takes 60.5 us for the first of these (66 here, from bf16 or 8 bits),
+// 11.1 for 512 rows of 1536 and 384 (10.4 from bf16, 13.4 from 8 bits) and 251 for the odd widths (29).
 #include <string.h>
 
 #include "abi_util.h"
