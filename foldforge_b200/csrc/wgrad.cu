@@ -31,8 +31,8 @@
 // Rows that have to be padded (n 129, k 68, 90000 rows): 14 us for that, 12 for the products, 4 for the sum.
 // Reading such rows through the codes' rings took 97 us for the products alone (lines to write back) where
 // padding and products took 18 + 14.
-// A bf16 library product with a bf16 result takes 60.5 us for the first of these (66 here, from bf16 or 8 bits),
-// 11.1 for 512 rows of 1536 and 384 (10.4 from bf16, 13.4 from 8 bits) and 251 for the odd widths (29).
+// A bf16 library product with a bf16 result takes 60.3 us for the first of these (65 to 66 here, from bf16 or 8 bits),
+// 10.9 for 512 rows of 1536 and 384 (10.4 from bf16, 12.4 from 8 bits) and 251 for the odd widths (29).
 #include <string.h>
 
 #include "abi_util.h"
@@ -536,20 +536,26 @@ struct WgradPlan {
 
 // Tiles of 256 channels of dY by 128 of X, or 128 by 256 for few of dY: larger tiles read each operand less
 // often.
-WgradPlan plan(int64_t rows, int n, int k) {
+WgradPlan plan(int64_t rows, int n, int k, bool pad, bool codes) {
   WgradPlan p;
   p.bn = n <= 64 ? 64 : n <= 128 ? 128 : 256;
   p.mb = p.bn == 256 || k <= 128 ? 1 : 2;
   const int64_t tiles = static_cast<int64_t>((n + p.bn - 1) / p.bn) * ((k + 128 * p.mb - 1) / (128 * p.mb));
   p.tiles = static_cast<int>(tiles);
   // The number of splits that ends first, in stages' time: waves of CTAs, each with its own start and end
-  // (about 6 stages), and for the partial sums a second kernel and a pass over them.
+  // (about 6 stages), and for the partial sums a pass over them (1 for 2^20 sums) and a second kernel, which
+  // starts while the products end: 1 stage of an 8-bit X (0.7 us), 3 of the shorter ones of a bf16 X (0.5 us),
+  // and 8 beside a padding kernel, where the host's third launch is what a short call waits for. Against 8 in
+  // each case, calls issued back to back, 8 bits: 1024 rows, n 1536, k 384 in 13.7 us for 18.5, 512 rows, n 512,
+  // k 128 in 10.3 for 13.1. With 1 in each case 512 rows, n 558, k 11 took 11.6 us for 10.5, and 512 rows,
+  // n = k = 1024 in bf16 up to 11.4 for 10.3.
+  const int second = pad ? 8 : codes ? 1 : 3;
   const int64_t steps = (rows + kRows - 1) / kRows;
   int64_t best = 1, best_cost = -1;
   for (int64_t s = 1; s <= kSms && s <= steps; ++s) {
     if (s > 1 && tiles * s > 4 * kSms) break;  // enough tiles to fill the SMs
     const int64_t waves = (tiles * s + kSms - 1) / kSms;
-    const int64_t cost = waves * ((steps + s - 1) / s + 6) + (s > 1 ? 8 + s * n * k / (1 << 19) : 0);
+    const int64_t cost = waves * ((steps + s - 1) / s + 6) + (s > 1 ? second + s * n * k / (1 << 20) : 0);
     if (best_cost < 0 || cost < best_cost) {
       best = s;
       best_cost = cost;
@@ -599,18 +605,19 @@ size_t pad_bytes(int64_t rows, int width) { return (static_cast<size_t>(rows) * 
 }  // namespace
 
 size_t weight_grad_workspace_bytes(int64_t rows, int n, int k, bool codes) {
-  size_t bytes = partial_bytes(plan(rows, n, k), n, k);
-  if (n % 8 != 0) bytes += pad_bytes(rows, n);
-  if (k % (codes ? 16 : 8) != 0) bytes += pad_bytes(rows, k);
+  const bool pad_dy = n % 8 != 0, pad_x = k % (codes ? 16 : 8) != 0;
+  size_t bytes = partial_bytes(plan(rows, n, k, pad_dy || pad_x, codes), n, k);
+  if (pad_dy) bytes += pad_bytes(rows, n);
+  if (pad_x) bytes += pad_bytes(rows, k);
   return bytes;
 }
 
 int weight_grad_forward(const void* dy, const void* x, const uint8_t* codes, const uint8_t* scales, float* dw,
                         void* workspace, int64_t rows, int n, int k, const DeviceInfo& info, cudaStream_t stream) {
-  const WgradPlan pl = plan(rows, n, k);
+  const bool pad_dy = n % 8 != 0, pad_x = k % (codes != nullptr ? 16 : 8) != 0;
+  const WgradPlan pl = plan(rows, n, k, pad_dy || pad_x, codes != nullptr);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   uint8_t* pad = ws + partial_bytes(pl, n, k);
-  const bool pad_dy = n % 8 != 0, pad_x = k % (codes != nullptr ? 16 : 8) != 0;
   const void* const from_dy = dy;
   const void* const from_x = codes != nullptr ? static_cast<const void*>(codes) : x;
   const uint8_t* const from_scales = codes != nullptr ? scales : nullptr;
