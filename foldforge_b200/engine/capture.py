@@ -5,15 +5,51 @@ FoldForge's execution policy captures the trunk once and replays it
 The b200 kernels are capturable: they allocate nothing, never synchronise the host, and
 take every buffer as an argument. Weights are packed on the eager warm-up call, before
 capture.
+
+A graph knows a packed weight image by its address alone, and a module replaces its image when its
+weights change: what an op hands out under capture is kept here, by the :class:`GraphedCall` that
+captures it or else (a capture of the caller's own) as long as the module lives. A replay goes on
+reading the image it was captured with.
 """
 
 from __future__ import annotations
 
-from collections.abc import Callable, Sequence
+import threading
+from collections.abc import Callable, Iterator, Sequence
+from contextlib import contextmanager
+from weakref import WeakKeyDictionary
 
 import torch
+from torch import nn
 
 Tensor = torch.Tensor
+_holder = threading.local()  # .images: the list of the capture that runs on this thread
+_of_modules: WeakKeyDictionary[nn.Module, list[Tensor]] = WeakKeyDictionary()
+
+
+def capturing() -> bool:
+    """Whether the current stream is being captured into a graph."""
+    return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+
+
+@contextmanager
+def holding(images: list[Tensor]) -> Iterator[None]:
+    """Images that ops of this thread hand out under capture meanwhile go to ``images``."""
+    before = getattr(_holder, "images", None)
+    _holder.images = images
+    try:
+        yield
+    finally:
+        _holder.images = before
+
+
+def keep_image(module: nn.Module, image: Tensor) -> None:
+    """Keep an image of ``module`` that a graph being captured reads."""
+    images = getattr(_holder, "images", None)
+    if images is None:
+        images = _of_modules.setdefault(module, [])
+    if not any(kept is image for kept in images):
+        images.append(image)
 
 
 class GraphedCall:
@@ -35,7 +71,8 @@ class GraphedCall:
         torch.cuda.current_stream().wait_stream(stream)
         torch.cuda.synchronize()
         self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph), torch.no_grad():
+        self.images: list[Tensor] = []
+        with torch.cuda.graph(self.graph), torch.no_grad(), holding(self.images):
             self.static_outputs = fn(*self.static_inputs)
         torch.cuda.synchronize()
 

@@ -23,6 +23,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from foldforge_b200.engine import capture
 from foldforge_b200.engine.modules import (
     MasterWeights,
     _check_backend,
@@ -171,6 +172,8 @@ class TokenDiT(MasterWeights, nn.Module):
         if self._packed is None or self._packed[0] != key:
             with torch.no_grad():
                 self._packed = (key, kernels.dit_prepare(self._weights(), device))
+        if capture.capturing():
+            capture.keep_image(self, self._packed[1])
         return self._packed[1]
 
     def _conditioning(self, cond: Tensor, pair: Tensor, packed: Tensor) -> Tensor:

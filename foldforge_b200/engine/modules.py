@@ -20,18 +20,21 @@ applies the reference equations there too.
 
 from __future__ import annotations
 
+from contextvars import ContextVar
 from dataclasses import dataclass
 
 import torch
 import torch.nn.functional as F
 from torch import nn
 
-from foldforge_b200.engine import training
+from foldforge_b200.engine import capture, training
 
 Tensor = torch.Tensor
 #: channels of a LayerNorm whose gradient the b200 kernels take (a row is held in one block's registers)
 MAX_TRAINED_CHANNELS = 8192
 MASKED_UPDATES = ("zero", "compute")
+#: the op whose forward pass trains in this context
+_training_op: ContextVar[nn.Module | None] = ContextVar("_training_op", default=None)
 
 
 class BackendUnsupported(RuntimeError):
@@ -227,7 +230,7 @@ class _PairOp(MasterWeights, nn.Module):
         super().__init__()
         self.backend = "pytorch"
         self.masked_update = "zero"
-        self._packed: tuple[tuple, Tensor] | None = None
+        self._packed: tuple[tuple | None, Tensor] | None = None
 
     def set_backend(self, name: str) -> None:
         _check_backend(self, name)
@@ -256,12 +259,36 @@ class _PairOp(MasterWeights, nn.Module):
 
     def _cached_pack(self, pack) -> Tensor:
         """The packed device image of the weights, rebuilt only when a parameter changed
-        (its storage or version): ``pack(weights)`` gets the state dict then."""
+        (its storage or version): ``pack(weights)`` gets the state dict then. A pass that trains packs
+        one for itself and leaves the shared one to its readers (:meth:`_train`); one packed under
+        capture belongs to the graph, which fills it when it runs."""
+        captured, trains = capture.capturing(), _training_op.get() is self
         key = tuple((p.data_ptr(), p._version) for p in self.parameters())
-        if self._packed is None or self._packed[0] != key:
+        cached = self._packed
+        if trains or cached is None or cached[0] != key:
             with torch.no_grad():
-                self._packed = (key, pack(dict(self.state_dict())))
-        return self._packed[1]
+                image = pack(dict(self.state_dict()))
+            if not (trains or captured):
+                self._packed = (key, image)
+        else:
+            image = cached[1]
+        if captured:
+            capture.keep_image(self, image)
+        return image
+
+    def _train(self, run, *args) -> Tensor:
+        """``run(*args)`` as the forward half of a pass that trains. Weights in training change from step to step,
+        through ``.data`` too, which leaves their version as it was, and the backward pass reads the weights
+        themselves: an image is packed for every such pass. The next pass without gradients packs again as
+        well, unless every weight is frozen."""
+        cached = self._packed
+        if cached is not None and any(p.requires_grad for p in self.parameters()):
+            self._packed = (None, cached[1])
+        token = _training_op.set(self)
+        try:
+            return run(*args)
+        finally:
+            _training_op.reset(token)
 
     def _key_mask(self, x: Tensor, key_mask: Tensor | None) -> Tensor:
         if key_mask is None:
@@ -504,16 +531,14 @@ class Transition(_PairOp):
     def _forward_b200(self, x: Tensor, key_mask: Tensor | None = None) -> Tensor:
         if not self._trains(x):
             return self._run_b200(x, key_mask)
-        # weights in training change from step to step, through .data too, which leaves their version as it
-        # was: they are packed again, so that both passes see the same ones
-        self._packed = None
         mask = None
         if self._masked_zero() and key_mask is not None:
             mask = key_mask.bool()
             if x.dim() == 4:
                 mask = mask[:, :, None] & mask[:, None, :]
         weights = (self.ln_in.weight, self.ln_in.bias, self.expand_a.weight, self.expand_b.weight, self.squeeze.weight)
-        return training.transition(x, mask, lambda t: self._run_b200(t, key_mask), self.checkpoint, self.ln_in.eps, *weights)
+        return training.transition(x, mask, lambda t: self._train(self._run_b200, t, key_mask), self.checkpoint,
+                                   self.ln_in.eps, *weights)
 
     def _run_b200(self, x: Tensor, key_mask: Tensor | None) -> Tensor:
         from foldforge_b200 import kernels
