@@ -533,7 +533,8 @@ class Transition(_PairOp):
             return self._run_b200(x, key_mask)
         mask = None
         if self._masked_zero() and key_mask is not None:
-            mask = key_mask.bool()
+            # as the kernels read it: a value that is 0 in 8 bits (0.5, 256) masks
+            mask = key_mask if key_mask.dtype == torch.bool else key_mask.to(torch.uint8).bool()
             if x.dim() == 4:
                 mask = mask[:, :, None] & mask[:, None, :]
         weights = (self.ln_in.weight, self.ln_in.bias, self.expand_a.weight, self.expand_b.weight, self.squeeze.weight)
