@@ -92,6 +92,19 @@ struct Lanes {
     f32x2_split(t, a, b);
     return a + b;
   }
+  // the sum as a tree: equal values add up without rounding
+  __device__ __forceinline__ float tree() const {
+    uint64_t t[VEC / 2];
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) t[i] = p[i];
+#pragma unroll
+    for (int n = VEC / 4; n > 0; n /= 2)
+#pragma unroll
+      for (int i = 0; i < n; ++i) t[i] = add_f32x2(t[i], t[i + n]);
+    float a, b;
+    f32x2_split(t[0], a, b);
+    return a + b;
+  }
   // the sum of products with `o`
   __device__ __forceinline__ float dot(const Lanes& o) const {
     uint64_t t = mul_f32x2(p[0], o.p[0]);
@@ -121,6 +134,7 @@ struct Lanes<1> {
     return Lanes(g(f, o.f));
   }
   __device__ __forceinline__ float sum() const { return f; }
+  __device__ __forceinline__ float tree() const { return f; }
   __device__ __forceinline__ float dot(const Lanes& o) const { return f * o.f; }
   __device__ __forceinline__ float get(int) const { return f; }
 };

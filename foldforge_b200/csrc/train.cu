@@ -25,6 +25,16 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 
+// The sum of N (a power of two) values as a tree, in which equal values add up without rounding.
+template <int N>
+__device__ __forceinline__ float tree_sum(float (&v)[N]) {
+#pragma unroll
+  for (int n = N / 2; n > 0; n /= 2)
+#pragma unroll
+    for (int i = 0; i < n; ++i) v[i] += v[i + n];
+  return v[0];
+}
+
 // Sums `v` over the GROUP threads that share a row (4 to 32, or the whole block). The block form
 // needs all threads; `scratch` holds one slot a warp and is used in turn (two buffers) so that one
 // barrier a sum is enough.
@@ -44,10 +54,10 @@ __device__ __forceinline__ void group_sum(float (&v)[NSUM], float* scratch, int&
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < NSUM; ++k) {
-      float t = 0.f;
+      float w[kWarps];
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) t += s[k * kWarps + w];
-      v[k] = t;
+      for (int i = 0; i < kWarps; ++i) w[i] = s[k * kWarps + i];
+      v[k] = tree_sum(w);
     }
   }
 }
@@ -337,21 +347,36 @@ __global__ void __launch_bounds__(kThreads, NV * VEC * sizeof(T) <= 32 ? 2 : 1)
     for (int u0 = 0; u0 < U; u0 += kTogether) {
       typename Raw<T, VEC>::type v[kTogether][NV];
       Lanes<VEC> f[kTogether][NV];
-      float m[kTogether], r[kTogether];
+      // The mean of a row that does not vary is its value to the last bit: the sums are trees, in which equal
+      // values add up without rounding, and that is all there is to a full row (c is a power of two). Of
+      // other rows each vector's sum, or that of two single elements, has the first channel taken off as often
+      // as it holds it, before 3 or 5 of them add up. For 65536 x 384 bf16 that costs 0.6 us of 21.6; taking it
+      // off every element of every row 1.3.
+      float m[kTogether], r[kTogether], x0[kTogether];
 #pragma unroll
       for (int u = 0; u < kTogether; ++u) {
-        m[u] = 0.f;
+        constexpr int kSum = VEC > 1 ? 1 : 2;  // of NV vectors
+        float sums[NV / kSum];
+        x0[u] = FULL ? 0.f : static_cast<float>(have[(u0 + u) * kGroups * c]);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           v[u][i] = read(u0 + u, i);
           f[u][i] = widen<T, VEC>(v[u][i]);
-          m[u] += f[u][i].sum();
         }
+#pragma unroll
+        for (int i = 0; i < NV; i += kSum) {
+          const int col = (i * GROUP + t) * VEC;
+          float a = f[u][i].tree();
+          if constexpr (kSum == 2) a += f[u][i + 1].tree();
+          if constexpr (!FULL) a = col < c ? fmaf(kSum == 2 && col + GROUP < c ? -2.f : -static_cast<float>(VEC), x0[u], a) : 0.f;
+          sums[i / kSum] = a;
+        }
+        m[u] = tree_sum(sums);
       }
       group_sum<GROUP>(m, scratch, turn_of);
 #pragma unroll
       for (int u = 0; u < kTogether; ++u) {
-        m[u] *= inv_c;
+        m[u] = fmaf(m[u], inv_c, x0[u]);
         r[u] = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) r[u] += squares(f[u][i], m[u], i);
