@@ -192,7 +192,8 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_train(const Tensor& x_in, const Op
 }
 
 std::tuple<Tensor, OptTensor, OptTensor> layer_norm_backward(const Tensor& dy_in, const Tensor& kept, bool checkpoint, const Tensor& stats_in,
-                                                             const OptTensor& weight, bool bias, const OptTensor& residual_in) {
+                                                             const OptTensor& weight, bool weight_gradient, bool bias,
+                                                             const OptTensor& residual_in) {
   at::NoGradGuard no_grad;
   const char* name = "layer_norm_backward";
   const Tensor dy = aligned(rows_of(name, dy_in));
@@ -206,7 +207,7 @@ std::tuple<Tensor, OptTensor, OptTensor> layer_norm_backward(const Tensor& dy_in
   need_cuda(name, dy);
   Call call(dy);
   const Tensor dx = like(dy, dy.sizes());
-  if (w) dweight = floats(dy, {c});
+  if (w && weight_gradient) dweight = floats(dy, {c});
   if (bias) dbias = floats(dy, {c});
   const int dtype = dtype_of(dy.scalar_type());
   const size_t size = dweight || dbias ? entries.layernorm_bwd_workspace_bytes(rows, static_cast<int>(c), dtype) : 0;

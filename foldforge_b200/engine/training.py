@@ -76,6 +76,14 @@ def _kept(ctx, kind: str, saved: Tensor):
     return saved if kind == "exact" else kernels.Checkpoint8(saved, ctx.shape, ctx.dtype)
 
 
+def _norm_backward(dy: Tensor, saved, weight: Tensor | None, want_weight: bool, want_bias: bool, **kwargs):
+    from foldforge_b200 import kernels
+
+    if weight is not None and not want_weight:
+        kwargs["weight_gradient"] = False
+    return kernels.layer_norm_backward(dy, saved, weight, bias=want_bias, **kwargs)
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float, kind: str) -> Tensor:
@@ -95,8 +103,9 @@ class _LayerNorm(torch.autograd.Function):
         _refuse_capture()
         kept, stats, weight = ctx.saved_tensors
         saved = kernels.LayerNormSaved(_kept(ctx, ctx.kind, kept), stats)
-        dx, dweight, dbias = kernels.layer_norm_backward(dy, saved, weight, bias=ctx.has_bias)
-        return dx, dweight, dbias, None, None
+        wanted = ctx.needs_input_grad
+        dx, dweight, dbias = _norm_backward(dy, saved, weight, wanted[1], ctx.has_bias and wanted[2])
+        return dx if wanted[0] else None, dweight, dbias, None, None
 
 
 def layer_norm(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float, kind: str) -> Tensor:
@@ -132,8 +141,16 @@ class _Transition(torch.autograd.Function):
         keep = None if mask is None else mask.reshape(rows, 1)
         expand = torch.cat([expand_a, expand_b]).to(x.dtype)  # [2 h, c]
         expand_t, squeeze_t = expand.t().contiguous(), squeeze.t().to(x.dtype).contiguous()
+        # the gradients that are asked for; the norm's kernel forms dx with its sums over the rows
+        want_x, want_ln_weight, want_ln_bias, want_a, want_b, want_squeeze = (ctx.needs_input_grad[i] for i in (0, 5, 6, 7, 8, 9))
+        want_expand, want_norm = want_a or want_b, want_x or want_ln_weight or want_ln_bias
         dx: list[Tensor] = []
-        sums: list[Tensor] = []
+        sums: dict[str, Tensor] = {}
+
+        def add(name: str, part: Tensor | None) -> None:
+            if part is not None:
+                sums[name] = sums[name].add_(part) if name in sums else part
+
         for first in range(0, rows, CHUNK_ROWS):
             part = slice(first, min(first + CHUNK_ROWS, rows))
             xp, gd = x[part], g[part]
@@ -141,19 +158,30 @@ class _Transition(torch.autograd.Function):
                 xp, gd = torch.where(keep[part], xp, 0.0), torch.where(keep[part], gd, 0.0)
             v, saved = kernels.layer_norm_train(xp, ln_weight, ln_bias, ctx.eps)
             ab = kernels.gemm_nt(v, expand)
-            dab, hidden = kernels.swiglu_backward(kernels.gemm_nt(gd, squeeze_t), ab, output=True)
+            dab = kernels.swiglu_backward(kernels.gemm_nt(gd, squeeze_t), ab, output=want_squeeze)
             del ab
-            dv = kernels.gemm_nt(dab, expand_t)
-            dxp, dln_weight, dln_bias = kernels.layer_norm_backward(dv, saved, ln_weight, residual=g[part])
-            dx.append(dxp)
-            new = [dln_weight, dln_bias, kernels.weight_grad(dab, v), kernels.weight_grad(gd, hidden)]
-            sums = new if not sums else [s.add_(t) for s, t in zip(sums, new)]
-        if not dx:  # no rows
-            dx = [x]
-            sums = [torch.zeros_like(t, dtype=torch.float32) for t in (ln_weight, ln_bias, expand, squeeze)]
-        dln_weight, dln_bias, dexpand, dsqueeze = sums
-        all_dx = (dx[0] if len(dx) == 1 else torch.cat(dx)).view(ctx.shape)
-        return all_dx, None, None, None, None, dln_weight, dln_bias, dexpand[:h], dexpand[h:], dsqueeze
+            if want_squeeze:
+                dab, hidden = dab
+                add("squeeze", kernels.weight_grad(gd, hidden))
+                del hidden
+            if want_expand:
+                add("expand", kernels.weight_grad(dab, v))
+            if want_norm:
+                dxp, dln_weight, dln_bias = _norm_backward(kernels.gemm_nt(dab, expand_t), saved, ln_weight, want_ln_weight,
+                                                           want_ln_bias, residual=g[part] if want_x else None)
+                add("ln_weight", dln_weight)
+                add("ln_bias", dln_bias)
+                if want_x:
+                    dx.append(dxp)
+        if rows == 0:
+            dx = [torch.empty_like(x)]
+            sums = {name: torch.zeros_like(t, dtype=torch.float32) for name, t in
+                    (("ln_weight", ln_weight), ("ln_bias", ln_bias), ("expand", expand), ("squeeze", squeeze))}
+        all_dx = (dx[0] if len(dx) == 1 else torch.cat(dx)).view(ctx.shape) if want_x else None
+        dexpand = sums.get("expand")
+        return (all_dx, None, None, None, None, sums.get("ln_weight") if want_ln_weight else None,
+                sums.get("ln_bias") if want_ln_bias else None, dexpand[:h] if want_a else None,
+                dexpand[h:] if want_b else None, sums.get("squeeze") if want_squeeze else None)
 
 
 def transition(x: Tensor, mask: Tensor | None, run, kind: str, eps: float, *weights: Tensor) -> Tensor:

@@ -568,13 +568,13 @@ def layer_norm_train(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps:
     return y, LayerNormSaved(Checkpoint8(kept, x.shape, x.dtype) if checkpoint else kept, stats)
 
 
-def layer_norm_backward(dy: Tensor, saved: LayerNormSaved, weight: Tensor | None, *, bias: bool = True,
-                        residual: Tensor | None = None) -> tuple[Tensor, Tensor | None, Tensor | None]:
+def layer_norm_backward(dy: Tensor, saved: LayerNormSaved, weight: Tensor | None, *, weight_gradient: bool = True,
+                        bias: bool = True, residual: Tensor | None = None) -> tuple[Tensor, Tensor | None, Tensor | None]:
     """``(dx, dweight, dbias)`` of :func:`layer_norm_train`: ``dx`` (plus ``residual``, the gradient that
     reaches x around the norm) in ``dy``'s dtype, the others fp32, reduced over the rows in a fixed order
-    (``None`` without ``weight`` / ``bias``)."""
+    (``None`` without ``weight`` or its ``weight_gradient``, and without ``bias``)."""
     kept, packed = _unpacked("layer_norm_backward", saved.x, dy.shape, dy.dtype)
-    return _lib.binding().layer_norm_backward(dy, kept, packed, saved.stats, weight, bias, residual)
+    return _lib.binding().layer_norm_backward(dy, kept, packed, saved.stats, weight, weight_gradient, bias, residual)
 
 
 def weight_grad(dy: Tensor, x: Tensor | Checkpoint8) -> Tensor:
