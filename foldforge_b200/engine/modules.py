@@ -32,6 +32,8 @@ from foldforge_b200.engine import capture, training
 Tensor = torch.Tensor
 #: channels of a LayerNorm whose gradient the b200 kernels take (a row is held in one block's registers)
 MAX_TRAINED_CHANNELS = 8192
+#: channels of either operand of a weight gradient
+MAX_WEIGHT_GRAD_CHANNELS = 1 << 20
 MASKED_UPDATES = ("zero", "compute")
 #: the op whose forward pass trains in this context
 _training_op: ContextVar[nn.Module | None] = ContextVar("_training_op", default=None)
@@ -483,6 +485,8 @@ class Transition(_PairOp):
             return f"activations are {x.dtype}; the b200 gradient takes bf16 (master precision)"
         if self.d % 8 or self.n * self.d % 16 or self.d > MAX_TRAINED_CHANNELS:
             return f"widths ({self.d}, {self.n} x {self.d}) (the b200 gradient takes a multiple of 8)"
+        if 2 * self.n * self.d > MAX_WEIGHT_GRAD_CHANNELS:
+            return f"{2 * self.n * self.d} hidden channels (a b200 weight gradient takes at most {MAX_WEIGHT_GRAD_CHANNELS})"
         return training.capture_reason()
 
     def unsupported(self, x: Tensor, key_mask: Tensor | None = None) -> str | None:
