@@ -20,11 +20,11 @@ namespace {
 
 // A block packs kPackRows rows, kPackColumns of each at a time: all threads write the image, then one thread a
 // row and sum adds up the columns in turn from shared memory (wsum and bias have that order). A pair transition, which
-// a training step packs in every forward pass, is packed in 106 us; with one thread for the whole of a row
+// a training step packs in every forward pass, is packed in 72 us; with one thread for the whole of a row
 // it took 411.
-constexpr int kPackRows = 8, kPackColumns = 128, kPackThreads = 128;
+constexpr int kPackRows = 8, kPackColumns = 128;
 
-__global__ void __launch_bounds__(kPackThreads)
+__global__ void __launch_bounds__(kPackColumns)
     pack_weight_kernel(const float* __restrict__ w, int rows, int k, const float* __restrict__ gamma,
                        const float* __restrict__ beta, uint8_t* __restrict__ image, int row_offset, int image_rows,
                        float* __restrict__ wsum, float* __restrict__ bias, float scale) {
@@ -34,18 +34,22 @@ __global__ void __launch_bounds__(kPackThreads)
   const int here = rows - first < kPackRows ? rows - first : kPackRows;
   float s = 0.f, bsum = 0.f;
   for (int c0 = 0; c0 < k; c0 += kPackColumns) {
-    const int n = k - c0 < kPackColumns ? k - c0 : kPackColumns;
-    for (int i = threadIdx.x; i < here * kPackColumns; i += kPackThreads) {
-      const int r = i / kPackColumns, j = i % kPackColumns, c = c0 + j;
-      if (j >= n) continue;
-      const float v = w[static_cast<int64_t>(first + r) * k + c];
+    const int n = k - c0 < kPackColumns ? k - c0 : kPackColumns, j = threadIdx.x, c = c0 + j;
+    if (j < n) {  // a thread has the same column of every row
       const float g = gamma ? gamma[c] : 1.0f;
-      const __nv_bfloat16 q = __float2bfloat16_rn(v * g * scale);
       uint8_t* block = image + static_cast<int64_t>(c / 64) * image_rows * 128;
-      *reinterpret_cast<__nv_bfloat16*>(block + sw128_offset(row_offset + first + r, c % 64)) = q;
-      packed[r][j] = __bfloat162float(q);
-      plain[r][j] = v;
-      if (r == 0) shift[j] = beta ? beta[c] : 0.f;
+      shift[j] = beta ? beta[c] : 0.f;
+      float v[kPackRows];
+#pragma unroll
+      for (int r = 0; r < kPackRows; ++r) v[r] = r < here ? w[static_cast<int64_t>(first + r) * k + c] : 0.f;
+#pragma unroll
+      for (int r = 0; r < kPackRows; ++r) {
+        if (r >= here) break;
+        const __nv_bfloat16 q = __float2bfloat16_rn(v[r] * g * scale);
+        *reinterpret_cast<__nv_bfloat16*>(block + sw128_offset(row_offset + first + r, c % 64)) = q;
+        packed[r][j] = __bfloat162float(q);
+        plain[r][j] = v[r];
+      }
     }
     __syncthreads();
     if (warp == 0 && lane < here && wsum) {
@@ -66,7 +70,7 @@ __global__ void __launch_bounds__(kPackThreads)
 
 int launch_pack_weight(const float* w, int rows, int k, const float* gamma, const float* beta, uint8_t* image,
                        int row_offset, int image_rows, float* wsum, float* bias, cudaStream_t stream, float scale) {
-  pack_weight_kernel<<<(rows + kPackRows - 1) / kPackRows, kPackThreads, 0, stream>>>(
+  pack_weight_kernel<<<(rows + kPackRows - 1) / kPackRows, kPackColumns, 0, stream>>>(
       w, rows, k, gamma, beta, image, row_offset, image_rows, wsum, bias, scale);
   return static_cast<int>(cudaGetLastError());
 }
