@@ -3,10 +3,12 @@
 //
 // Measured on one B200 (device time, L2 holding other data; a plain copy moves 6.5 TB/s):
 //   LayerNorm, 262144 x 128 bf16 (a pair tensor of 512 tokens)   forward 21 us (6.4 TB/s), writing a
-//     checkpoint too 29 us (5.8); backward 36 us (5.6), from a checkpoint 37 us (4.6), and 3 us for the sums
+//     checkpoint too 29 us (5.8); backward 36 us (5.6), from a checkpoint 37 us (4.6), and 4 us for the sums
 //     over the blocks. With rows loaded straight to registers instead of rings the four took 32 / 43 / 45 / 50 us:
-//     what was in flight was limited by the registers, at 16 warps an SM. With a checkpoint the conversions
-//     weigh as well (58 and 60% of issue slots in a profile of these two at 30 and 39 us).
+//     what was in flight was limited by the registers, at 16 warps an SM. With a checkpoint, work on the
+//     values weighs as well: 59 and 62% of issue slots in a profile of these two, the memory's pins at 46 and 41%.
+//     (The backward pass from a checkpoint has 4 to 8 bytes of a thread's registers spilled where rows are
+//     full, the forward pass of 1025 to 4096 channels in whole blocks of 16 bytes 16 to 40.)
 //   LayerNorm, 4099 x 4096 bf16 with a checkpoint   19 us + 25 us + 4 us
 //   checkpoint, 524288 x 64 bf16   packed in 15 us, read back in 12 us
 //   gated unit, 65536 x 2 x 512 bf16 with a checkpoint   49 us (5.5 TB/s), backward 50 us (4.1)
