@@ -270,12 +270,19 @@ class _PairOp(MasterWeights, nn.Module):
         if trains or cached is None or cached[0] != key:
             with torch.no_grad():
                 image = pack(dict(self.state_dict()))
+            image._streams = set()  # whose readers the allocator knows of
             if not (trains or captured):
                 self._packed = (key, image)
         else:
             image = cached[1]
         if captured:
             capture.keep_image(self, image)
+        elif (device := image.get_device()) >= 0:
+            # it is replaced one day, perhaps by a call on another stream than its readers': its memory waits for them
+            stream = torch._C._cuda_getCurrentRawStream(device)
+            if stream not in image._streams:
+                image.record_stream(torch.cuda.current_stream(device))
+                image._streams.add(stream)
         return image
 
     def _train(self, run, *args) -> Tensor:

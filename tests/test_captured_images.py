@@ -195,3 +195,29 @@ def test_a_captured_image_of_the_token_transformer_outlives_changed_weights(monk
         block.weight.add_(1.0)
     block._pack(torch.device("cpu"))
     assert alive(made) == [True, True]
+
+
+def test_an_image_is_recorded_on_the_streams_that_read_it(packs, monkeypatch):
+    """So that the memory of one that is replaced waits for them; a captured one is held instead."""
+
+    class Image:
+        def __init__(self):
+            self.streams = []
+
+        def get_device(self):
+            return 0
+
+        def record_stream(self, stream):
+            self.streams.append(stream)
+
+    module, image = op(128), Image()
+    for stream in ("one", "two", "one"):
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda device, s=stream: s)
+        monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index, s=stream: hash(s), raising=False)
+        assert module._cached_pack(lambda weights: image) is image
+    assert image.streams == ["one", "two"]
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_initialized", lambda: True)
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        module._cached_pack(lambda weights: image)
+    assert len(image.streams) == 2

@@ -48,3 +48,28 @@ def test_replays_between_training_steps(d, shape, frozen):
     assert torch.equal(again(x), now) and torch.equal(graphed(x), want)
     torch.cuda.synchronize()
     assert _lib.device_error() == 0
+
+
+def test_the_memory_of_a_replaced_image_waits_for_another_streams_reader():
+    torch.manual_seed(0)
+    module = Transition(128, 4).cuda()
+    module.set_backend("b200")
+    x = torch.randn(1, 20, 20, 128, device="cuda").to(BF16)
+    with torch.no_grad():
+        want = module(x)
+        image = module._packed[1]
+        address, size = image.data_ptr(), image.numel()
+        del image
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(100_000_000)  # about 50 ms
+            got = module(x)
+        module.squeeze.weight.mul_(2.0)
+        module(x)  # replaces the image
+        others = [torch.zeros(size, dtype=torch.uint8, device="cuda") for _ in range(8)]
+        assert not side.query() and address not in [t.data_ptr() for t in others]
+        side.synchronize()
+    assert torch.equal(got, want)
+    torch.cuda.synchronize()
+    assert _lib.device_error() == 0
