@@ -1,5 +1,5 @@
-// The torch-facing calls of the training operators: argument checks, outputs, workspaces, device and
-// stream, then one call of the C ABI (include/foldforge_b200.h). A call of one token's row costs what the
+// The torch-facing calls of the training operators and of those around an attention: argument checks,
+// outputs, workspaces, device and stream, then one call of the C ABI (include/foldforge_b200.h). A call of one token's row costs what the
 // host needs to issue it: about 14 us by ctypes from Python, 7 us from here.
 //
 // The entry points come in as addresses (bind()), so this module does not link the kernels' library.
@@ -35,6 +35,11 @@ struct Entries {
   decltype(&ffb_weight_grad) weight_grad;
   decltype(&ffb_swiglu_train_fwd) swiglu_train_fwd;
   decltype(&ffb_swiglu_bwd) swiglu_bwd;
+  decltype(&ffb_rotary_fwd) rotary_fwd;
+  decltype(&ffb_qk_norm_rotary_fwd) qk_norm_rotary_fwd;
+  decltype(&ffb_qk_norm_rotary_bwd_workspace_bytes) qk_norm_rotary_bwd_workspace_bytes;
+  decltype(&ffb_qk_norm_rotary_bwd) qk_norm_rotary_bwd;
+  decltype(&ffb_dropout) dropout;
 } entries;
 
 [[noreturn]] void raise(const char* name, int status, const std::string& message) {
@@ -284,6 +289,192 @@ std::tuple<Tensor, OptTensor> swiglu_backward(const Tensor& dh_in, const Tensor&
   return {dab, out};
 }
 
+// ---- around an attention: heads [tokens, heads, channels] or [batch, tokens, heads, channels] as they lie
+constexpr int64_t kMostHeadChannels = 512;
+
+struct Heads {
+  Tensor t;
+  ffb_heads view{};
+  const ffb_heads* at() const { return t.defined() ? &view : nullptr; }
+};
+
+// `like`: the tensor whose dtype, device and (but for the heads, where `heads`) shape this one has; an output's
+// channels have to be dense as they lie.
+Heads heads_of(const char* name, const char* what, const Tensor& t_in, const Tensor& like, bool heads, bool output = false) {
+  const int64_t dim = like.dim();
+  bool same = t_in.dim() == dim && t_in.scalar_type() == like.scalar_type() && t_in.device() == like.device();
+  for (int64_t i = 0; same && i < dim; ++i) same = t_in.size(i) == like.size(i) || (heads && i == dim - 2);
+  if (!same) refuse(name, std::string(what) + " is " + text(t_in) + ", beside " + text(like));
+  Heads h;
+  const bool dense_rows = t_in.stride(-1) == 1 || t_in.size(-1) <= 1;
+  if (output && !dense_rows) refuse(name, std::string(what) + "'s channels are " + std::to_string(t_in.stride(-1)) + " elements apart");
+  h.t = dense_rows ? t_in : t_in.contiguous();
+  h.view = {h.t.data_ptr(), dim == 4 ? h.t.stride(0) : 0, h.t.stride(dim - 3), h.t.stride(dim - 2), h.t.size(dim - 2)};
+  return h;
+}
+
+// q, the first tensor of a call
+Heads first_heads(const char* name, const Tensor& q) {
+  if (q.scalar_type() != at::kBFloat16 && q.scalar_type() != at::kFloat)
+    refuse(name, std::string("dtype ") + c10::toString(q.scalar_type()) + " (takes bf16 or fp32)");
+  if (q.dim() != 3 && q.dim() != 4) refuse(name, "shape " + text(q.sizes()) + " is neither [tokens, heads, channels] nor [batch, tokens, heads, channels]");
+  if (q.size(-1) < 1 || q.size(-1) > kMostHeadChannels)
+    refuse(name, std::to_string(q.size(-1)) + " channels a head (1 to " + std::to_string(kMostHeadChannels) + ")");
+  return heads_of(name, "q", q, q, false);
+}
+
+Heads output_heads(const char* name, const char* what, const Heads& x, const OptTensor& out) {
+  return heads_of(name, what, out ? *out : like(x.t, x.t.sizes()), x.t, false, true);
+}
+
+using Table = std::tuple<Tensor, Tensor, int64_t, bool>;  // quarter turns, the pairs' axes, axes, interleaved
+
+struct Rotary {
+  Tensor positions, quarters, axes;
+  ffb_rotary params{};
+};
+Rotary rotary_of(const char* name, const Tensor& q, const OptTensor& positions, const std::optional<Table>& table, bool inverse) {
+  Rotary r;
+  if (positions.has_value() != table.has_value()) refuse(name, "positions and their table go together");
+  if (!table) return r;
+  int64_t axes;
+  bool interleaved;
+  std::tie(r.quarters, r.axes, axes, interleaved) = *table;
+  r.positions = *positions;
+  const int64_t pairs = r.quarters.numel(), d = r.positions.dim(), qd = q.dim();
+  if (r.quarters.dim() != 1 || r.quarters.scalar_type() != at::kDouble || r.axes.sizes() != r.quarters.sizes() ||
+      r.axes.scalar_type() != at::kInt || r.quarters.device() != q.device() || r.axes.device() != q.device() ||
+      !r.quarters.is_contiguous() || !r.axes.is_contiguous())
+    refuse(name, "the table is " + text(r.quarters) + " and " + text(r.axes) + ", beside " + text(q));
+  if (pairs > q.size(-1) / 2) refuse(name, std::to_string(pairs) + " pairs of " + std::to_string(q.size(-1)) + " channels");
+  const at::ScalarType type = r.positions.scalar_type();
+  if (type != at::kInt && type != at::kLong && type != at::kFloat)
+    refuse(name, std::string("positions are ") + c10::toString(type) + " (takes int32, int64 or fp32)");
+  const int64_t batch = qd == 4 ? q.size(0) : 1;
+  if (r.positions.device() != q.device() || d < 2 || d > 3 || r.positions.size(d - 2) != q.size(qd - 3) ||
+      (d == 3 && r.positions.size(0) != batch && r.positions.size(0) != 1))
+    refuse(name, "positions are " + text(r.positions) + ", beside " + text(q));
+  if (axes < 1 || r.positions.size(d - 1) < axes)
+    refuse(name, "positions of " + std::to_string(r.positions.size(d - 1)) + " axes for a table of " + std::to_string(axes));
+  r.params = {r.positions.data_ptr(), d == 3 && r.positions.size(0) > 1 ? r.positions.stride(0) : 0, r.positions.stride(d - 2),
+              r.positions.stride(d - 1), r.quarters.data_ptr<double>(), r.axes.data_ptr<int32_t>(),
+              type == at::kInt ? FFB_POSITION_I32 : type == at::kLong ? FFB_POSITION_I64 : FFB_POSITION_F32,
+              static_cast<int>(axes), static_cast<int>(pairs), interleaved, inverse};
+  return r;
+}
+
+int64_t batch_of(const Tensor& q) { return q.dim() == 4 ? q.size(0) : 1; }
+int64_t tokens_of(const Tensor& q) { return q.size(-3); }
+
+std::tuple<Tensor, OptTensor> heads_forward(const char* name, bool norm, const Tensor& q_in, const OptTensor& k_in,
+                                            const OptTensor& positions, const std::optional<Table>& table, bool inverse,
+                                            const OptTensor& q_weight, const OptTensor& k_weight, double eps,
+                                            const OptTensor& q_out_in, const OptTensor& k_out_in) {
+  at::NoGradGuard no_grad;
+  const Heads q = first_heads(name, q_in);
+  Heads k, q_out, k_out;
+  if (k_in) k = heads_of(name, "k", *k_in, q_in, true);
+  if (!k_in && (k_weight || k_out_in)) refuse(name, "k's weight or output without k");
+  const Rotary r = rotary_of(name, q_in, positions, table, inverse);
+  OptTensor qw, kw;
+  if (q_weight) qw = vector(name, "q's weight", q.t, *q_weight);
+  if (k_weight) kw = vector(name, "k's weight", q.t, *k_weight);
+  if (q_out_in) output_heads(name, "q's output", q, q_out_in);
+  if (k_out_in) output_heads(name, "k's output", k, k_out_in);
+  need_cuda(name, q.t);
+  Call call(q.t);
+  q_out = output_heads(name, "q's output", q, q_out_in);
+  if (k_in) k_out = output_heads(name, "k's output", k, k_out_in);
+  const int channels = static_cast<int>(q.t.size(-1)), dtype = dtype_of(q.t.scalar_type());
+  const int64_t batch = batch_of(q.t), tokens = tokens_of(q.t);
+  check(name, norm ? entries.qk_norm_rotary_fwd(q.at(), k.at(), q_out.at(), k_out.at(), pointer(qw), pointer(kw),
+                                                static_cast<float>(eps), &r.params, batch, tokens, channels, dtype, call.stream)
+                   : entries.rotary_fwd(q.at(), k.at(), q_out.at(), k_out.at(), &r.params, batch, tokens, channels, dtype, call.stream));
+  return {q_out.t, k_in ? OptTensor(k_out.t) : OptTensor()};
+}
+
+std::tuple<Tensor, OptTensor> rotary(const Tensor& q, const OptTensor& k, const Tensor& positions, const Table& table, bool inverse,
+                                     const OptTensor& q_out, const OptTensor& k_out) {
+  return heads_forward("rotary", false, q, k, positions, table, inverse, {}, {}, 0.0, q_out, k_out);
+}
+
+std::tuple<Tensor, OptTensor> qk_norm_rotary(const Tensor& q, const OptTensor& k, const OptTensor& positions,
+                                             const std::optional<Table>& table, const OptTensor& q_weight, const OptTensor& k_weight,
+                                             double eps, const OptTensor& q_out, const OptTensor& k_out) {
+  return heads_forward("qk_norm_rotary", true, q, k, positions, table, false, q_weight, k_weight, eps, q_out, k_out);
+}
+
+std::tuple<Tensor, OptTensor, OptTensor, OptTensor> qk_norm_rotary_backward(
+    const Tensor& dq_out, const OptTensor& dk_out, const Tensor& q_in, const OptTensor& k_in, const OptTensor& positions,
+    const std::optional<Table>& table, const OptTensor& q_weight, const OptTensor& k_weight, double eps, bool weight_gradient,
+    const OptTensor& dq_in, const OptTensor& dk_in) {
+  at::NoGradGuard no_grad;
+  const char* name = "qk_norm_rotary_backward";
+  const Heads q = first_heads(name, q_in);
+  const Heads dy_q = heads_of(name, "the gradient of q's output", dq_out, q_in, false);
+  Heads k, dy_k, dq, dk;
+  if (k_in.has_value() != dk_out.has_value()) refuse(name, "k and the gradient of its output go together");
+  if (!k_in && (k_weight || dk_in)) refuse(name, "k's weight or gradient without k");
+  if (k_in) {
+    k = heads_of(name, "k", *k_in, q_in, true);
+    dy_k = heads_of(name, "the gradient of k's output", *dk_out, *k_in, false);
+  }
+  const Rotary r = rotary_of(name, q_in, positions, table, false);
+  OptTensor qw, kw, dqw, dkw, ws;
+  if (q_weight) qw = vector(name, "q's weight", q.t, *q_weight);
+  if (k_weight) kw = vector(name, "k's weight", q.t, *k_weight);
+  if (dq_in) output_heads(name, "q's gradient", q, dq_in);
+  if (dk_in) output_heads(name, "k's gradient", k, dk_in);
+  need_cuda(name, q.t);
+  Call call(q.t);
+  dq = output_heads(name, "q's gradient", q, dq_in);
+  if (k_in) dk = output_heads(name, "k's gradient", k, dk_in);
+  const int64_t batch = batch_of(q.t), tokens = tokens_of(q.t), c = q.t.size(-1);
+  const int channels = static_cast<int>(c), dtype = dtype_of(q.t.scalar_type());
+  size_t size = 0;
+  if (weight_gradient && (qw || kw)) {
+    if (qw) dqw = floats(q.t, {c});
+    if (kw) dkw = floats(q.t, {c});
+    size = entries.qk_norm_rotary_bwd_workspace_bytes(batch, tokens, q.view.heads, k_in ? k.view.heads : 0, channels, dtype);
+    if (size) ws = bytes(q.t, static_cast<int64_t>(size));
+  }
+  check(name, entries.qk_norm_rotary_bwd(dy_q.at(), dy_k.at(), q.at(), k.at(), dq.at(), dk.at(), pointer(qw), pointer(kw), pointer(dqw),
+                                         pointer(dkw), static_cast<float>(eps), &r.params, ws ? ws->data_ptr() : nullptr, size, batch,
+                                         tokens, channels, dtype, call.stream));
+  return {dq.t, k_in ? OptTensor(dk.t) : OptTensor(), dqw, dkw};
+}
+
+// x dropped and scaled (plus the residual) in out_dtype; axes: those whose positions share a mask, ascending
+Tensor dropout(const char* name, const Tensor& x_in, double p, uint64_t seed, uint64_t offset, const OptTensor& device_seed,
+               const OptTensor& residual_in, const std::vector<int64_t>& axes, at::ScalarType out_dtype) {
+  at::NoGradGuard no_grad;
+  for (const at::ScalarType t : {x_in.scalar_type(), out_dtype})
+    if (t != at::kBFloat16 && t != at::kFloat) refuse(name, std::string("dtype ") + c10::toString(t) + " (takes bf16 or fp32)");
+  if (!(p >= 0.0 && p <= 1.0)) refuse(name, "p = " + std::to_string(p));
+  int64_t outer = 1, shared = 1, inner = 1;
+  if (axes.empty()) {
+    inner = x_in.numel();
+  } else {
+    for (size_t i = 0; i < axes.size(); ++i)
+      if (axes[i] < 0 || axes[i] >= x_in.dim() || axes[i] != axes[0] + static_cast<int64_t>(i))
+        refuse(name, "shared axes " + text(axes) + " of " + text(x_in.sizes()) + " (axes beside one another)");
+    for (int64_t i = 0; i < x_in.dim(); ++i) (i < axes.front() ? outer : i > axes.back() ? inner : shared) *= x_in.size(i);
+  }
+  OptTensor residual;
+  if (residual_in) residual = beside(name, "residual", x_in, *residual_in, x_in.sizes(), out_dtype);
+  if (device_seed && (device_seed->scalar_type() != at::kLong || device_seed->dim() != 1 || device_seed->size(0) != 2 ||
+                      !device_seed->is_contiguous() || device_seed->device() != x_in.device()))
+    refuse(name, "seed is " + text(*device_seed) + ", not Long [2] on " + x_in.device().str());
+  need_cuda(name, x_in);
+  Call call(x_in);
+  const Tensor x = dense(x_in);
+  const Tensor out = at::empty(x.sizes(), x.options().dtype(out_dtype).requires_grad(false));
+  check(name, entries.dropout(x.data_ptr(), dtype_of(x.scalar_type()), residual ? residual->data_ptr() : nullptr, out.data_ptr(),
+                              dtype_of(out_dtype), outer, shared, inner, p, seed, offset,
+                              device_seed ? reinterpret_cast<const uint64_t*>(device_seed->data_ptr<int64_t>()) : nullptr, call.stream));
+  return out;
+}
+
 template <typename F>
 void take(const py::dict& addresses, const char* name, F& f) {
   f = reinterpret_cast<F>(addresses[name].cast<uintptr_t>());
@@ -303,6 +494,11 @@ PYBIND11_MODULE(_binding, m) {
     take(a, "ffb_weight_grad", entries.weight_grad);
     take(a, "ffb_swiglu_train_fwd", entries.swiglu_train_fwd);
     take(a, "ffb_swiglu_bwd", entries.swiglu_bwd);
+    take(a, "ffb_rotary_fwd", entries.rotary_fwd);
+    take(a, "ffb_qk_norm_rotary_fwd", entries.qk_norm_rotary_fwd);
+    take(a, "ffb_qk_norm_rotary_bwd_workspace_bytes", entries.qk_norm_rotary_bwd_workspace_bytes);
+    take(a, "ffb_qk_norm_rotary_bwd", entries.qk_norm_rotary_bwd);
+    take(a, "ffb_dropout", entries.dropout);
   });
   m.def("checkpoint_pack", &checkpoint_pack);
   m.def("checkpoint_unpack", &checkpoint_unpack);
@@ -311,4 +507,8 @@ PYBIND11_MODULE(_binding, m) {
   m.def("weight_grad", &weight_grad);
   m.def("swiglu_train", &swiglu_train);
   m.def("swiglu_backward", &swiglu_backward);
+  m.def("rotary", &rotary);
+  m.def("qk_norm_rotary", &qk_norm_rotary);
+  m.def("qk_norm_rotary_backward", &qk_norm_rotary_backward);
+  m.def("dropout", &dropout);
 }

@@ -197,5 +197,49 @@ size_t weight_grad_workspace_bytes(int64_t rows, int n, int k, bool codes);
 int weight_grad_forward(const void* dy, const void* x, const uint8_t* codes, const uint8_t* scales, float* dw,
                         void* workspace, int64_t rows, int n, int k, const DeviceInfo& info, cudaStream_t stream);
 
-}  // namespace ffb
+// ---- around an attention: norm of q and k per head with positions' rotation (heads.cu), dropout (dropout.cu)
+constexpr int kMaxHeadChannels = 512;  // a head is held in one warp's registers
+constexpr int kMaxPositionAxes = 16;
 
+// [batch, tokens, heads, channels], channels dense, strides in elements
+struct HeadView {
+  void* data;
+  int64_t batch, token, head;
+};
+enum PositionType : int { kPositionI32 = 0, kPositionI64 = 1, kPositionF32 = 2 };
+struct RotaryParams {
+  const void* positions;  // [batch, tokens, axes], strides in elements
+  int type, axes;
+  int64_t batch, token, axis;
+  const double* quarters;  // [pairs]: quarter turns a unit of position
+  const int32_t* pair_axes;
+  int pairs, interleaved, inverse;
+};
+struct HeadsParams {
+  HeadView x[2], dy[2], out[2];  // q and k; dy: backward only
+  const float* weight[2];        // null: 1
+  float* dweight[2];             // null: not wanted
+  int heads[2];
+  int batch, tokens, channels;
+  float eps;
+  int norm;
+  RotaryParams rotary;
+};
+size_t heads_bwd_workspace_bytes(int64_t tokens, int q_heads, int k_heads, int channels, int is_f32);
+int launch_heads(const HeadsParams& p, int is_f32, cudaStream_t stream);
+int launch_heads_bwd(const HeadsParams& p, void* workspace, int is_f32, cudaStream_t stream);
+
+// out = residual + keep(x) scale; x as [outer, shared, inner], one mask for the shared positions
+struct DropoutParams {
+  const void* x;
+  const void* residual;  // of out's type, or null
+  void* out;
+  int64_t outer, shared, inner;
+  uint64_t threshold;  // an element stays where its 32-bit word is at least this
+  float scale;
+  uint64_t seed, offset;
+  const uint64_t* device_seed;  // [seed, offset to add] read by the kernel, or null
+};
+int launch_dropout(const DropoutParams& p, int x_is_f32, int out_is_f32, cudaStream_t stream);
+
+}  // namespace ffb

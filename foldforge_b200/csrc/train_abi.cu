@@ -1,4 +1,6 @@
-// The C ABI of the training operators: argument checks around train.cu and wgrad.cu.
+// The C ABI of the training operators: argument checks around train.cu, wgrad.cu and dropout.cu.
+#include <math.h>
+
 #include "../../include/foldforge_b200.h"
 #include "abi_util.h"
 #include "kernels.h"
@@ -196,6 +198,39 @@ int ffb_swiglu_bwd(const void* dh, const void* ab, const uint8_t* codes, const u
   if (st != FFB_OK) return st;
   return cuda_status(launch_swiglu_bwd(dh, ab, codes, scales, dab, out, rows, h, dtype == FFB_F32, as_stream(stream)),
                      "swiglu_bwd launch");
+}
+
+int ffb_dropout(const void* x, int x_dtype, const void* residual, void* out, int out_dtype, int64_t outer,
+                int64_t shared, int64_t inner, double p, uint64_t seed, uint64_t offset, const uint64_t* device_seed,
+                void* stream) {
+  if (outer < 0 || shared < 0 || inner < 0)
+    return fail(FFB_ERR_ARG, "dropout: outer=%lld shared=%lld inner=%lld", (long long)outer, (long long)shared, (long long)inner);
+  const int64_t most = int64_t(1) << 46;
+  if ((shared > 0 && outer > most / shared) || (inner > 0 && outer * shared > most / inner))
+    return fail(FFB_ERR_UNSUPPORTED, "dropout: too many elements");
+  if ((x_dtype != FFB_BF16 && x_dtype != FFB_F32) || (out_dtype != FFB_BF16 && out_dtype != FFB_F32))
+    return fail(FFB_ERR_UNSUPPORTED, "dropout: dtypes %d and %d", x_dtype, out_dtype);
+  if (!(p >= 0.0 && p <= 1.0)) return fail(FFB_ERR_ARG, "dropout: p = %g", p);
+  const int64_t n = outer * shared * inner;
+  if (n == 0) return FFB_OK;
+  if (!x || !out) return fail(FFB_ERR_ARG, "dropout: null pointer");
+  if (off_element(x, x_dtype) || off_element(out, out_dtype) || off_element(residual, out_dtype) ||
+      (reinterpret_cast<uintptr_t>(device_seed) & 7u) != 0)
+    return fail(FFB_ERR_ARG, "dropout: misaligned pointer");
+  const auto overlap = [&](const void* a, int a_dtype) {
+    const char *pa = static_cast<const char*>(a), *po = static_cast<const char*>(out);
+    if (a == nullptr || (a == out && a_dtype == out_dtype)) return false;
+    return pa < po + n * element_size(out_dtype) && po < pa + n * element_size(a_dtype);
+  };
+  if (overlap(x, x_dtype) || overlap(residual, out_dtype)) return fail(FFB_ERR_ARG, "dropout: out overlaps an input");
+  DeviceInfo info;
+  const int st = device_info(&info);
+  if (st != FFB_OK) return st;
+  // at most 2^32, which no word reaches: with p = 1 all are dropped
+  const uint64_t threshold = static_cast<uint64_t>(llrint(p * 4294967296.0));
+  const DropoutParams d{x, residual, out, outer, shared, inner, threshold, p < 1.0 ? static_cast<float>(1.0 / (1.0 - p)) : 0.f,
+                        seed, offset, device_seed};
+  return cuda_status(launch_dropout(d, x_dtype == FFB_F32, out_dtype == FFB_F32, as_stream(stream)), "dropout launch");
 }
 
 }  // extern "C"

@@ -9,6 +9,9 @@ before anything is launched.
 from __future__ import annotations
 
 import ctypes
+import math
+import operator
+from collections.abc import Sequence
 from typing import NamedTuple
 
 import torch
@@ -599,3 +602,119 @@ def swiglu_backward(dh: Tensor, saved: Tensor | Checkpoint8, *, output: bool = F
         kept, packed = _unpacked("swiglu_backward", saved, (*dh.shape[:-1], 2 * dh.shape[-1]) if dh.dim() else (), dh.dtype)
     dab, out = _lib.binding().swiglu_backward(dh, kept, packed, output)
     return (dab, out) if output else dab
+
+
+# --------------------------------------------------------------------------- around an attention
+# csrc/heads.cu, csrc/dropout.cu behind csrc/binding.cpp. Heads are [tokens, heads, channels] or [batch, tokens,
+# heads, channels] in bf16 or fp32, at most 512 channels, of any strides (read as they lie where a head's channels
+# are dense: q and k of a projection's [q | k | v] rows, or of a head-major tensor, are views).
+class RotaryTable(NamedTuple):
+    """Which channels a rotation turns and how fast (:func:`rotary_table`): for each pair its quarter turns
+    a unit of position (fp64) and its axis of the positions (int32), the number of axes, and how channels are
+    paired."""
+
+    quarters: Tensor
+    pair_axes: Tensor
+    axes: int
+    interleaved: bool
+
+
+def rotary_frequencies(channels: int, base: float = 10000.0) -> list[float]:
+    """The geometric ladder ``base^(-2 i / channels)`` of ``channels // 2`` pairs, in radians a position."""
+    return [base ** (-2.0 * i / channels) for i in range(channels // 2)]
+
+
+def rotary_table(frequencies: Sequence[float] | Tensor, axes: Sequence[int] | None = None, *, interleaved: bool = False,
+                 device: torch.device | str = "cuda") -> RotaryTable:
+    """The table of a rotation that turns a head's first ``2 len(frequencies)`` channels: pair i by
+    ``frequencies[i]`` radians a unit of the positions' axis ``axes[i]`` (0 without ``axes``). A pair is channels
+    ``(i, i + len)``, or with ``interleaved`` ``(2 i, 2 i + 1)``. For positions of several axes, give each axis a
+    ladder of its own: ``frequencies = rotary_frequencies(44) + rotary_frequencies(42) + ..``, ``axes = [0] * 22 +
+    [1] * 21 + ..``. Made once and kept beside the weights."""
+    f = torch.as_tensor(frequencies, dtype=torch.float64, device="cpu").detach()
+    if f.dim() != 1 or not bool(torch.isfinite(f).all()):
+        raise ValueError("frequencies must be a list of finite numbers")
+    a = [0] * f.numel() if axes is None else [int(i) for i in axes]
+    if len(a) != f.numel() or any(not 0 <= i < 16 for i in a):
+        raise ValueError(f"axes must name one of at most 16 axes for each of {f.numel()} pairs, got {a}")
+    return RotaryTable((f * (2.0 / math.pi)).to(device), torch.tensor(a, dtype=torch.int32).to(device), max(a, default=0) + 1,
+                       bool(interleaved))
+
+
+def rotary(q: Tensor, k: Tensor | None, positions: Tensor, table: RotaryTable, *, inverse: bool = False,
+           out: tuple[Tensor, Tensor | None] | None = None) -> tuple[Tensor, Tensor | None]:
+    """``q`` and ``k`` (of other heads, or ``None``) turned by their tokens' ``positions [tokens, axes]`` or ``[batch,
+    tokens, axes]`` (int32, int64 or fp32), with ``inverse`` back: also the gradients of q and k from those of the
+    outputs. ``out``: tensors to write instead of new ones (of any strides with dense channels; q and k
+    themselves, a cache's slots)."""
+    q_out, k_out = out or (None, None)
+    return _lib.binding().rotary(q, k, positions, table, inverse, q_out, k_out)
+
+
+def qk_norm_rotary(q: Tensor, k: Tensor | None, positions: Tensor | None, table: RotaryTable | None,
+                   q_weight: Tensor | None, k_weight: Tensor | None, eps: float = 1e-6, *,
+                   out: tuple[Tensor, Tensor | None] | None = None) -> tuple[Tensor, Tensor | None]:
+    """Each head of ``q`` and ``k`` divided by the root of its channels' mean square (plus ``eps``), times its weight
+    ``[channels]`` (``None``: 1) and turned as by :func:`rotary` (``positions`` and ``table`` ``None``: not turned).
+    The backward pass reads ``q`` and ``k`` themselves, which may not change until then."""
+    q_out, k_out = out or (None, None)
+    return _lib.binding().qk_norm_rotary(q, k, positions, table, q_weight, k_weight, eps, q_out, k_out)
+
+
+def qk_norm_rotary_backward(dq_out: Tensor, dk_out: Tensor | None, q: Tensor, k: Tensor | None, positions: Tensor | None,
+                            table: RotaryTable | None, q_weight: Tensor | None, k_weight: Tensor | None,
+                            eps: float = 1e-6, *, weight_gradient: bool = True,
+                            out: tuple[Tensor, Tensor | None] | None = None):
+    """``(dq, dk, dq_weight, dk_weight)`` of :func:`qk_norm_rotary` from its outputs' gradients: ``dq`` and ``dk`` in q's
+    dtype (written to ``out`` where given), the weights' in fp32, summed over tokens and heads in a fixed order
+    (``None`` without the weight or ``weight_gradient``)."""
+    dq, dk = out or (None, None)
+    return _lib.binding().qk_norm_rotary_backward(dq_out, dk_out, q, k, positions, table, q_weight, k_weight, eps, weight_gradient,
+                                                  dq, dk)
+
+
+class DropoutSaved(NamedTuple):
+    """What a dropout's backward pass draws its mask from, and the activations' shape and dtypes."""
+
+    p: float
+    seed: int | Tensor
+    offset: int
+    shared: tuple[int, ...]
+    shape: torch.Size
+    dtype: torch.dtype
+    out_dtype: torch.dtype
+
+
+def _dropout(name: str, x: Tensor, residual: Tensor | None, saved: DropoutSaved, out_dtype: torch.dtype) -> Tensor:
+    seed = saved.seed
+    on_device = isinstance(seed, torch.Tensor)
+    return _lib.binding().dropout(name, x, saved.p, 0 if on_device else seed & (1 << 64) - 1, saved.offset & (1 << 64) - 1,
+                                  seed if on_device else None, residual, saved.shared, out_dtype)
+
+
+def dropout_train(x: Tensor, p: float, seed: int | Tensor, *, offset: int = 0, residual: Tensor | None = None,
+                  shared: int | tuple[int, ...] | None = None) -> tuple[Tensor, DropoutSaved]:
+    """``residual + keep(x) / (1 - p)`` in ``residual``'s dtype (or without it ``keep(x) / (1 - p)`` in x's), an element
+    of ``x`` (bf16 or fp32) kept with probability ``1 - p`` and else counted as 0, whatever it holds; and what the
+    backward pass reads (no mask). The choice follows from ``seed``, ``offset`` and the element's place alone:
+    calls of one step take another ``offset`` each. ``shared``: an axis (or axes beside one another) of ``x``
+    whose positions share a mask. ``seed`` as an int64 tensor ``[seed, offset]`` on the device is read by the kernel
+    (its offset adds to ``offset``), so that a captured step draws other masks once the tensor changes; it may
+    not change between a forward pass and its backward pass."""
+    if shared is None:
+        axes: tuple[int, ...] = ()
+    else:
+        axes = tuple(sorted(i + x.dim() if i < 0 else i for i in ((shared,) if isinstance(shared, int) else shared)))
+    out_dtype = x.dtype if residual is None else residual.dtype
+    seed = seed if isinstance(seed, torch.Tensor) else operator.index(seed)
+    saved = DropoutSaved(float(p), seed, operator.index(offset), axes, x.shape, x.dtype, out_dtype)
+    return _dropout("dropout_train", x, residual, saved, out_dtype), saved
+
+
+def dropout_backward(dout: Tensor, saved: DropoutSaved) -> Tensor:
+    """The gradient of x of :func:`dropout_train`, in x's dtype, from the output's gradient (which is the
+    residual's own)."""
+    if dout.shape != saved.shape or dout.dtype != saved.out_dtype:
+        raise _lib.UnsupportedCall("dropout_backward", 2, f"the gradient is {dout.dtype} {tuple(dout.shape)}, not {saved.out_dtype} "
+                                                          f"{tuple(saved.shape)}")
+    return _dropout("dropout_backward", dout, None, saved, saved.dtype)

@@ -388,6 +388,64 @@ int ffb_swiglu_train_fwd(const void* ab, void* out, uint8_t* codes, uint8_t* sca
 int ffb_swiglu_bwd(const void* dh, const void* ab, const uint8_t* codes, const uint8_t* scales, void* dab, void* out,
                    int64_t rows, int h, int dtype, void* stream);
 
+/* ---- Around an attention: the norm of queries and keys of each head with the rotation by their positions,
+ * and dropout from a counter-based generator.
+ *
+ * ffb_heads: a tensor [batch, tokens, heads, channels], its channels dense, the other strides in elements
+ * (0 repeats; an output's positions have to be distinct): a head-major tensor, or q as it lies in a
+ * projection's [q | k | v] rows, is a view of this form.
+ * ffb_rotary: a head's first 2 pairs channels are turned in pairs, (i, i + pairs) or with `interleaved`
+ * (2 i, 2 i + 1), by the angle positions[.., pair_axes[i]] * quarters[i] in quarter turns (found in 64
+ * bits), with `inverse` by the opposite angle; the channels behind them stay. positions: [batch, tokens,
+ * axes] of position_type (ffb_position_type), strides in elements (0 repeats); a pair whose axis is not one
+ * of `axes` becomes NaN. pairs may be 0 (positions, quarters and pair_axes are then not read).
+ *
+ * ffb_rotary_fwd: q_out, k_out = the rotation of q, k.
+ * ffb_qk_norm_rotary_fwd: the rotation of x rstd weight, rstd = 1 / sqrt(mean(x^2) + eps) over a head's
+ *   channels; q_weight, k_weight [channels] fp32 or NULL (1).
+ * ffb_qk_norm_rotary_bwd: from the outputs' gradients and q, k: g = the rotation back of dy, w = g weight,
+ *   xh = x rstd, dx = rstd (w - xh mean(w xh)), dweight = sum over tokens and heads of g xh (fp32, a fixed
+ *   order of sums; NULL where not wanted).
+ * channels <= 512, batch tokens < 2^31 - 1 (0: nothing but zero weight gradients); k, its outputs and weights may
+ * be left out (k NULL). dtype (ffb_dtype) is the activations'. An output may be its own input (the same
+ * address and strides); else outputs overlap neither inputs nor each other, but may interleave with them
+ * in rows of one size (q and k of the same [q | k | v] rows).
+ *
+ * ffb_dropout: out = residual + keep x / (1 - p), or without residual (NULL) keep x / (1 - p); a dropped x
+ *   counts as 0 whatever it holds. x is read as [outer, shared, inner], the mask is of [outer, inner]: element
+ *   m stays where word m % 4 of Philox4x32-10 (Salmon et al., "Parallel random numbers: as easy as 1, 2, 3",
+ *   2011) with key = seed and counter = (m / 4, offset) is at least p 2^32 (rounded). x and out (and the
+ *   residual with it) may differ in dtype. device_seed (or NULL): two 64-bit numbers on the device, read by the
+ *   kernel: the seed, taken in the place of `seed`, and a number added to offset. 0 <= p <= 1. The backward pass
+ *   is the same call on the output's gradient without residual. out may be x or the residual. */
+typedef struct ffb_heads {
+  void* data;
+  int64_t batch_stride, token_stride, head_stride;
+  int64_t heads;
+} ffb_heads;
+typedef enum ffb_position_type { FFB_POSITION_I32 = 0, FFB_POSITION_I64 = 1, FFB_POSITION_F32 = 2 } ffb_position_type;
+typedef struct ffb_rotary {
+  const void* positions;
+  int64_t batch_stride, token_stride, axis_stride;
+  const double* quarters;
+  const int32_t* pair_axes;
+  int position_type, axes, pairs, interleaved, inverse;
+} ffb_rotary;
+int ffb_rotary_fwd(const ffb_heads* q, const ffb_heads* k, const ffb_heads* q_out, const ffb_heads* k_out,
+                   const ffb_rotary* rotary, int64_t batch, int64_t tokens, int channels, int dtype, void* stream);
+int ffb_qk_norm_rotary_fwd(const ffb_heads* q, const ffb_heads* k, const ffb_heads* q_out, const ffb_heads* k_out,
+                           const float* q_weight, const float* k_weight, float eps, const ffb_rotary* rotary,
+                           int64_t batch, int64_t tokens, int channels, int dtype, void* stream);
+size_t ffb_qk_norm_rotary_bwd_workspace_bytes(int64_t batch, int64_t tokens, int64_t q_heads, int64_t k_heads,
+                                              int channels, int dtype);
+int ffb_qk_norm_rotary_bwd(const ffb_heads* dq_out, const ffb_heads* dk_out, const ffb_heads* q, const ffb_heads* k,
+                           const ffb_heads* dq, const ffb_heads* dk, const float* q_weight, const float* k_weight,
+                           float* dq_weight, float* dk_weight, float eps, const ffb_rotary* rotary, void* workspace,
+                           size_t workspace_bytes, int64_t batch, int64_t tokens, int channels, int dtype, void* stream);
+int ffb_dropout(const void* x, int x_dtype, const void* residual, void* out, int out_dtype, int64_t outer,
+                int64_t shared, int64_t inner, double p, uint64_t seed, uint64_t offset, const uint64_t* device_seed,
+                void* stream);
+
 #ifdef __cplusplus
 }
 #endif
