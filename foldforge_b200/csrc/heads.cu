@@ -3,9 +3,12 @@
 //
 // A warp takes a token's heads, a team of lanes a head: a lane holds the same pairs of channels of every
 // head that comes to its team. So the warp finds the token's cosines and sines once for all heads (into
-// shared memory, each pair by one lane), folds the weight into them, and a head costs its loads, one sum over
-// the team and two multiply-adds a channel. In the backward pass a lane also adds up the weight's gradient of
-// its channels over all heads and tokens that it meets.
+// shared memory, each pair by one lane). In the backward pass a lane also adds up the weight's gradient of its
+// channels over all heads and tokens that it meets.
+//
+// Heads come through a ring in shared memory that belongs to the lane alone: each lane copies its own 16 bytes
+// asynchronously a few steps (and tokens) ahead, and needs no barrier to read them. What is in flight then does
+// not depend on registers.
 //
 // Angles: a position times the pair's frequency in quarter turns in 64 bits, less the nearest whole
 // number of them (exact), then sine and cosine in 32 bits of at most an eighth of a turn: a position of 2^20
@@ -26,36 +29,56 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 
-// cosine and sine of pair `j`'s angle at a token
-__device__ __forceinline__ float2 turn_of(const RotaryParams& r, int64_t at, int j) {
-  const int axis = r.pair_axes[j];
-  if (axis < 0 || axis >= r.axes) return make_float2(__int_as_float(0x7FFFFFFF), __int_as_float(0x7FFFFFFF));
-  const int64_t i = at + axis * r.axis;
-  double place;
-  if (r.type == kPositionI64)
-    place = static_cast<double>(static_cast<const int64_t*>(r.positions)[i]);
-  else if (r.type == kPositionI32)
-    place = static_cast<double>(static_cast<const int32_t*>(r.positions)[i]);
-  else
-    place = static_cast<double>(static_cast<const float*>(r.positions)[i]);
-  const double quarters = place * r.quarters[j];
-  const double whole = rint(quarters);
-  float s, c;
-  sincospif(0.5f * static_cast<float>(quarters - whole), &s, &c);
-  // the whole quarter turns, modulo 4
-  const int k = static_cast<int>(whole - 4.0 * rint(0.25 * whole)) & 3;
-  const float cos = k == 0 ? c : k == 1 ? -s : k == 2 ? -c : s;
-  const float sin = k == 0 ? s : k == 1 ? c : k == 2 ? -s : -c;
-  return make_float2(cos, r.inverse ? -sin : sin);
+// Cosine and sine of an angle of at most an eighth of a turn, r quarter turns (|r| <= 1/2): polynomials in r^2
+// through Chebyshev's nodes, off by less than 0.2 steps of 2^-24 before the roundings of their own evaluation.
+__device__ __forceinline__ float2 eighth_turn(float r) {
+  const float t = r * r;
+  const float s = r * fmaf(fmaf(fmaf(-0.0046021491289f, t, 0.0796802192926f), t, -0.6459634900093f), t, 1.5707963705063f);
+  const float c = fmaf(fmaf(fmaf(fmaf(0.0009036280680f, t, -0.0208600703627f), t, 0.2536692023277f), t, -1.2337005138397f), t, 1.0f);
+  return make_float2(c, s);
 }
 
-// A token's cosines and sines of `slots` pairs (those past the table's: no turn) to a warp's shared memory.
-__device__ __forceinline__ void find_turns(const RotaryParams& r, int64_t at, int slots, float* cosines, float* sines) {
+// cosine and sine of the angle of `quarters` quarter turns
+__device__ __forceinline__ float2 turn_of(double quarters, uint32_t inverse_sign) {
+  // the nearest whole number: 1.5 2^52 has a last place of 1, so the sum rounds to it, and its lowest bits are the
+  // number's. (Past 2^51 neighbouring doubles are half a quarter turn and more apart.)
+  double whole = quarters + 6755399441055744.0;
+  int k = __double2loint(whole);
+  whole -= 6755399441055744.0;
+  if (!(fabs(quarters) < 2251799813685248.0)) {
+    whole = rint(quarters);
+    k = static_cast<int>(whole - 4.0 * rint(0.25 * whole));
+  }
+  const float2 t = eighth_turn(static_cast<float>(quarters - whole));
+  // k quarter turns more
+  const float cos = k & 1 ? t.y : t.x, sin = k & 1 ? t.x : t.y;
+  return make_float2(__uint_as_float(__float_as_uint(cos) ^ (((k + 1) & 2) << 30)),
+                     __uint_as_float(__float_as_uint(sin) ^ ((k & 2) << 30) ^ inverse_sign));
+}
+
+// A token's position on axis `lane` (0 past the last axis).
+__device__ __forceinline__ double place_of(const RotaryParams& r, uint32_t b, uint32_t t) {
+  const int axis = threadIdx.x & 31;
+  if (r.pairs == 0 || axis >= r.axes) return 0.0;
+  const int64_t i = b * r.batch + t * r.token + axis * r.axis;
+  if (r.type == kPositionI64) return static_cast<double>(static_cast<const int64_t*>(r.positions)[i]);
+  if (r.type == kPositionI32) return static_cast<double>(static_cast<const int32_t*>(r.positions)[i]);
+  return static_cast<double>(static_cast<const float*>(r.positions)[i]);
+}
+
+// A token's cosines and sines of `slots` pairs (those past the table's: no turn) to a warp's shared memory, from
+// its places on the lanes. A pair whose axis is not there becomes NaN.
+__device__ __forceinline__ void find_turns(const RotaryParams& r, double place, int slots, float* cosines, float* sines) {
   __syncwarp();
-  for (int j = threadIdx.x & 31; j < slots; j += 32) {
-    const float2 t = j < r.pairs ? turn_of(r, at, j) : make_float2(1.f, 0.f);
-    cosines[j] = t.x;
-    sines[j] = t.y;
+  for (int j = threadIdx.x & 31; j - static_cast<int>(threadIdx.x & 31) < slots; j += 32) {
+    const int axis = j < r.pairs ? r.pair_axes[j] : 0;
+    double at = __shfl_sync(0xFFFFFFFFu, place, axis & 31);
+    if (axis < 0 || axis >= r.axes) at = __longlong_as_double(0x7FF8000000000000LL);
+    const float2 t = j < r.pairs ? turn_of(at * r.quarters[j], r.inverse ? 0x80000000u : 0u) : make_float2(1.f, 0.f);
+    if (j < slots) {
+      cosines[j] = t.x;
+      sines[j] = t.y;
+    }
   }
   __syncwarp();
 }
@@ -126,42 +149,51 @@ struct Pairs {
 };
 
 // Where a lane's P pairs lie: runs of P channels at `a` and `b`, which are the pairs' first and second channels,
-// or with INTER two halves of a run in which both take turns. P = 1: single channels anywhere.
+// or with INTER two runs of P / 2 neighbouring pairs (a team's runs at `a` lie side by side, and so do those at `b`,
+// so that its accesses take whole sectors). P = 1: single channels anywhere. The pairs' angles lie at `table_a`
+// and with INTER the second run's at `table_b`.
 template <int P>
 struct Spot {
-  int a, b;    // element offsets in a head
-  int turned;  // how many of the pairs are turned: the first ones
+  int a, b;                // element offsets in a head
+  int table_a, table_b;
+  int turned_a, turned_b;  // how many of the pairs (with INTER of each run's) are turned: the first ones
   bool has_a, has_b;
 };
+__device__ __forceinline__ int clamped(int v, int most) { return v < 0 ? 0 : v < most ? v : most; }
 template <int P, bool INTER>
 __device__ __forceinline__ Spot<P> spot_of(const RotaryParams& r, int chunk, int channels) {
   Spot<P> s;
-  const int first = chunk * P, turned = r.pairs - first;  // the chunk's first pair
-  s.turned = turned < 0 ? 0 : turned < P ? turned : P;
-  if (!INTER && turned > 0 && !(P == 1 && r.interleaved)) {
-    s.a = first;
-    s.b = r.pairs + first;
+  if constexpr (INTER) {
+    s.table_a = chunk * (P / 2);
+    s.table_b = channels / 4 + s.table_a;
+    s.a = chunk * P;
+    s.b = channels / 2 + s.a;
+    s.turned_a = clamped(r.pairs - s.table_a, P / 2);
+    s.turned_b = clamped(r.pairs - s.table_b, P / 2);
+    s.has_a = s.has_b = s.a < channels / 2;
   } else {
-    s.a = 2 * first;
-    s.b = s.a + P;
+    s.table_a = s.table_b = chunk * P;
+    s.turned_a = s.turned_b = clamped(r.pairs - s.table_a, P);
+    const bool halves = s.turned_a > 0 && !(P == 1 && r.interleaved);
+    s.a = halves ? s.table_a : 2 * s.table_a;
+    s.b = halves ? r.pairs + s.table_a : s.a + P;
+    s.has_a = s.a + P <= channels;
+    s.has_b = s.b + P <= channels;
   }
-  s.has_a = s.a + P <= channels;
-  s.has_b = s.b + P <= channels;
   return s;
 }
 
 template <typename T, int P>
 struct RawPairs {
   Run<T, P> a, b;
-  __device__ __forceinline__ void load(const T* head, const Spot<P>& s, bool in) {
-    if (in && s.has_a)
-      a.load(head + s.a);
-    else
-      a.zero();
-    if (in && s.has_b)
-      b.load(head + s.b);
-    else
-      b.zero();
+  __device__ __forceinline__ void zero() {
+    a.zero();
+    b.zero();
+  }
+  // channels that are not there keep the zeros they were given
+  __device__ __forceinline__ void load(const T* head, const Spot<P>& s) {
+    if (s.has_a) a.load(head + s.a);
+    if (s.has_b) b.load(head + s.b);
   }
   __device__ __forceinline__ void store(T* head, const Spot<P>& s) const {
     if (s.has_a) a.store(head + s.a);
@@ -218,22 +250,27 @@ template <int P, bool INTER>
 __device__ __forceinline__ Pairs<P> weight_of(const float* weight, const Spot<P>& s) {
   if (weight == nullptr) return {Lanes<P>(1.f), Lanes<P>(1.f)};
   RawPairs<float, P> raw;
-  raw.a.zero();
-  raw.b.zero();
+  raw.zero();
   if (s.has_a) raw.a.load_again(weight + s.a);
   if (s.has_b) raw.b.load_again(weight + s.b);
   return widen<float, P, INTER>(raw);
 }
 
-template <int P>
-__device__ __forceinline__ Lanes<P> from_shared(const float* p) {
+// a table's values for a lane's pairs
+template <int P, bool INTER>
+__device__ __forceinline__ Lanes<P> from_table(const float* table, const Spot<P>& s) {
   Lanes<P> v;
   if constexpr (P == 1) {
-    v.f = *p;
+    v.f = table[s.table_a];
+  } else if constexpr (P == 4 && INTER) {
+    const float2 x = *reinterpret_cast<const float2*>(table + s.table_a), y = *reinterpret_cast<const float2*>(table + s.table_b);
+    v.p[0] = f32x2(x.x, x.y);
+    v.p[1] = f32x2(y.x, y.y);
   } else {
 #pragma unroll
     for (int i = 0; i < P / 4; ++i) {
-      const float4 t = reinterpret_cast<const float4*>(p)[i];
+      const float* from = INTER && i >= P / 8 ? table + s.table_b + 4 * (i - P / 8) : table + s.table_a + 4 * i;
+      const float4 t = *reinterpret_cast<const float4*>(from);
       v.p[2 * i] = f32x2(t.x, t.y);
       v.p[2 * i + 1] = f32x2(t.z, t.w);
     }
@@ -244,27 +281,29 @@ template <int P>
 __device__ __forceinline__ Lanes<P> negative(const Lanes<P>& v) {
   return v.each([](float f) { return -f; });
 }
-// the first `turned` pairs of y, the others of x: what is not turned never meets another channel's value
-template <int P>
-__device__ __forceinline__ void keep_unturned(Pairs<P>& y, const Pairs<P>& x, int turned) {
-  if (turned == P) return;
+// the turned pairs of y, the others of x: what is not turned never meets another channel's value
+template <int P, bool INTER>
+__device__ __forceinline__ void keep_unturned(Pairs<P>& y, const Pairs<P>& x, const Spot<P>& s) {
+  if (s.turned_a + (INTER ? s.turned_b : 0) == P) return;
   if constexpr (P == 1) {
     y = x;
   } else {
+    const auto turned = [&](int i) { return INTER && i >= P / 2 ? i - P / 2 < s.turned_b : i < s.turned_a; };
 #pragma unroll
     for (int i = 0; i < P; i += 2) {
-      y.a.p[i / 2] = f32x2(i < turned ? y.a.get(i) : x.a.get(i), i + 1 < turned ? y.a.get(i + 1) : x.a.get(i + 1));
-      y.b.p[i / 2] = f32x2(i < turned ? y.b.get(i) : x.b.get(i), i + 1 < turned ? y.b.get(i + 1) : x.b.get(i + 1));
+      y.a.p[i / 2] = f32x2(turned(i) ? y.a.get(i) : x.a.get(i), turned(i + 1) ? y.a.get(i + 1) : x.a.get(i + 1));
+      y.b.p[i / 2] = f32x2(turned(i) ? y.b.get(i) : x.b.get(i), turned(i + 1) ? y.b.get(i + 1) : x.b.get(i + 1));
     }
   }
 }
 
-// the sum over a team of `team` lanes, a power of two
-template <int U>
-__device__ __forceinline__ void team_sums(float (&v)[U], int team) {
-  for (int o = team / 2; o > 0; o >>= 1) {
+// the sums over a team of `team` lanes, a power of two
+template <int N>
+__device__ __forceinline__ void team_sums(float (&v)[N], int team) {
+#pragma unroll 1
+  for (int o = team >> 1; o > 0; o >>= 1) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] += __shfl_xor_sync(0xFFFFFFFFu, v[u], o);
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xFFFFFFFFu, v[i], o);
   }
 }
 
@@ -276,226 +315,405 @@ struct Plan {
   int per, shift, slots;
 };
 
-// Forward. NORM: the norm and its weight. q's heads come before k's. NV runs a lane, a team apart.
-template <typename T, int P, bool INTER, int NV, bool NORM>
-__global__ void __launch_bounds__(kThreads) heads_kernel(const __grid_constant__ HeadsParams p, const __grid_constant__ Plan plan) {
-  constexpr int U = P * NV >= 4 ? 2 : 4;  // heads of a team at a time
-  extern __shared__ __align__(16) float tables[];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-  const uint32_t id = blockIdx.x * kWarps + warp;
-  if (id >= plan.items) return;
-  const uint32_t token = plan.chunks.quotient(id), chunk = id - token * plan.chunks.d;
-  const uint32_t b = plan.tokens.quotient(token), t = token - b * plan.tokens.d;
-  const int team = 1 << plan.shift, teams = 32 >> plan.shift, mine = lane >> plan.shift;
-  float* cosines = tables + warp * 2 * plan.slots;
-  float* sines = cosines + plan.slots;
-  Spot<P> spot[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) spot[i] = spot_of<P, INTER>(p.rotary, (lane & (team - 1)) + i * team, p.channels);
-  const int first = chunk * plan.per, last = min(first + plan.per, p.heads[0] + p.heads[1]);
-  const float inverse_c = 1.0f / static_cast<float>(p.channels);
+// ---- a lane's ring of S slots for NT tensors
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
 
-  RawPairs<T, P> raw[U][NV];
-  const T* x = nullptr;
-  auto load = [&](int which, int h, int end) {
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int i = 0; i < NV; ++i) raw[u][i].load(x + (h + u * teams) * p.x[which].head, spot[i], h + u * teams < end);
-  };
-  bool fresh = true;  // no heads loaded yet
-#pragma unroll 1
-  for (int which = 0; which < 2; ++which) {
-    const int skip = which == 0 ? 0 : p.heads[0];
-    const int begin = max(first - skip, 0), end = min(last - skip, p.heads[which]);
-    if (begin >= end) continue;
-    const HeadView out = p.out[which];
-    x = static_cast<const T*>(p.x[which].data) + b * p.x[which].batch + t * p.x[which].token;
-    T* y = static_cast<T*>(out.data) + b * out.batch + t * out.token;
-    load(which, begin + mine, end);
-    if (fresh) find_turns(p.rotary, b * p.rotary.batch + t * p.rotary.token, plan.slots, cosines, sines);
-    fresh = false;
-    Pairs<P> c[NV], s[NV];  // cosines, and sines by the other channel's weight (a's negative)
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int at = ((lane & (team - 1)) + i * team) * P;
-      const Lanes<P> cosine = from_shared<P>(cosines + at), sine = from_shared<P>(sines + at);
-      if constexpr (NORM) {
-        const Pairs<P> w = weight_of<P, INTER>(p.weight[which], spot[i]);
-        c[i] = {cosine * w.a, cosine * w.b};
-        s[i] = {negative(sine * w.b), sine * w.a};
-      } else {
-        c[i] = {cosine, cosine};
-        s[i] = {negative(sine), sine};
-      }
-    }
-#pragma unroll 1
-    for (int h = begin; h < end; h += U * teams) {
-      Pairs<P> v[U][NV];
+// A warp's item: a token's heads `first` to `last` of q's and then k's, a phase each.
+struct Place {
+  uint32_t b, t;
+  int first, last;
+  __device__ __forceinline__ Place(const Plan& plan, uint32_t id) {
+    const uint32_t token = plan.chunks.quotient(id);
+    b = plan.tokens.quotient(token);
+    t = token - b * plan.tokens.d;
+    first = (id - token * plan.chunks.d) * plan.per;
+    last = first + plan.per;
+  }
+  __device__ __forceinline__ int begin(const HeadsParams& p, int which) const { return max(first - (which == 0 ? 0 : p.heads[0]), 0); }
+  __device__ __forceinline__ int end(const HeadsParams& p, int which) const {
+    return min(last - (which == 0 ? 0 : p.heads[0]), p.heads[which]);
+  }
+};
+
+template <int BYTES>
+__device__ __forceinline__ void read_shared(uint32_t* w, uint32_t from) {
+  if constexpr (BYTES == 16)
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(from) : "memory");
+  else
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(from) : "memory");
+}
+
+// A warp's loads of the steps of its items, U heads a team a step. Runs come through the ring, S steps ahead, each
+// lane's own 16 bytes by itself; single channels (P = 1) are held in registers one step ahead.
+template <typename T, int P, int NV, int NT, int U, int S>
+struct Stream {
+  static constexpr bool kAsync = P > 1;
+  static constexpr int kPiece = P * sizeof(T) >= 16 ? 16 : 8;                            // bytes of a copy
+  static constexpr int kPieces = kAsync ? P * static_cast<int>(sizeof(T)) / kPiece : 0;  // of a run
+  static constexpr int kSlot = U * NV * NT * 2 * kPieces * kPiece * kThreads;            // bytes of a slot for the block
+  static constexpr int kBytes = kAsync ? S * kSlot : 0;
+
+  const HeadsParams& p;
+  const Plan& plan;
+  const Spot<P> (&spot)[NV];
+  uint32_t id, slot, last_slot;  // addresses of this lane's piece
+  int which, mine, left, steps;
+  Place place;
+  int64_t step[NT];  // elements from a step's heads to the next's
+  const T* at[NT];
+  RawPairs<T, P> next[kAsync ? 1 : U][NV][NT];
+
+  __device__ __forceinline__ Stream(const HeadsParams& params, const Plan& plan_of, const Spot<P> (&spots)[NV], uint32_t first, uint8_t* smem)
+      : p(params), plan(plan_of), spot(spots), id(first), which(-1), mine((threadIdx.x & 31) >> plan_of.shift), left(0), place(plan_of, first) {
+    slot = smem_u32(smem) + threadIdx.x * kPiece;
+    last_slot = slot + (S - 1) * kSlot;
+    if constexpr (!kAsync) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int i = 0; i < NV; ++i) v[u][i] = widen<T, P, INTER>(raw[u][i]);
-      if (h + U * teams < end) load(which, h + U * teams + mine, end);
-      float rstd[U];
-      if constexpr (NORM) {
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          rstd[u] = 0.f;
-#pragma unroll
-          for (int i = 0; i < NV; ++i) rstd[u] += v[u][i].a.dot(v[u][i].a) + v[u][i].b.dot(v[u][i].b);
-        }
-        team_sums(rstd, team);
-#pragma unroll
-        for (int u = 0; u < U; ++u) rstd[u] = rsqrtf(rstd[u] * inverse_c + p.eps);
+          for (int k = 0; k < NT; ++k) next[u][i][k].zero();
+    }
+    enter();
+#pragma unroll 1
+    for (int k = 0; k < (kAsync ? S : 1); ++k) fetch();
+  }
+
+  // to the next phase that has heads, of this item or the next
+  __device__ __forceinline__ void enter() {
+    const int teams = 32 >> plan.shift;
+    while (id < plan.items) {
+      if (++which == 2) {
+        id += gridDim.x * kWarps;
+        which = -1;
+        if (id < plan.items) place = Place(plan, id);
+        continue;
       }
+      const int begin = place.begin(p, which), count = place.end(p, which) - begin;
+      if (count <= 0) continue;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int head = h + mine + u * teams;
+      for (int k = 0; k < NT; ++k) {
+        const HeadView& v = k == 0 ? p.x[which] : p.dy[which];
+        at[k] = static_cast<const T*>(v.data) + (place.b * v.batch + place.t * v.token + (begin + mine) * v.head);
+        step[k] = U * teams * v.head;
+      }
+      left = (count - mine + teams - 1) >> (5 - plan.shift);
+      steps = (count + U * teams - 1) / (U * teams);
+      return;
+    }
+  }
+
+  // starts the loads of the next step
+  __device__ __forceinline__ void fetch() {
+    if (id < plan.items) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          Pairs<P> n = v[u][i];
-          if constexpr (NORM) n = {n.a * Lanes<P>(rstd[u]), n.b * Lanes<P>(rstd[u])};
-          Pairs<P> turned = {fma(n.a, c[i].a, n.b * s[i].a), fma(n.b, c[i].b, n.a * s[i].b)};
-          // a cosine of 1 leaves the weight
-          keep_unturned(turned, {n.a * c[i].a, n.b * c[i].b}, spot[i].turned);
-          if (head < end) narrow<T, P, INTER>(turned).store(y + head * out.head, spot[i]);
+      for (int u = 0; u < U; ++u)
+        if (u < left) {
+#pragma unroll
+          for (int k = 0; k < NT; ++k) {
+            const T* from = at[k] + (U == 1 ? 0 : u * (step[k] / U));
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+              if constexpr (kAsync) {
+                if (spot[i].has_a) {  // runs are whole: both are there
+                  const uint32_t to = slot + ((u * NV + i) * NT + k) * 2 * kPieces * (kPiece * kThreads);
+#pragma unroll
+                  for (int c = 0; c < kPieces; ++c) {
+                    copy_async<kPiece>(to + c * (kPiece * kThreads), from + spot[i].a + c * kPiece / sizeof(T));
+                    copy_async<kPiece>(to + (kPieces + c) * (kPiece * kThreads), from + spot[i].b + c * kPiece / sizeof(T));
+                  }
+                }
+              } else {
+                next[u][i][k].load(from, spot[i]);
+              }
+            }
+          }
         }
+      left -= U;
+#pragma unroll
+      for (int k = 0; k < NT; ++k) at[k] += step[k];
+      if (--steps == 0) enter();
+    }
+    if constexpr (kAsync) {
+      commit_copies();
+      slot = slot == last_slot ? last_slot - (S - 1) * kSlot : slot + kSlot;
+    }
+  }
+
+  // The oldest step's values; then its slot is free (nobody else reads it). The caller fetches the next after it
+  // has widened them. What comes for channels and heads that are not there means nothing.
+  __device__ __forceinline__ void take(RawPairs<T, P> (&raw)[U][NV][NT]) {
+    if constexpr (kAsync) wait_copies<S - 1>();
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < NT; ++k) {
+          if constexpr (kAsync) {
+            const uint32_t from = slot + ((u * NV + i) * NT + k) * 2 * kPieces * (kPiece * kThreads);
+#pragma unroll
+            for (int c = 0; c < kPieces; ++c) {
+              read_shared<kPiece>(raw[u][i][k].a.w + c * (kPiece / 4), from + c * (kPiece * kThreads));
+              read_shared<kPiece>(raw[u][i][k].b.w + c * (kPiece / 4), from + (kPieces + c) * (kPiece * kThreads));
+            }
+          } else {
+            raw[u][i][k] = next[u][i][k];
+          }
+        }
+  }
+};
+
+// heads of a team at a time
+template <int P, int NV>
+constexpr int kAtOnce = P > 1 || NV >= 4 ? 1 : 4 / NV;
+
+// Slots of the rings, and blocks that an SM holds. 65536 tokens of 40 heads x 128 in bf16: forward 214 us with two
+// blocks (111 registers a thread) and 3, 4 or 6 slots, 260 with three (80 registers, 150 bytes of them spilled);
+// backward 371 us with 3 slots, 384 with 6, 398 with one block, 624 with three.
+constexpr int kForwardSlots = 3, kBackwardSlots = 3;
+template <typename T, int P, int NV>
+constexpr int kResident = P * NV * static_cast<int>(sizeof(T)) > 16 || NV > 2 ? 1 : 2;
+
+// Forward. NORM: the norm and its weight. ALL: every pair is turned. NV runs a lane, a team apart.
+template <typename T, int P, bool INTER, int NV, bool ALL, bool NORM>
+__global__ void __launch_bounds__(kThreads, kResident<T, P, NV>)
+    heads_kernel(const __grid_constant__ HeadsParams p, const __grid_constant__ Plan plan) {
+  constexpr int U = kAtOnce<P, NV>;
+  using Heads = Stream<T, P, NV, 1, U, kForwardSlots>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int lane = threadIdx.x & 31, team = 1 << plan.shift, teams = 32 >> plan.shift, mine = lane >> plan.shift;
+  const uint32_t first = blockIdx.x * kWarps + threadIdx.x / 32;
+  if (first >= plan.items) return;
+  float* cosines = reinterpret_cast<float*>(smem + Heads::kBytes) + threadIdx.x / 32 * 2 * plan.slots;
+  float* sines = cosines + plan.slots;
+  const float inverse_c = 1.0f / static_cast<float>(p.channels);
+  Spot<P> spot[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) spot[i] = spot_of<P, INTER>(p.rotary, (lane & (team - 1)) + i * team, p.channels);
+  Heads stream(p, plan, spot, first, smem);
+  Place after(plan, first);
+  double ahead = place_of(p.rotary, after.b, after.t);  // the next item's
+#pragma unroll 1
+  for (uint32_t id = first; id < plan.items; id += gridDim.x * kWarps) {
+    const Place place = after;
+    find_turns(p.rotary, ahead, plan.slots, cosines, sines);
+    if (id + gridDim.x * kWarps < plan.items) {
+      after = Place(plan, id + gridDim.x * kWarps);
+      ahead = place_of(p.rotary, after.b, after.t);
+    }
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which) {
+      const int begin = place.begin(p, which), count = place.end(p, which) - begin;
+      if (count <= 0) continue;
+      const HeadView& out = p.out[which];
+      T* y_head = static_cast<T*>(out.data) + (place.b * out.batch + place.t * out.token + (begin + mine) * out.head);
+      const int64_t out_head = teams * out.head;
+      int left = (count - mine + teams - 1) >> (5 - plan.shift);
+      Pairs<P> c[NV], s[NV];  // cosines, and sines by the other channel's weight (a's negative)
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const Lanes<P> cosine = from_table<P, INTER>(cosines, spot[i]), sine = from_table<P, INTER>(sines, spot[i]);
+        if constexpr (NORM) {
+          const Pairs<P> w = weight_of<P, INTER>(p.weight[which], spot[i]);
+          c[i] = {cosine * w.a, cosine * w.b};
+          s[i] = {negative(sine) * w.b, sine * w.a};
+        } else {
+          c[i] = {cosine, cosine};
+          s[i] = {negative(sine), sine};
+        }
+      }
+#pragma unroll 1
+      for (int step = (count + U * teams - 1) / (U * teams); step > 0; --step) {
+        RawPairs<T, P> raw[U][NV][1];
+        Pairs<P> v[U][NV];
+        stream.take(raw);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int i = 0; i < NV; ++i) v[u][i] = widen<T, P, INTER>(raw[u][i][0]);
+        stream.fetch();
+        if constexpr (NORM) {
+          float rstd[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            rstd[u] = 0.f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+              const float sum = v[u][i].a.dot(v[u][i].a) + v[u][i].b.dot(v[u][i].b);
+              rstd[u] += P == 1 || spot[i].has_a ? sum : 0.f;
+            }
+          }
+          team_sums(rstd, team);
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            rstd[u] = rsqrtf(rstd[u] * inverse_c + p.eps);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[u][i] = {v[u][i].a * Lanes<P>(rstd[u]), v[u][i].b * Lanes<P>(rstd[u])};
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (u < left) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+              const Pairs<P>& n = v[u][i];
+              Pairs<P> y = {fma(n.a, c[i].a, n.b * s[i].a), fma(n.b, c[i].b, n.a * s[i].b)};
+              // a cosine of 1 leaves the weight
+              if constexpr (!ALL) keep_unturned<P, INTER>(y, {n.a * c[i].a, n.b * c[i].b}, spot[i]);
+              narrow<T, P, INTER>(y).store(y_head + u * out_head, spot[i]);
+            }
+          }
+        left -= U;
+        y_head += U * out_head;
       }
     }
   }
 }
 
-// Backward: g = dy turned back, w = g weight, xh = x rstd: dx = rstd (w - xh mean(w xh)); the first q_blocks
-// blocks take q's heads, the others k's, each over its tokens. A block's sums of g xh go to row blockIdx.x of the
-// partial sums.
-template <typename T, int P, bool INTER, int NV>
-__global__ void __launch_bounds__(kThreads)
-    heads_bwd_kernel(const __grid_constant__ HeadsParams p, const __grid_constant__ Plan q_plan, const __grid_constant__ Plan k_plan,
-                     int q_blocks, float* part) {
-  constexpr int U = P * NV >= 4 ? 1 : 2;
-  extern __shared__ __align__(16) float tables[];
-  const int which = static_cast<int>(blockIdx.x) < q_blocks ? 0 : 1;
-  const Plan& plan = which == 0 ? q_plan : k_plan;
-  const uint32_t block = blockIdx.x - (which == 0 ? 0 : q_blocks), blocks = which == 0 ? q_blocks : gridDim.x - q_blocks;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-  const int team = 1 << plan.shift, teams = 32 >> plan.shift, mine = lane >> plan.shift;
-  float* cosines = tables + warp * 2 * plan.slots;
+// Backward: g = dy turned back, w = g weight, xh = x rstd: dx = rstd (w - xh mean(w xh)). A block's sums of g xh
+// over its items go to its rows of the partial sums, q's rows before k's.
+template <typename T, int P, bool INTER, int NV, bool ALL>
+__global__ void __launch_bounds__(kThreads, kResident<T, P, NV>)
+    heads_bwd_kernel(const __grid_constant__ HeadsParams p, const __grid_constant__ Plan plan, float* partial) {
+  constexpr int U = kAtOnce<P, NV>;
+  using Heads = Stream<T, P, NV, 2, U, kBackwardSlots>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, team = 1 << plan.shift, teams = 32 >> plan.shift, mine = lane >> plan.shift;
+  const uint32_t first = blockIdx.x * kWarps + warp;
+  float* cosines = reinterpret_cast<float*>(smem + Heads::kBytes) + warp * 2 * plan.slots;
   float* sines = cosines + plan.slots;
-  const HeadView xv = p.x[which], dyv = p.dy[which], outv = p.out[which];
   const float inverse_c = 1.0f / static_cast<float>(p.channels);
   Spot<P> spot[NV];
-  Pairs<P> w[NV], dw[NV];
+  Pairs<P> dw[2][NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     spot[i] = spot_of<P, INTER>(p.rotary, (lane & (team - 1)) + i * team, p.channels);
-    w[i] = weight_of<P, INTER>(p.weight[which], spot[i]);
-    dw[i] = {Lanes<P>(0.f), Lanes<P>(0.f)};
+    dw[0][i] = dw[1][i] = {Lanes<P>(0.f), Lanes<P>(0.f)};
   }
-  for (uint32_t id = block * kWarps + warp; id < plan.items; id += blocks * kWarps) {
-    const uint32_t token = plan.chunks.quotient(id), chunk = id - token * plan.chunks.d;
-    const uint32_t b = plan.tokens.quotient(token), t = token - b * plan.tokens.d;
-    const int begin = chunk * plan.per, end = min(begin + plan.per, p.heads[which]);
-    const T* x = static_cast<const T*>(xv.data) + b * xv.batch + t * xv.token;
-    const T* dy = static_cast<const T*>(dyv.data) + b * dyv.batch + t * dyv.token;
-    T* dx = static_cast<T*>(outv.data) + b * outv.batch + t * outv.token;
-    RawPairs<T, P> raw_x[U][NV], raw_g[U][NV];
-    auto load = [&](int h) {
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int head = h + u * teams;
-          raw_x[u][i].load(x + head * xv.head, spot[i], head < end);
-          raw_g[u][i].load(dy + head * dyv.head, spot[i], head < end);
-        }
-    };
-    load(begin + mine);
-    find_turns(p.rotary, b * p.rotary.batch + t * p.rotary.token, plan.slots, cosines, sines);
-    Lanes<P> c[NV], s[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int at = ((lane & (team - 1)) + i * team) * P;
-      c[i] = from_shared<P>(cosines + at);
-      s[i] = from_shared<P>(sines + at);
-    }
+  Heads stream(p, plan, spot, first, smem);
+  Place after(plan, first);
+  double ahead = first < plan.items ? place_of(p.rotary, after.b, after.t) : 0.0;  // the next item's
 #pragma unroll 1
-    for (int h = begin; h < end; h += U * teams) {
-      Pairs<P> v[U][NV], g[U][NV];
-      float sums[2 * U];
+  for (uint32_t id = first; id < plan.items; id += gridDim.x * kWarps) {
+    const Place place = after;
+    find_turns(p.rotary, ahead, plan.slots, cosines, sines);
+    if (id + gridDim.x * kWarps < plan.items) {
+      after = Place(plan, id + gridDim.x * kWarps);
+      ahead = place_of(p.rotary, after.b, after.t);
+    }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        sums[2 * u] = sums[2 * u + 1] = 0.f;
+    for (int which = 0; which < 2; ++which) {
+      const int begin = place.begin(p, which), count = place.end(p, which) - begin;
+      if (count <= 0) continue;
+      const HeadView& out = p.out[which];
+      T* dx_head = static_cast<T*>(out.data) + (place.b * out.batch + place.t * out.token + (begin + mine) * out.head);
+      const int64_t out_head = teams * out.head;
+      int left = (count - mine + teams - 1) >> (5 - plan.shift);
+      Pairs<P> w[NV];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) w[i] = weight_of<P, INTER>(p.weight[which], spot[i]);
+#pragma unroll 1
+      for (int step = (count + U * teams - 1) / (U * teams); step > 0; --step) {
+        RawPairs<T, P> raw[U][NV][2];
+        Pairs<P> v[U][NV], g[U][NV];
+        stream.take(raw);
+        float sums[2 * U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) sums[2 * u] = sums[2 * u + 1] = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-          v[u][i] = widen<T, P, INTER>(raw_x[u][i]);
-          const Pairs<P> d = widen<T, P, INTER>(raw_g[u][i]);
-          g[u][i] = {fma(d.a, c[i], d.b * s[i]), fma(d.b, c[i], negative(d.a * s[i]))};
-          keep_unturned(g[u][i], d, spot[i].turned);
-          sums[2 * u] += v[u][i].a.dot(v[u][i].a) + v[u][i].b.dot(v[u][i].b);
-          sums[2 * u + 1] += (v[u][i].a * w[i].a).dot(g[u][i].a) + (v[u][i].b * w[i].b).dot(g[u][i].b);
-        }
-      }
-      if (h + U * teams < end) load(h + U * teams + mine);
-      team_sums(sums, team);
+          const Lanes<P> c = from_table<P, INTER>(cosines, spot[i]), s = from_table<P, INTER>(sines, spot[i]);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int head = h + mine + u * teams;
-        const float rstd = rsqrtf(sums[2 * u] * inverse_c + p.eps);
-        const float along = -rstd * (sums[2 * u + 1] * rstd * inverse_c);  // -rstd mean(w xh)
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const Pairs<P> xh = {v[u][i].a * Lanes<P>(rstd), v[u][i].b * Lanes<P>(rstd)};
-          if (head < end) {
-            dw[i] = {fma(g[u][i].a, xh.a, dw[i].a), fma(g[u][i].b, xh.b, dw[i].b)};
-            const Pairs<P> y = {fma(xh.a, Lanes<P>(along), g[u][i].a * w[i].a * Lanes<P>(rstd)),
-                                fma(xh.b, Lanes<P>(along), g[u][i].b * w[i].b * Lanes<P>(rstd))};
-            narrow<T, P, INTER>(y).store(dx + head * outv.head, spot[i]);
+          for (int u = 0; u < U; ++u) {
+            v[u][i] = widen<T, P, INTER>(raw[u][i][0]);
+            const Pairs<P> d = widen<T, P, INTER>(raw[u][i][1]);
+            g[u][i] = {fma(d.a, c, d.b * s), fma(d.b, c, negative(d.a * s))};
+            if constexpr (!ALL) keep_unturned<P, INTER>(g[u][i], d, spot[i]);
+            const float squares = v[u][i].a.dot(v[u][i].a) + v[u][i].b.dot(v[u][i].b);
+            const float along = (v[u][i].a * w[i].a).dot(g[u][i].a) + (v[u][i].b * w[i].b).dot(g[u][i].b);
+            sums[2 * u] += P == 1 || spot[i].has_a ? squares : 0.f;
+            sums[2 * u + 1] += P == 1 || spot[i].has_a ? along : 0.f;
           }
         }
+        stream.fetch();
+        team_sums(sums, team);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (u < left) {
+            const float rstd = rsqrtf(sums[2 * u] * inverse_c + p.eps);
+            const float along = -rstd * rstd * (sums[2 * u + 1] * rstd * inverse_c);  // -rstd^2 mean(w xh)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+              const Pairs<P> gr = {g[u][i].a * Lanes<P>(rstd), g[u][i].b * Lanes<P>(rstd)};
+              dw[which][i] = {fma(gr.a, v[u][i].a, dw[which][i].a), fma(gr.b, v[u][i].b, dw[which][i].b)};
+              const Pairs<P> y = {fma(v[u][i].a, Lanes<P>(along), gr.a * w[i].a), fma(v[u][i].b, Lanes<P>(along), gr.b * w[i].b)};
+              narrow<T, P, INTER>(y).store(dx_head + u * out_head, spot[i]);
+            }
+          }
+        left -= U;
+        dx_head += U * out_head;
       }
     }
   }
-  if (part == nullptr) return;
+  if (partial == nullptr) return;
   let_next_kernel_start();
   // the warp's teams by shuffles, then the warps through shared memory, each sum in a fixed order
-  __syncthreads();
-  float* row = tables + warp * p.channels;
+  float* sums = reinterpret_cast<float*>(smem);
+  float* row = sums + warp * p.channels;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    for (int o = 16; o >= team; o >>= 1) {
-      dw[i].a = dw[i].a.each([&](float f) { return f + __shfl_xor_sync(0xFFFFFFFFu, f, o); });
-      dw[i].b = dw[i].b.each([&](float f) { return f + __shfl_xor_sync(0xFFFFFFFFu, f, o); });
-    }
-    if (mine == 0) {
+  for (int which = 0; which < 2; ++which) {
+    if (p.dweight[which] == nullptr) continue;
+    __syncthreads();
 #pragma unroll
-      for (int j = 0; j < P; ++j) {
-        if (spot[i].has_a) row[INTER && P > 1 ? spot[i].a + 2 * j : spot[i].a + j] = dw[i].a.get(j);
-        if (spot[i].has_b) row[INTER && P > 1 ? spot[i].a + 2 * j + 1 : spot[i].b + j] = dw[i].b.get(j);
+    for (int i = 0; i < NV; ++i) {
+      for (int o = 16; o >= team; o >>= 1) {
+        dw[which][i].a = dw[which][i].a.each([&](float f) { return f + __shfl_xor_sync(0xFFFFFFFFu, f, o); });
+        dw[which][i].b = dw[which][i].b.each([&](float f) { return f + __shfl_xor_sync(0xFFFFFFFFu, f, o); });
+      }
+      if (lane < team) {
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+          const int at = !INTER ? spot[i].a + j : j < P / 2 ? spot[i].a + 2 * j : spot[i].b + 2 * j - P;
+          if (spot[i].has_a) row[at] = dw[which][i].a.get(j);
+          if (spot[i].has_b) row[INTER ? at + 1 : spot[i].b + j] = dw[which][i].b.get(j);
+        }
       }
     }
-  }
-  __syncthreads();
-  for (int c = threadIdx.x; c < p.channels; c += kThreads) {
-    float a = 0.f;
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.channels; c += kThreads) {
+      float a = 0.f;
 #pragma unroll
-    for (int k = 0; k < kWarps; ++k) a += tables[k * p.channels + c];
-    part[static_cast<int64_t>(blockIdx.x) * p.channels + c] = a;
+      for (int k = 0; k < kWarps; ++k) a += sums[k * p.channels + c];
+      partial[(static_cast<int64_t>(which) * gridDim.x + blockIdx.x) * p.channels + c] = a;
+    }
   }
 }
 
 // a weight's gradient from the blocks' partial sums (q's rows first), in a fixed order: 32 channels a block
 __global__ void __launch_bounds__(1024)
-    heads_reduce_kernel(const float* __restrict__ part, float* dq_weight, float* dk_weight, int q_blocks, int blocks, int channels) {
+    heads_reduce_kernel(const float* __restrict__ part, float* dq_weight, float* dk_weight, int blocks, int channels) {
   __shared__ float s[32][33];
   const int lane = threadIdx.x & 31, r = threadIdx.x / 32, c = blockIdx.x * 32 + lane;
   float* out = blockIdx.y == 0 ? dq_weight : dk_weight;
-  const int first = blockIdx.y == 0 ? 0 : q_blocks, last = blockIdx.y == 0 ? q_blocks : blocks;
+  const float* rows = part + static_cast<int64_t>(blockIdx.y) * blocks * channels;
   wait_for_kernel_before();
   if (out == nullptr) return;
   float v = 0.f;
   if (c < channels)
-    for (int i = first + r; i < last; i += 32) v += part[static_cast<int64_t>(i) * channels + c];
+    for (int i = r; i < blocks; i += 32) v += rows[static_cast<int64_t>(i) * channels + c];
   s[r][lane] = v;
   __syncthreads();
   if (r == 0 && c < channels) {
@@ -525,15 +743,18 @@ bool runs_of(const HeadsParams& p, int P, int size, bool backward) {
   return true;
 }
 
-// Calls f(P, INTER, NV as integral constants, lanes a team at least): runs of 16 bytes where they are whole and aligned
+// Calls f(P, INTER, NV, ALL as integral constants, lanes a team at least): runs of 16 bytes where they are whole and aligned
 // (fp32 heads of more than 256 channels in two of them), else of half that, else single channels.
 template <typename T, typename F>
 int dispatch_heads(const HeadsParams& p, bool backward, F&& f) {
   const int size = sizeof(T);
   const auto runs = [&](auto P) {
     const int lanes = p.channels / (2 * decltype(P)::value);
-    return p.rotary.interleaved ? f(P, std::true_type{}, std::integral_constant<int, 1>{}, lanes)
-                                : f(P, std::false_type{}, std::integral_constant<int, 1>{}, lanes);
+    const std::integral_constant<int, 1> one;
+    const std::true_type yes;
+    const std::false_type no;
+    if (2 * p.rotary.pairs == p.channels) return p.rotary.interleaved ? f(P, yes, one, yes, lanes) : f(P, no, one, yes, lanes);
+    return p.rotary.interleaved ? f(P, yes, one, no, lanes) : f(P, no, one, no, lanes);
   };
   if (sizeof(T) == 4 && runs_of(p, 4, size, backward)) return runs(std::integral_constant<int, 4>{});
   if (runs_of(p, 8, size, backward)) return runs(std::integral_constant<int, 8>{});
@@ -541,10 +762,10 @@ int dispatch_heads(const HeadsParams& p, bool backward, F&& f) {
   const int pairs = (p.channels + 1) / 2;
   const std::integral_constant<int, 1> one;
   const std::false_type apart;
-  if (pairs <= 32) return f(one, apart, std::integral_constant<int, 1>{}, pairs);
-  if (pairs <= 64) return f(one, apart, std::integral_constant<int, 2>{}, 32);
-  if (pairs <= 128) return f(one, apart, std::integral_constant<int, 4>{}, 32);
-  return f(one, apart, std::integral_constant<int, 8>{}, 32);
+  if (pairs <= 32) return f(one, apart, std::integral_constant<int, 1>{}, apart, pairs);
+  if (pairs <= 64) return f(one, apart, std::integral_constant<int, 2>{}, apart, 32);
+  if (pairs <= 128) return f(one, apart, std::integral_constant<int, 4>{}, apart, 32);
+  return f(one, apart, std::integral_constant<int, 8>{}, apart, 32);
 }
 
 // Items of `per` heads: all of a token's where the tokens keep the GPU's warps busy, else no more than a team
@@ -565,51 +786,57 @@ Plan plan_of(const HeadsParams& p, int heads, int lanes, int run, int nv) {
   return plan;
 }
 
+constexpr int kMostBlocks = 148 * 2;
+
+int blocks_of(const Plan& plan, int resident) {
+  const int64_t want = (static_cast<int64_t>(plan.items) + kWarps - 1) / kWarps, most = 148 * resident;
+  return static_cast<int>(want < most ? want : most);
+}
+
 template <typename T>
 int heads(const HeadsParams& p, cudaStream_t stream) {
-  return dispatch_heads<T>(p, false, [&](auto run, auto inter, auto nv, int lanes) {
+  return dispatch_heads<T>(p, false, [&](auto run, auto inter, auto nv, auto all, int lanes) {
     constexpr int P = decltype(run)::value, NV = decltype(nv)::value;
+    constexpr bool INTER = decltype(inter)::value, ALL = decltype(all)::value;
     const Plan plan = plan_of(p, p.heads[0] + p.heads[1], lanes, P, NV);
-    const unsigned grid = (plan.items + kWarps - 1) / kWarps;
-    const size_t smem = sizeof(float) * kWarps * 2 * plan.slots;
-    auto kernel = p.norm ? heads_kernel<T, P, decltype(inter)::value, NV, true> : heads_kernel<T, P, decltype(inter)::value, NV, false>;
-    kernel<<<grid, kThreads, smem, stream>>>(p, plan);
+    const size_t smem = Stream<T, P, NV, 1, kAtOnce<P, NV>, kForwardSlots>::kBytes + sizeof(float) * kWarps * 2 * plan.slots;
+    auto kernel = p.norm ? heads_kernel<T, P, INTER, NV, ALL, true> : heads_kernel<T, P, INTER, NV, ALL, false>;
+    if (smem > 48 * 1024) {
+      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+      if (e != cudaSuccess) return static_cast<int>(e);
+    }
+    kernel<<<blocks_of(plan, kResident<T, P, NV>), kThreads, smem, stream>>>(p, plan);
     return static_cast<int>(cudaGetLastError());
   });
 }
 
-constexpr int kMostBlocks = 148 * 2;
-
 template <typename T>
 int heads_bwd(const HeadsParams& p, float* part, cudaStream_t stream) {
   const bool sums = p.dweight[0] != nullptr || p.dweight[1] != nullptr;
-  return dispatch_heads<T>(p, true, [&](auto run, auto inter, auto nv, int lanes) {
+  return dispatch_heads<T>(p, true, [&](auto run, auto inter, auto nv, auto all, int lanes) {
     constexpr int P = decltype(run)::value, NV = decltype(nv)::value;
-    Plan plan[2] = {plan_of(p, p.heads[0] > 0 ? p.heads[0] : 1, lanes, P, NV), plan_of(p, p.heads[1] > 0 ? p.heads[1] : 1, lanes, P, NV)};
-    int blocks[2];
-    for (int i = 0; i < 2; ++i) {
-      if (p.heads[i] == 0) plan[i].items = 0;
-      const int64_t want = (static_cast<int64_t>(plan[i].items) + kWarps - 1) / kWarps;
-      const int64_t share = kMostBlocks * static_cast<int64_t>(p.heads[i]) / (p.heads[0] + p.heads[1]);
-      const int64_t most = share > 0 ? share : 1;
-      blocks[i] = static_cast<int>(want < most ? want : most);
-      if (p.dweight[i] != nullptr && blocks[i] == 0) blocks[i] = 1;  // writes zeros
-    }
-    size_t smem = sizeof(float) * kWarps * 2 * plan[0].slots;
+    constexpr bool INTER = decltype(inter)::value, ALL = decltype(all)::value;
+    const Plan plan = plan_of(p, p.heads[0] + p.heads[1], lanes, P, NV);
+    size_t smem = Stream<T, P, NV, 2, kAtOnce<P, NV>, kBackwardSlots>::kBytes + sizeof(float) * kWarps * 2 * plan.slots;
     if (smem < sizeof(float) * kWarps * p.channels) smem = sizeof(float) * kWarps * p.channels;
-    const int grid = blocks[0] + blocks[1];
-    heads_bwd_kernel<T, P, decltype(inter)::value, NV><<<grid, kThreads, smem, stream>>>(p, plan[0], plan[1], blocks[0], sums ? part : nullptr);
+    auto kernel = heads_bwd_kernel<T, P, INTER, NV, ALL>;
+    if (smem > 48 * 1024) {
+      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+      if (e != cudaSuccess) return static_cast<int>(e);
+    }
+    const int blocks = blocks_of(plan, kResident<T, P, NV>);
+    kernel<<<blocks, kThreads, smem, stream>>>(p, plan, sums ? part : nullptr);
     const int rc = static_cast<int>(cudaGetLastError());
     if (rc != 0 || !sums) return rc;
     return launch_after(heads_reduce_kernel, dim3((p.channels + 31) / 32, 2), 1024, 0, stream, static_cast<const float*>(part),
-                        p.dweight[0], p.dweight[1], blocks[0], grid, p.channels);
+                        p.dweight[0], p.dweight[1], blocks, p.channels);
   });
 }
 
 }  // namespace
 
 size_t heads_bwd_workspace_bytes(int64_t, int, int, int channels, int) {
-  return static_cast<size_t>(kMostBlocks + 2) * channels * sizeof(float);
+  return static_cast<size_t>(2 * kMostBlocks) * channels * sizeof(float);
 }
 int launch_heads(const HeadsParams& p, int is_f32, cudaStream_t stream) {
   return is_f32 ? heads<float>(p, stream) : heads<__nv_bfloat16>(p, stream);
