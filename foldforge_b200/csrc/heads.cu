@@ -56,9 +56,8 @@ __device__ __forceinline__ float2 turn_of(double quarters, uint32_t inverse_sign
                      __uint_as_float(__float_as_uint(sin) ^ ((k & 2) << 30) ^ inverse_sign));
 }
 
-// A token's position on axis `lane` (0 past the last axis).
-__device__ __forceinline__ double place_of(const RotaryParams& r, uint32_t b, uint32_t t) {
-  const int axis = threadIdx.x & 31;
+// A token's position on axis `axis` (0 past the last axis).
+__device__ __forceinline__ double place_of(const RotaryParams& r, uint32_t b, uint32_t t, int axis) {
   if (r.pairs == 0 || axis >= r.axes) return 0.0;
   const int64_t i = b * r.batch + t * r.token + axis * r.axis;
   if (r.type == kPositionI64) return static_cast<double>(static_cast<const int64_t*>(r.positions)[i]);
@@ -66,19 +65,47 @@ __device__ __forceinline__ double place_of(const RotaryParams& r, uint32_t b, ui
   return static_cast<double>(static_cast<const float*>(r.positions)[i]);
 }
 
-// A token's cosines and sines of `slots` pairs (those past the table's: no turn) to a warp's shared memory, from
-// its places on the lanes. A pair whose axis is not there becomes NaN.
-__device__ __forceinline__ void find_turns(const RotaryParams& r, double place, int slots, float* cosines, float* sines) {
-  __syncwarp();
-  for (int j = threadIdx.x & 31; j - static_cast<int>(threadIdx.x & 31) < slots; j += 32) {
-    const int axis = j < r.pairs ? r.pair_axes[j] : 0;
-    double at = __shfl_sync(0xFFFFFFFFu, place, axis & 31);
-    if (axis < 0 || axis >= r.axes) at = __longlong_as_double(0x7FF8000000000000LL);
-    const float2 t = j < r.pairs ? turn_of(at * r.quarters[j], r.inverse ? 0x80000000u : 0u) : make_float2(1.f, 0.f);
-    if (j < slots) {
-      cosines[j] = t.x;
-      sines[j] = t.y;
+// What a block reads again for every token, from its start on in shared memory, so that the first token waits for
+// one load's time and not for several one after the other: the pairs' frequencies and axes, q's and k's weights.
+struct Constants {
+  double* quarters;  // [slots]; NaN where a pair's axis is not there
+  int* axes;
+  float* weights;  // [2][channels, to a multiple of 4]
+  __host__ __device__ static int padded(int channels) { return (channels + 3) / 4 * 4; }
+  __host__ __device__ static int bytes(int slots, int channels) { return slots * 12 + padded(channels) * 8; }
+  __device__ __forceinline__ Constants(const HeadsParams& p, int slots, uint8_t* smem) {
+    quarters = reinterpret_cast<double*>(smem);
+    weights = reinterpret_cast<float*>(quarters + slots);
+    axes = reinterpret_cast<int*>(weights + 2 * padded(p.channels));
+    const RotaryParams& r = p.rotary;
+    for (int j = threadIdx.x; j < r.pairs; j += kThreads) {
+      const int axis = r.pair_axes[j];
+      const double q = r.quarters[j];
+      const bool there = axis >= 0 && axis < r.axes;
+      quarters[j] = there ? q : __longlong_as_double(0x7FF8000000000000LL);
+      axes[j] = there ? axis : 0;
     }
+    for (int c = threadIdx.x; c < 2 * padded(p.channels); c += kThreads) {
+      const int which = c >= padded(p.channels), i = c - which * padded(p.channels);
+      weights[c] = p.weight[which] != nullptr && i < p.channels ? p.weight[which][i] : 1.f;
+    }
+  }
+  __device__ __forceinline__ const float* weight(const HeadsParams& p, int which) const { return weights + which * padded(p.channels); }
+};
+
+// A token's cosines and sines of `slots` pairs (those past the table's: no turn) to a crew's shared memory, from
+// its places on the crew's lanes.
+__device__ __forceinline__ void find_turns(const RotaryParams& r, const Constants& constants, double place, int slots, int crew_lanes,
+                                           float* cosines, float* sines) {
+  __syncwarp();
+  const int lane = threadIdx.x & (crew_lanes - 1), before = (threadIdx.x & 31) - lane;
+  for (int first = 0; first < slots; first += crew_lanes) {
+    const int j = first + lane;
+    const double at = __shfl_sync(0xFFFFFFFFu, place, before + (j < r.pairs ? constants.axes[j] : 0));
+    if (j >= slots) continue;
+    const float2 t = j < r.pairs ? turn_of(at * constants.quarters[j], r.inverse ? 0x80000000u : 0u) : make_float2(1.f, 0.f);
+    cosines[j] = t.x;
+    sines[j] = t.y;
   }
   __syncwarp();
 }
@@ -99,10 +126,10 @@ struct Run {
       }
     }
   }
-  __device__ __forceinline__ void load_again(const T* p) {  // what every token reads
+  __device__ __forceinline__ void load_plain(const T* p) {  // whole 16 bytes
 #pragma unroll
     for (int i = 0; i < static_cast<int>(sizeof(w)) / 16; ++i) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
+      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
       memcpy(w + 4 * i, &v, 16);
     }
   }
@@ -136,7 +163,7 @@ template <typename T>
 struct Run<T, 1> {
   T v;
   __device__ __forceinline__ void load(const T* p) { v = *p; }
-  __device__ __forceinline__ void load_again(const T* p) { v = __ldg(p); }
+  __device__ __forceinline__ void load_plain(const T* p) { v = *p; }
   __device__ __forceinline__ void store(T* p) const { *p = v; }
   __device__ __forceinline__ void zero() { v = static_cast<T>(0.f); }
   __device__ __forceinline__ float get(int) const { return static_cast<float>(v); }
@@ -245,14 +272,13 @@ __device__ __forceinline__ RawPairs<T, P> narrow(const Pairs<P>& v) {
   return raw;
 }
 
-// a weight's values at a lane's pairs (1 without a weight, 0 where there is no channel)
+// a weight's values (in shared memory) at a lane's pairs, 0 where there is no channel
 template <int P, bool INTER>
 __device__ __forceinline__ Pairs<P> weight_of(const float* weight, const Spot<P>& s) {
-  if (weight == nullptr) return {Lanes<P>(1.f), Lanes<P>(1.f)};
   RawPairs<float, P> raw;
   raw.zero();
-  if (s.has_a) raw.a.load_again(weight + s.a);
-  if (s.has_b) raw.b.load_again(weight + s.b);
+  if (s.has_a) raw.a.load_plain(weight + s.a);
+  if (s.has_b) raw.b.load_plain(weight + s.b);
   return widen<float, P, INTER>(raw);
 }
 
@@ -307,12 +333,24 @@ __device__ __forceinline__ void team_sums(float (&v)[N], int team) {
   }
 }
 
-// How a launch's warps share its work: items are a token's next `per` heads; teams of 2^shift lanes; `slots`
-// pairs in a warp's table.
+// How a launch shares its work: an item is a token's next `per` heads, and a crew of 2^crew lanes takes it in teams
+// of 2^shift lanes (a warp is one crew, or several where a token's heads do not fill it: its crews then take one
+// item each, all of the same steps). `slots` pairs in a crew's table.
 struct Plan {
   uint32_t items;
   Divisor chunks, tokens;
-  int per, shift, slots;
+  int per, shift, crew, slots;
+};
+// A lane's place in its warp.
+struct Lane {
+  int lane, team, teams, mine;  // lanes a team, teams a crew, this one's team in its crew
+  int to_teams;                 // log2 of teams
+  uint32_t crew, crews;         // this one's crew in the warp, crews a warp
+  __device__ __forceinline__ explicit Lane(const Plan& plan)
+      : lane(threadIdx.x & 31), team(1 << plan.shift), teams(1 << (plan.crew - plan.shift)),
+        mine((lane & ((1 << plan.crew) - 1)) >> plan.shift), to_teams(plan.crew - plan.shift),
+        crew(static_cast<uint32_t>(lane) >> plan.crew), crews(32u >> plan.crew) {}
+  __device__ __forceinline__ int teams_heads(int count) const { return (count - mine + teams - 1) >> to_teams; }  // of `count` heads
 };
 
 // ---- a lane's ring of S slots for NT tensors
@@ -329,11 +367,14 @@ __device__ __forceinline__ void wait_copies() {
   asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
 }
 
-// A warp's item: a token's heads `first` to `last` of q's and then k's, a phase each.
+// A crew's item: a token's heads `first` to `last` of q's and then k's, a phase each. Past the last item nothing is
+// there, but phases and steps are an item's.
 struct Place {
   uint32_t b, t;
   int first, last;
-  __device__ __forceinline__ Place(const Plan& plan, uint32_t id) {
+  bool there;
+  __device__ __forceinline__ Place(const Plan& plan, uint32_t id) : there(id < plan.items) {
+    if (!there) id = 0;
     const uint32_t token = plan.chunks.quotient(id);
     b = plan.tokens.quotient(token);
     t = token - b * plan.tokens.d;
@@ -367,15 +408,17 @@ struct Stream {
   const HeadsParams& p;
   const Plan& plan;
   const Spot<P> (&spot)[NV];
-  uint32_t id, slot, last_slot;  // addresses of this lane's piece
-  int which, mine, left, steps;
+  const Lane& my;
+  uint32_t id, slot, last_slot;  // the warp's first item; addresses of this lane's piece
+  int which, left, steps;
   Place place;
-  int64_t step[NT];  // elements from a step's heads to the next's
+  int64_t step[NT];  // elements from one of the team's heads to the next
   const T* at[NT];
   RawPairs<T, P> next[kAsync ? 1 : U][NV][NT];
 
-  __device__ __forceinline__ Stream(const HeadsParams& params, const Plan& plan_of, const Spot<P> (&spots)[NV], uint32_t first, uint8_t* smem)
-      : p(params), plan(plan_of), spot(spots), id(first), which(-1), mine((threadIdx.x & 31) >> plan_of.shift), left(0), place(plan_of, first) {
+  __device__ __forceinline__ Stream(const HeadsParams& params, const Plan& plan_of, const Spot<P> (&spots)[NV], const Lane& lane, uint32_t first,
+                                    uint8_t* smem)
+      : p(params), plan(plan_of), spot(spots), my(lane), id(first), which(-1), left(0), place(plan_of, first + lane.crew) {
     slot = smem_u32(smem) + threadIdx.x * kPiece;
     last_slot = slot + (S - 1) * kSlot;
     if constexpr (!kAsync) {
@@ -393,12 +436,11 @@ struct Stream {
 
   // to the next phase that has heads, of this item or the next
   __device__ __forceinline__ void enter() {
-    const int teams = 32 >> plan.shift;
     while (id < plan.items) {
       if (++which == 2) {
-        id += gridDim.x * kWarps;
+        id += gridDim.x * kWarps * my.crews;
         which = -1;
-        if (id < plan.items) place = Place(plan, id);
+        if (id < plan.items) place = Place(plan, id + my.crew);
         continue;
       }
       const int begin = place.begin(p, which), count = place.end(p, which) - begin;
@@ -406,11 +448,11 @@ struct Stream {
 #pragma unroll
       for (int k = 0; k < NT; ++k) {
         const HeadView& v = k == 0 ? p.x[which] : p.dy[which];
-        at[k] = static_cast<const T*>(v.data) + (place.b * v.batch + place.t * v.token + (begin + mine) * v.head);
-        step[k] = U * teams * v.head;
+        at[k] = static_cast<const T*>(v.data) + (place.b * v.batch + place.t * v.token + (begin + my.mine) * v.head);
+        step[k] = my.teams * v.head;
       }
-      left = (count - mine + teams - 1) >> (5 - plan.shift);
-      steps = (count + U * teams - 1) / (U * teams);
+      left = place.there ? my.teams_heads(count) : 0;
+      steps = (count + U * my.teams - 1) / (U * my.teams);
       return;
     }
   }
@@ -423,7 +465,7 @@ struct Stream {
         if (u < left) {
 #pragma unroll
           for (int k = 0; k < NT; ++k) {
-            const T* from = at[k] + (U == 1 ? 0 : u * (step[k] / U));
+            const T* from = at[k] + u * step[k];
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
               if constexpr (kAsync) {
@@ -443,7 +485,7 @@ struct Stream {
         }
       left -= U;
 #pragma unroll
-      for (int k = 0; k < NT; ++k) at[k] += step[k];
+      for (int k = 0; k < NT; ++k) at[k] += U * step[k];
       if (--steps == 0) enter();
     }
     if constexpr (kAsync) {
@@ -478,14 +520,14 @@ struct Stream {
 
 // heads of a team at a time
 template <int P, int NV>
-constexpr int kAtOnce = P > 1 || NV >= 4 ? 1 : 4 / NV;
+constexpr int kAtOnce = P > 1 || NV > 2 ? 1 : 4 / NV;
 
 // Slots of the rings, and blocks that an SM holds. 65536 tokens of 40 heads x 128 in bf16: forward 214 us with two
 // blocks (111 registers a thread) and 3, 4 or 6 slots, 260 with three (80 registers, 150 bytes of them spilled);
 // backward 371 us with 3 slots, 384 with 6, 398 with one block, 624 with three.
 constexpr int kForwardSlots = 3, kBackwardSlots = 3;
 template <typename T, int P, int NV>
-constexpr int kResident = P * NV * static_cast<int>(sizeof(T)) > 16 || NV > 2 ? 1 : 2;
+constexpr int kResident = P * static_cast<int>(sizeof(T)) > 16 || NV > 3 ? 1 : 2;
 
 // Forward. NORM: the norm and its weight. ALL: every pair is turned. NV runs a lane, a team apart.
 template <typename T, int P, bool INTER, int NV, bool ALL, bool NORM>
@@ -494,40 +536,43 @@ __global__ void __launch_bounds__(kThreads, kResident<T, P, NV>)
   constexpr int U = kAtOnce<P, NV>;
   using Heads = Stream<T, P, NV, 1, U, kForwardSlots>;
   extern __shared__ __align__(16) uint8_t smem[];
-  const int lane = threadIdx.x & 31, team = 1 << plan.shift, teams = 32 >> plan.shift, mine = lane >> plan.shift;
-  const uint32_t first = blockIdx.x * kWarps + threadIdx.x / 32;
-  if (first >= plan.items) return;
-  float* cosines = reinterpret_cast<float*>(smem + Heads::kBytes) + threadIdx.x / 32 * 2 * plan.slots;
+  const Lane my(plan);
+  const int warp = threadIdx.x / 32, tables = kWarps * my.crews;
+  const uint32_t first = (blockIdx.x * kWarps + warp) * my.crews, stride = gridDim.x * tables;  // the warp's items
+  float* cosines = reinterpret_cast<float*>(smem + Heads::kBytes) + (warp * my.crews + my.crew) * 2 * plan.slots;
   float* sines = cosines + plan.slots;
   const float inverse_c = 1.0f / static_cast<float>(p.channels);
   Spot<P> spot[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) spot[i] = spot_of<P, INTER>(p.rotary, (lane & (team - 1)) + i * team, p.channels);
-  Heads stream(p, plan, spot, first, smem);
-  Place after(plan, first);
-  double ahead = place_of(p.rotary, after.b, after.t);  // the next item's
+  for (int i = 0; i < NV; ++i) spot[i] = spot_of<P, INTER>(p.rotary, (my.lane & (my.team - 1)) + i * my.team, p.channels);
+  const int crew_lanes = 1 << plan.crew, axis = my.lane & (crew_lanes - 1);
+  Place after(plan, first + my.crew);
+  double ahead = place_of(p.rotary, after.b, after.t, axis);  // the next item's
+  Heads stream(p, plan, spot, my, first, smem);
+  const Constants constants(p, plan.slots, smem + Heads::kBytes + tables * 2 * plan.slots * sizeof(float));
+  __syncthreads();
 #pragma unroll 1
-  for (uint32_t id = first; id < plan.items; id += gridDim.x * kWarps) {
+  for (uint32_t id = first; id < plan.items; id += stride) {
     const Place place = after;
-    find_turns(p.rotary, ahead, plan.slots, cosines, sines);
-    if (id + gridDim.x * kWarps < plan.items) {
-      after = Place(plan, id + gridDim.x * kWarps);
-      ahead = place_of(p.rotary, after.b, after.t);
+    find_turns(p.rotary, constants, ahead, plan.slots, crew_lanes, cosines, sines);
+    if (id + stride < plan.items) {
+      after = Place(plan, id + stride + my.crew);
+      ahead = place_of(p.rotary, after.b, after.t, axis);
     }
 #pragma unroll 1
     for (int which = 0; which < 2; ++which) {
       const int begin = place.begin(p, which), count = place.end(p, which) - begin;
       if (count <= 0) continue;
       const HeadView& out = p.out[which];
-      T* y_head = static_cast<T*>(out.data) + (place.b * out.batch + place.t * out.token + (begin + mine) * out.head);
-      const int64_t out_head = teams * out.head;
-      int left = (count - mine + teams - 1) >> (5 - plan.shift);
+      T* y_head = static_cast<T*>(out.data) + (place.b * out.batch + place.t * out.token + (begin + my.mine) * out.head);
+      const int64_t out_head = my.teams * out.head;
+      int left = place.there ? my.teams_heads(count) : 0;
       Pairs<P> c[NV], s[NV];  // cosines, and sines by the other channel's weight (a's negative)
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const Lanes<P> cosine = from_table<P, INTER>(cosines, spot[i]), sine = from_table<P, INTER>(sines, spot[i]);
         if constexpr (NORM) {
-          const Pairs<P> w = weight_of<P, INTER>(p.weight[which], spot[i]);
+          const Pairs<P> w = weight_of<P, INTER>(constants.weight(p, which), spot[i]);
           c[i] = {cosine * w.a, cosine * w.b};
           s[i] = {negative(sine) * w.b, sine * w.a};
         } else {
@@ -536,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, kResident<T, P, NV>)
         }
       }
 #pragma unroll 1
-      for (int step = (count + U * teams - 1) / (U * teams); step > 0; --step) {
+      for (int step = (count + U * my.teams - 1) / (U * my.teams); step > 0; --step) {
         RawPairs<T, P> raw[U][NV][1];
         Pairs<P> v[U][NV];
         stream.take(raw);
@@ -556,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, kResident<T, P, NV>)
               rstd[u] += P == 1 || spot[i].has_a ? sum : 0.f;
             }
           }
-          team_sums(rstd, team);
+          team_sums(rstd, my.team);
 #pragma unroll
           for (int u = 0; u < U; ++u) {
             rstd[u] = rsqrtf(rstd[u] * inverse_c + p.eps);
@@ -591,42 +636,46 @@ __global__ void __launch_bounds__(kThreads, kResident<T, P, NV>)
   constexpr int U = kAtOnce<P, NV>;
   using Heads = Stream<T, P, NV, 2, U, kBackwardSlots>;
   extern __shared__ __align__(16) uint8_t smem[];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, team = 1 << plan.shift, teams = 32 >> plan.shift, mine = lane >> plan.shift;
-  const uint32_t first = blockIdx.x * kWarps + warp;
-  float* cosines = reinterpret_cast<float*>(smem + Heads::kBytes) + warp * 2 * plan.slots;
+  const Lane my(plan);
+  const int warp = threadIdx.x / 32, tables = kWarps * my.crews;
+  const uint32_t first = (blockIdx.x * kWarps + warp) * my.crews, stride = gridDim.x * tables;  // the warp's items
+  float* cosines = reinterpret_cast<float*>(smem + Heads::kBytes) + (warp * my.crews + my.crew) * 2 * plan.slots;
   float* sines = cosines + plan.slots;
   const float inverse_c = 1.0f / static_cast<float>(p.channels);
   Spot<P> spot[NV];
   Pairs<P> dw[2][NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    spot[i] = spot_of<P, INTER>(p.rotary, (lane & (team - 1)) + i * team, p.channels);
+    spot[i] = spot_of<P, INTER>(p.rotary, (my.lane & (my.team - 1)) + i * my.team, p.channels);
     dw[0][i] = dw[1][i] = {Lanes<P>(0.f), Lanes<P>(0.f)};
   }
-  Heads stream(p, plan, spot, first, smem);
-  Place after(plan, first);
-  double ahead = first < plan.items ? place_of(p.rotary, after.b, after.t) : 0.0;  // the next item's
+  const int crew_lanes = 1 << plan.crew, axis = my.lane & (crew_lanes - 1);
+  Place after(plan, first + my.crew);
+  double ahead = place_of(p.rotary, after.b, after.t, axis);  // the next item's
+  Heads stream(p, plan, spot, my, first, smem);
+  const Constants constants(p, plan.slots, smem + Heads::kBytes + tables * 2 * plan.slots * sizeof(float));
+  __syncthreads();
 #pragma unroll 1
-  for (uint32_t id = first; id < plan.items; id += gridDim.x * kWarps) {
+  for (uint32_t id = first; id < plan.items; id += stride) {
     const Place place = after;
-    find_turns(p.rotary, ahead, plan.slots, cosines, sines);
-    if (id + gridDim.x * kWarps < plan.items) {
-      after = Place(plan, id + gridDim.x * kWarps);
-      ahead = place_of(p.rotary, after.b, after.t);
+    find_turns(p.rotary, constants, ahead, plan.slots, crew_lanes, cosines, sines);
+    if (id + stride < plan.items) {
+      after = Place(plan, id + stride + my.crew);
+      ahead = place_of(p.rotary, after.b, after.t, axis);
     }
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       const int begin = place.begin(p, which), count = place.end(p, which) - begin;
       if (count <= 0) continue;
       const HeadView& out = p.out[which];
-      T* dx_head = static_cast<T*>(out.data) + (place.b * out.batch + place.t * out.token + (begin + mine) * out.head);
-      const int64_t out_head = teams * out.head;
-      int left = (count - mine + teams - 1) >> (5 - plan.shift);
+      T* dx_head = static_cast<T*>(out.data) + (place.b * out.batch + place.t * out.token + (begin + my.mine) * out.head);
+      const int64_t out_head = my.teams * out.head;
+      int left = place.there ? my.teams_heads(count) : 0;
       Pairs<P> w[NV];
 #pragma unroll
-      for (int i = 0; i < NV; ++i) w[i] = weight_of<P, INTER>(p.weight[which], spot[i]);
+      for (int i = 0; i < NV; ++i) w[i] = weight_of<P, INTER>(constants.weight(p, which), spot[i]);
 #pragma unroll 1
-      for (int step = (count + U * teams - 1) / (U * teams); step > 0; --step) {
+      for (int step = (count + U * my.teams - 1) / (U * my.teams); step > 0; --step) {
         RawPairs<T, P> raw[U][NV][2];
         Pairs<P> v[U][NV], g[U][NV];
         stream.take(raw);
@@ -649,7 +698,7 @@ __global__ void __launch_bounds__(kThreads, kResident<T, P, NV>)
           }
         }
         stream.fetch();
-        team_sums(sums, team);
+        team_sums(sums, my.team);
 #pragma unroll
         for (int u = 0; u < U; ++u)
           if (u < left) {
@@ -679,11 +728,11 @@ __global__ void __launch_bounds__(kThreads, kResident<T, P, NV>)
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      for (int o = 16; o >= team; o >>= 1) {
+      for (int o = 16; o >= my.team; o >>= 1) {
         dw[which][i].a = dw[which][i].a.each([&](float f) { return f + __shfl_xor_sync(0xFFFFFFFFu, f, o); });
         dw[which][i].b = dw[which][i].b.each([&](float f) { return f + __shfl_xor_sync(0xFFFFFFFFu, f, o); });
       }
-      if (lane < team) {
+      if (my.lane < my.team) {
 #pragma unroll
         for (int j = 0; j < P; ++j) {
           const int at = !INTER ? spot[i].a + j : j < P / 2 ? spot[i].a + 2 * j : spot[i].b + 2 * j - P;
@@ -764,32 +813,50 @@ int dispatch_heads(const HeadsParams& p, bool backward, F&& f) {
   const std::false_type apart;
   if (pairs <= 32) return f(one, apart, std::integral_constant<int, 1>{}, apart, pairs);
   if (pairs <= 64) return f(one, apart, std::integral_constant<int, 2>{}, apart, 32);
+  if (pairs <= 96) return f(one, apart, std::integral_constant<int, 3>{}, apart, 32);
   if (pairs <= 128) return f(one, apart, std::integral_constant<int, 4>{}, apart, 32);
   return f(one, apart, std::integral_constant<int, 8>{}, apart, 32);
 }
 
-// Items of `per` heads: all of a token's where the tokens keep the GPU's warps busy, else no more than a team
-// takes at once.
-Plan plan_of(const HeadsParams& p, int heads, int lanes, int run, int nv) {
-  Plan plan{0, Divisor(1), Divisor(static_cast<uint32_t>(p.tokens)), heads, 0, 0};
+// How a token's heads are cut into items: an item costs its token's angles, about as long as two steps take, and
+// its steps, and the GPU's warps take the items in rounds. All heads in one item where there are many tokens,
+// single steps where there are few.
+Plan plan_of(const HeadsParams& p, int lanes, int run, int nv, int at_once, int resident) {
+  const int heads = p.heads[0] + p.heads[1], larger = p.heads[0] > p.heads[1] ? p.heads[0] : p.heads[1];
+  Plan plan{0, Divisor(1), Divisor(static_cast<uint32_t>(p.tokens)), heads, 0, 0, 0};
   while ((1 << plan.shift) < lanes) ++plan.shift;
-  plan.slots = (run * nv) << plan.shift;
-  const int64_t tokens = static_cast<int64_t>(p.batch) * p.tokens;
-  const int at_once = 32 >> plan.shift;
-  int64_t chunks = (148 * 16 + tokens - 1) / tokens;
-  const int64_t most = (heads + at_once - 1) / at_once;
-  if (chunks > most) chunks = most;
-  plan.per = static_cast<int>((heads + chunks * at_once - 1) / (chunks * at_once)) * at_once;
-  chunks = (heads + plan.per - 1) / plan.per;
-  plan.chunks = Divisor(static_cast<uint32_t>(chunks));
-  plan.items = static_cast<uint32_t>(tokens * chunks);
+  plan.slots = (((run * nv) << plan.shift) + 3) / 4 * 4;
+  plan.crew = plan.shift;
+  while (plan.crew < 5 && (at_once << (plan.crew - plan.shift) < larger || (p.rotary.pairs > 0 && 1 << plan.crew < p.rotary.axes))) ++plan.crew;
+  const int64_t tokens = static_cast<int64_t>(p.batch) * p.tokens, crews = 148 * kWarps * static_cast<int64_t>(resident) * (32 >> plan.crew);
+  const int step = at_once << (plan.crew - plan.shift), steps = (heads + step - 1) / step;
+  int64_t best = 0;
+  for (int of = steps; of >= 1; of = (of + 1) / 2) {  // steps an item
+    const int64_t chunks = (steps + of - 1) / of, rounds = (tokens * chunks + crews - 1) / crews, cost = rounds * (2 + of);
+    if (best == 0 || cost < best) {
+      best = cost;
+      plan.per = of * step;
+      plan.chunks = Divisor(static_cast<uint32_t>(chunks));
+      plan.items = static_cast<uint32_t>(tokens * chunks);
+    }
+    // crews of one warp take the same steps
+    if (of == 1 || plan.crew < 5 || tokens * chunks >= int64_t(1) << 29) break;
+  }
+  if (plan.crew < 5) {
+    plan.per = heads;
+    plan.chunks = Divisor(1);
+    plan.items = static_cast<uint32_t>(tokens);
+  }
   return plan;
+}
+size_t table_bytes(const Plan& plan, int channels) {
+  return sizeof(float) * kWarps * (32 >> plan.crew) * 2 * plan.slots + Constants::bytes(plan.slots, channels);
 }
 
 constexpr int kMostBlocks = 148 * 2;
 
 int blocks_of(const Plan& plan, int resident) {
-  const int64_t want = (static_cast<int64_t>(plan.items) + kWarps - 1) / kWarps, most = 148 * resident;
+  const int64_t warp_items = kWarps * (32 >> plan.crew), want = (plan.items + warp_items - 1) / warp_items, most = 148 * resident;
   return static_cast<int>(want < most ? want : most);
 }
 
@@ -798,8 +865,8 @@ int heads(const HeadsParams& p, cudaStream_t stream) {
   return dispatch_heads<T>(p, false, [&](auto run, auto inter, auto nv, auto all, int lanes) {
     constexpr int P = decltype(run)::value, NV = decltype(nv)::value;
     constexpr bool INTER = decltype(inter)::value, ALL = decltype(all)::value;
-    const Plan plan = plan_of(p, p.heads[0] + p.heads[1], lanes, P, NV);
-    const size_t smem = Stream<T, P, NV, 1, kAtOnce<P, NV>, kForwardSlots>::kBytes + sizeof(float) * kWarps * 2 * plan.slots;
+    const Plan plan = plan_of(p, lanes, P, NV, kAtOnce<P, NV>, kResident<T, P, NV>);
+    const size_t smem = Stream<T, P, NV, 1, kAtOnce<P, NV>, kForwardSlots>::kBytes + table_bytes(plan, p.channels);
     auto kernel = p.norm ? heads_kernel<T, P, INTER, NV, ALL, true> : heads_kernel<T, P, INTER, NV, ALL, false>;
     if (smem > 48 * 1024) {
       const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
@@ -816,8 +883,8 @@ int heads_bwd(const HeadsParams& p, float* part, cudaStream_t stream) {
   return dispatch_heads<T>(p, true, [&](auto run, auto inter, auto nv, auto all, int lanes) {
     constexpr int P = decltype(run)::value, NV = decltype(nv)::value;
     constexpr bool INTER = decltype(inter)::value, ALL = decltype(all)::value;
-    const Plan plan = plan_of(p, p.heads[0] + p.heads[1], lanes, P, NV);
-    size_t smem = Stream<T, P, NV, 2, kAtOnce<P, NV>, kBackwardSlots>::kBytes + sizeof(float) * kWarps * 2 * plan.slots;
+    const Plan plan = plan_of(p, lanes, P, NV, kAtOnce<P, NV>, kResident<T, P, NV>);
+    size_t smem = Stream<T, P, NV, 2, kAtOnce<P, NV>, kBackwardSlots>::kBytes + table_bytes(plan, p.channels);
     if (smem < sizeof(float) * kWarps * p.channels) smem = sizeof(float) * kWarps * p.channels;
     auto kernel = heads_bwd_kernel<T, P, INTER, NV, ALL>;
     if (smem > 48 * 1024) {

@@ -212,7 +212,9 @@ def test_without_weights_positions_or_k():
     frozen = kernels.qk_norm_rotary_backward(dq, dk, q, k, turn.positions, turn.table, None, w, EPS, weight_gradient=False)
     assert frozen[3] is None and torch.equal(frozen[0], out[0]) and torch.equal(frozen[1], out[1])
     only = kernels.qk_norm_rotary_backward(dk, None, k, None, turn.positions, turn.table, w, None, EPS)
-    assert torch.equal(only[0], out[1]) and only[1] is None and torch.equal(only[2], out[3])
+    assert torch.equal(only[0], out[1]) and only[1] is None
+    # alone, k's heads are shared out in another way, so its sums have another order: both lie within the sums' bound
+    check([only[2]], [dw], [edw], [F32])
 
 
 @pytest.mark.parametrize("shape", [(0, 4, 64), (2, 0, 4, 64), (0, 5, 4, 64), (5, 0, 64)])
