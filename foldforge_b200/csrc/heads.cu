@@ -818,9 +818,9 @@ int dispatch_heads(const HeadsParams& p, bool backward, F&& f) {
   return f(one, apart, std::integral_constant<int, 8>{}, apart, 32);
 }
 
-// How a token's heads are cut into items: an item costs its token's angles, about as long as two steps take, and
-// its steps, and the GPU's warps take the items in rounds. All heads in one item where there are many tokens,
-// single steps where there are few.
+// How a token's heads are cut into items: an item costs its token's angles, about as long as a step takes, and its
+// steps, and the GPU's warps take the items in rounds. All heads in one item where there are many tokens, single
+// steps where there are few. (Single steps everywhere: 65536 tokens of 40 heads x 128 599 us for 229.)
 Plan plan_of(const HeadsParams& p, int lanes, int run, int nv, int at_once, int resident) {
   const int heads = p.heads[0] + p.heads[1], larger = p.heads[0] > p.heads[1] ? p.heads[0] : p.heads[1];
   Plan plan{0, Divisor(1), Divisor(static_cast<uint32_t>(p.tokens)), heads, 0, 0, 0};
@@ -832,7 +832,7 @@ Plan plan_of(const HeadsParams& p, int lanes, int run, int nv, int at_once, int 
   const int step = at_once << (plan.crew - plan.shift), steps = (heads + step - 1) / step;
   int64_t best = 0;
   for (int of = steps; of >= 1; of = (of + 1) / 2) {  // steps an item
-    const int64_t chunks = (steps + of - 1) / of, rounds = (tokens * chunks + crews - 1) / crews, cost = rounds * (2 + of);
+    const int64_t chunks = (steps + of - 1) / of, rounds = (tokens * chunks + crews - 1) / crews, cost = rounds * (1 + of);
     if (best == 0 || cost < best) {
       best = cost;
       plan.per = of * step;

@@ -47,7 +47,7 @@ OP_CLASSES: dict[str, tuple[str, ...]] = {
     "msa_pwa": ("MSAPairWeightedAveraging",),
     "single_attention": ("AttentionPairBias",),
     "transition": ("Transition",),
-    "layernorm": ("LayerNorm",),
+    "layernorm": ("LayerNorm", "QKNorm"),
     "conditioning": (),
     "dit_blocks": ("TokenDiT",),
     "atom_blocks": (),

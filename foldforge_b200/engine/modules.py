@@ -21,6 +21,7 @@ applies the reference equations there too.
 from __future__ import annotations
 
 from contextvars import ContextVar
+from copy import deepcopy
 from dataclasses import dataclass
 
 import torch
@@ -34,6 +35,8 @@ Tensor = torch.Tensor
 MAX_TRAINED_CHANNELS = 8192
 #: channels of either operand of a weight gradient
 MAX_WEIGHT_GRAD_CHANNELS = 1 << 20
+#: channels of a head that the b200 norm of queries and keys takes
+MAX_HEAD_CHANNELS = 512
 MASKED_UPDATES = ("zero", "compute")
 #: the op whose forward pass trains in this context
 _training_op: ContextVar[nn.Module | None] = ContextVar("_training_op", default=None)
@@ -123,6 +126,119 @@ class LayerNorm(nn.LayerNorm):
         if self._trains(x):
             return training.layer_norm(x, self.weight, self.bias, self.eps, self.checkpoint)
         return kernels.layer_norm(x, self.weight, self.bias, self.eps)
+
+
+class QKNorm(nn.Module):
+    """Queries and keys before an attention: each head divided by the root of its channels' mean square, times a
+    weight (``q_weight``, ``k_weight`` ``[d_head]``, fp32 under any cast), then turned in pairs by its token's
+    positions where the module has ``frequencies`` (radians a unit of position for each pair, on axis ``axes[i]``
+    of the positions; :func:`foldforge_b200.kernels.rotary_frequencies` makes a ladder). Called as ``qk_norm(q
+    [.., tokens, heads, d_head], k [.., tokens, other heads, d_head], positions [.., tokens, axes])``; returns
+    both. Not a residual module. With ``checkpoint`` set it has a gradient on b200."""
+
+    backends = ("pytorch", "b200")
+    dispatches_policy = True
+
+    #: what the b200 backend keeps for a backward pass (``foldforge_b200.engine.training``)
+    checkpoint: str | None = None
+
+    def __init__(self, d_head: int, *, frequencies=None, axes=None, interleaved: bool = False, eps: float = 1e-6,
+                 elementwise_affine: bool = True) -> None:
+        super().__init__()
+        self.d_head, self.eps, self.backend = d_head, eps, "pytorch"
+        self.q_weight = nn.Parameter(torch.ones(d_head)) if elementwise_affine else None
+        self.k_weight = nn.Parameter(torch.ones(d_head)) if elementwise_affine else None
+        self.frequencies = None if frequencies is None else tuple(float(f) for f in frequencies)
+        self.axes = (0,) * len(self.frequencies or ()) if axes is None else tuple(int(a) for a in axes)
+        self.interleaved = interleaved
+        if self.frequencies is not None and (2 * len(self.frequencies) > d_head or len(self.axes) != len(self.frequencies)):
+            raise ValueError(f"{len(self.frequencies)} frequencies on axes {self.axes} for heads of {d_head} channels")
+        self._tables: dict[torch.device, object] = {}
+
+    def _apply(self, fn, recurse=True):  # noqa: ANN001
+        out = super()._apply(fn, recurse)
+        for p in self.parameters(recurse=False):
+            if p.dtype != torch.float32:
+                p.data = p.data.float()
+        return out
+
+    def __deepcopy__(self, memo):
+        copy = self.__new__(type(self))
+        memo[id(self)] = copy
+        copy.__dict__.update({k: ({} if k == "_tables" else deepcopy(v, memo)) for k, v in self.__dict__.items()})
+        return copy
+
+    def set_backend(self, name: str) -> None:
+        _check_backend(self, name)
+        self.backend = name
+
+    def set_checkpoint(self, name: str | None) -> None:
+        self.checkpoint = training.check_name(name)
+
+    def table(self, device: torch.device):
+        """The rotation's table on ``device``, made once."""
+        from foldforge_b200 import kernels
+
+        if self.frequencies is None:
+            return None
+        if device not in self._tables:
+            self._tables[device] = kernels.rotary_table(self.frequencies, self.axes, interleaved=self.interleaved, device=device)
+        return self._tables[device]
+
+    def _trains(self, *ts: Tensor) -> bool:
+        return self.checkpoint is not None and training.needs_gradient(self, *ts)
+
+    def unsupported(self, q: Tensor, k: Tensor, positions: Tensor | None = None) -> str | None:
+        if self.backend == "pytorch":
+            return None
+        trains = self._trains(q, k)
+        reason = _device_reason(q, k, positions) if trains else _cuda_reason(q, k, positions)
+        if reason is None and not trains and training.needs_gradient(self):
+            reason = "autograd is not supported by the b200 kernels (inference only)"
+        if reason or (reason := _library_reason()):
+            return reason
+        if q.dtype not in (torch.bfloat16, torch.float32) or k.dtype != q.dtype:
+            return f"dtypes {q.dtype} and {k.dtype} (both bf16 or both fp32)"
+        if q.dim() not in (3, 4) or self.d_head > MAX_HEAD_CHANNELS:
+            return f"q {tuple(q.shape)} (b200: [tokens, heads, d] or [batch, tokens, heads, d], d at most {MAX_HEAD_CHANNELS})"
+        if positions is not None and positions.dtype not in (torch.int32, torch.int64, torch.float32):
+            return f"positions are {positions.dtype} (b200: int32, int64 or fp32)"
+        if trains and positions is not None and positions.requires_grad:
+            return "positions have no gradient"
+        if self.frequencies is not None and torch.device(q.device) not in self._tables and training.capture_reason():
+            return "the rotation's table is made by the first call, which is not captured"
+        return training.capture_reason() if trains else None
+
+    def forward(self, q: Tensor, k: Tensor, positions: Tensor | None = None):
+        if (positions is None) != (self.frequencies is None):
+            raise ValueError("positions go with frequencies" if positions is None else "positions for a module without frequencies")
+        return _dispatch(self, q, k, positions)
+
+    def _forward_pytorch(self, q: Tensor, k: Tensor, positions: Tensor | None = None):
+        def normal(x: Tensor, weight: Tensor | None) -> Tensor:
+            v = x.float()
+            v = v * torch.rsqrt(v.square().mean(-1, keepdim=True) + self.eps)
+            v = v if weight is None else v * weight
+            if positions is None:
+                return v.to(x.dtype)
+            n = len(self.frequencies)
+            angle = positions[..., list(self.axes)].double() * torch.tensor(self.frequencies, dtype=torch.float64, device=x.device)
+            cos, sin = angle[..., None, :].cos().float(), angle[..., None, :].sin().float()
+            if self.interleaved:
+                a, b = v[..., 0:2 * n:2], v[..., 1:2 * n:2]
+                turned = torch.stack([a * cos - b * sin, b * cos + a * sin], -1).flatten(-2)
+            else:
+                a, b = v[..., :n], v[..., n:2 * n]
+                turned = torch.cat([a * cos - b * sin, b * cos + a * sin], -1)
+            return torch.cat([turned, v[..., 2 * n:]], -1).to(x.dtype)
+
+        return normal(q, self.q_weight), normal(k, self.k_weight)
+
+    def _forward_b200(self, q: Tensor, k: Tensor, positions: Tensor | None = None):
+        from foldforge_b200 import kernels
+
+        args = (q, k, positions, self.table(q.device), self.q_weight, self.k_weight, self.eps)
+        return training.qk_norm_rotary(*args, self.checkpoint) if self._trains(q, k) else kernels.qk_norm_rotary(*args)
 
 
 # --------------------------------------------------------------------------- helpers
@@ -218,6 +334,10 @@ def _ln(x: Tensor, norm: nn.LayerNorm) -> Tensor:
     return F.layer_norm(x, norm.normalized_shape, w, b, norm.eps)
 
 
+#: the fused b200 ops add their residual themselves
+_DROPOUT_REASON = "dropout of the update (the b200 op adds its residual itself)"
+
+
 class _PairOp(MasterWeights, nn.Module):
     """Shared plumbing of the pair ops: backend selection, refusals, the packed-weight cache."""
 
@@ -227,6 +347,9 @@ class _PairOp(MasterWeights, nn.Module):
     dead = False
     #: channels the b200 kernels are built for
     b200_channels = 128
+    #: the rate at which training mode drops the update (``_Dropped`` ops), and the axis that shares a mask
+    dropout: float = 0.0
+    dropout_shared = -3
 
     def __init__(self) -> None:
         super().__init__()
@@ -238,8 +361,11 @@ class _PairOp(MasterWeights, nn.Module):
         _check_backend(self, name)
         self.backend = name
 
+    def _drops(self) -> bool:
+        return self.training and self.dropout > 0
+
     def _pair_reason(self, x: Tensor, key_mask: Tensor | None) -> str | None:
-        reason = _cuda_reason(x, key_mask) or _library_reason()
+        reason = _cuda_reason(x, key_mask) or _library_reason() or (_DROPOUT_REASON if self._drops() else None)
         if reason:
             return reason
         if x.dtype not in (torch.bfloat16, torch.float32):
@@ -312,11 +438,25 @@ class _PairOp(MasterWeights, nn.Module):
     def _zero_masked(self, x: Tensor, delta: Tensor, key_mask: Tensor | None) -> Tensor:
         if self._masked_zero() and key_mask is not None:
             delta = delta * _pair_mask(key_mask, x)[..., None]
+        return self._add(x, delta)
+
+    def _add(self, x: Tensor, delta: Tensor) -> Tensor:
+        """The residual and its update, which training mode may drop."""
+        if self._drops():
+            return training.dropout_add(x, delta, self.dropout, self.dropout_shared)
         return (x.float() + delta).to(x.dtype)
 
 
+class _Dropped:
+    """An op whose update training mode drops once :meth:`set_dropout` is called (off otherwise, whatever
+    ``p_drop`` says)."""
+
+    def set_dropout(self, p: float | None = None) -> None:
+        self.dropout = training.check_rate(self.p_drop if p is None else p)
+
+
 # --------------------------------------------------------------------------- triangle multiplication
-class TriangleMultiplication(_PairOp):
+class TriangleMultiplication(_Dropped, _PairOp):
     """Triangle multiplicative update, outgoing or incoming, residual included.
 
     Reference equations: ``legacy/reference/triangle.py:19-50`` (``triangle_update``),
@@ -379,7 +519,7 @@ class TriangleMultiplication(_PairOp):
 TRIANGLE_ATTENTION_MODELS: dict[str, str] = {"af3": "TriangleAttentionAF3"}
 
 
-class TriangleAttention(_PairOp):
+class TriangleAttention(_Dropped, _PairOp):
     """Triangle attention around the starting (rows) or ending (columns) node.
 
     ``TriangleAttention(..., model=key)`` builds the class of ``key``; only AF3's
@@ -401,6 +541,7 @@ class TriangleAttention(_PairOp):
         hidden = d_hidden * n_head if d_hidden else d_pair
         self.d_pair, self.n_head, self.starting, self.p_drop, self.model = d_pair, n_head, starting, p_drop, model
         self.d_head = hidden // n_head
+        self.dropout_shared = -3 if starting else -2  # one mask for all rows, around the ending node for all columns
         self.ln_pair = LayerNorm(d_pair)
         self.to_bias = nn.Linear(d_pair, n_head, bias=False)
         self.to_query = nn.Linear(d_pair, hidden, bias=False)
@@ -722,7 +863,7 @@ class OuterProductMean(_PairOp):
         return kernels.outer_product_mean(msa, row_mask, packed, count_offset=self.count_offset)
 
 
-class MSAPairWeightedAveraging(_PairOp):
+class MSAPairWeightedAveraging(_Dropped, _PairOp):
     """MSA pair-weighted averaging with residual: per head, the pair's logits ``W_b LN(z)[i, j]``
     (minus 1e9 at columns no MSA row has) give softmax weights over j that average the values
     ``W_v LN(msa)`` of each MSA row; sigmoid-gated by ``W_g LN(msa)``, projected back by ``W_o``
@@ -747,7 +888,7 @@ class MSAPairWeightedAveraging(_PairOp):
             return None
         if (self.d_msa, self.d_pair, self.n_head, self.d_hidden) != (64, 128, 8, 8):
             return f"widths ({self.d_msa}, {self.d_pair}, {self.n_head} x {self.d_hidden}) (b200: 64, 128, 8 x 8)"
-        reason = _cuda_reason(msa, pair, key_mask) or _library_reason()
+        reason = _cuda_reason(msa, pair, key_mask) or _library_reason() or (_DROPOUT_REASON if self._drops() else None)
         if reason:
             return reason
         if msa.dtype != torch.bfloat16 or pair.dtype != torch.bfloat16:
@@ -770,7 +911,7 @@ class MSAPairWeightedAveraging(_PairOp):
         v = _linear(x, self.to_value).reshape(b, s, n, self.n_head, self.d_hidden)
         avg = torch.einsum("bhij,bsjhc->bsihc", weights, v).reshape(b, s, n, -1)
         delta = _linear(torch.sigmoid(_linear(x, self.to_gate)) * avg, self.to_out)
-        return (msa.float() + delta).to(msa.dtype)
+        return self._add(msa, delta)
 
     @honours_dead
     def _forward_b200(self, msa: Tensor, pair: Tensor, key_mask: Tensor | None = None) -> Tensor:
@@ -822,15 +963,15 @@ class PairformerBlock(MasterWeights, nn.Module):
         self.config = config
         self.backend = "pytorch"
         c = config.d_pair
-        self.tri_multi_outgoing = TriangleMultiplication(c, config.d_hidden_tri_multi, outgoing=True)
-        self.tri_multi_incoming = TriangleMultiplication(c, config.d_hidden_tri_multi, outgoing=False)
+        self.tri_multi_outgoing = TriangleMultiplication(c, config.d_hidden_tri_multi, outgoing=True, p_drop=config.p_drop)
+        self.tri_multi_incoming = TriangleMultiplication(c, config.d_hidden_tri_multi, outgoing=False, p_drop=config.p_drop)
         if config.use_triangle_attention:
             self.tri_atten_starting = TriangleAttention(c, config.n_head_tri_attention,
                                                         d_hidden=config.d_hidden_tri_attention, starting=True,
-                                                        model=config.model)
+                                                        p_drop=config.p_drop, model=config.model)
             self.tri_atten_ending = TriangleAttention(c, config.n_head_tri_attention,
                                                       d_hidden=config.d_hidden_tri_attention, starting=False,
-                                                      model=config.model)
+                                                      p_drop=config.p_drop, model=config.model)
         self.transition_pair = Transition(c, config.pair_transition_n)
         if config.d_single > 0:
             self.single_attention = AttentionPairBias(config.d_single, c, config.n_head_single,

@@ -1,4 +1,4 @@
-"""Gradients of the engine ops on the ``b200`` backend.
+"""Gradients of the engine ops on the ``b200`` backend, and the dropout of their updates.
 
 An op's ``checkpoint`` says what its forward pass keeps for the backward pass, and with that whether the
 op has one on b200 at all:
@@ -17,6 +17,13 @@ are asked for are formed.
 A backward pass is not captured into a CUDA graph: autograd keeps a leaf's accumulation on the stream of
 the graph that made it first, and capturing another while that one lives ends the process. A captured
 training step calls the functions of :mod:`foldforge_b200.kernels` itself.
+
+:func:`set_dropout` turns on the dropout of the pair and MSA updates (``TriangleMultiplication``,
+``TriangleAttention``, ``MSAPairWeightedAveraging``), which is off otherwise: in training mode an update is
+dropped before its residual is added, one mask for all rows (for all columns around the ending node). The
+masks come from a counter-based generator and are not stored; their seeds from torch's default CPU generator
+(``torch.manual_seed``), which activation checkpointing restores. The b200 backend's fused ops add their
+residual themselves, so an op whose dropout is on runs the ``pytorch`` backend.
 """
 
 from __future__ import annotations
@@ -44,6 +51,21 @@ def set_checkpoint(model: nn.Module, name: str | None) -> list[str]:
     for _, m in found:
         m.set_checkpoint(name)
     return [path for path, _ in found]
+
+
+def set_dropout(model: nn.Module, p: float | None = None) -> list[str]:
+    """Drop the updates of every op under ``model`` that takes dropout with rate ``p`` (``None``: the op's own
+    ``p_drop``; 0: none) while it is in training mode; their names."""
+    found = [(path, m) for path, m in model.named_modules() if hasattr(m, "set_dropout")]
+    for _, m in found:
+        m.set_dropout(p)
+    return [path for path, _ in found]
+
+
+def check_rate(p: float) -> float:
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"a dropout rate lies in [0, 1], got {p!r}")
+    return float(p)
 
 
 def needs_gradient(module: nn.Module, *inputs: Tensor) -> bool:
@@ -191,3 +213,106 @@ def transition(x: Tensor, mask: Tensor | None, run, kind: str, eps: float, *weig
     """``run(x)`` with a gradient. ``mask`` (bool, the shape of x without its channels): where the update is
     kept; ``weights``: LayerNorm weight and bias, expand_a, expand_b, squeeze."""
     return _Transition.apply(x, mask, run, kind, eps, *weights)
+
+
+class _QKNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q: Tensor, k: Tensor | None, positions: Tensor | None, table, q_weight: Tensor | None,
+                k_weight: Tensor | None, eps: float, kind: str):
+        from foldforge_b200 import kernels
+
+        ctx.table, ctx.eps, ctx.kind = table, eps, kind
+        kept: list[Tensor | None] = [q, k]
+        if kind != "exact":
+            ctx.kept_as = [None if t is None else (t.shape, t.dtype) for t in kept]
+            kept = [None if t is None else kernels.checkpoint_pack(t).data for t in kept]
+        ctx.save_for_backward(*kept, positions, q_weight, k_weight)
+        q_out, k_out = kernels.qk_norm_rotary(q, k, positions, table, q_weight, k_weight, eps)
+        return q_out, k_out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq_out: Tensor | None, dk_out: Tensor | None):
+        from foldforge_b200 import kernels
+
+        _refuse_capture()
+        q, k, positions, q_weight, k_weight = ctx.saved_tensors
+        if ctx.kind != "exact":
+            q, k = (None if t is None else kernels.checkpoint_unpack(kernels.Checkpoint8(t, *as_was))
+                    for t, as_was in zip((q, k), ctx.kept_as, strict=True))
+        wanted = ctx.needs_input_grad
+        dq, dk, dq_weight, dk_weight = kernels.qk_norm_rotary_backward(
+            dq_out, dk_out, q, k, positions, ctx.table, q_weight, k_weight, ctx.eps, weight_gradient=wanted[4] or wanted[5])
+        return (dq if wanted[0] else None, dk if wanted[1] else None, None, None, dq_weight if wanted[4] else None,
+                dk_weight if wanted[5] else None, None, None)
+
+
+def qk_norm_rotary(q: Tensor, k: Tensor | None, positions: Tensor | None, table, q_weight: Tensor | None,
+                   k_weight: Tensor | None, eps: float, kind: str) -> tuple[Tensor, Tensor | None]:
+    """:func:`foldforge_b200.kernels.qk_norm_rotary` with a gradient (none for the positions)."""
+    if positions is not None and positions.requires_grad:
+        raise ValueError("positions have no gradient")
+    return _QKNorm.apply(q, k, positions, table, q_weight, k_weight, eps, kind)
+
+
+# --------------------------------------------------------------------------- dropout
+def dropout_keep(shape, p: float, seed: int, offset: int = 0, shared: tuple[int, ...] = (), device=None) -> Tensor:
+    """The mask (True: kept) that :func:`foldforge_b200.kernels.dropout_train` draws, in integer operations on any
+    device: element m of ``shape`` without its ``shared`` axes stays where word m % 4 of Philox4x32-10 (Salmon et
+    al., "Parallel random numbers: as easy as 1, 2, 3", 2011) at counter m // 4 is at least p 2^32."""
+    low = (1 << 32) - 1
+    seed, offset = seed & (1 << 64) - 1, offset & (1 << 64) - 1
+    small = [1 if i in shared else n for i, n in enumerate(shape)]
+    count = torch.Size(small).numel()
+    group = torch.arange(-(-count // 4), dtype=torch.int64, device=device)
+    c = [group & low, group >> 32, torch.full_like(group, offset & low), torch.full_like(group, offset >> 32)]
+    k = [seed & low, seed >> 32]
+    for _ in range(10):
+        a, b = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57  # 64-bit products wrap and keep their bits
+        c = [(b >> 32 & low) ^ c[1] ^ k[0], b & low, (a >> 32 & low) ^ c[3] ^ k[1], a & low]
+        k = [k[0] + 0x9E3779B9 & low, k[1] + 0xBB67AE85 & low]
+    words = torch.stack(c, -1).flatten()[:count]
+    return (words >= round(p * 2**32)).view(small).expand(shape)
+
+
+def _on_b200(*ts: Tensor) -> bool:
+    return all(t.is_cuda and t.dtype in (torch.bfloat16, torch.float32) for t in ts) and \
+        torch.cuda.get_device_capability(ts[0].device) == (10, 0)
+
+
+def _dropped(x: Tensor, residual: Tensor | None, p: float, seed: int, shared: int, dtype: torch.dtype) -> Tensor:
+    """``residual + keep(x) / (1 - p)``, or without residual in ``dtype``"""
+    from foldforge_b200 import kernels
+
+    axes = (shared % x.dim(),)
+    if _on_b200(x, *(() if residual is None else (residual,))) and (residual is not None or dtype in (torch.bfloat16, torch.float32)):
+        if residual is not None:
+            return kernels.dropout_train(x, p, seed, residual=residual, shared=axes)[0]
+        return kernels.dropout_backward(x, kernels.DropoutSaved(p, seed, 0, axes, x.shape, dtype, x.dtype))
+    keep = dropout_keep(x.shape, p, seed, shared=axes, device=x.device)
+    out = torch.where(keep, x.float() * (1.0 / (1.0 - p) if p < 1 else 0.0), 0.0)
+    return out.to(dtype) if residual is None else (residual.float() + out).to(residual.dtype)
+
+
+class _DropoutAdd(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, residual: Tensor, update: Tensor, p: float, seed: int, shared: int) -> Tensor:
+        ctx.drawn, ctx.dtype = (p, seed, shared), update.dtype
+        return _dropped(update, residual, p, seed, shared, residual.dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g: Tensor):
+        p, seed, shared = ctx.drawn
+        update = _dropped(g, None, p, seed, shared, ctx.dtype) if ctx.needs_input_grad[1] else None
+        return g if ctx.needs_input_grad[0] else None, update, None, None, None
+
+
+def dropout_add(residual: Tensor, update: Tensor, p: float, shared: int) -> Tensor:
+    """``residual`` plus ``update`` dropped with rate ``p``, one mask for all positions of axis ``shared``; in
+    ``residual``'s dtype, with a gradient. The mask's seed comes from torch's default CPU generator."""
+    if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("dropout draws its seed on the host: a captured graph would repeat one mask "
+                           "(kernels.dropout_train reads a seed on the device)")
+    seed = int(torch.empty((), dtype=torch.int64).random_())
+    return _DropoutAdd.apply(residual, update, p, seed, shared)
