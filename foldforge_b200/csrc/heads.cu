@@ -351,6 +351,13 @@ struct Lane {
         mine((lane & ((1 << plan.crew) - 1)) >> plan.shift), to_teams(plan.crew - plan.shift),
         crew(static_cast<uint32_t>(lane) >> plan.crew), crews(32u >> plan.crew) {}
   __device__ __forceinline__ int teams_heads(int count) const { return (count - mine + teams - 1) >> to_teams; }  // of `count` heads
+  // steps of U (a power of two) heads a team
+  template <int U>
+  __device__ __forceinline__ int steps(int count) const {
+    constexpr int kShift = U == 1 ? 0 : U == 2 ? 1 : 2;
+    static_assert(U == 1 << kShift);
+    return (count + (U << to_teams) - 1) >> (to_teams + kShift);
+  }
 };
 
 // ---- a lane's ring of S slots for NT tensors
@@ -452,7 +459,7 @@ struct Stream {
         step[k] = my.teams * v.head;
       }
       left = place.there ? my.teams_heads(count) : 0;
-      steps = (count + U * my.teams - 1) / (U * my.teams);
+      steps = my.template steps<U>(count);
       return;
     }
   }
@@ -581,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, kResident<T, P, NV>)
         }
       }
 #pragma unroll 1
-      for (int step = (count + U * my.teams - 1) / (U * my.teams); step > 0; --step) {
+      for (int step = my.steps<U>(count); step > 0; --step) {
         RawPairs<T, P> raw[U][NV][1];
         Pairs<P> v[U][NV];
         stream.take(raw);
@@ -675,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, kResident<T, P, NV>)
 #pragma unroll
       for (int i = 0; i < NV; ++i) w[i] = weight_of<P, INTER>(constants.weight(p, which), spot[i]);
 #pragma unroll 1
-      for (int step = (count + U * my.teams - 1) / (U * my.teams); step > 0; --step) {
+      for (int step = my.steps<U>(count); step > 0; --step) {
         RawPairs<T, P> raw[U][NV][2];
         Pairs<P> v[U][NV], g[U][NV];
         stream.take(raw);
