@@ -4,6 +4,7 @@
 //
 // The entry points come in as addresses (bind()), so this module does not link the kernels' library.
 // Refusals and errors raise the exceptions of foldforge_b200._lib.
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -105,9 +106,14 @@ Tensor vector(const char* name, const char* what, const Tensor& x, const Tensor&
   return aligned(t.scalar_type() == at::kFloat ? dense(t) : t.to(at::kFloat).contiguous());
 }
 
-Tensor bytes(const Tensor& x, int64_t n) { return at::empty({n}, x.options().dtype(at::kByte).requires_grad(false)); }
-Tensor floats(const Tensor& x, c10::IntArrayRef shape) { return at::empty(shape, x.options().dtype(at::kFloat).requires_grad(false)); }
-Tensor like(const Tensor& x, c10::IntArrayRef shape) { return at::empty(shape, x.options().requires_grad(false)); }
+// New tensors on x's CUDA device, from the allocator without the dispatcher (a call of a token's q and k makes two, its
+// backward pass five)
+Tensor made(const Tensor& x, c10::IntArrayRef shape, at::ScalarType dtype) {
+  return Tensor(at::detail::empty_cuda(shape, dtype, x.device(), std::nullopt));
+}
+Tensor bytes(const Tensor& x, int64_t n) { return made(x, {n}, at::kByte); }
+Tensor floats(const Tensor& x, c10::IntArrayRef shape) { return made(x, shape, at::kFloat); }
+Tensor like(const Tensor& x, c10::IntArrayRef shape) { return made(x, shape, x.scalar_type()); }
 
 // ---- checkpoints: codes, then (from the next multiple of 16 bytes on) scales
 int64_t scales_at(int64_t codes) { return (codes + 15) / 16 * 16; }
@@ -165,7 +171,7 @@ Tensor checkpoint_unpack(const Tensor& data_in, const std::vector<int64_t>& shap
   const Kept k = kept_of(name, data_in, data_in, true, shape, dtype);
   need_cuda(name, data_in);
   Call call(data_in);
-  const Tensor x = at::empty(shape, data_in.options().dtype(dtype));
+  const Tensor x = made(data_in, shape, dtype);
   const int64_t c = shape.back();
   check(name, entries.checkpoint_unpack(k.codes, k.scales, x.data_ptr(), x.numel() / c, static_cast<int>(c), dtype_of(dtype), call.stream));
   return x;
@@ -468,7 +474,7 @@ Tensor dropout(const char* name, const Tensor& x_in, double p, uint64_t seed, ui
   need_cuda(name, x_in);
   Call call(x_in);
   const Tensor x = dense(x_in);
-  const Tensor out = at::empty(x.sizes(), x.options().dtype(out_dtype).requires_grad(false));
+  const Tensor out = made(x, x.sizes(), out_dtype);
   check(name, entries.dropout(x.data_ptr(), dtype_of(x.scalar_type()), residual ? residual->data_ptr() : nullptr, out.data_ptr(),
                               dtype_of(out_dtype), outer, shared, inner, p, seed, offset,
                               device_seed ? reinterpret_cast<const uint64_t*>(device_seed->data_ptr<int64_t>()) : nullptr, call.stream));

@@ -76,7 +76,7 @@ def build_binding() -> Path:
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_API_INCLUDE_EXTENSION_H",
            *[f"-I{p}" for p in includes], str(src), "-o", str(BINDING), f"-L{libs}", f"-Wl,-rpath,{libs}", "-lc10", "-lc10_cuda",
-           "-ltorch_cpu", "-ltorch_python", "-ltorch"]
+           "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-ltorch"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)

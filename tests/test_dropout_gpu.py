@@ -194,6 +194,23 @@ def test_elements_past_32_bits(shared, inner):
     assert torch.equal(out, dx)
 
 
+def test_narrow_shared_rows_and_views_past_32_bits():
+    """2^31 and more elements where masks lie closer than rows of 32, and a tensor that starts off 16 bytes."""
+    shape = (180_000_000, 3, 4)
+    x = torch.ones(shape, device="cuda", dtype=BF16)
+    out = kernels.dropout_train(x, 0.5, 8, shared=1)[0]
+    index = torch.arange((shape[0] - 1000) * 4, shape[0] * 4, device="cuda")
+    keep = (ref.words(index, 8, 0) >= 2**31).view(1000, 1, 4).expand(1000, 3, 4)
+    assert torch.equal(out[-1000:] != 0, keep)
+    del out
+    flat = x.view(-1)[1:]
+    out = kernels.dropout_train(flat, 0.5, 9)[0]
+    index = torch.arange(flat.numel() - 5000, flat.numel(), device="cuda")
+    assert torch.equal(out[-5000:] != 0, ref.words(index, 9, 0) >= 2**31)
+    del x, flat, out
+    torch.cuda.empty_cache()
+
+
 def test_counters_past_32_bits():
     """More than 2^34 elements, whose groups of four take the counter's second word."""
     n = 2**34 + 1000

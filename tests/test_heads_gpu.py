@@ -305,6 +305,18 @@ def test_offsets_past_32_bits():
         assert torch.equal(far, want)
 
 
+@pytest.mark.parametrize("t,hq,hk,d,pairs,axes", [(70001, 1, 1, 16, 8, 1), (70001, 2, 1, 24, 12, 1), (40009, 4, 4, 32, 16, 3),
+                                                  (40009, 4, 4, 32, 15, 5), (40009, 3, 1, 7, 3, 9), (1, 3, 3, 16, 8, 2), (33, 0, 2, 32, 16, 1)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_tokens_that_share_a_warp(t, hq, hk, d, pairs, axes, dtype):
+    """Few small heads: several tokens a warp, a number of them that leaves lanes without one."""
+    g = gen(t + d)
+    turn = Turn(g, 1, t, pairs, axes)
+    q, k = values(g, 1, t, hq, d, dtype=dtype), values(g, 1, t, hk, d, dtype=dtype)
+    dq, dk = values(g, 1, t, hq, d, dtype=dtype, size=1e-2), values(g, 1, t, hk, d, dtype=dtype, size=1e-2)
+    run_norm(q, k, dq, dk, turn, weights(g, d), weights(g, d))
+
+
 def test_more_tokens_than_a_grid_takes_at_once():
     g = gen(6)
     turn = Turn(g, 1, 120000, 8)
