@@ -699,8 +699,8 @@ def dropout_train(x: Tensor, p: float, seed: int | Tensor, *, offset: int = 0, r
     backward pass reads (no mask). The choice follows from ``seed``, ``offset`` and the element's place alone:
     calls of one step take another ``offset`` each. ``shared``: an axis (or axes beside one another) of ``x``
     whose positions share a mask. ``seed`` as an int64 tensor ``[seed, offset]`` on the device is read by the kernel
-    (its offset adds to ``offset``), so that a captured step draws other masks once the tensor changes; it may
-    not change between a forward pass and its backward pass."""
+    (its offset adds to ``offset``), so that a captured step draws other masks once the tensor changes (a number
+    stays what it was when the graph was captured); it may not change between a forward pass and its backward pass."""
     if shared is None:
         axes: tuple[int, ...] = ()
     else:

@@ -42,7 +42,7 @@ def heads(x: Tensor, angle: Tensor, interleaved: bool, weight: Tensor | None = N
     ``(outputs, bounds)``: y, and dx, dweight."""
     v, n, c = x.double(), angle.shape[-1], x.shape[-1]
     w = torch.ones(c, dtype=torch.float64, device=x.device) if weight is None else weight.double()
-    # cosine and sine: the angle's fp32 rounding (at most pi / 4 of a step), one step of the functions, and
+    # cosine and sine: the angle's fp32 rounding (at most pi / 4 of a step), the functions (less than 2 steps), and
     # angles found in 64 bits: at most 4 steps of 1; products and the sum: 3 more
     turn = 8 * STEP
     if eps is None:
