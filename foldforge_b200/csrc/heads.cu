@@ -14,18 +14,21 @@
 // number of them (exact), then sine and cosine in 32 bits of at most an eighth of a turn: a position of 2^20
 // keeps the digits that a 32-bit product would lose.
 //
-// Measured on one B200 (device time, inputs past L2; a plain copy moves 6.55 TB/s):
-//   65536 tokens, 32 + 8 heads x 128 bf16          forward 214 us (6.3 TB/s), backward 371 to 380 (5.4)
+// Measured on one B200 (device time, inputs past L2; a plain copy moves 6.55 TB/s; boxes differ by 5%):
+//   65536 tokens, 32 + 8 heads x 128 bf16          forward 214 us (6.3 TB/s), backward 339 (5.9)
 //   2 x 24960 tokens, 24 + 24 heads x 128 bf16     rotation alone 207 us (5.9 TB/s)
-//   500000 tokens, 4 + 4 heads x 32 bf16           forward 152 us (3.4 TB/s), backward 219 (3.5)
+//   65536 tokens, 16 + 16 heads x 48 bf16          forward 85 us (4.8 TB/s), backward 143 (4.2)
+//   500000 tokens, 4 + 4 heads x 32 bf16           forward 131 us (3.9 TB/s), backward 192 (4.0)
 //   65536 tokens, 8 + 8 heads x 37 bf16            forward 150 us (1.0 TB/s), backward 231 (1.0)
-// In the first case 16 warps an SM issue in 60% of the slots: 13 instructions for 32 channels forward and 23 backward.
-// A token costs about as much as four steps of its heads (angles, addresses, the weight's values), which is what
-// bounds few heads a token; single channels, for heads that are not whole runs, cost five times a run's instructions.
+// In the first case 16 warps an SM issue in 60% of the slots: 13 instructions for 32 channels forward and 22 backward.
+// A token costs a crew about as much as two to four steps of its heads (angles, addresses, the weight's values), so
+// crews of a warp share it where the issue is the limit (plan_of); single channels, for heads that are not whole
+// runs, cost five times a run's instructions.
 // Before the ring, with heads loaded straight to registers: forward 247 us, backward 670 (or 461 with half the
-// channels a lane). Without effect or slower: three blocks an SM, more slots, a table of negative sines, q and k in
-// blocks of their own (a token's angles are then found twice: forward 264 us), single channels in rows of several
-// tokens a warp (65536 x 16 heads x 37 117 us for 150, but 151 channels 350 for 330 and 301 in fp32 390 for 240).
+// channels a lane). Without effect or slower: three blocks an SM, more slots, a table of negative sines, two heads of a
+// team at a time, q and k in blocks of their own (a token's angles are then found twice: forward 264 us), single
+// channels in rows of several tokens a warp (65536 x 16 heads x 37 117 us for 150, but 151 channels 350 for 330 and 301
+// in fp32 390 for 240).
 #include <string.h>
 
 #include <type_traits>
@@ -542,9 +545,9 @@ struct Stream {
 template <int P, int NV>
 constexpr int kAtOnce = P > 1 || NV > 2 ? 1 : 4 / NV;
 
-// Slots of the rings, and blocks that an SM holds. 65536 tokens of 40 heads x 128 in bf16: forward 214 us with two
-// blocks (111 registers a thread) and 3, 4 or 6 slots, 260 with three (80 registers, 150 bytes of them spilled);
-// backward 371 us with 3 slots, 384 with 6, 398 with one block, 624 with three.
+// Slots of the rings, and blocks that an SM holds. 65536 tokens of 40 heads x 128 in bf16, a warp a token: forward 214 us
+// with two blocks (111 registers a thread) and 3, 4 or 6 slots, 260 with three (80 registers, 150 bytes of them
+// spilled); backward 371 us with 3 slots, 384 with 6, 398 with one block, 624 with three.
 constexpr int kForwardSlots = 3, kBackwardSlots = 3;
 template <typename T, int P, int NV>
 constexpr int kResident = P * static_cast<int>(sizeof(T)) > 16 || NV > 3 ? 1 : 2;
@@ -838,36 +841,45 @@ int dispatch_heads(const HeadsParams& p, bool backward, F&& f) {
   return f(one, apart, std::integral_constant<int, 8>{}, apart, 32);
 }
 
-// How a token's heads are cut into items: an item costs its token's angles, about as long as a step takes, and its
-// steps, and the GPU's warps take the items in rounds. All heads in one item where there are many tokens, single
-// steps where there are few. (Single steps everywhere: 65536 tokens of 40 heads x 128 599 us for 229.)
-Plan plan_of(const HeadsParams& p, int lanes, int run, int nv, int at_once, int resident) {
-  const int heads = p.heads[0] + p.heads[1], larger = p.heads[0] > p.heads[1] ? p.heads[0] : p.heads[1];
-  Plan plan{0, Divisor(1), Divisor(static_cast<uint32_t>(p.tokens)), heads, 0, 0, 0};
-  while ((1 << plan.shift) < lanes) ++plan.shift;
-  plan.slots = (((run * nv) << plan.shift) + 3) / 4 * 4;
-  plan.crew = plan.shift;
-  while (plan.crew < 5 && (at_once << (plan.crew - plan.shift) < larger || (p.rotary.pairs > 0 && 1 << plan.crew < p.rotary.axes))) ++plan.crew;
-  const int64_t tokens = static_cast<int64_t>(p.batch) * p.tokens, crews = 148 * kWarps * static_cast<int64_t>(resident) * (32 >> plan.crew);
-  const int step = at_once << (plan.crew - plan.shift), steps = (heads + step - 1) / step;
-  int64_t best = 0;
-  for (int of = steps; of >= 1; of = (of + 1) / 2) {  // steps an item
-    const int64_t chunks = (steps + of - 1) / of, rounds = (tokens * chunks + crews - 1) / crews, cost = rounds * (1 + of);
-    if (best == 0 || cost < best) {
-      best = cost;
-      plan.per = of * step;
-      plan.chunks = Divisor(static_cast<uint32_t>(chunks));
-      plan.items = static_cast<uint32_t>(tokens * chunks);
+// How tokens' heads are cut into items. An item's issue time, in fortieths of a step of runs of 8: fixed work
+// (addresses, the weight's values) of about two steps, a quarter of one for each round of the crew's lanes over the
+// pairs' angles, and its steps; its memory time, the bytes of its heads, where the issue of a full step of 1 KB an
+// input takes 40 and its memory 57 (44 of a backward step, which issues more for its three KB; fp32 a quarter more). The GPU's crews take
+// the items in rounds. Smaller crews share the fixed work among more tokens of a warp and take more steps, which
+// helps where the issue is the limit (65536 tokens of 32 heads x 24: 68 -> 35 us forward, 84 -> 52 backward; of 32 x
+// 48 104 -> 88 and 174 -> 141) and not where the memory is (40 x 128: 214 -> 218 forward). Where there are few
+// tokens, a whole warp takes a token, or a part of its heads.
+Plan plan_of(const HeadsParams& p, int lanes, int run, int nv, int at_once, int resident, int size, bool backward) {
+  const int heads = p.heads[0] + p.heads[1];
+  Plan best{0, Divisor(1), Divisor(static_cast<uint32_t>(p.tokens)), heads, 0, 0, 0};
+  while ((1 << best.shift) < lanes) ++best.shift;
+  best.slots = (((run * nv) << best.shift) + 3) / 4 * 4;
+  const int64_t tokens = static_cast<int64_t>(p.batch) * p.tokens, warps = 148 * kWarps * static_cast<int64_t>(resident);
+  int64_t least = 0;
+  const auto consider = [&](int crew, int per, int64_t chunks, int64_t steps) {
+    const int64_t items = tokens * chunks, crews = warps * (32 >> crew), full = 16 * items / crews;
+    const int64_t rounds = full < 16 ? 16 : full + 8;  // sixteenths; the last one is half a round in the mean
+    const int64_t issue = 80 + 10 * ((best.slots + (1 << crew) - 1) >> crew) + (run == 4 ? 25 : 40) * steps;
+    const int64_t memory = (backward ? 44 : 57) * static_cast<int64_t>(per) * p.channels * (size == 4 ? 5 : 2) / 1024 * (32 >> crew);
+    const int64_t cost = rounds * (issue > memory ? issue : memory);
+    if (least != 0 && cost >= least) return;
+    least = cost;
+    best.crew = crew;
+    best.per = per;
+    best.chunks = Divisor(static_cast<uint32_t>(chunks));
+    best.items = static_cast<uint32_t>(items);
+  };
+  for (int crew = 5; crew >= best.shift; --crew) {
+    if (p.rotary.pairs > 0 && 1 << crew < p.rotary.axes) break;
+    const int step = at_once << (crew - best.shift);
+    consider(crew, heads, 1, (p.heads[0] + step - 1) / step + (p.heads[1] + step - 1) / step);
+    if (crew < 5) continue;  // crews of one warp take the same steps
+    for (int of = (heads + step - 1) / step / 2; of >= 1 && tokens < warps; of /= 2) {  // steps an item
+      consider(crew, of * step, (heads + of * step - 1) / (of * step), of);
+      if (of == 1) break;
     }
-    // crews of one warp take the same steps
-    if (of == 1 || plan.crew < 5 || tokens * chunks >= int64_t(1) << 29) break;
   }
-  if (plan.crew < 5) {
-    plan.per = heads;
-    plan.chunks = Divisor(1);
-    plan.items = static_cast<uint32_t>(tokens);
-  }
-  return plan;
+  return best;
 }
 size_t table_bytes(const Plan& plan, int channels) {
   return sizeof(float) * kWarps * (32 >> plan.crew) * 2 * plan.slots + Constants::bytes(plan.slots, channels);
@@ -885,7 +897,7 @@ int heads(const HeadsParams& p, cudaStream_t stream) {
   return dispatch_heads<T>(p, false, [&](auto run, auto inter, auto nv, auto all, int lanes) {
     constexpr int P = decltype(run)::value, NV = decltype(nv)::value;
     constexpr bool INTER = decltype(inter)::value, ALL = decltype(all)::value;
-    const Plan plan = plan_of(p, lanes, P, NV, kAtOnce<P, NV>, kResident<T, P, NV>);
+    const Plan plan = plan_of(p, lanes, P, NV, kAtOnce<P, NV>, kResident<T, P, NV>, sizeof(T), false);
     const size_t smem = Stream<T, P, NV, 1, kAtOnce<P, NV>, kForwardSlots>::kBytes + table_bytes(plan, p.channels);
     auto kernel = p.norm ? heads_kernel<T, P, INTER, NV, ALL, true> : heads_kernel<T, P, INTER, NV, ALL, false>;
     if (smem > 48 * 1024) {
@@ -903,7 +915,7 @@ int heads_bwd(const HeadsParams& p, float* part, cudaStream_t stream) {
   return dispatch_heads<T>(p, true, [&](auto run, auto inter, auto nv, auto all, int lanes) {
     constexpr int P = decltype(run)::value, NV = decltype(nv)::value;
     constexpr bool INTER = decltype(inter)::value, ALL = decltype(all)::value;
-    const Plan plan = plan_of(p, lanes, P, NV, kAtOnce<P, NV>, kResident<T, P, NV>);
+    const Plan plan = plan_of(p, lanes, P, NV, kAtOnce<P, NV>, kResident<T, P, NV>, sizeof(T), true);
     size_t smem = Stream<T, P, NV, 2, kAtOnce<P, NV>, kBackwardSlots>::kBytes + table_bytes(plan, p.channels);
     if (smem < sizeof(float) * kWarps * p.channels) smem = sizeof(float) * kWarps * p.channels;
     auto kernel = heads_bwd_kernel<T, P, INTER, NV, ALL>;
