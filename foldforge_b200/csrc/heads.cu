@@ -10,104 +10,37 @@
 // asynchronously a few steps (and tokens) ahead, and needs no barrier to read them. What is in flight then does
 // not depend on registers.
 //
-// Angles: a position times the pair's frequency in quarter turns in 64 bits, less the nearest whole
-// number of them (exact), then sine and cosine in 32 bits of at most an eighth of a turn: a position of 2^20
-// keeps the digits that a 32-bit product would lose.
+// Heads that are not whole runs of 8 or 16 bytes a lane take heads_any.cu.
 //
 // Measured on one B200 (device time, inputs past L2; a plain copy moves 6.55 TB/s; boxes differ by 5%):
 //   65536 tokens, 32 + 8 heads x 128 bf16          forward 214 us (6.3 TB/s), backward 339 (5.9)
 //   2 x 24960 tokens, 24 + 24 heads x 128 bf16     rotation alone 207 us (5.9 TB/s)
 //   65536 tokens, 16 + 16 heads x 48 bf16          forward 85 us (4.8 TB/s), backward 143 (4.2)
 //   500000 tokens, 4 + 4 heads x 32 bf16           forward 131 us (3.9 TB/s), backward 192 (4.0)
-//   65536 tokens, 8 + 8 heads x 37 bf16            forward 150 us (1.0 TB/s), backward 231 (1.0)
 // In the first case 16 warps an SM issue in 60% of the slots: 13 instructions for 32 channels forward and 22 backward.
 // A token costs a crew about as much as two to four steps of its heads (angles, addresses, the weight's values), so
-// crews of a warp share it where the issue is the limit (plan_of); single channels, for heads that are not whole
-// runs, cost five times a run's instructions.
+// crews of a warp share it where the issue is the limit (plan_of).
 // Before the ring, with heads loaded straight to registers: forward 247 us, backward 670 (or 461 with half the
 // channels a lane). Without effect or slower: three blocks an SM, more slots, a table of negative sines, two heads of a
-// team at a time, q and k in blocks of their own (a token's angles are then found twice: forward 264 us), single
-// channels in rows of several tokens a warp (65536 x 16 heads x 37 117 us for 150, but 151 channels 350 for 330 and 301
-// in fp32 390 for 240).
+// team at a time, q and k in blocks of their own (a token's angles are then found twice: forward 264 us).
 #include <string.h>
 
 #include <type_traits>
 
-#include "abi_util.h"
-#include "common.cuh"
-#include "kernels.h"
+#include "heads.cuh"
 #include "launch.cuh"
 #include "mx8.cuh"
 
 namespace ffb {
+namespace heads {
 namespace {
-
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
-
-// Cosine and sine of an angle of at most an eighth of a turn, r quarter turns (|r| <= 1/2): polynomials in r^2
-// through Chebyshev's nodes, off by less than 0.2 steps of 2^-24 before the roundings of their own evaluation.
-__device__ __forceinline__ float2 eighth_turn(float r) {
-  const float t = r * r;
-  const float s = r * fmaf(fmaf(fmaf(-0.0046021491289f, t, 0.0796802192926f), t, -0.6459634900093f), t, 1.5707963705063f);
-  const float c = fmaf(fmaf(fmaf(fmaf(0.0009036280680f, t, -0.0208600703627f), t, 0.2536692023277f), t, -1.2337005138397f), t, 1.0f);
-  return make_float2(c, s);
-}
-
-// cosine and sine of the angle of `quarters` quarter turns
-__device__ __forceinline__ float2 turn_of(double quarters, uint32_t inverse_sign) {
-  // the nearest whole number: 1.5 2^52 has a last place of 1, so the sum rounds to it, and its lowest bits are the
-  // number's. (Past 2^51 neighbouring doubles are half a quarter turn and more apart.)
-  double whole = quarters + 6755399441055744.0;
-  int k = __double2loint(whole);
-  whole -= 6755399441055744.0;
-  if (!(fabs(quarters) < 2251799813685248.0)) {
-    whole = rint(quarters);
-    k = static_cast<int>(whole - 4.0 * rint(0.25 * whole));
-  }
-  const float2 t = eighth_turn(static_cast<float>(quarters - whole));
-  // k quarter turns more
-  const float cos = k & 1 ? t.y : t.x, sin = k & 1 ? t.x : t.y;
-  return make_float2(__uint_as_float(__float_as_uint(cos) ^ (((k + 1) & 2) << 30)),
-                     __uint_as_float(__float_as_uint(sin) ^ ((k & 2) << 30) ^ inverse_sign));
-}
 
 // A token's position on axis `axis` (0 past the last axis).
 __device__ __forceinline__ double place_of(const RotaryParams& r, uint32_t b, uint32_t t, int axis) {
   if (r.pairs == 0 || axis >= r.axes) return 0.0;
   const int64_t i = b * r.batch + t * r.token + axis * r.axis;
-  if (r.type == kPositionI64) return static_cast<double>(static_cast<const int64_t*>(r.positions)[i]);
-  if (r.type == kPositionI32) return static_cast<double>(static_cast<const int32_t*>(r.positions)[i]);
-  return static_cast<double>(static_cast<const float*>(r.positions)[i]);
+  return position_at(r, i);
 }
-
-// What a block reads again for every token, from its start on in shared memory, so that the first token waits for
-// one load's time and not for several one after the other: the pairs' frequencies and axes, q's and k's weights.
-struct Constants {
-  double* quarters;  // [slots]; NaN where a pair's axis is not there
-  int* axes;
-  float* weights;  // [2][channels, to a multiple of 4]
-  __host__ __device__ static int padded(int channels) { return (channels + 3) / 4 * 4; }
-  __host__ __device__ static int bytes(int slots, int channels) { return slots * 12 + padded(channels) * 8; }
-  __device__ __forceinline__ Constants(const HeadsParams& p, int slots, uint8_t* smem) {
-    quarters = reinterpret_cast<double*>(smem);
-    weights = reinterpret_cast<float*>(quarters + slots);
-    axes = reinterpret_cast<int*>(weights + 2 * padded(p.channels));
-    const RotaryParams& r = p.rotary;
-    for (int j = threadIdx.x; j < r.pairs; j += kThreads) {
-      const int axis = r.pair_axes[j];
-      const double q = r.quarters[j];
-      const bool there = axis >= 0 && axis < r.axes;
-      quarters[j] = there ? q : __longlong_as_double(0x7FF8000000000000LL);
-      axes[j] = there ? axis : 0;
-    }
-    for (int c = threadIdx.x; c < 2 * padded(p.channels); c += kThreads) {
-      const int which = c >= padded(p.channels), i = c - which * padded(p.channels);
-      weights[c] = p.weight[which] != nullptr && i < p.channels ? p.weight[which][i] : 1.f;
-    }
-  }
-  __device__ __forceinline__ const float* weight(const HeadsParams& p, int which) const { return weights + which * padded(p.channels); }
-};
 
 // A token's cosines and sines of `slots` pairs (those past the table's: no turn) to a crew's shared memory, from
 // its places on the crew's lanes.
@@ -130,19 +63,7 @@ __device__ __forceinline__ void find_turns(const RotaryParams& r, const Constant
 template <typename T, int P>
 struct Run {
   uint32_t w[P * sizeof(T) / 4];
-  __device__ __forceinline__ void load(const T* p) {
-    if constexpr (sizeof(w) == 8) {
-      const uint2 v = __ldcs(reinterpret_cast<const uint2*>(p));
-      memcpy(w, &v, 8);
-    } else {
-#pragma unroll
-      for (int i = 0; i < static_cast<int>(sizeof(w)) / 16; ++i) {
-        const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p) + i);
-        memcpy(w + 4 * i, &v, 16);
-      }
-    }
-  }
-  __device__ __forceinline__ void load_plain(const T* p) {  // whole 16 bytes
+  __device__ __forceinline__ void load(const T* p) {  // whole 16 bytes
 #pragma unroll
     for (int i = 0; i < static_cast<int>(sizeof(w)) / 16; ++i) {
       const uint4 v = reinterpret_cast<const uint4*>(p)[i];
@@ -158,10 +79,6 @@ struct Run {
         reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
     }
   }
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(w)) / 4; ++i) w[i] = 0;
-  }
   __device__ __forceinline__ float get(int i) const {
     if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
     return i & 1 ? bf16_hi(w[i / 2]) : bf16_lo(w[i / 2]);
@@ -175,16 +92,6 @@ struct Run {
     }
   }
 };
-template <typename T>
-struct Run<T, 1> {
-  T v;
-  __device__ __forceinline__ void load(const T* p) { v = *p; }
-  __device__ __forceinline__ void load_plain(const T* p) { v = *p; }
-  __device__ __forceinline__ void store(T* p) const { *p = v; }
-  __device__ __forceinline__ void zero() { v = static_cast<T>(0.f); }
-  __device__ __forceinline__ float get(int) const { return static_cast<float>(v); }
-};
-
 // A lane's P pairs of a head: their first channels `a` and second channels `b`.
 template <int P>
 struct Pairs {
@@ -193,14 +100,14 @@ struct Pairs {
 
 // Where a lane's P pairs lie: runs of P channels at `a` and `b`, which are the pairs' first and second channels,
 // or with INTER two runs of P / 2 neighbouring pairs (a team's runs at `a` lie side by side, and so do those at `b`,
-// so that its accesses take whole sectors). P = 1: single channels anywhere. The pairs' angles lie at `table_a`
-// and with INTER the second run's at `table_b`.
+// so that its accesses take whole sectors). The pairs' angles lie at `table_a` and with INTER the second run's at
+// `table_b`.
 template <int P>
 struct Spot {
   int a, b;                // element offsets in a head
   int table_a, table_b;
   int turned_a, turned_b;  // how many of the pairs (with INTER of each run's) are turned: the first ones
-  bool has_a, has_b;
+  bool there;              // whether the lane has a run
 };
 __device__ __forceinline__ int clamped(int v, int most) { return v < 0 ? 0 : v < most ? v : most; }
 template <int P, bool INTER>
@@ -213,15 +120,13 @@ __device__ __forceinline__ Spot<P> spot_of(const RotaryParams& r, int chunk, int
     s.b = channels / 2 + s.a;
     s.turned_a = clamped(r.pairs - s.table_a, P / 2);
     s.turned_b = clamped(r.pairs - s.table_b, P / 2);
-    s.has_a = s.has_b = s.a < channels / 2;
+    s.there = s.a < channels / 2;
   } else {
     s.table_a = s.table_b = chunk * P;
     s.turned_a = s.turned_b = clamped(r.pairs - s.table_a, P);
-    const bool halves = s.turned_a > 0 && !(P == 1 && r.interleaved);
-    s.a = halves ? s.table_a : 2 * s.table_a;
-    s.b = halves ? r.pairs + s.table_a : s.a + P;
-    s.has_a = s.a + P <= channels;
-    s.has_b = s.b + P <= channels;
+    s.a = s.turned_a > 0 ? s.table_a : 2 * s.table_a;
+    s.b = s.turned_a > 0 ? r.pairs + s.table_a : s.a + P;
+    s.there = chunk * 2 * P < channels;
   }
   return s;
 }
@@ -229,38 +134,25 @@ __device__ __forceinline__ Spot<P> spot_of(const RotaryParams& r, int chunk, int
 template <typename T, int P>
 struct RawPairs {
   Run<T, P> a, b;
-  __device__ __forceinline__ void zero() {
-    a.zero();
-    b.zero();
-  }
-  // channels that are not there keep the zeros they were given
-  __device__ __forceinline__ void load(const T* head, const Spot<P>& s) {
-    if (s.has_a) a.load(head + s.a);
-    if (s.has_b) b.load(head + s.b);
-  }
   __device__ __forceinline__ void store(T* head, const Spot<P>& s) const {
-    if (s.has_a) a.store(head + s.a);
-    if (s.has_b) b.store(head + s.b);
+    if (!s.there) return;
+    a.store(head + s.a);
+    b.store(head + s.b);
   }
 };
 template <typename T, int P, bool INTER>
 __device__ __forceinline__ Pairs<P> widen(const RawPairs<T, P>& raw) {
   Pairs<P> v;
-  if constexpr (P == 1) {
-    v.a.f = raw.a.get(0);
-    v.b.f = raw.b.get(0);
-  } else {
 #pragma unroll
-    for (int i = 0; i < P; i += 2) {
-      if constexpr (INTER) {
-        const Run<T, P>& run = i < P / 2 ? raw.a : raw.b;
-        const int e = 2 * i - (i < P / 2 ? 0 : P);
-        v.a.p[i / 2] = f32x2(run.get(e), run.get(e + 2));
-        v.b.p[i / 2] = f32x2(run.get(e + 1), run.get(e + 3));
-      } else {
-        v.a.p[i / 2] = f32x2(raw.a.get(i), raw.a.get(i + 1));
-        v.b.p[i / 2] = f32x2(raw.b.get(i), raw.b.get(i + 1));
-      }
+  for (int i = 0; i < P; i += 2) {
+    if constexpr (INTER) {
+      const Run<T, P>& run = i < P / 2 ? raw.a : raw.b;
+      const int e = 2 * i - (i < P / 2 ? 0 : P);
+      v.a.p[i / 2] = f32x2(run.get(e), run.get(e + 2));
+      v.b.p[i / 2] = f32x2(run.get(e + 1), run.get(e + 3));
+    } else {
+      v.a.p[i / 2] = f32x2(raw.a.get(i), raw.a.get(i + 1));
+      v.b.p[i / 2] = f32x2(raw.b.get(i), raw.b.get(i + 1));
     }
   }
   return v;
@@ -268,33 +160,28 @@ __device__ __forceinline__ Pairs<P> widen(const RawPairs<T, P>& raw) {
 template <typename T, int P, bool INTER>
 __device__ __forceinline__ RawPairs<T, P> narrow(const Pairs<P>& v) {
   RawPairs<T, P> raw;
-  if constexpr (P == 1) {
-    raw.a.v = static_cast<T>(v.a.f);
-    raw.b.v = static_cast<T>(v.b.f);
-  } else {
 #pragma unroll
-    for (int i = 0; i < P; i += 2) {
-      if constexpr (INTER) {
-        Run<T, P>& run = i < P / 2 ? raw.a : raw.b;
-        const int e = 2 * i - (i < P / 2 ? 0 : P);
-        run.set_two(e, v.a.get(i), v.b.get(i));
-        run.set_two(e + 2, v.a.get(i + 1), v.b.get(i + 1));
-      } else {
-        raw.a.set_two(i, v.a.get(i), v.a.get(i + 1));
-        raw.b.set_two(i, v.b.get(i), v.b.get(i + 1));
-      }
+  for (int i = 0; i < P; i += 2) {
+    if constexpr (INTER) {
+      Run<T, P>& run = i < P / 2 ? raw.a : raw.b;
+      const int e = 2 * i - (i < P / 2 ? 0 : P);
+      run.set_two(e, v.a.get(i), v.b.get(i));
+      run.set_two(e + 2, v.a.get(i + 1), v.b.get(i + 1));
+    } else {
+      raw.a.set_two(i, v.a.get(i), v.a.get(i + 1));
+      raw.b.set_two(i, v.b.get(i), v.b.get(i + 1));
     }
   }
   return raw;
 }
 
-// a weight's values (in shared memory) at a lane's pairs, 0 where there is no channel
+// a weight's values (in shared memory) at a lane's pairs
 template <int P, bool INTER>
 __device__ __forceinline__ Pairs<P> weight_of(const float* weight, const Spot<P>& s) {
+  if (!s.there) return {Lanes<P>(0.f), Lanes<P>(0.f)};
   RawPairs<float, P> raw;
-  raw.zero();
-  if (s.has_a) raw.a.load_plain(weight + s.a);
-  if (s.has_b) raw.b.load_plain(weight + s.b);
+  raw.a.load(weight + s.a);
+  raw.b.load(weight + s.b);
   return widen<float, P, INTER>(raw);
 }
 
@@ -302,9 +189,7 @@ __device__ __forceinline__ Pairs<P> weight_of(const float* weight, const Spot<P>
 template <int P, bool INTER>
 __device__ __forceinline__ Lanes<P> from_table(const float* table, const Spot<P>& s) {
   Lanes<P> v;
-  if constexpr (P == 1) {
-    v.f = table[s.table_a];
-  } else if constexpr (P == 4 && INTER) {
+  if constexpr (P == 4 && INTER) {
     const float2 x = *reinterpret_cast<const float2*>(table + s.table_a), y = *reinterpret_cast<const float2*>(table + s.table_b);
     v.p[0] = f32x2(x.x, x.y);
     v.p[1] = f32x2(y.x, y.y);
@@ -327,15 +212,11 @@ __device__ __forceinline__ Lanes<P> negative(const Lanes<P>& v) {
 template <int P, bool INTER>
 __device__ __forceinline__ void keep_unturned(Pairs<P>& y, const Pairs<P>& x, const Spot<P>& s) {
   if (s.turned_a + (INTER ? s.turned_b : 0) == P) return;
-  if constexpr (P == 1) {
-    y = x;
-  } else {
-    const auto turned = [&](int i) { return INTER && i >= P / 2 ? i - P / 2 < s.turned_b : i < s.turned_a; };
+  const auto turned = [&](int i) { return INTER && i >= P / 2 ? i - P / 2 < s.turned_b : i < s.turned_a; };
 #pragma unroll
-    for (int i = 0; i < P; i += 2) {
-      y.a.p[i / 2] = f32x2(turned(i) ? y.a.get(i) : x.a.get(i), turned(i + 1) ? y.a.get(i + 1) : x.a.get(i + 1));
-      y.b.p[i / 2] = f32x2(turned(i) ? y.b.get(i) : x.b.get(i), turned(i + 1) ? y.b.get(i + 1) : x.b.get(i + 1));
-    }
+  for (int i = 0; i < P; i += 2) {
+    y.a.p[i / 2] = f32x2(turned(i) ? y.a.get(i) : x.a.get(i), turned(i + 1) ? y.a.get(i + 1) : x.a.get(i + 1));
+    y.b.p[i / 2] = f32x2(turned(i) ? y.b.get(i) : x.b.get(i), turned(i + 1) ? y.b.get(i + 1) : x.b.get(i + 1));
   }
 }
 
@@ -367,13 +248,7 @@ struct Lane {
         mine((lane & ((1 << plan.crew) - 1)) >> plan.shift), to_teams(plan.crew - plan.shift),
         crew(static_cast<uint32_t>(lane) >> plan.crew), crews(32u >> plan.crew) {}
   __device__ __forceinline__ int teams_heads(int count) const { return (count - mine + teams - 1) >> to_teams; }  // of `count` heads
-  // steps of U (a power of two) heads a team
-  template <int U>
-  __device__ __forceinline__ int steps(int count) const {
-    constexpr int kShift = U == 1 ? 0 : U == 2 ? 1 : 2;
-    static_assert(U == 1 << kShift);
-    return (count + (U << to_teams) - 1) >> (to_teams + kShift);
-  }
+  __device__ __forceinline__ int steps(int count) const { return (count + teams - 1) >> to_teams; }
 };
 
 // ---- a lane's ring of S slots for NT tensors
@@ -418,43 +293,33 @@ __device__ __forceinline__ void read_shared(uint32_t* w, uint32_t from) {
     asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(from) : "memory");
 }
 
-// A warp's loads of the steps of its items, U heads a team a step. Runs come through the ring, S steps ahead, each
-// lane's own 16 bytes by itself; single channels (P = 1) are held in registers one step ahead.
-template <typename T, int P, int NV, int NT, int U, int S>
+// A warp's loads of the steps of its items, a head of every team a step: through the ring, S steps ahead, each lane's own
+// 16 bytes by itself.
+template <typename T, int P, int NT, int S>
 struct Stream {
-  static constexpr bool kAsync = P > 1;
-  static constexpr int kPiece = P * sizeof(T) >= 16 ? 16 : 8;                            // bytes of a copy
-  static constexpr int kPieces = kAsync ? P * static_cast<int>(sizeof(T)) / kPiece : 0;  // of a run
-  static constexpr int kSlot = U * NV * NT * 2 * kPieces * kPiece * kThreads;            // bytes of a slot for the block
-  static constexpr int kBytes = kAsync ? S * kSlot : 0;
+  static constexpr int kPiece = P * sizeof(T) >= 16 ? 16 : 8;                  // bytes of a copy
+  static constexpr int kPieces = P * static_cast<int>(sizeof(T)) / kPiece;     // of a run
+  static constexpr int kRow = kPiece * kThreads;                               // bytes of a piece of all threads
+  static constexpr int kSlot = NT * 2 * kPieces * kRow, kBytes = S * kSlot;    // bytes of a slot and of the ring
 
   const HeadsParams& p;
   const Plan& plan;
-  const Spot<P> (&spot)[NV];
+  const Spot<P>& spot;
   const Lane& my;
   uint32_t id, slot, last_slot;  // the warp's first item; addresses of this lane's piece
   int which, left, steps;
   Place place;
   int64_t step[NT];  // elements from one of the team's heads to the next
   const T* at[NT];
-  RawPairs<T, P> next[kAsync ? 1 : U][NV][NT];
 
-  __device__ __forceinline__ Stream(const HeadsParams& params, const Plan& plan_of, const Spot<P> (&spots)[NV], const Lane& lane, uint32_t first,
+  __device__ __forceinline__ Stream(const HeadsParams& params, const Plan& plan_of, const Spot<P>& spot_of, const Lane& lane, uint32_t first,
                                     uint8_t* smem)
-      : p(params), plan(plan_of), spot(spots), my(lane), id(first), which(-1), left(0), place(plan_of, first + lane.crew) {
+      : p(params), plan(plan_of), spot(spot_of), my(lane), id(first), which(-1), left(0), place(plan_of, first + lane.crew) {
     slot = smem_u32(smem) + threadIdx.x * kPiece;
     last_slot = slot + (S - 1) * kSlot;
-    if constexpr (!kAsync) {
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-          for (int k = 0; k < NT; ++k) next[u][i][k].zero();
-    }
     enter();
 #pragma unroll 1
-    for (int k = 0; k < (kAsync ? S : 1); ++k) fetch();
+    for (int k = 0; k < S; ++k) fetch();
   }
 
   // to the next phase that has heads, of this item or the next
@@ -475,7 +340,7 @@ struct Stream {
         step[k] = my.teams * v.head;
       }
       left = place.there ? my.teams_heads(count) : 0;
-      steps = my.template steps<U>(count);
+      steps = my.steps(count);
       return;
     }
   }
@@ -483,81 +348,52 @@ struct Stream {
   // starts the loads of the next step
   __device__ __forceinline__ void fetch() {
     if (id < plan.items) {
+      if (left > 0 && spot.there) {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (u < left) {
+        for (int k = 0; k < NT; ++k)
 #pragma unroll
-          for (int k = 0; k < NT; ++k) {
-            const T* from = at[k] + u * step[k];
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-              if constexpr (kAsync) {
-                if (spot[i].has_a) {  // runs are whole: both are there
-                  const uint32_t to = slot + ((u * NV + i) * NT + k) * 2 * kPieces * (kPiece * kThreads);
-#pragma unroll
-                  for (int c = 0; c < kPieces; ++c) {
-                    copy_async<kPiece>(to + c * (kPiece * kThreads), from + spot[i].a + c * kPiece / sizeof(T));
-                    copy_async<kPiece>(to + (kPieces + c) * (kPiece * kThreads), from + spot[i].b + c * kPiece / sizeof(T));
-                  }
-                }
-              } else {
-                next[u][i][k].load(from, spot[i]);
-              }
-            }
+          for (int c = 0; c < kPieces; ++c) {
+            const uint32_t to = slot + (k * 2 * kPieces + c) * kRow;
+            copy_async<kPiece>(to, at[k] + spot.a + c * kPiece / sizeof(T));
+            copy_async<kPiece>(to + kPieces * kRow, at[k] + spot.b + c * kPiece / sizeof(T));
           }
-        }
-      left -= U;
+      }
+      --left;
 #pragma unroll
-      for (int k = 0; k < NT; ++k) at[k] += U * step[k];
+      for (int k = 0; k < NT; ++k) at[k] += step[k];
       if (--steps == 0) enter();
     }
-    if constexpr (kAsync) {
-      commit_copies();
-      slot = slot == last_slot ? last_slot - (S - 1) * kSlot : slot + kSlot;
-    }
+    commit_copies();
+    slot = slot == last_slot ? last_slot - (S - 1) * kSlot : slot + kSlot;
   }
 
   // The oldest step's values; then its slot is free (nobody else reads it). The caller fetches the next after it
   // has widened them. What comes for channels and heads that are not there means nothing.
-  __device__ __forceinline__ void take(RawPairs<T, P> (&raw)[U][NV][NT]) {
-    if constexpr (kAsync) wait_copies<S - 1>();
+  __device__ __forceinline__ void take(RawPairs<T, P> (&raw)[NT]) {
+    wait_copies<S - 1>();
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int k = 0; k < NT; ++k)
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int k = 0; k < NT; ++k) {
-          if constexpr (kAsync) {
-            const uint32_t from = slot + ((u * NV + i) * NT + k) * 2 * kPieces * (kPiece * kThreads);
-#pragma unroll
-            for (int c = 0; c < kPieces; ++c) {
-              read_shared<kPiece>(raw[u][i][k].a.w + c * (kPiece / 4), from + c * (kPiece * kThreads));
-              read_shared<kPiece>(raw[u][i][k].b.w + c * (kPiece / 4), from + (kPieces + c) * (kPiece * kThreads));
-            }
-          } else {
-            raw[u][i][k] = next[u][i][k];
-          }
-        }
+      for (int c = 0; c < kPieces; ++c) {
+        const uint32_t from = slot + (k * 2 * kPieces + c) * kRow;
+        read_shared<kPiece>(raw[k].a.w + c * (kPiece / 4), from);
+        read_shared<kPiece>(raw[k].b.w + c * (kPiece / 4), from + kPieces * kRow);
+      }
   }
 };
-
-// heads of a team at a time
-template <int P, int NV>
-constexpr int kAtOnce = P > 1 || NV > 2 ? 1 : 4 / NV;
 
 // Slots of the rings, and blocks that an SM holds. 65536 tokens of 40 heads x 128 in bf16, a warp a token: forward 214 us
 // with two blocks (111 registers a thread) and 3, 4 or 6 slots, 260 with three (80 registers, 150 bytes of them
 // spilled); backward 371 us with 3 slots, 384 with 6, 398 with one block, 624 with three.
 constexpr int kForwardSlots = 3, kBackwardSlots = 3;
-template <typename T, int P, int NV>
-constexpr int kResident = P * static_cast<int>(sizeof(T)) > 16 || NV > 3 ? 1 : 2;
+template <typename T, int P>
+constexpr int kResident = P * static_cast<int>(sizeof(T)) > 16 ? 1 : 2;
 
-// Forward. NORM: the norm and its weight. ALL: every pair is turned. NV runs a lane, a team apart.
-template <typename T, int P, bool INTER, int NV, bool ALL, bool NORM>
-__global__ void __launch_bounds__(kThreads, kResident<T, P, NV>)
+// Forward. NORM: the norm and its weight. ALL: every pair is turned.
+template <typename T, int P, bool INTER, bool ALL, bool NORM>
+__global__ void __launch_bounds__(kThreads, kResident<T, P>)
     heads_kernel(const __grid_constant__ HeadsParams p, const __grid_constant__ Plan plan) {
-  constexpr int U = kAtOnce<P, NV>;
-  using Heads = Stream<T, P, NV, 1, U, kForwardSlots>;
+  using Heads = Stream<T, P, 1, kForwardSlots>;
   extern __shared__ __align__(16) uint8_t smem[];
   const Lane my(plan);
   const int warp = threadIdx.x / 32, tables = kWarps * my.crews;
@@ -565,9 +401,7 @@ __global__ void __launch_bounds__(kThreads, kResident<T, P, NV>)
   float* cosines = reinterpret_cast<float*>(smem + Heads::kBytes) + (warp * my.crews + my.crew) * 2 * plan.slots;
   float* sines = cosines + plan.slots;
   const float inverse_c = 1.0f / static_cast<float>(p.channels);
-  Spot<P> spot[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) spot[i] = spot_of<P, INTER>(p.rotary, (my.lane & (my.team - 1)) + i * my.team, p.channels);
+  const Spot<P> spot = spot_of<P, INTER>(p.rotary, my.lane & (my.team - 1), p.channels);
   const int crew_lanes = 1 << plan.crew, axis = my.lane & (crew_lanes - 1);
   Place after(plan, first + my.crew);
   double ahead = place_of(p.rotary, after.b, after.t, axis);  // the next item's
@@ -590,62 +424,37 @@ __global__ void __launch_bounds__(kThreads, kResident<T, P, NV>)
       T* y_head = static_cast<T*>(out.data) + (place.b * out.batch + place.t * out.token + (begin + my.mine) * out.head);
       const int64_t out_head = my.teams * out.head;
       int left = place.there ? my.teams_heads(count) : 0;
-      Pairs<P> c[NV], s[NV];  // cosines, and sines by the other channel's weight (a's negative)
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const Lanes<P> cosine = from_table<P, INTER>(cosines, spot[i]), sine = from_table<P, INTER>(sines, spot[i]);
-        if constexpr (NORM) {
-          const Pairs<P> w = weight_of<P, INTER>(constants.weight(p, which), spot[i]);
-          c[i] = {cosine * w.a, cosine * w.b};
-          s[i] = {negative(sine) * w.b, sine * w.a};
-        } else {
-          c[i] = {cosine, cosine};
-          s[i] = {negative(sine), sine};
-        }
+      Pairs<P> c, s;  // cosines, and sines by the other channel's weight (a's negative)
+      const Lanes<P> cosine = from_table<P, INTER>(cosines, spot), sine = from_table<P, INTER>(sines, spot);
+      if constexpr (NORM) {
+        const Pairs<P> w = weight_of<P, INTER>(constants.weight(p, which), spot);
+        c = {cosine * w.a, cosine * w.b};
+        s = {negative(sine) * w.b, sine * w.a};
+      } else {
+        c = {cosine, cosine};
+        s = {negative(sine), sine};
       }
 #pragma unroll 1
-      for (int step = my.steps<U>(count); step > 0; --step) {
-        RawPairs<T, P> raw[U][NV][1];
-        Pairs<P> v[U][NV];
+      for (int step = my.steps(count); step > 0; --step) {
+        RawPairs<T, P> raw[1];
         stream.take(raw);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int i = 0; i < NV; ++i) v[u][i] = widen<T, P, INTER>(raw[u][i][0]);
+        Pairs<P> v = widen<T, P, INTER>(raw[0]);
         stream.fetch();
         if constexpr (NORM) {
-          float rstd[U];
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            rstd[u] = 0.f;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-              const float sum = v[u][i].a.dot(v[u][i].a) + v[u][i].b.dot(v[u][i].b);
-              rstd[u] += P == 1 || spot[i].has_a ? sum : 0.f;
-            }
-          }
-          team_sums(rstd, my.team);
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            rstd[u] = rsqrtf(rstd[u] * inverse_c + p.eps);
-#pragma unroll
-            for (int i = 0; i < NV; ++i) v[u][i] = {v[u][i].a * Lanes<P>(rstd[u]), v[u][i].b * Lanes<P>(rstd[u])};
-          }
+          float sum[1] = {v.a.dot(v.a) + v.b.dot(v.b)};
+          if (!spot.there) sum[0] = 0.f;
+          team_sums(sum, my.team);
+          const Lanes<P> rstd(rsqrtf(sum[0] * inverse_c + p.eps));
+          v = {v.a * rstd, v.b * rstd};
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (u < left) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-              const Pairs<P>& n = v[u][i];
-              Pairs<P> y = {fma(n.a, c[i].a, n.b * s[i].a), fma(n.b, c[i].b, n.a * s[i].b)};
-              // a cosine of 1 leaves the weight
-              if constexpr (!ALL) keep_unturned<P, INTER>(y, {n.a * c[i].a, n.b * c[i].b}, spot[i]);
-              narrow<T, P, INTER>(y).store(y_head + u * out_head, spot[i]);
-            }
-          }
-        left -= U;
-        y_head += U * out_head;
+        if (left > 0) {
+          Pairs<P> y = {fma(v.a, c.a, v.b * s.a), fma(v.b, c.b, v.a * s.b)};
+          // a cosine of 1 leaves the weight
+          if constexpr (!ALL) keep_unturned<P, INTER>(y, {v.a * c.a, v.b * c.b}, spot);
+          narrow<T, P, INTER>(y).store(y_head, spot);
+        }
+        --left;
+        y_head += out_head;
       }
     }
   }
@@ -653,11 +462,10 @@ __global__ void __launch_bounds__(kThreads, kResident<T, P, NV>)
 
 // Backward: g = dy turned back, w = g weight, xh = x rstd: dx = rstd (w - xh mean(w xh)). A block's sums of g xh
 // over its items go to its rows of the partial sums, q's rows before k's.
-template <typename T, int P, bool INTER, int NV, bool ALL>
-__global__ void __launch_bounds__(kThreads, kResident<T, P, NV>)
+template <typename T, int P, bool INTER, bool ALL>
+__global__ void __launch_bounds__(kThreads, kResident<T, P>)
     heads_bwd_kernel(const __grid_constant__ HeadsParams p, const __grid_constant__ Plan plan, float* partial) {
-  constexpr int U = kAtOnce<P, NV>;
-  using Heads = Stream<T, P, NV, 2, U, kBackwardSlots>;
+  using Heads = Stream<T, P, 2, kBackwardSlots>;
   extern __shared__ __align__(16) uint8_t smem[];
   const Lane my(plan);
   const int warp = threadIdx.x / 32, tables = kWarps * my.crews;
@@ -665,13 +473,9 @@ __global__ void __launch_bounds__(kThreads, kResident<T, P, NV>)
   float* cosines = reinterpret_cast<float*>(smem + Heads::kBytes) + (warp * my.crews + my.crew) * 2 * plan.slots;
   float* sines = cosines + plan.slots;
   const float inverse_c = 1.0f / static_cast<float>(p.channels);
-  Spot<P> spot[NV];
-  Pairs<P> dw[2][NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    spot[i] = spot_of<P, INTER>(p.rotary, (my.lane & (my.team - 1)) + i * my.team, p.channels);
-    dw[0][i] = dw[1][i] = {Lanes<P>(0.f), Lanes<P>(0.f)};
-  }
+  const Spot<P> spot = spot_of<P, INTER>(p.rotary, my.lane & (my.team - 1), p.channels);
+  Pairs<P> dw[2];
+  dw[0] = dw[1] = {Lanes<P>(0.f), Lanes<P>(0.f)};
   const int crew_lanes = 1 << plan.crew, axis = my.lane & (crew_lanes - 1);
   Place after(plan, first + my.crew);
   double ahead = place_of(p.rotary, after.b, after.t, axis);  // the next item's
@@ -694,49 +498,29 @@ __global__ void __launch_bounds__(kThreads, kResident<T, P, NV>)
       T* dx_head = static_cast<T*>(out.data) + (place.b * out.batch + place.t * out.token + (begin + my.mine) * out.head);
       const int64_t out_head = my.teams * out.head;
       int left = place.there ? my.teams_heads(count) : 0;
-      Pairs<P> w[NV];
-#pragma unroll
-      for (int i = 0; i < NV; ++i) w[i] = weight_of<P, INTER>(constants.weight(p, which), spot[i]);
+      const Pairs<P> w = weight_of<P, INTER>(constants.weight(p, which), spot);
 #pragma unroll 1
-      for (int step = my.steps<U>(count); step > 0; --step) {
-        RawPairs<T, P> raw[U][NV][2];
-        Pairs<P> v[U][NV], g[U][NV];
+      for (int step = my.steps(count); step > 0; --step) {
+        RawPairs<T, P> raw[2];
         stream.take(raw);
-        float sums[2 * U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) sums[2 * u] = sums[2 * u + 1] = 0.f;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const Lanes<P> c = from_table<P, INTER>(cosines, spot[i]), s = from_table<P, INTER>(sines, spot[i]);
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            v[u][i] = widen<T, P, INTER>(raw[u][i][0]);
-            const Pairs<P> d = widen<T, P, INTER>(raw[u][i][1]);
-            g[u][i] = {fma(d.a, c, d.b * s), fma(d.b, c, negative(d.a * s))};
-            if constexpr (!ALL) keep_unturned<P, INTER>(g[u][i], d, spot[i]);
-            const float squares = v[u][i].a.dot(v[u][i].a) + v[u][i].b.dot(v[u][i].b);
-            const float along = (v[u][i].a * w[i].a).dot(g[u][i].a) + (v[u][i].b * w[i].b).dot(g[u][i].b);
-            sums[2 * u] += P == 1 || spot[i].has_a ? squares : 0.f;
-            sums[2 * u + 1] += P == 1 || spot[i].has_a ? along : 0.f;
-          }
-        }
+        const Lanes<P> c = from_table<P, INTER>(cosines, spot), s = from_table<P, INTER>(sines, spot);
+        const Pairs<P> v = widen<T, P, INTER>(raw[0]), d = widen<T, P, INTER>(raw[1]);
+        Pairs<P> g = {fma(d.a, c, d.b * s), fma(d.b, c, negative(d.a * s))};
+        if constexpr (!ALL) keep_unturned<P, INTER>(g, d, spot);
+        float sums[2] = {v.a.dot(v.a) + v.b.dot(v.b), (v.a * w.a).dot(g.a) + (v.b * w.b).dot(g.b)};
+        if (!spot.there) sums[0] = sums[1] = 0.f;
         stream.fetch();
         team_sums(sums, my.team);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (u < left) {
-            const float rstd = rsqrtf(sums[2 * u] * inverse_c + p.eps);
-            const float along = -rstd * rstd * (sums[2 * u + 1] * rstd * inverse_c);  // -rstd^2 mean(w xh)
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-              const Pairs<P> gr = {g[u][i].a * Lanes<P>(rstd), g[u][i].b * Lanes<P>(rstd)};
-              dw[which][i] = {fma(gr.a, v[u][i].a, dw[which][i].a), fma(gr.b, v[u][i].b, dw[which][i].b)};
-              const Pairs<P> y = {fma(v[u][i].a, Lanes<P>(along), gr.a * w[i].a), fma(v[u][i].b, Lanes<P>(along), gr.b * w[i].b)};
-              narrow<T, P, INTER>(y).store(dx_head + u * out_head, spot[i]);
-            }
-          }
-        left -= U;
-        dx_head += U * out_head;
+        if (left > 0) {
+          const float rstd = rsqrtf(sums[0] * inverse_c + p.eps);
+          const Lanes<P> along(-rstd * rstd * (sums[1] * rstd * inverse_c));  // -rstd^2 mean(w xh)
+          const Pairs<P> gr = {g.a * Lanes<P>(rstd), g.b * Lanes<P>(rstd)};
+          dw[which] = {fma(gr.a, v.a, dw[which].a), fma(gr.b, v.b, dw[which].b)};
+          const Pairs<P> y = {fma(v.a, along, gr.a * w.a), fma(v.b, along, gr.b * w.b)};
+          narrow<T, P, INTER>(y).store(dx_head, spot);
+        }
+        --left;
+        dx_head += out_head;
       }
     }
   }
@@ -749,19 +533,16 @@ __global__ void __launch_bounds__(kThreads, kResident<T, P, NV>)
   for (int which = 0; which < 2; ++which) {
     if (p.dweight[which] == nullptr) continue;
     __syncthreads();
+    for (int o = 16; o >= my.team; o >>= 1) {
+      dw[which].a = dw[which].a.each([&](float f) { return f + __shfl_xor_sync(0xFFFFFFFFu, f, o); });
+      dw[which].b = dw[which].b.each([&](float f) { return f + __shfl_xor_sync(0xFFFFFFFFu, f, o); });
+    }
+    if (my.lane < my.team && spot.there) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      for (int o = 16; o >= my.team; o >>= 1) {
-        dw[which][i].a = dw[which][i].a.each([&](float f) { return f + __shfl_xor_sync(0xFFFFFFFFu, f, o); });
-        dw[which][i].b = dw[which][i].b.each([&](float f) { return f + __shfl_xor_sync(0xFFFFFFFFu, f, o); });
-      }
-      if (my.lane < my.team) {
-#pragma unroll
-        for (int j = 0; j < P; ++j) {
-          const int at = !INTER ? spot[i].a + j : j < P / 2 ? spot[i].a + 2 * j : spot[i].b + 2 * j - P;
-          if (spot[i].has_a) row[at] = dw[which][i].a.get(j);
-          if (spot[i].has_b) row[INTER ? at + 1 : spot[i].b + j] = dw[which][i].b.get(j);
-        }
+      for (int j = 0; j < P; ++j) {
+        const int at = !INTER ? spot.a + j : j < P / 2 ? spot.a + 2 * j : spot.b + 2 * j - P;
+        row[at] = dw[which].a.get(j);
+        row[INTER ? at + 1 : spot.b + j] = dw[which].b.get(j);
       }
     }
     __syncthreads();
@@ -815,30 +596,24 @@ bool runs_of(const HeadsParams& p, int P, int size, bool backward) {
   return true;
 }
 
-// Calls f(P, INTER, NV, ALL as integral constants, lanes a team at least): runs of 16 bytes where they are whole and aligned
-// (fp32 heads of more than 256 channels in two of them), else of half that, else single channels.
+constexpr int kNoRuns = -1;
+
+// Calls f(P, INTER, ALL as integral constants, lanes a team at least): runs of 16 bytes where they are whole and aligned
+// (fp32 heads of more than 256 channels in two of them), else of half that, else kNoRuns.
 template <typename T, typename F>
 int dispatch_heads(const HeadsParams& p, bool backward, F&& f) {
   const int size = sizeof(T);
   const auto runs = [&](auto P) {
     const int lanes = p.channels / (2 * decltype(P)::value);
-    const std::integral_constant<int, 1> one;
     const std::true_type yes;
     const std::false_type no;
-    if (2 * p.rotary.pairs == p.channels) return p.rotary.interleaved ? f(P, yes, one, yes, lanes) : f(P, no, one, yes, lanes);
-    return p.rotary.interleaved ? f(P, yes, one, no, lanes) : f(P, no, one, no, lanes);
+    if (2 * p.rotary.pairs == p.channels) return p.rotary.interleaved ? f(P, yes, yes, lanes) : f(P, no, yes, lanes);
+    return p.rotary.interleaved ? f(P, yes, no, lanes) : f(P, no, no, lanes);
   };
   if (sizeof(T) == 4 && runs_of(p, 4, size, backward)) return runs(std::integral_constant<int, 4>{});
   if (runs_of(p, 8, size, backward)) return runs(std::integral_constant<int, 8>{});
   if (sizeof(T) == 2 && runs_of(p, 4, size, backward)) return runs(std::integral_constant<int, 4>{});
-  const int pairs = (p.channels + 1) / 2;
-  const std::integral_constant<int, 1> one;
-  const std::false_type apart;
-  if (pairs <= 32) return f(one, apart, std::integral_constant<int, 1>{}, apart, pairs);
-  if (pairs <= 64) return f(one, apart, std::integral_constant<int, 2>{}, apart, 32);
-  if (pairs <= 96) return f(one, apart, std::integral_constant<int, 3>{}, apart, 32);
-  if (pairs <= 128) return f(one, apart, std::integral_constant<int, 4>{}, apart, 32);
-  return f(one, apart, std::integral_constant<int, 8>{}, apart, 32);
+  return kNoRuns;
 }
 
 // How tokens' heads are cut into items. An item's issue time, in fortieths of a step of runs of 8: fixed work
@@ -849,11 +624,11 @@ int dispatch_heads(const HeadsParams& p, bool backward, F&& f) {
 // helps where the issue is the limit (65536 tokens of 32 heads x 24: 68 -> 35 us forward, 84 -> 52 backward; of 32 x
 // 48 104 -> 88 and 174 -> 141) and not where the memory is (40 x 128: 214 -> 218 forward). Where there are few
 // tokens, a whole warp takes a token, or a part of its heads.
-Plan plan_of(const HeadsParams& p, int lanes, int run, int nv, int at_once, int resident, int size, bool backward) {
+Plan plan_of(const HeadsParams& p, int lanes, int run, int resident, int size, bool backward) {
   const int heads = p.heads[0] + p.heads[1];
   Plan best{0, Divisor(1), Divisor(static_cast<uint32_t>(p.tokens)), heads, 0, 0, 0};
   while ((1 << best.shift) < lanes) ++best.shift;
-  best.slots = (((run * nv) << best.shift) + 3) / 4 * 4;
+  best.slots = run << best.shift;
   const int64_t tokens = static_cast<int64_t>(p.batch) * p.tokens, warps = 148 * kWarps * static_cast<int64_t>(resident);
   int64_t least = 0;
   const auto consider = [&](int crew, int per, int64_t chunks, int64_t steps) {
@@ -871,7 +646,7 @@ Plan plan_of(const HeadsParams& p, int lanes, int run, int nv, int at_once, int 
   };
   for (int crew = 5; crew >= best.shift; --crew) {
     if (p.rotary.pairs > 0 && 1 << crew < p.rotary.axes) break;
-    const int step = at_once << (crew - best.shift);
+    const int step = 1 << (crew - best.shift);
     consider(crew, heads, 1, (p.heads[0] + step - 1) / step + (p.heads[1] + step - 1) / step);
     if (crew < 5) continue;  // crews of one warp take the same steps
     for (int of = (heads + step - 1) / step / 2; of >= 1 && tokens < warps; of /= 2) {  // steps an item
@@ -885,64 +660,69 @@ size_t table_bytes(const Plan& plan, int channels) {
   return sizeof(float) * kWarps * (32 >> plan.crew) * 2 * plan.slots + Constants::bytes(plan.slots, channels);
 }
 
-constexpr int kMostBlocks = 148 * 2;
-
 int blocks_of(const Plan& plan, int resident) {
   const int64_t warp_items = kWarps * (32 >> plan.crew), want = (plan.items + warp_items - 1) / warp_items, most = 148 * resident;
   return static_cast<int>(want < most ? want : most);
 }
 
 template <typename T>
-int heads(const HeadsParams& p, cudaStream_t stream) {
-  return dispatch_heads<T>(p, false, [&](auto run, auto inter, auto nv, auto all, int lanes) {
-    constexpr int P = decltype(run)::value, NV = decltype(nv)::value;
+int forward(const HeadsParams& p, cudaStream_t stream) {
+  const int rc = dispatch_heads<T>(p, false, [&](auto run, auto inter, auto all, int lanes) {
+    constexpr int P = decltype(run)::value;
     constexpr bool INTER = decltype(inter)::value, ALL = decltype(all)::value;
-    const Plan plan = plan_of(p, lanes, P, NV, kAtOnce<P, NV>, kResident<T, P, NV>, sizeof(T), false);
-    const size_t smem = Stream<T, P, NV, 1, kAtOnce<P, NV>, kForwardSlots>::kBytes + table_bytes(plan, p.channels);
-    auto kernel = p.norm ? heads_kernel<T, P, INTER, NV, ALL, true> : heads_kernel<T, P, INTER, NV, ALL, false>;
+    const Plan plan = plan_of(p, lanes, P, kResident<T, P>, sizeof(T), false);
+    const size_t smem = Stream<T, P, 1, kForwardSlots>::kBytes + table_bytes(plan, p.channels);
+    auto kernel = p.norm ? heads_kernel<T, P, INTER, ALL, true> : heads_kernel<T, P, INTER, ALL, false>;
     if (smem > 48 * 1024) {
       const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
       if (e != cudaSuccess) return static_cast<int>(e);
     }
-    kernel<<<blocks_of(plan, kResident<T, P, NV>), kThreads, smem, stream>>>(p, plan);
+    kernel<<<blocks_of(plan, kResident<T, P>), kThreads, smem, stream>>>(p, plan);
     return static_cast<int>(cudaGetLastError());
   });
+  return rc == kNoRuns ? forward_any<T>(p, stream) : rc;
 }
 
 template <typename T>
-int heads_bwd(const HeadsParams& p, float* part, cudaStream_t stream) {
+int backward(const HeadsParams& p, float* part, cudaStream_t stream) {
   const bool sums = p.dweight[0] != nullptr || p.dweight[1] != nullptr;
-  return dispatch_heads<T>(p, true, [&](auto run, auto inter, auto nv, auto all, int lanes) {
-    constexpr int P = decltype(run)::value, NV = decltype(nv)::value;
+  const int rc = dispatch_heads<T>(p, true, [&](auto run, auto inter, auto all, int lanes) {
+    constexpr int P = decltype(run)::value;
     constexpr bool INTER = decltype(inter)::value, ALL = decltype(all)::value;
-    const Plan plan = plan_of(p, lanes, P, NV, kAtOnce<P, NV>, kResident<T, P, NV>, sizeof(T), true);
-    size_t smem = Stream<T, P, NV, 2, kAtOnce<P, NV>, kBackwardSlots>::kBytes + table_bytes(plan, p.channels);
+    const Plan plan = plan_of(p, lanes, P, kResident<T, P>, sizeof(T), true);
+    size_t smem = Stream<T, P, 2, kBackwardSlots>::kBytes + table_bytes(plan, p.channels);
     if (smem < sizeof(float) * kWarps * p.channels) smem = sizeof(float) * kWarps * p.channels;
-    auto kernel = heads_bwd_kernel<T, P, INTER, NV, ALL>;
+    auto kernel = heads_bwd_kernel<T, P, INTER, ALL>;
     if (smem > 48 * 1024) {
       const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
       if (e != cudaSuccess) return static_cast<int>(e);
     }
-    const int blocks = blocks_of(plan, kResident<T, P, NV>);
+    const int blocks = blocks_of(plan, kResident<T, P>);
     kernel<<<blocks, kThreads, smem, stream>>>(p, plan, sums ? part : nullptr);
-    const int rc = static_cast<int>(cudaGetLastError());
-    if (rc != 0 || !sums) return rc;
-    return launch_after(heads_reduce_kernel, dim3((p.channels + 31) / 32, 2), 1024, 0, stream, static_cast<const float*>(part),
-                        p.dweight[0], p.dweight[1], blocks, p.channels);
+    const int launched = static_cast<int>(cudaGetLastError());
+    return launched != 0 || !sums ? launched : reduce(part, p, blocks, stream);
   });
+  return rc == kNoRuns ? backward_any<T>(p, part, stream) : rc;
 }
 
 }  // namespace
 
+int reduce(const float* part, const HeadsParams& p, int blocks, cudaStream_t stream) {
+  return launch_after(heads_reduce_kernel, dim3((p.channels + 31) / 32, 2), 1024, 0, stream, part, p.dweight[0], p.dweight[1], blocks,
+                      p.channels);
+}
+
+}  // namespace heads
+
 size_t heads_bwd_workspace_bytes(int64_t, int, int, int channels, int) {
-  return static_cast<size_t>(2 * kMostBlocks) * channels * sizeof(float);
+  return static_cast<size_t>(2 * heads::kMostBlocks) * channels * sizeof(float);
 }
 int launch_heads(const HeadsParams& p, int is_f32, cudaStream_t stream) {
-  return is_f32 ? heads<float>(p, stream) : heads<__nv_bfloat16>(p, stream);
+  return is_f32 ? heads::forward<float>(p, stream) : heads::forward<__nv_bfloat16>(p, stream);
 }
 int launch_heads_bwd(const HeadsParams& p, void* workspace, int is_f32, cudaStream_t stream) {
   float* part = static_cast<float*>(workspace);
-  return is_f32 ? heads_bwd<float>(p, part, stream) : heads_bwd<__nv_bfloat16>(p, part, stream);
+  return is_f32 ? heads::backward<float>(p, part, stream) : heads::backward<__nv_bfloat16>(p, part, stream);
 }
 
 }  // namespace ffb

@@ -306,15 +306,41 @@ def test_offsets_past_32_bits():
 
 
 @pytest.mark.parametrize("t,hq,hk,d,pairs,axes", [(70001, 1, 1, 16, 8, 1), (70001, 2, 1, 24, 12, 1), (40009, 4, 4, 32, 16, 3),
-                                                  (40009, 4, 4, 32, 15, 5), (40009, 3, 1, 7, 3, 9), (1, 3, 3, 16, 8, 2), (33, 0, 2, 32, 16, 1)])
+                                                  (40009, 4, 4, 32, 15, 5), (40009, 3, 1, 7, 3, 9), (1, 3, 3, 16, 8, 2), (33, 0, 2, 32, 16, 1),
+                                                  (40009, 16, 16, 48, 24, 1), (30011, 9, 4, 24, 8, 2), (20011, 10, 3, 128, 64, 3),
+                                                  (20011, 7, 5, 80, 40, 1), (20011, 6, 6, 56, 28, 1)])
+@pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("dtype", [BF16, F32])
-def test_tokens_that_share_a_warp(t, hq, hk, d, pairs, axes, dtype):
-    """Few small heads: several tokens a warp, a number of them that leaves lanes without one."""
+def test_tokens_that_share_a_warp(t, hq, hk, d, pairs, axes, dtype, interleaved):
+    """Many tokens: several a warp, a number of them that leaves lanes without one."""
     g = gen(t + d)
-    turn = Turn(g, 1, t, pairs, axes)
+    turn = Turn(g, 1, t, pairs, axes, interleaved)
     q, k = values(g, 1, t, hq, d, dtype=dtype), values(g, 1, t, hk, d, dtype=dtype)
     dq, dk = values(g, 1, t, hq, d, dtype=dtype, size=1e-2), values(g, 1, t, hk, d, dtype=dtype, size=1e-2)
     run_norm(q, k, dq, dk, turn, weights(g, d), weights(g, d))
+
+
+@pytest.mark.parametrize("d", [24, 48, 64, 33])
+def test_many_tokens_in_place(d):
+    """q and k of packed rows over themselves, a batch with positions of its own, tokens before the batch in memory."""
+    g = gen(d + 1)
+    b, t = 3, 9001
+    turn = Turn(g, b, t, d // 2, 2)
+    qw, kw = weights(g, d), weights(g, d)
+    rows = values(g, t, b, 7, d).transpose(0, 1)
+    q, k = rows[:, :, :4], rows[:, :, 4:6]
+    kept = rows.clone()
+    want = kernels.qk_norm_rotary(q, k, turn.positions, turn.table, qw, kw, EPS)
+    for x, y, w in zip((q, k), want, (qw, kw), strict=True):
+        check([y], *ref.heads(x, turn.angles(), False, w, EPS), [BF16])
+    got = kernels.qk_norm_rotary(q, k, turn.positions, turn.table, qw, kw, EPS, out=(q, k))
+    assert got[0].data_ptr() == rows.data_ptr()
+    assert torch.equal(rows[:, :, :4], want[0]) and torch.equal(rows[:, :, 4:6], want[1]) and torch.equal(rows[:, :, 6:], kept[:, :, 6:])
+    rows.copy_(kept)
+    dq, dk = values(g, b, t, 4, d, size=1e-2), values(g, b, t, 2, d, size=1e-2)
+    want = kernels.qk_norm_rotary_backward(dq, dk, q, k, turn.positions, turn.table, qw, kw, EPS)
+    got = kernels.qk_norm_rotary_backward(dq, dk, q, k, turn.positions, turn.table, qw, kw, EPS, out=(dq, dk))  # over the gradients
+    assert all(torch.equal(x, y) for x, y in zip(got, want, strict=True)) and torch.equal(dq, want[0])
 
 
 def test_more_tokens_than_a_grid_takes_at_once():
