@@ -2,15 +2,16 @@
 // alignment, a lane a pair of single channels.
 //
 // A warp takes an item of up to 32 rows (a row: one head of one token), of several tokens where a token has few
-// heads. Each lane first finds one row's addresses, then all of them the tokens' angles (into shared memory), and the
-// rows follow in batches of U a team. The sums of a batch go through one another: lanes trade halves of the rows at the
-// first steps, so that U sums over a team take U - 1 exchanges and a few more instead of five each.
+// heads. Each lane first finds one row's addresses; the first batch of rows (U a team) is on its way while all of them
+// find the tokens' angles (into shared memory), and each next one while its predecessor is worked on. The sums of a
+// batch go through one another: lanes trade halves of the rows at the first steps, so that U sums over a team take
+// U - 1 exchanges and a few more instead of five each.
 //
 // Measured on one B200 (us; in brackets as heads.cu's rings of one token an item did it, with single channels):
-//   65536 tokens, 8 + 8 heads x 37 bf16     forward 111 (150), backward 163 (232)
-//   65536 tokens, 8 + 8 heads x 151 bf16    forward 260 (334), backward 370 (414)
-//   79000 tokens, 2 + 2 heads x 51 fp32     forward 51 (107), backward 69 (137)
-//   20000 tokens, 4 + 4 heads x 500 bf16    forward 197 (170), backward 264 (182): no registers are left for a batch
+//   65536 tokens, 8 + 8 heads x 37 bf16     forward 109 (150), backward 162 (232)
+//   65536 tokens, 8 + 8 heads x 151 bf16    forward 254 (334), backward 363 (414)
+//   79000 tokens, 2 + 2 heads x 51 fp32     forward 51 (107), backward 68 (137)
+//   20000 tokens, 4 + 4 heads x 500 bf16    forward 184 (170), backward 250 (182): no registers are left for a batch
 // Bound by instructions: 2-byte loads and stores, and at 37 channels 19 of 32 lanes. Rows staged through shared memory
 // by asynchronous copies of the 16 bytes around them instead: 37 channels 125 and 202, 151 298 and 532.
 #include <type_traits>
@@ -46,19 +47,20 @@ struct Rows {
   int64_t* places;            // [kRows]: of the item's tokens' positions
   int* tables;                // [kRows]
   float2* turns;
-  int count;
+  int count, tokens;
 
   static __host__ __device__ int bytes(int turns) { return (NT + 2) * kRows * 8 + kRows * 4 + turns * 8; }
-  __device__ __forceinline__ Rows(uint8_t* smem, int turns_of)
+  __device__ __forceinline__ explicit Rows(uint8_t* smem)
       : offsets(reinterpret_cast<int64_t(*)[kRows]>(smem)), places(offsets[NT + 1]), tables(reinterpret_cast<int*>(places + kRows)),
-        turns(reinterpret_cast<float2*>(tables + kRows)), count(0) {}
-  __device__ __forceinline__ void prepare(const HeadsParams& p, const AnyPlan& plan, const Constants& constants, int which, uint32_t id) {
+        turns(reinterpret_cast<float2*>(tables + kRows)), count(0), tokens(0) {}
+  // an item's rows
+  __device__ __forceinline__ void enter(const HeadsParams& p, const AnyPlan& plan, int which, uint32_t id) {
     const Phase& phase = plan.phase[which];
     const RotaryParams& r = p.rotary;
     const int lane = threadIdx.x & 31;
     const uint32_t group = phase.chunks.quotient(id), first = group * phase.tokens;
     const int head0 = static_cast<int>(id - group * phase.chunks.d) * phase.heads;
-    const int tokens = min(static_cast<uint32_t>(phase.tokens), plan.total - first);
+    tokens = min(static_cast<uint32_t>(phase.tokens), plan.total - first);
     count = tokens * min(phase.heads, p.heads[which] - head0);
     __syncwarp();
     if (lane < count) {
@@ -76,7 +78,10 @@ struct Rows {
       places[lane] = b * r.batch + t * r.token;
     }
     __syncwarp();
-    for (int e = lane; e < tokens * r.pairs; e += 32) {
+  }
+  // its tokens' angles
+  __device__ __forceinline__ void find_turns(const RotaryParams& r, const AnyPlan& plan, const Constants& constants) {
+    for (int e = threadIdx.x & 31; e < tokens * r.pairs; e += 32) {
       const int of = static_cast<int>(plan.pairs.quotient(e)), j = e - of * r.pairs;
       turns[e] = turn_of(position_at(r, places[of] + constants.axes[j] * r.axis) * constants.quarters[j], r.inverse ? 0x80000000u : 0u);
     }
@@ -173,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, kResident<NV>)
   extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, team = 1 << plan.shift, teams = 32 >> plan.shift, mine = lane >> plan.shift;
   const int warp_bytes = Rows<1>::bytes(plan.turns);
-  Rows<1> rows(smem + warp * warp_bytes, plan.turns);
+  Rows<1> rows(smem + warp * warp_bytes);
   const Constants constants(p, plan.table, smem + kWarps * warp_bytes);
   __syncthreads();
   const float inverse_c = 1.0f / static_cast<float>(p.channels);
@@ -195,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, kResident<NV>)
     const Share share(which);
 #pragma unroll 1
     for (uint32_t id = share.first; id < plan.phase[which].items; id += share.stride) {
-      rows.prepare(p, plan, constants, which, id);
+      rows.enter(p, plan, which, id);
       const auto fetch = [&](int base) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -205,6 +210,7 @@ __global__ void __launch_bounds__(kThreads, kResident<NV>)
         }
       };
       fetch(0);
+      rows.find_turns(p.rotary, plan, constants);
 #pragma unroll 1
       for (int base = 0; base < rows.count; base += U * teams) {
         float2 v[U][NV];
@@ -249,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, kResident<NV>)
   extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, team = 1 << plan.shift, teams = 32 >> plan.shift, mine = lane >> plan.shift;
   const int warp_bytes = Rows<2>::bytes(plan.turns);
-  Rows<2> rows(smem + warp * warp_bytes, plan.turns);
+  Rows<2> rows(smem + warp * warp_bytes);
   const Constants constants(p, plan.table, smem + kWarps * warp_bytes);
   float* sums_of = reinterpret_cast<float*>(smem + kWarps * warp_bytes + Constants::bytes(plan.table, p.channels));
   __syncthreads();
@@ -278,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, kResident<NV>)
     const Share share(which);
 #pragma unroll 1
     for (uint32_t id = share.first; id < plan.phase[which].items; id += share.stride) {
-      rows.prepare(p, plan, constants, which, id);
+      rows.enter(p, plan, which, id);
       const auto fetch = [&](int base) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -292,6 +298,7 @@ __global__ void __launch_bounds__(kThreads, kResident<NV>)
         }
       };
       fetch(0);
+      rows.find_turns(p.rotary, plan, constants);
 #pragma unroll 1
       for (int base = 0; base < rows.count; base += U * teams) {
         float2 v[U][NV], g[U][NV];
@@ -359,12 +366,12 @@ __global__ void __launch_bounds__(kThreads, kResident<NV>)
 }
 
 // ------------------------------------------------------------------ launches
-AnyPlan plan_of(const HeadsParams& p, int lanes, int at_once) {
+AnyPlan plan_of(const HeadsParams& p, int lanes, int at_once, int resident) {
   AnyPlan plan{{{0, Divisor(1), Divisor(1), 1, 1}, {0, Divisor(1), Divisor(1), 1, 1}},
                Divisor(static_cast<uint32_t>(p.tokens)), Divisor(static_cast<uint32_t>(p.rotary.pairs > 0 ? p.rotary.pairs : 1)),
                static_cast<uint32_t>(static_cast<int64_t>(p.batch) * p.tokens), 0, 0, (p.rotary.pairs + 3) / 4 * 4, true};
   while ((1 << plan.shift) < lanes) ++plan.shift;
-  const int step = at_once * (32 >> plan.shift);
+  const int step = at_once * (32 >> plan.shift), phases = p.heads[0] > 0 && p.heads[1] > 0 ? 2 : 1;
   int most_tokens = 1;
   for (int i = 0; i < 2; ++i) {
     if (p.heads[i] == 0) continue;
@@ -374,13 +381,31 @@ AnyPlan plan_of(const HeadsParams& p, int lanes, int at_once) {
       if (p.rotary.pairs > 0 && tokens * p.rotary.pairs > kItemPairs) tokens = kItemPairs / p.rotary.pairs;
       if (tokens < 1) tokens = 1;
     }
-    // smaller items where there are not enough for the GPU's warps: fewer tokens, then a step's heads
-    const int64_t total = plan.total, enough = 148 * 16;
-    while (tokens > 1 && (total + tokens - 1) / tokens * chunks < enough) tokens /= 2;
-    while (tokens == 1 && heads > step && total * chunks < enough) {
-      heads = (heads + 1) / 2 > step ? (heads + 1) / 2 : step;
-      chunks = (p.heads[i] + heads - 1) / heads;
+    // Fewer tokens an item, then fewer heads, where that saves time: rounds of items by their batches and half a batch for
+    // what an item costs besides. In two rounds also at 3% more, since shorter items spread better: 2100 tokens of
+    // 30 heads x 248 bf16 backward 41 us for 53. 3584 of 8 x 32, 30 channels turned: four tokens an item 6.9 us, two
+    // 8.8, one 9.4; 8000 of 16 x 37 backward: four 33.3, two 30.8.
+    const int64_t total = plan.total, warps = 148 * kWarps * resident / phases;
+    const auto rounds = [&](int of_tokens, int of_heads) {
+      const int64_t items = (total + of_tokens - 1) / of_tokens * ((p.heads[i] + of_heads - 1) / of_heads);
+      return (items + warps - 1) / warps;
+    };
+    const auto cost = [&](int of_tokens, int of_heads) {  // in half batches
+      return rounds(of_tokens, of_heads) * (2 * ((of_tokens * of_heads + step - 1) / step) + 1);
+    };
+    int64_t least = cost(tokens, heads);
+    for (int t = tokens, h = heads; t > 1 || h > step;) {
+      if (t > 1)
+        t /= 2;
+      else
+        h = (h + 1) / 2 > step ? (h + 1) / 2 : step;
+      const int64_t now = cost(t, h);
+      if (now * (rounds(t, h) <= 2 ? 31 : 32) >= least * 32) continue;
+      least = now;
+      tokens = t;
+      heads = h;
     }
+    chunks = (p.heads[i] + heads - 1) / heads;
     if ((total + tokens - 1) / tokens * chunks >= int64_t(1) << 31) plan.fits = false;
     plan.phase[i] = {static_cast<uint32_t>((total + tokens - 1) / tokens * chunks), Divisor(static_cast<uint32_t>(chunks)),
                      Divisor(static_cast<uint32_t>(heads)), tokens, heads};
@@ -419,7 +444,7 @@ template <typename T>
 int forward_any(const HeadsParams& p, cudaStream_t stream) {
   return dispatch(p.channels, [&](auto nv, int lanes) {
     constexpr int NV = decltype(nv)::value;
-    const AnyPlan plan = plan_of(p, lanes, kForwardRows<NV>);
+    const AnyPlan plan = plan_of(p, lanes, kForwardRows<NV>, kResident<NV>);
     if (!plan.fits) return static_cast<int>(cudaErrorInvalidValue);
     const size_t smem = kWarps * Rows<1>::bytes(plan.turns) + Constants::bytes(plan.table, p.channels);
     auto kernel = p.norm ? forward_kernel<T, NV, true> : forward_kernel<T, NV, false>;
@@ -435,7 +460,7 @@ int backward_any(const HeadsParams& p, float* part, cudaStream_t stream) {
   const bool sums = p.dweight[0] != nullptr || p.dweight[1] != nullptr;
   return dispatch(p.channels, [&](auto nv, int lanes) {
     constexpr int NV = decltype(nv)::value;
-    const AnyPlan plan = plan_of(p, lanes, kBackwardRows<NV>);
+    const AnyPlan plan = plan_of(p, lanes, kBackwardRows<NV>, kResident<NV>);
     if (!plan.fits) return static_cast<int>(cudaErrorInvalidValue);
     const size_t smem = kWarps * Rows<2>::bytes(plan.turns) + Constants::bytes(plan.table, p.channels) +
                         sizeof(float) * kWarps * Constants::padded(p.channels);
