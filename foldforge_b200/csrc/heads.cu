@@ -17,7 +17,7 @@
 //   2 x 24960 tokens, 24 + 24 heads x 128 bf16     rotation alone 207 us (5.9 TB/s)
 //   65536 tokens, 16 + 16 heads x 48 bf16          forward 85 us (4.8 TB/s), backward 143 (4.2)
 //   500000 tokens, 4 + 4 heads x 32 bf16           forward 131 us (3.9 TB/s), backward 192 (4.0)
-// In the first case 16 warps an SM issue in 60% of the slots: 13 instructions for 32 channels forward and 22 backward.
+// In the first case 16 warps an SM issue in 60% of the slots: 13 instructions for 32 channels forward and 21 backward.
 // A token costs a crew about as much as two to four steps of its heads (angles, addresses, the weight's values), so
 // crews of a warp share it where the issue is the limit (plan_of).
 // Before the ring, with heads loaded straight to registers: forward 247 us, backward 670 (or 461 with half the
