@@ -414,7 +414,8 @@ int ffb_swiglu_bwd(const void* dh, const void* ab, const uint8_t* codes, const u
  * ffb_dropout: out = residual + keep x / (1 - p), or without residual (NULL) keep x / (1 - p); a dropped x
  *   counts as 0 whatever it holds. x is read as [outer, shared, inner], the mask is of [outer, inner]: element
  *   m stays where word m % 4 of Philox4x32-10 (Salmon et al., "Parallel random numbers: as easy as 1, 2, 3",
- *   2011) with key = seed and counter = (m / 4, offset) is at least p 2^32 (rounded). x and out (and the
+ *   2011) with key = seed and counter = (m / 4, offset) is at least p 2^32 (rounded). x / (1 - p) (a product with
+ *   1 / (1 - p) in fp32) and the sum are rounded to fp32 each, the sum then to out's type. x and out (and the
  *   residual with it) may differ in dtype. device_seed (or NULL): two 64-bit numbers on the device, read by the
  *   kernel: the seed, taken in the place of `seed`, and a number added to offset. 0 <= p <= 1. The backward pass
  *   is the same call on the output's gradient without residual. out may be x or the residual. */
