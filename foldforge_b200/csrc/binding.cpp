@@ -333,6 +333,16 @@ Heads output_heads(const char* name, const char* what, const Heads& x, const Opt
   return heads_of(name, what, out ? *out : like(x.t, x.t.sizes()), x.t, false, true);
 }
 
+// A tensor of the caller's to write. Nothing here is recorded: one that autograd follows would keep the gradient of what it
+// held before. (Called outside the guard.)
+void need_unfollowed(const char* name, const char* what, const OptTensor& out) {
+  if (out && out->requires_grad() && at::GradMode::is_enabled()) refuse(name, std::string(what) + " to write requires a gradient");
+}
+// counts it as written, so that a backward pass which kept it (or memory that it shares) refuses to read it
+void written(const OptTensor& out) {
+  if (out && !out->is_inference()) out->unsafeGetTensorImpl()->bump_version();
+}
+
 using Table = std::tuple<Tensor, Tensor, int64_t, bool>;  // quarter turns, the pairs' axes, axes, interleaved
 
 struct Rotary {
@@ -376,6 +386,8 @@ std::tuple<Tensor, OptTensor> heads_forward(const char* name, bool norm, const T
                                             const OptTensor& positions, const std::optional<Table>& table, bool inverse,
                                             const OptTensor& q_weight, const OptTensor& k_weight, double eps,
                                             const OptTensor& q_out_in, const OptTensor& k_out_in) {
+  need_unfollowed(name, "q's output", q_out_in);
+  need_unfollowed(name, "k's output", k_out_in);
   at::NoGradGuard no_grad;
   const Heads q = first_heads(name, q_in);
   Heads k, q_out, k_out;
@@ -396,6 +408,8 @@ std::tuple<Tensor, OptTensor> heads_forward(const char* name, bool norm, const T
   check(name, norm ? entries.qk_norm_rotary_fwd(q.at(), k.at(), q_out.at(), k_out.at(), pointer(qw), pointer(kw),
                                                 static_cast<float>(eps), &r.params, batch, tokens, channels, dtype, call.stream)
                    : entries.rotary_fwd(q.at(), k.at(), q_out.at(), k_out.at(), &r.params, batch, tokens, channels, dtype, call.stream));
+  written(q_out_in);
+  written(k_out_in);
   return {q_out.t, k_in ? OptTensor(k_out.t) : OptTensor()};
 }
 
@@ -414,8 +428,10 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor> qk_norm_rotary_backward(
     const Tensor& dq_out, const OptTensor& dk_out, const Tensor& q_in, const OptTensor& k_in, const OptTensor& positions,
     const std::optional<Table>& table, const OptTensor& q_weight, const OptTensor& k_weight, double eps, bool weight_gradient,
     const OptTensor& dq_in, const OptTensor& dk_in) {
-  at::NoGradGuard no_grad;
   const char* name = "qk_norm_rotary_backward";
+  need_unfollowed(name, "q's gradient", dq_in);
+  need_unfollowed(name, "k's gradient", dk_in);
+  at::NoGradGuard no_grad;
   const Heads q = first_heads(name, q_in);
   const Heads dy_q = heads_of(name, "the gradient of q's output", dq_out, q_in, false);
   Heads k, dy_k, dq, dk;
@@ -447,6 +463,8 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor> qk_norm_rotary_backward(
   check(name, entries.qk_norm_rotary_bwd(dy_q.at(), dy_k.at(), q.at(), k.at(), dq.at(), dk.at(), pointer(qw), pointer(kw), pointer(dqw),
                                          pointer(dkw), static_cast<float>(eps), &r.params, ws ? ws->data_ptr() : nullptr, size, batch,
                                          tokens, channels, dtype, call.stream));
+  written(dq_in);
+  written(dk_in);
   return {dq.t, k_in ? OptTensor(dk.t) : OptTensor(), dqw, dkw};
 }
 

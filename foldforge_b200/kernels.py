@@ -646,7 +646,8 @@ def rotary(q: Tensor, k: Tensor | None, positions: Tensor, table: RotaryTable, *
     """``q`` and ``k`` (of other heads, or ``None``) turned by their tokens' ``positions [tokens, axes]`` or ``[batch,
     tokens, axes]`` (int32, int64 or fp32), with ``inverse`` back: also the gradients of q and k from those of the
     outputs. ``out``: tensors to write instead of new ones (of any strides with dense channels; q and k
-    themselves, a cache's slots)."""
+    themselves, a cache's slots). Nothing is recorded for autograd, so an output that requires a gradient is refused while
+    gradients are recorded; a backward pass that kept one finds it changed."""
     q_out, k_out = out or (None, None)
     return _lib.binding().rotary(q, k, positions, table, inverse, q_out, k_out)
 
