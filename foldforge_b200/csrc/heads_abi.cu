@@ -78,26 +78,35 @@ bool same_view(const Sizes& s, const ffb_heads& a, const ffb_heads& b) {
          (s.tokens == 1 || a.token_stride == b.token_stride) && (a.heads == 1 || a.head_stride == b.head_stride);
 }
 
-// Two views share no element: they lie apart, or side by side in rows of one size (a row a token, and rows
-// apart), each within its own part of every row.
-bool apart(const Sizes& s, const ffb_heads& a, const ffb_heads& b) {
-  const char *pa = static_cast<const char*>(a.data), *pb = static_cast<const char*>(b.data);
-  if (pa + extent(s, a) * s.element <= pb || pb + extent(s, b) * s.element <= pa) return true;
-  if ((s.batch > 1 && a.batch_stride != b.batch_stride) || (s.tokens > 1 && a.token_stride != b.token_stride)) return false;
-  int64_t row = 0;  // a row's size
-  if (s.batch > 1 && s.tokens > 1) {
-    const bool token_inside = a.token_stride <= a.batch_stride;
-    row = token_inside ? a.token_stride : a.batch_stride;
-    if ((token_inside ? a.batch_stride : a.token_stride) / (token_inside ? s.tokens : s.batch) < row) return false;
-  } else if (s.batch > 1 || s.tokens > 1) {
-    row = s.batch > 1 ? a.batch_stride : a.token_stride;
-  } else {
-    return false;
+// Where b starts behind a, and their sizes and strides on the batch, the tokens and the heads, in elements.
+struct Beside {
+  int64_t delta, channels, na[3], nb[3], sa[3], sb[3];
+};
+// Two views share no element over the axes of the set `left`: one ends before the other begins, or an axis that they step
+// along alike has steps that reach over both of their parts, and within a step these share none.
+bool apart(const Beside& v, unsigned left) {
+  int64_t wa = v.channels, wb = v.channels;
+  for (int i = 0; i < 3; ++i)
+    if (left >> i & 1) {
+      wa += (v.na[i] - 1) * v.sa[i];
+      wb += (v.nb[i] - 1) * v.sb[i];
+    }
+  if (wa <= v.delta || wb <= -v.delta) return true;
+  for (int i = 0; i < 3; ++i) {
+    if (!(left >> i & 1) || (v.na[i] == 1 && v.nb[i] == 1)) continue;
+    const int64_t step = v.na[i] > 1 ? v.sa[i] : v.sb[i];
+    if (v.na[i] > 1 && v.nb[i] > 1 && v.sb[i] != step) continue;
+    const int64_t a_end = wa - (v.na[i] - 1) * v.sa[i], b_end = v.delta + wb - (v.nb[i] - 1) * v.sb[i];
+    const int64_t span = (a_end > b_end ? a_end : b_end) - (v.delta < 0 ? v.delta : 0);
+    if (span <= step && apart(v, left & ~(1u << i))) return true;
   }
-  const int64_t wa = (a.heads - 1) * a.head_stride + s.channels, wb = (b.heads - 1) * b.head_stride + s.channels;
-  const int64_t bytes = pb - pa, delta = bytes / s.element;
+  return false;
+}
+bool apart(const Sizes& s, const ffb_heads& a, const ffb_heads& b) {
+  const int64_t bytes = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.data)) - static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.data));
   if (bytes % s.element != 0) return false;
-  return delta >= 0 ? wa <= delta && delta + wb <= row : wb <= -delta && wa - delta <= row;
+  return apart(Beside{bytes / s.element, s.channels, {s.batch, s.tokens, a.heads}, {s.batch, s.tokens, b.heads},
+                      {a.batch_stride, a.token_stride, a.head_stride}, {b.batch_stride, b.token_stride, b.head_stride}}, 7u);
 }
 
 int check_rotary(const Sizes& s, const ffb_rotary* r) {

@@ -408,8 +408,8 @@ int ffb_swiglu_bwd(const void* dh, const void* ab, const uint8_t* codes, const u
  *   order of sums; NULL where not wanted).
  * channels <= 512, batch tokens < 2^31 - 1 (0: nothing but zero weight gradients); k, its outputs and weights may
  * be left out (k NULL). dtype (ffb_dtype) is the activations'. An output may be its own input (the same
- * address and strides); else outputs overlap neither inputs nor each other, but may interleave with them
- * in rows of one size (q and k of the same [q | k | v] rows).
+ * address and strides); else outputs share no element with inputs or each other, but may lie between them as
+ * parts of one tensor, its axes in any order (q and k of the same [q | k | v] rows, of one head-major tensor).
  *
  * ffb_dropout: out = residual + keep x / (1 - p), or without residual (NULL) keep x / (1 - p); a dropped x
  *   counts as 0 whatever it holds. x is read as [outer, shared, inner], the mask is of [outer, inner]: element

@@ -71,3 +71,36 @@ def test_versions_of_outputs():
         other = torch.empty_like(q)
         kernels.rotary(q, None, positions, table, out=(other, None))
         assert torch.equal(other, want)
+
+
+# --------------------------------------------------------------------------- outputs that lie between others
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("d", [48, 37])
+@pytest.mark.parametrize("order", [(0, 2, 1, 3), (1, 2, 0, 3), (2, 0, 1, 3), (2, 1, 0, 3), (0, 1, 2, 3)])
+def test_parts_of_one_tensor(order, d, dtype):
+    """q and k as parts of one tensor of a batch, its axes in any order in memory (head-major among them), and as
+    channels side by side in the same heads: in place and into another such tensor, the rest left as it was."""
+    b, t = 3, 21
+    positions, table = turning(b, t, 24)
+    g = gen(d)
+
+    def made(heads, channels):
+        sizes = (b, t, heads, channels)
+        memory = torch.randn([sizes[a] for a in order], device="cuda", generator=g).to(dtype)
+        return memory.permute([order.index(a) for a in range(4)])
+
+    for x, at in ((made(9, d), lambda x: (x[:, :, :4], x[:, :, 4:6], x[:, :, 6:])),
+                  (made(3, 3 * d), lambda x: (x[..., 2 * d:], x[..., :d], x[..., d:2 * d]))):
+        q, k, rest = at(x)
+        w = 1 + 0.2 * torch.randn(d, device="cuda", generator=g)
+        kept = rest.clone()
+        want = kernels.qk_norm_rotary(q.contiguous(), k.contiguous(), positions, table, w, w)
+        target = torch.empty_like(x).copy_(x)
+        assert target.stride() == x.stride()
+        kernels.qk_norm_rotary(q, k, positions, table, w, w, out=at(target)[:2])
+        dq, dk = kernels.qk_norm_rotary_backward(*want, q, k, positions, table, w, w)[:2]
+        gradients = torch.empty_like(x).copy_(x)
+        kernels.qk_norm_rotary_backward(*want, q, k, positions, table, w, w, out=at(gradients)[:2])
+        kernels.qk_norm_rotary(q, k, positions, table, w, w, out=(q, k))
+        for got, parts in ((at(x), want), (at(target), want), (at(gradients), (dq, dk))):
+            assert torch.equal(got[0], parts[0]) and torch.equal(got[1], parts[1]) and torch.equal(got[2], kept)
