@@ -314,5 +314,5 @@ def dropout_add(residual: Tensor, update: Tensor, p: float, shared: int) -> Tens
     if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("dropout draws its seed on the host: a captured graph would repeat one mask "
                            "(kernels.dropout_train reads a seed on the device)")
-    seed = int(torch.empty((), dtype=torch.int64).random_())
+    seed = int(torch.empty((), dtype=torch.int64, device="cpu").random_())  # whatever the default device
     return _DropoutAdd.apply(residual, update, p, seed, shared)
