@@ -637,8 +637,8 @@ def rotary_table(frequencies: Sequence[float] | Tensor, axes: Sequence[int] | No
     a = [0] * f.numel() if axes is None else [int(i) for i in axes]
     if len(a) != f.numel() or any(not 0 <= i < 16 for i in a):
         raise ValueError(f"axes must name one of at most 16 axes for each of {f.numel()} pairs, got {a}")
-    return RotaryTable((f * (2.0 / math.pi)).to(device), torch.tensor(a, dtype=torch.int32).to(device), max(a, default=0) + 1,
-                       bool(interleaved))
+    pair_axes = torch.tensor(a, dtype=torch.int32, device="cpu")  # whatever the default device
+    return RotaryTable((f * (2.0 / math.pi)).to(device), pair_axes.to(device), max(a, default=0) + 1, bool(interleaved))
 
 
 def rotary(q: Tensor, k: Tensor | None, positions: Tensor, table: RotaryTable, *, inverse: bool = False,

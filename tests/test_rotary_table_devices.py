@@ -1,0 +1,19 @@
+"""A rotation's table is made on the device that is asked for, whatever the default device."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from foldforge_b200 import kernels
+from foldforge_b200.engine.modules import QKNorm
+
+
+@pytest.mark.parametrize("device", ["cpu", "meta"])
+def test_tables_under_another_default_device(device):
+    want = kernels.rotary_table([1.0, 0.1], [1, 0], device="cpu")
+    with torch.device(device):
+        got = kernels.rotary_table([1.0, 0.1], [1, 0], device="cpu")
+        table = QKNorm(8, frequencies=[1.0, 0.1], axes=[1, 0]).table(torch.device("cpu"))
+    for t in (got, table):
+        assert torch.equal(t.quarters, want.quarters) and torch.equal(t.pair_axes, want.pair_axes) and t.axes == 2
