@@ -195,7 +195,7 @@ class QKNorm(nn.Module):
         reason = _device_reason(q, k, positions) if trains else _cuda_reason(q, k, positions)
         if reason is None and not trains and training.needs_gradient(self):
             reason = "autograd is not supported by the b200 kernels (inference only)"
-        if reason or (reason := _library_reason()):
+        if reason or (reason := _library_reason(binding=True)):
             return reason
         if q.dtype not in (torch.bfloat16, torch.float32) or k.dtype != q.dtype:
             return f"dtypes {q.dtype} and {k.dtype} (both bf16 or both fp32)"
@@ -269,11 +269,12 @@ def _cuda_reason(*ts: Tensor | None) -> str | None:
     return None
 
 
-def _library_reason() -> str | None:
+def _library_reason(binding: bool = False) -> str | None:
+    """Why the kernels' library (or the compiled ``binding`` to it) cannot be used."""
     from foldforge_b200 import _lib
 
     try:
-        _lib.load()
+        _lib.binding() if binding else _lib.load()
     except _lib.LibraryMissing as exc:
         return str(exc)
     return None

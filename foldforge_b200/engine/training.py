@@ -276,8 +276,17 @@ def dropout_keep(shape, p: float, seed: int, offset: int = 0, shared: tuple[int,
 
 
 def _on_b200(*ts: Tensor) -> bool:
-    return all(t.is_cuda and t.dtype in (torch.bfloat16, torch.float32) for t in ts) and \
-        torch.cuda.get_device_capability(ts[0].device) == (10, 0)
+    """Whether the kernel takes these tensors; where it is not built, the ops' pytorch backend does without."""
+    from foldforge_b200 import _lib
+
+    if not all(t.is_cuda and t.dtype in (torch.bfloat16, torch.float32) for t in ts) or \
+            torch.cuda.get_device_capability(ts[0].device) != (10, 0):
+        return False
+    try:
+        _lib.binding()
+    except _lib.LibraryMissing:
+        return False
+    return True
 
 
 def _dropped(x: Tensor, residual: Tensor | None, p: float, seed: int, shared: int, dtype: torch.dtype) -> Tensor:
