@@ -1,6 +1,6 @@
 // The torch-facing calls of the training operators and of those around an attention: argument checks,
-// outputs, workspaces, device and stream, then one call of the C ABI (include/foldforge_b200.h). A call of one token's row costs what the
-// host needs to issue it: about 14 us by ctypes from Python, 7 us from here.
+// outputs, workspaces, device and stream, then one call of the C ABI (include/foldforge_b200.h). A call of
+// one token's row costs what the host needs to issue it: about 14 us by ctypes from Python, 7 us from here.
 //
 // The entry points come in as addresses (bind()), so this module does not link the kernels' library.
 // Refusals and errors raise the exceptions of foldforge_b200._lib.

@@ -3,13 +3,15 @@
 // backward pass draws it again, and neither the grid nor a tensor's layout enters it.
 //
 // Measured on one B200 (device time, inputs past L2; a plain copy moves 6.55 TB/s):
-//   512 x 512 x 128 bf16, a mask for all rows       forward 28.7 us (7.0 TB/s, part of it still in L2), backward 20.5
-//   16384 x 4096 bf16, each element for itself      forward 65.3 us (6.2 TB/s), backward 64.2 (4.2)
-//   8192 x 4096 fp32, each element for itself       forward 61.3 us (6.6 TB/s), backward 42.0 (6.4)
+//   512 x 512 x 128 bf16, a mask for all rows       forward 28.8 us (7.0 TB/s, part of it still in L2), backward 21.6
+//   16384 x 4096 bf16, each element for itself      forward 66.7 us (6.0 TB/s), backward 67.9 (4.0)
+//   8192 x 4096 fp32, each element for itself       forward 61.2 us (6.6 TB/s), backward 43.0 (6.2)
+//   700 x 700 x 33 bf16, a mask for all rows        forward 30.8 us (3.2 TB/s), backward 28.7: single elements
+//   1500 x 1500 x 16 bf16, a mask for all columns   forward 69 us (3.1 TB/s), backward 66: closer than 32 elements
 // The generator bounds the bf16 backward pass where every element has its own word: ten rounds of two 32 x 32
 // bit products for four elements. A product takes its pipe four cycles a warp (its counter: 66% busy), the
-// exclusive ors, comparisons and conversions another pipe two each (62%), and 21 instructions an element
-// issue in 60% of the slots. What helped there: the rounds' keys in the launch's parameters (86 -> 69 us with the
+// exclusive ors, comparisons and conversions another pipe two each (62%), and 23 instructions an element
+// issue in 68% of the slots. What helped there: the rounds' keys in the launch's parameters (86 -> 69 us with the
 // next), a predicated addition for a selection, products that a block's threads share. Without effect or
 // slower: one or four vectors a thread, blocks that loop.
 #include "kernels.h"

@@ -15,7 +15,8 @@
 // Measured on one B200 (device time, inputs past L2; a plain copy moves 6.55 TB/s; boxes differ by 5%):
 //   65536 tokens, 32 + 8 heads x 128 bf16          forward 214 us (6.3 TB/s), backward 339 (5.9)
 //   2 x 24960 tokens, 24 + 24 heads x 128 bf16     rotation alone 207 us (5.9 TB/s)
-//   65536 tokens, 16 + 16 heads x 48 bf16          forward 85 us (4.8 TB/s), backward 143 (4.2)
+//   65536 tokens, 16 + 16 heads x 48 bf16          forward 86 us (4.7 TB/s), backward 141 (4.3)
+//   65536 tokens, 16 + 16 heads x 24 bf16          forward 67 us (3.0 TB/s), backward 109 (2.8)
 //   500000 tokens, 4 + 4 heads x 32 bf16           forward 131 us (3.9 TB/s), backward 192 (4.0)
 // In the first case 16 warps an SM issue in 60% of the slots: 13 instructions for 32 channels forward and 21 backward.
 // A token costs a crew about as much as two to four steps of its heads (angles, addresses, the weight's values), so
@@ -382,9 +383,10 @@ struct Stream {
   }
 };
 
-// Slots of the rings, and blocks that an SM holds. 65536 tokens of 40 heads x 128 in bf16, a warp a token: forward 214 us
-// with two blocks (111 registers a thread) and 3, 4 or 6 slots, 260 with three (80 registers, 150 bytes of them
-// spilled); backward 371 us with 3 slots, 384 with 6, 398 with one block, 624 with three.
+// Slots of the rings, and blocks that an SM holds. 65536 tokens of 40 heads x 128 in bf16: forward 214 us with two blocks
+// (111 registers a thread) and 3, 4 or 6 slots, 260 with three (80 registers, 150 bytes of them spilled). Backward,
+// compared when a warp took a token (plan_of's crews now take 339 to 355 us): 371 us with 3 slots, 384 with 6, 398 with
+// one block, 624 with three. At two blocks the bf16 backward kernels' 128 registers spill 14 to 62 bytes.
 constexpr int kForwardSlots = 3, kBackwardSlots = 3;
 template <typename T, int P>
 constexpr int kResident = P * static_cast<int>(sizeof(T)) > 16 ? 1 : 2;
@@ -621,9 +623,9 @@ int dispatch_heads(const HeadsParams& p, bool backward, F&& f) {
 // pairs' angles, and its steps; its memory time, the bytes of its heads, where the issue of a full step of 1 KB an
 // input takes 40 and its memory 57 (44 of a backward step, which issues more for its three KB; fp32 a quarter more). The GPU's crews take
 // the items in rounds. Smaller crews share the fixed work among more tokens of a warp and take more steps, which
-// helps where the issue is the limit (65536 tokens of 32 heads x 24: 68 -> 35 us forward, 84 -> 52 backward; of 32 x
-// 48 104 -> 88 and 174 -> 141) and not where the memory is (40 x 128: 214 -> 218 forward). Where there are few
-// tokens, a whole warp takes a token, or a part of its heads.
+// helps where the issue is the limit (65536 tokens of 16 heads x 24: 68 -> 39 us forward, 84 -> 62 backward; of 32 x 24
+// 86 -> 67 and 114 -> 109; of 32 x 48 104 -> 86 and 174 -> 141) and not where the memory is (40 x 128: 214 -> 218
+// forward). Where there are few tokens, a whole warp takes a token, or a part of its heads.
 Plan plan_of(const HeadsParams& p, int lanes, int run, int resident, int size, bool backward) {
   const int heads = p.heads[0] + p.heads[1];
   Plan best{0, Divisor(1), Divisor(static_cast<uint32_t>(p.tokens)), heads, 0, 0, 0};

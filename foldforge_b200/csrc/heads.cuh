@@ -17,7 +17,8 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMostBlocks = 148 * 4;  // rows of partial gradients of q's, and as many of k's
 
 // Cosine and sine of an angle of at most an eighth of a turn, r quarter turns (|r| <= 1/2): polynomials in r^2
-// through Chebyshev's nodes, off by less than 0.2 steps of 2^-24 before the roundings of their own evaluation.
+// through Chebyshev's nodes. With coefficients in 32 bits they are off by 0.12 (cosine) and 0.4 (sine) steps of 2^-24; with
+// the roundings of r and of their evaluation by 1.3 and 1.7 (20 million angles).
 __device__ __forceinline__ float2 eighth_turn(float r) {
   const float t = r * r;
   const float s = r * fmaf(fmaf(fmaf(-0.0046021491289f, t, 0.0796802192926f), t, -0.6459634900093f), t, 1.5707963705063f);

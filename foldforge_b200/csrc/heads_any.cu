@@ -12,6 +12,8 @@
 //   65536 tokens, 8 + 8 heads x 151 bf16    forward 254 (334), backward 363 (414)
 //   79000 tokens, 2 + 2 heads x 51 fp32     forward 51 (107), backward 68 (137)
 //   20000 tokens, 4 + 4 heads x 500 bf16    forward 184 (170), backward 250 (182): no registers are left for a batch
+//   500000 tokens, 4 + 4 heads x 32 bf16    forward 234, backward 327 with 15 pairs in halves (16 pairs are whole runs
+//                                           and take heads.cu's rings: 130 and 194)
 // Bound by instructions: 2-byte loads and stores, and at 37 channels 19 of 32 lanes. Rows staged through shared memory
 // by asynchronous copies of the 16 bytes around them instead: 37 channels 125 and 202, 151 298 and 532.
 #include <type_traits>

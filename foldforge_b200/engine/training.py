@@ -7,12 +7,12 @@ op has one on b200 at all:
 * ``"exact"``: its input as it is.
 * ``"mxfp8"``: its input in 8 bits (33 bytes for 32 channels, :class:`foldforge_b200.kernels.Checkpoint8`).
 
-``LayerNorm`` and ``Transition`` have gradients; :func:`set_checkpoint` sets them for a whole model. A
+``LayerNorm``, ``Transition`` and ``QKNorm`` have gradients; :func:`set_checkpoint` sets them for a whole model. A
 transition's forward pass runs the kernels it runs without gradients and gives the same output; its backward
 pass computes the hidden activations again from the kept input, in bf16 with sums in fp32 (the ``pytorch``
 backend holds them in fp32). ``LayerNorm``'s forward pass is a kernel of its own, which keeps the rows'
 statistics: its output is the one without gradients but for the order of its sums. Only the gradients that
-are asked for are formed.
+are asked for are formed (``QKNorm``'s kernel forms those of q and k in one pass, whichever is asked for).
 
 A backward pass is not captured into a CUDA graph: autograd keeps a leaf's accumulation on the stream of
 the graph that made it first, and capturing another while that one lives ends the process. A captured
