@@ -58,7 +58,7 @@ def set_dropout(model: nn.Module, p: float | None = None) -> list[str]:
     ``p_drop``; 0: none) while it is in training mode; their names. The factories give their ops no rate: ``None``
     is refused where that would leave every op without one."""
     found = [(path, m) for path, m in model.named_modules() if hasattr(m, "set_dropout")]
-    if p is None and found and all(m.p_drop == 0 for _, m in found):
+    if p is None and found and all(getattr(m, "p_drop", None) == 0 for _, m in found):
         raise ValueError(f"no op of {type(model).__name__} has a p_drop of its own: give a rate")
     for _, m in found:
         m.set_dropout(p)

@@ -36,3 +36,14 @@ def test_ops_with_and_without_a_rate():
     names = training.set_dropout(model)
     assert len(names) == 8 and dropping(model) == names[:4]
     assert training.set_dropout(Transition(8)) == []  # nothing to drop
+
+
+def test_an_op_of_another_kind_keeps_its_own_rate():
+    """A module of the user's that takes dropout in its own way decides what no rate means."""
+
+    class Op(torch.nn.Module):
+        def set_dropout(self, p=None):
+            self.dropout = 0.3 if p is None else p
+
+    op = Op()
+    assert training.set_dropout(op) == [""] and op.dropout == 0.3
