@@ -21,7 +21,6 @@ applies the reference equations there too.
 from __future__ import annotations
 
 from contextvars import ContextVar
-from copy import deepcopy
 from dataclasses import dataclass
 
 import torch
@@ -162,11 +161,8 @@ class QKNorm(nn.Module):
                 p.data = p.data.float()
         return out
 
-    def __deepcopy__(self, memo):
-        copy = self.__new__(type(self))
-        memo[id(self)] = copy
-        copy.__dict__.update({k: ({} if k == "_tables" else deepcopy(v, memo)) for k, v in self.__dict__.items()})
-        return copy
+    def __getstate__(self):  # copied or stored, it makes its tables again, wherever it then is
+        return {**self.__dict__, "_tables": {}}
 
     def set_backend(self, name: str) -> None:
         _check_backend(self, name)
